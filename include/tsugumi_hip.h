@@ -684,6 +684,123 @@ tsg_status tsg_prefill_int4_qmm(tsg_ctx* ctx, tsg_stream stream, const uint8_t* 
                                 const uint16_t* x, uint16_t* y, uint32_t t, uint32_t n,
                                 uint32_t k);
 
+/* ------------------------------------------------------------ attention ---
+ * The attention half of a decoder layer, between the Q, K, V projections
+ * (tsg_qmv_int4*, tsg_prefill_int4_qmm) and the O projection, over a paged
+ * key/value cache in HBM. No counterpart entries: the reference's attention
+ * encoders are outside this library's path; these are its own.
+ *
+ * Sequence s of a batch has lengths[s] tokens in the cache, this call's rows
+ * among them: row i of its n rows is at position p = lengths[s] - n + i. Its
+ * token t lies in slot t % page_tokens of page page_table[s * table_stride +
+ * t / page_tokens]. A row with p < 0 (a padded row, a sequence of length 0) is
+ * no token: nothing of it is appended and its outputs are zeros. Rows behind
+ * the last sequence's (row_starts) are left as they were.
+ *
+ * page_table, lengths and row_starts are read on the device, so a captured
+ * graph replays with what they then hold. A page id past the cache's pages, a
+ * sequence longer than its table, or row starts that fall or pass `rows` leave
+ * NaN in the rows concerned (query rows of an append included; nothing of them
+ * goes to the cache) and tsg_ctx_synchronize reports TSG_ERR_INVALID_ARGUMENT;
+ * the rows that share a kernel tile with them may be NaN as well. */
+
+/* What the cache holds: fp16, or OCP e4m3 codes c standing for c * scale. */
+typedef enum tsg_kv_type { TSG_KV_F16 = 0, TSG_KV_E4M3 = 1 } tsg_kv_type;
+
+/* One kind of attention layer. q_heads a multiple of kv_heads (query head h
+ * reads key head h / (q_heads / kv_heads)), at most 1024; head_dim a multiple
+ * of 8 (e4m3: of 16) up to 512; page_tokens a power of two in 16...4096.
+ * Key j is visible at position p iff j <= p and (window == 0 or p - j < window
+ * or j < sinks); sinks need a window. scale multiplies q . k. k_scale and
+ * v_scale (1e-6...1e6) are the e4m3 cache's and 1 for fp16. */
+typedef struct tsg_attn_config {
+    uint32_t q_heads, kv_heads, head_dim, page_tokens;
+    tsg_kv_type kv_type;
+    uint32_t window, sinks;
+    float scale, k_scale, v_scale;
+} tsg_attn_config;
+
+/* The cache's two pools, caller-owned. Element e of token slot t of key head h
+ * of page i is at i * page_stride + h * head_stride + t * token_stride + e
+ * (elements; multiples of 16 bytes). Heads and pages must not overlap; either
+ * of heads and tokens may be the inner one. */
+typedef struct tsg_kv_pages {
+    void* k;
+    void* v;
+    uint32_t num_pages, token_stride;
+    uint64_t head_stride, page_stride;
+} tsg_kv_pages;
+
+/* The sequences of one call. row_starts [num_seqs + 1]: sequence s has rows
+ * row_starts[s] .. row_starts[s + 1] - 1 of the row buffers, which hold `rows`
+ * rows; NULL: every sequence has rows / num_seqs of them. */
+typedef struct tsg_attn_batch {
+    const uint32_t* page_table;
+    const uint32_t* lengths;
+    const uint32_t* row_starts;
+    uint32_t table_stride, num_seqs, rows;
+} tsg_attn_batch;
+
+/* Projected rows, fp16: row r of q at q + r * q_stride (elements), its heads
+ * head_dim apart; the three may lie in one fused buffer. */
+typedef struct tsg_attn_rows {
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    uint32_t q_stride, k_stride, v_stride;
+} tsg_attn_rows;
+
+/* Head norms (bf16 weights [head_dim]; NULL: no norm) and position rotation:
+ * the first rotary_dim elements (a multiple of 16, 0: none) of a query or key
+ * head turn in pairs by position * inv_freq[i], pairs (i, i + rotary_dim / 2)
+ * or, interleaved, (2i, 2i + 1); inv_freq [rotary_dim / 2] on the device.
+ * normalize_v: values are divided by their root mean square too. */
+typedef struct tsg_attn_norm_rope {
+    const uint16_t* q_weight;
+    const uint16_t* k_weight;
+    const float* inv_freq;
+    uint32_t rotary_dim, interleaved, normalize_v;
+    float eps;
+} tsg_attn_norm_rope;
+
+typedef struct tsg_attn tsg_attn; /* one kind of attention layer and its scratch */
+
+/* The checks the entry points below make of these arguments, without a device
+ * (pages and batch may be NULL: not checked). */
+tsg_status tsg_attn_check(const tsg_attn_config* config, const tsg_kv_pages* pages,
+                          const tsg_attn_batch* batch);
+/* Calls on one tsg_attn run in stream order (they share its scratch); two
+ * tsg_attn may run beside each other. Destroyed before its context. */
+tsg_status tsg_attn_create(tsg_ctx* ctx, const tsg_attn_config* config, tsg_attn** out);
+void tsg_attn_destroy(tsg_attn* attn);
+
+/* Norms, rotation and cache write in one pass: for every row, q heads ->
+ * q_out (fp16), k heads -> the cache, v heads -> the cache (not rotated):
+ *   y = x * w / sqrt(mean(x^2) + eps), then (a cos t - b sin t, b cos t + a sin t)
+ * in fp32 (the angle t in fp64) with one rounding at the end; e4m3 codes are of
+ * y / scale, clamped to +-448. k and v may be the same rows. q_out may be q
+ * itself (same address and stride) and otherwise shares no element with the
+ * inputs. q, k, v, q_out rows on 16 bytes. */
+tsg_status tsg_attn_append(tsg_attn* attn, tsg_stream stream, const tsg_kv_pages* pages,
+                           const tsg_attn_batch* batch, const tsg_attn_rows* rows,
+                           const tsg_attn_norm_rope* norm_rope, uint16_t* q_out,
+                           uint32_t q_out_stride);
+/* out[row, head] = sum_j softmax_j(scale * q . k_j) v_j over the visible keys
+ * (zeros where there are none), softmax and sums in fp32, for 1...8 rows of
+ * every sequence (a decoded token, a speculative block). What lies in the
+ * cache at keys a row does not see, NaN and infinities among it, does not
+ * reach the row. Returns TSG_ERR_DECLINED for more than 8 rows a sequence;
+ * row_starts must be NULL. q and out rows on 16 bytes; out must not share an
+ * element with q. */
+tsg_status tsg_attn_decode(tsg_attn* attn, tsg_stream stream, const tsg_kv_pages* pages,
+                           const tsg_attn_batch* batch, const uint16_t* q, uint32_t q_stride,
+                           uint16_t* out, uint32_t out_stride);
+/* The same for any number of rows of each sequence, ragged or uniform: a
+ * prompt, or the next chunk of one. */
+tsg_status tsg_attn_prefill(tsg_attn* attn, tsg_stream stream, const tsg_kv_pages* pages,
+                            const tsg_attn_batch* batch, const uint16_t* q, uint32_t q_stride,
+                            uint16_t* out, uint32_t out_stride);
+
 /* ----------------------------------------------------------- layer tail ----
  * The Gemma decoder-layer tail after the MoE FFN, per row (fp16 h2, h1,
  * hidden; bf16 norm weights):

@@ -15,6 +15,9 @@ include/tsugumi_hip.h (libtsugumi_hip.so). Names follow the reference:
     ManifestReader + PackedExpertsLayoutReader -> MoEPack (install reader + layer upload)
     SharedExpertInt4        -> SharedExpertInt4 (Gemma's dense int4 MLP)
 
+The attention half of the layer (Attention, PagedKVCache, AttentionBatch,
+HeadNormRope) is this library's own.
+
 Device buffers are torch CUDA tensors (plumbing only); `stream` defaults to
 torch's current stream. Every call raises TsgError on a non-OK status; there
 is no CPU fallback.
@@ -26,7 +29,8 @@ import ctypes as C
 import numpy as np
 
 from . import _abi
-from ._abi import (TSG_ACT_GELU_TANH, TSG_ACT_SILU, TSG_AFFINE, TSG_SYM, ExpertOffsets,
+from ._abi import (TSG_ACT_GELU_TANH, TSG_ACT_SILU, TSG_AFFINE, TSG_ERR_INVALID_ARGUMENT,
+                   TSG_KV_E4M3, TSG_KV_F16, TSG_SYM, ExpertOffsets,
                    RoutedBlock, TokenExpertPair, TsgError, check, load)
 
 __all__ = [
@@ -34,6 +38,7 @@ __all__ = [
     "PrefillRouter", "PrefillMoEGrouping",
     "PrefillRoutedGEMMPlanner", "PrefillGroupedRoutedMoE", "PrefillMoE", "ResidentLayer",
     "MoEPack", "SharedExpertInt4", "PrefillLayerTail", "FusedLayerTail", "PrefillInt4QMM",
+    "Attention", "PagedKVCache", "AttentionBatch", "HeadNormRope",
     "ExpertOffsets", "TsgError", "PAIR_DTYPE", "BLOCK_DTYPE", "GROUP_DTYPE", "TILE_DTYPE",
     "generators", "load",
 ]
@@ -86,6 +91,15 @@ def _stream(stream) -> int | None:
     if _current_stream is None:
         _current_stream = _stream_reader()
     return _current_stream()
+
+
+def _current_stream_of(device: int) -> int:
+    """torch's current stream on `device`, which need not be the current one."""
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    if raw is not None and torch.cuda.is_initialized():
+        return raw(device)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def _np_ptr(a: np.ndarray):
@@ -827,6 +841,183 @@ class FusedLayerTail:
         check(self.lib.tsg_fused_layer_tail(
             self.ctx.handle, _stream(stream), _ptr(h2), _ptr(h1), _ptr(hidden),
             _ptr(post_ffn2_weight), _ptr(post_ffn_weight), d, eps, layer_scalar))
+
+
+def _refuse(text: str):
+    raise TsgError(TSG_ERR_INVALID_ARGUMENT, text)
+
+
+def _types(*names):
+    """torch's types of these names (bit patterns travel as 16-bit integers too)."""
+    import torch
+    return tuple(getattr(torch, n) for n in names if hasattr(torch, n))
+
+
+class PagedKVCache:
+    """A layer's key and value pools (tsg_kv_pages) on torch CUDA tensors of
+    shape [pages, kv_heads, page_tokens, head_dim], contiguous or views with
+    the heads inside the tokens (the last dimension contiguous)."""
+
+    def __init__(self, attn: "Attention", k, v):
+        c = attn.config
+        shape = (c.kv_heads, c.page_tokens, c.head_dim)
+        types = _types("float8_e4m3fn", "uint8") if c.kv_type == TSG_KV_E4M3 \
+            else _types("float16", "int16", "uint16")
+        for t in (k, v):
+            if not t.is_cuda or t.device.index != attn.ctx.device:
+                _refuse("cache pages must be on the context's device")
+            if t.dim() != 4 or tuple(t.shape[1:]) != shape:
+                _refuse(f"cache pages of shape {tuple(t.shape)}, not [pages, {shape}]")
+            if t.dtype not in types:
+                _refuse(f"cache pages of {t.dtype}, not {types[0]}")
+            if t.stride(3) != 1:
+                _refuse("a cache row's elements must be contiguous")
+        if k.shape != v.shape or k.stride() != v.stride():
+            _refuse("key and value pages differ in shape or strides")
+        page, head, token, _ = k.stride()
+        # a stride over one element is any number in torch; the library wants a real one
+        self._keep = (k, v)
+        self.pages = _abi.KVPages(k.data_ptr(), v.data_ptr(), k.shape[0], token,
+                                  head if shape[0] > 1 else 0, page if k.shape[0] > 1 else 0)
+        self._ref = C.addressof(self.pages)
+        check(attn.lib.tsg_attn_check(C.addressof(c), self._ref, None))
+
+
+class AttentionBatch:
+    """The sequences of one call (tsg_attn_batch): page_table [seqs, pages] and
+    lengths [seqs] of 32-bit integers; row_starts [seqs + 1] for ragged rows."""
+
+    def __init__(self, attn: "Attention", page_table, lengths, rows: int, row_starts=None):
+        for t in (page_table, lengths, row_starts):
+            if t is None:
+                continue
+            if not t.is_cuda or t.device.index != attn.ctx.device:
+                _refuse("batch tensors must be on the context's device")
+            if t.dtype not in _types("int32", "uint32") or not t.is_contiguous():
+                _refuse("batch tensors must be contiguous 32-bit integers")
+        if page_table.dim() != 2 or lengths.dim() != 1 or \
+                page_table.shape[0] != lengths.shape[0]:
+            _refuse("page_table must be [seqs, pages] and lengths [seqs]")
+        seqs = lengths.shape[0]
+        if row_starts is not None and tuple(row_starts.shape) != (seqs + 1,):
+            _refuse("row_starts must be [seqs + 1]")
+        self._keep = (page_table, lengths, row_starts)
+        self.rows = int(rows)
+        self.batch = _abi.AttnBatch(_ptr(page_table), _ptr(lengths), _ptr(row_starts),
+                                    page_table.shape[1], seqs, self.rows)
+        self._ref = C.addressof(self.batch)
+        check(attn.lib.tsg_attn_check(C.addressof(attn.config), None, self._ref))
+
+
+class HeadNormRope:
+    """Head norms (bf16 weights [head_dim] or None) and position rotation
+    (inv_freq: fp32 [rotary_dim / 2] or None) of tsg_attn_append."""
+
+    def __init__(self, q_weight=None, k_weight=None, inv_freq=None, interleaved: bool = False,
+                 normalize_v: bool = False, eps: float = 1e-6):
+        bits = _types("bfloat16", "int16", "uint16")
+        for t, types in ((q_weight, bits), (k_weight, bits), (inv_freq, _types("float32"))):
+            if t is not None and (t.dim() != 1 or t.dtype not in types):
+                _refuse("norm weights are bf16 [head_dim], inv_freq is fp32 [rotary_dim / 2]")
+        self.widths = {int(t.shape[0]) for t in (q_weight, k_weight) if t is not None}
+        self._keep = (q_weight, k_weight, inv_freq)
+        self.norm_rope = _abi.AttnNormRope(
+            _ptr(q_weight), _ptr(k_weight), _ptr(inv_freq),
+            0 if inv_freq is None else 2 * inv_freq.shape[0], int(interleaved), int(normalize_v),
+            eps)
+        self._ref = C.addressof(self.norm_rope)
+
+
+class Attention:
+    """One kind of attention layer (tsg_attn): append, decode and prefill over a
+    paged cache. scale defaults to head_dim ** -0.5. Row operands are fp16
+    tensors [rows, heads, head_dim] or [rows, heads * head_dim], rows any
+    16-byte multiple apart. Work goes to `stream`, or to torch's current stream
+    of the context's device."""
+
+    def __init__(self, ctx: Context, q_heads: int, kv_heads: int, head_dim: int,
+                 page_tokens: int, kv_type: str = "f16", window: int = 0, sinks: int = 0,
+                 scale: float | None = None, k_scale: float = 1.0, v_scale: float = 1.0):
+        self.handle = None
+        self.ctx = ctx
+        self.lib = ctx.lib
+        types = {"f16": TSG_KV_F16, "e4m3": TSG_KV_E4M3}
+        if kv_type not in types:
+            _refuse(f"unknown cache type {kv_type!r}")
+        if scale is None:
+            scale = float(head_dim) ** -0.5 if head_dim > 0 else 1.0
+        self.config = _abi.AttnConfig(q_heads, kv_heads, head_dim, page_tokens, types[kv_type],
+                                      window, sinks, scale, k_scale, v_scale)
+        h = C.c_void_p()
+        check(self.lib.tsg_attn_create(ctx.handle, C.addressof(self.config), C.byref(h)))
+        self.handle = h
+        self._half = _types("float16", "int16", "uint16")
+        self._q_width, self._kv_width = q_heads * head_dim, kv_heads * head_dim
+
+    def cache(self, k, v) -> PagedKVCache:
+        return PagedKVCache(self, k, v)
+
+    def batch(self, page_table, lengths, rows, row_starts=None) -> AttentionBatch:
+        return AttentionBatch(self, page_table, lengths, rows, row_starts)
+
+    def _rows(self, t, rows: int, heads: int, width: int):
+        """Address and row stride of a row operand."""
+        shape, strides = t.shape, t.stride()
+        if t.dtype not in self._half or not t.is_cuda or t.get_device() != self.ctx.device:
+            _refuse("row operands must be fp16 tensors on the context's device")
+        if len(shape) == 2:
+            fits = shape[1] == width and strides[1] == 1
+        else:
+            fits = (len(shape) == 3 and shape[1] == heads and shape[1] * shape[2] == width
+                    and strides[2] == 1 and (heads == 1 or strides[1] == shape[2]))
+        if not fits or shape[0] < rows:
+            _refuse(f"row operand of shape {tuple(shape)}, strides {strides}: not {rows} rows of "
+                    f"{width}")
+        return t.data_ptr(), strides[0] if shape[0] > 1 else width
+
+    def _on(self, stream):
+        if stream is not None:
+            return stream if isinstance(stream, int) else stream.cuda_stream
+        return _current_stream_of(self.ctx.device)
+
+    def encode_append(self, cache, batch, q, k, v, norm_rope, q_out, stream=None):
+        """Norms, rotation and cache write of the batch's rows; q_out gets the
+        query heads (it may be q)."""
+        c, n = self.config, batch.rows
+        if norm_rope.widths - {c.head_dim}:
+            _refuse("norm weights must be [head_dim]")
+        q, qs = self._rows(q, n, c.q_heads, self._q_width)
+        k, ks = self._rows(k, n, c.kv_heads, self._kv_width)
+        v, vs = self._rows(v, n, c.kv_heads, self._kv_width)
+        out, os = self._rows(q_out, n, c.q_heads, self._q_width)
+        rows = _abi.AttnRows(q, k, v, qs, ks, vs)
+        check(self.lib.tsg_attn_append(self.handle, self._on(stream), cache._ref, batch._ref,
+                                       C.addressof(rows), norm_rope._ref, out, os))
+
+    def _attend(self, call, cache, batch, q, out, stream):
+        c, n = self.config, batch.rows
+        q, qs = self._rows(q, n, c.q_heads, self._q_width)
+        out, os = self._rows(out, n, c.q_heads, self._q_width)
+        check(call(self.handle, self._on(stream), cache._ref, batch._ref, q, qs, out, os))
+
+    def encode_decode(self, cache, batch, q, out, stream=None):
+        """Attention of 1..8 new tokens of every sequence."""
+        self._attend(self.lib.tsg_attn_decode, cache, batch, q, out, stream)
+
+    def encode_prefill(self, cache, batch, q, out, stream=None):
+        """Attention of a prompt's rows, or of the next chunk of one."""
+        self._attend(self.lib.tsg_attn_prefill, cache, batch, q, out, stream)
+
+    def close(self) -> None:
+        if getattr(self, "handle", None) and getattr(self.ctx, "handle", None):
+            self.lib.tsg_attn_destroy(self.handle)
+        self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 class generators:

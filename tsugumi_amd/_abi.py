@@ -30,6 +30,7 @@ GROUPING_ERRORS = {
 
 TSG_AFFINE, TSG_SYM = 0, 1
 TSG_ACT_GELU_TANH, TSG_ACT_SILU = 0, 1
+TSG_KV_F16, TSG_KV_E4M3 = 0, 1
 
 
 class ExpertOffsets(C.Structure):
@@ -84,6 +85,40 @@ class Int4Projection(C.Structure):
     and the [rows, cols] shape of one int4 matrix."""
     _fields_ = [("weights", C.c_void_p), ("scales", C.c_void_p), ("biases", C.c_void_p),
                 ("rows", C.c_uint32), ("cols", C.c_uint32)]
+
+
+class AttnConfig(C.Structure):
+    """tsg_attn_config: one kind of attention layer."""
+    _fields_ = [("q_heads", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("page_tokens", C.c_uint32), ("kv_type", C.c_int), ("window", C.c_uint32),
+                ("sinks", C.c_uint32), ("scale", C.c_float), ("k_scale", C.c_float),
+                ("v_scale", C.c_float)]
+
+
+class KVPages(C.Structure):
+    """tsg_kv_pages: the cache's two pools, strides in elements."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("num_pages", C.c_uint32),
+                ("token_stride", C.c_uint32), ("head_stride", C.c_uint64),
+                ("page_stride", C.c_uint64)]
+
+
+class AttnBatch(C.Structure):
+    """tsg_attn_batch: the sequences of one attention call."""
+    _fields_ = [("page_table", C.c_void_p), ("lengths", C.c_void_p), ("row_starts", C.c_void_p),
+                ("table_stride", C.c_uint32), ("num_seqs", C.c_uint32), ("rows", C.c_uint32)]
+
+
+class AttnRows(C.Structure):
+    """tsg_attn_rows: projected query, key and value rows."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("q_stride", C.c_uint32), ("k_stride", C.c_uint32), ("v_stride", C.c_uint32)]
+
+
+class AttnNormRope(C.Structure):
+    """tsg_attn_norm_rope: head norms and position rotation."""
+    _fields_ = [("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("inv_freq", C.c_void_p),
+                ("rotary_dim", C.c_uint32), ("interleaved", C.c_uint32),
+                ("normalize_v", C.c_uint32), ("eps", C.c_float)]
 
 
 P = C.c_void_p
@@ -164,6 +199,12 @@ SIGNATURES = {
                                               U32, U32]),
     "tsg_prefill_moe_reduce_token_major": (C.c_int, [P, P, P, P, P, U32, U32, U32]),
     "tsg_prefill_int4_qmm": (C.c_int, [P, P, P, P, P, P, P, U32, U32, U32]),
+    "tsg_attn_check": (C.c_int, [P, P, P]),
+    "tsg_attn_create": (C.c_int, [P, P, C.POINTER(P)]),
+    "tsg_attn_destroy": (None, [P]),
+    "tsg_attn_append": (C.c_int, [P, P, P, P, P, P, P, U32]),
+    "tsg_attn_decode": (C.c_int, [P, P, P, P, P, U32, P, U32]),
+    "tsg_attn_prefill": (C.c_int, [P, P, P, P, P, U32, P, U32]),
     "tsg_prefill_layer_tail": (C.c_int, [P, P, P, P, P, P, P, U32, U32, U32, U32, U32,
                                          C.c_float, C.c_float]),
     "tsg_fused_layer_tail": (C.c_int, [P, P, P, P, P, P, P, U32, C.c_float, C.c_float]),

@@ -1,0 +1,537 @@
+// attn.hip — the attention half of a decoder layer over a paged key/value
+// cache: the plan object, the checks, and the append (head norms, rotation,
+// cache write).
+#include "attn_internal.hpp"
+
+#include <cmath>
+#include <new>
+
+namespace tsg {
+namespace {
+
+constexpr uint32_t kMaxHeads = 1024;
+constexpr uint32_t kMaxHeadDim = 512;
+constexpr uint32_t kMinPage = 16, kMaxPage = 4096;
+constexpr uint64_t kMaxCapacity = 1u << 30;  // tokens a page table may hold
+constexpr uint32_t kMaxAttnRows = 1u << 22;
+
+bool is16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool is4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+bool is2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
+
+uint32_t cell_bytes(const tsg_attn_config& c) { return c.kv_type == TSG_KV_E4M3 ? 1u : 2u; }
+
+}  // namespace
+
+tsg_status check_attn_config(const tsg_attn_config* c) {
+    TSG_REQUIRE(c, TSG_ERR_INVALID_ARGUMENT, "attention config is NULL");
+    TSG_REQUIRE(c->kv_heads > 0 && c->q_heads > 0 && c->q_heads <= kMaxHeads,
+                TSG_ERR_INVALID_ARGUMENT, "head counts must be in 1...%u", kMaxHeads);
+    TSG_REQUIRE(c->q_heads % c->kv_heads == 0, TSG_ERR_INVALID_ARGUMENT,
+                "%u query heads do not share %u key heads evenly", c->q_heads, c->kv_heads);
+    TSG_REQUIRE(c->kv_type == TSG_KV_F16 || c->kv_type == TSG_KV_E4M3, TSG_ERR_INVALID_ARGUMENT,
+                "unknown cache type %d", (int)c->kv_type);
+    const uint32_t step = 16u / cell_bytes(*c);
+    TSG_REQUIRE(c->head_dim > 0 && c->head_dim <= kMaxHeadDim && c->head_dim % step == 0,
+                TSG_ERR_UNSUPPORTED, "head_dim %u: a multiple of %u up to %u (16-byte cache rows)",
+                c->head_dim, step, kMaxHeadDim);
+    TSG_REQUIRE(c->page_tokens >= kMinPage && c->page_tokens <= kMaxPage &&
+                    (c->page_tokens & (c->page_tokens - 1u)) == 0,
+                TSG_ERR_UNSUPPORTED, "page_tokens %u: a power of two in %u...%u", c->page_tokens,
+                kMinPage, kMaxPage);
+    TSG_REQUIRE(c->window <= kMaxCapacity && c->sinks <= kMaxCapacity, TSG_ERR_INVALID_ARGUMENT,
+                "window or sinks above %llu", (unsigned long long)kMaxCapacity);
+    TSG_REQUIRE(c->window > 0 || c->sinks == 0, TSG_ERR_INVALID_ARGUMENT,
+                "sinks without a window: every token is visible already");
+    TSG_REQUIRE(std::isfinite(c->scale) && std::fabs(c->scale) <= 1e6f, TSG_ERR_INVALID_ARGUMENT,
+                "scale must be finite and at most 1e6");
+    // the scales' own reciprocals and products with `scale` stay normal fp32
+    const auto scale_ok = [](float s) { return s >= 1e-6f && s <= 1e6f; };
+    TSG_REQUIRE(scale_ok(c->k_scale) && scale_ok(c->v_scale), TSG_ERR_INVALID_ARGUMENT,
+                "k_scale and v_scale must be in 1e-6...1e6");
+    TSG_REQUIRE(c->kv_type == TSG_KV_E4M3 || (c->k_scale == 1.0f && c->v_scale == 1.0f),
+                TSG_ERR_INVALID_ARGUMENT, "an fp16 cache takes no scales (k_scale = v_scale = 1)");
+    return TSG_OK;
+}
+
+tsg_status check_attn_pages(const tsg_attn_config& c, const tsg_kv_pages* p) {
+    TSG_REQUIRE(p && p->k && p->v, TSG_ERR_INVALID_ARGUMENT, "NULL cache pages");
+    TSG_REQUIRE(p->num_pages > 0, TSG_ERR_INVALID_ARGUMENT, "a cache needs at least one page");
+    const uint32_t step = 16u / cell_bytes(c);
+    TSG_REQUIRE(is16(p->k) && is16(p->v), TSG_ERR_ALIGNMENT, "cache pages must be 16-byte aligned");
+    TSG_REQUIRE(p->token_stride % step == 0 && p->head_stride % step == 0 &&
+                    p->page_stride % step == 0,
+                TSG_ERR_ALIGNMENT, "cache strides must be multiples of 16 bytes");
+    // 64-bit products: page_tokens <= 2^12, token_stride < 2^32, heads <= 2^10
+    TSG_REQUIRE(p->head_stride < (1ull << 40) && p->page_stride < (1ull << 44),
+                TSG_ERR_INVALID_ARGUMENT, "cache stride too large");
+    const uint64_t run = (uint64_t)(c.page_tokens - 1u) * p->token_stride + c.head_dim;
+    const uint64_t across = (uint64_t)(c.kv_heads - 1u) * p->head_stride;
+    TSG_REQUIRE(p->token_stride >= c.head_dim, TSG_ERR_INVALID_ARGUMENT, "token stride is too small");
+    TSG_REQUIRE(c.kv_heads == 1 || p->head_stride >= run ||
+                    (p->head_stride >= c.head_dim && p->token_stride >= across + c.head_dim),
+                TSG_ERR_INVALID_ARGUMENT, "head stride is too small: heads overlap");
+    TSG_REQUIRE(p->num_pages == 1 || p->page_stride >= run + across, TSG_ERR_INVALID_ARGUMENT,
+                "page stride is too small: pages overlap");
+    // the kernels address a head's tokens within a page by 32-bit byte offsets
+    TSG_REQUIRE(run * cell_bytes(c) <= 0x7fffffffu, TSG_ERR_UNSUPPORTED,
+                "a page's rows of one head must span less than 2 GiB");
+    return TSG_OK;
+}
+
+tsg_status check_attn_batch(const tsg_attn_config& c, const tsg_attn_batch* b) {
+    TSG_REQUIRE(b, TSG_ERR_INVALID_ARGUMENT, "attention batch is NULL");
+    TSG_REQUIRE(b->num_seqs > 0, TSG_ERR_INVALID_ARGUMENT, "numSeqs must be positive");
+    TSG_REQUIRE(b->rows > 0 && b->rows <= kMaxAttnRows, TSG_ERR_INVALID_ARGUMENT,
+                "rows must be in 1...%u", kMaxAttnRows);
+    TSG_REQUIRE(b->num_seqs <= kMaxAttnRows, TSG_ERR_INVALID_ARGUMENT, "too many sequences");
+    TSG_REQUIRE(b->page_table && b->lengths, TSG_ERR_INVALID_ARGUMENT,
+                "NULL page table or lengths");
+    TSG_REQUIRE(is4(b->page_table) && is4(b->lengths) && is4(b->row_starts), TSG_ERR_ALIGNMENT,
+                "page table, lengths and row starts must be 4-byte aligned");
+    TSG_REQUIRE(b->table_stride > 0 && (uint64_t)b->table_stride * c.page_tokens <= kMaxCapacity,
+                TSG_ERR_INVALID_ARGUMENT, "a page table holds 1...%llu tokens",
+                (unsigned long long)kMaxCapacity);
+    TSG_REQUIRE(b->row_starts || b->rows % b->num_seqs == 0, TSG_ERR_INVALID_ARGUMENT,
+                "%u rows do not divide over %u sequences (give row starts)", b->rows, b->num_seqs);
+    return TSG_OK;
+}
+
+tsg_status attn_args(const tsg_attn* attn, const tsg_kv_pages* pages, const tsg_attn_batch* batch,
+                     const uint16_t* q, uint32_t q_stride, uint16_t* out, uint32_t out_stride,
+                     AttnArgs* a) {
+    TSG_REQUIRE(attn, TSG_ERR_INVALID_ARGUMENT, "attn is NULL");
+    const tsg_attn_config& c = attn->cfg;
+    if (tsg_status s = check_attn_pages(c, pages)) return s;
+    if (tsg_status s = check_attn_batch(c, batch)) return s;
+    TSG_REQUIRE(q && out, TSG_ERR_INVALID_ARGUMENT, "NULL attention operand");
+    TSG_REQUIRE(q_stride >= c.q_heads * c.head_dim, TSG_ERR_INVALID_ARGUMENT,
+                "q stride is too small");
+    TSG_REQUIRE(out_stride >= c.q_heads * c.head_dim, TSG_ERR_INVALID_ARGUMENT,
+                "out stride is too small");
+    TSG_REQUIRE(is16(q) && is16(out) && q_stride % 8u == 0 && out_stride % 8u == 0,
+                TSG_ERR_ALIGNMENT, "q and out rows must be 16-byte aligned");
+    a->q = q;
+    a->out = out;
+    a->k = static_cast<const uint8_t*>(pages->k);
+    a->v = static_cast<const uint8_t*>(pages->v);
+    a->table = batch->page_table;
+    a->lengths = batch->lengths;
+    a->row_starts = batch->row_starts;
+    a->error = attn->ctx->counters + kSyncErrorWord;
+    a->page_stride = pages->page_stride * attn->cell;
+    a->head_stride = pages->head_stride * attn->cell;
+    a->token_stride = pages->token_stride * attn->cell;
+    a->q_stride = q_stride;
+    a->out_stride = out_stride;
+    a->table_stride = batch->table_stride;
+    a->num_seqs = batch->num_seqs;
+    a->rows = batch->rows;
+    a->seq_rows = batch->row_starts ? 0u : batch->rows / batch->num_seqs;
+    a->num_pages = pages->num_pages;
+    a->q_heads = c.q_heads;
+    a->kv_heads = c.kv_heads;
+    a->group = attn->group;
+    a->dim = c.head_dim;
+    a->page_shift = attn->page_shift;
+    a->window = c.window;
+    a->sinks = c.sinks;
+    a->scale_log2 = (float)((double)c.scale * c.k_scale * 1.4426950408889634);
+    a->v_scale = c.v_scale;
+    return TSG_OK;
+}
+
+namespace {
+
+// ------------------------------------------------------------------ append
+//
+// Head rows x of q and k: y = x w / sqrt(mean(x^2) + eps) in fp32, then the
+// rotation of pairs (a, b) by t = position * inv_freq: (a cos t - b sin t,
+// b cos t + a sin t), one rounding at the end (fp16, or e4m3 of y / scale). The
+// angle is formed in fp64, in revolutions, and only its fraction goes to fp32
+// (v_sin_f32 / v_cos_f32 take revolutions): at position 10^6 an fp32 product
+// would be off by 0.03 rad, the fraction is off by 2^-25 of a turn.
+
+struct AppendArgs {
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    uint16_t* q_out;
+    const uint16_t* q_weight;
+    const uint16_t* k_weight;
+    const float* inv_freq;
+    uint8_t* k_pages;
+    uint8_t* v_pages;
+    const uint32_t* table;
+    const uint32_t* lengths;
+    const uint32_t* row_starts;
+    uint32_t* error;
+    uint64_t page_stride, head_stride;  // bytes
+    uint32_t token_stride;              // bytes
+    uint32_t q_stride, k_stride, v_stride, q_out_stride;
+    uint32_t table_stride, num_seqs, rows, seq_rows, num_pages;
+    uint32_t q_heads, kv_heads, dim, page_shift;
+    uint32_t rot, interleaved, normalize_v;
+    uint32_t lanes_log2;     // lanes a head row takes, 16 elements each
+    uint32_t waves_per_row;
+    float eps, k_inv_scale, v_inv_scale;
+};
+
+typedef float f4a4_t __attribute__((ext_vector_type(4), aligned(4)));
+
+__device__ __forceinline__ void unpack8(uint4 u, float* y) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        y[2 * i] = f16_to_f32((uint16_t)(w[i] & 0xFFFFu));
+        y[2 * i + 1] = f16_to_f32((uint16_t)(w[i] >> 16));
+    }
+}
+
+__device__ __forceinline__ uint4 pack8_f16(const float* y) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        w[i] = (uint32_t)f32_to_f16(y[2 * i]) | ((uint32_t)f32_to_f16(y[2 * i + 1]) << 16);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// x / scale clamped to e4m3's largest value, NaN kept.
+__device__ __forceinline__ float e4m3_range(float x, float inv_scale) {
+    const float y = x * inv_scale;
+    return y > 448.0f ? 448.0f : (y < -448.0f ? -448.0f : y);
+}
+
+__device__ __forceinline__ uint2 pack8_e4m3(const float* y, float inv_scale) {
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        int u = 0;
+        u = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_range(y[4 * i], inv_scale),
+                                            e4m3_range(y[4 * i + 1], inv_scale), u, false);
+        u = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_range(y[4 * i + 2], inv_scale),
+                                            e4m3_range(y[4 * i + 3], inv_scale), u, true);
+        w[i] = (uint32_t)u;
+    }
+    return make_uint2(w[0], w[1]);
+}
+
+// A wave takes one row's heads, 64 >> lanes_log2 of them: queries, then keys,
+// then values. Lane j of a head holds two 8-element chunks; for split pairs
+// chunk c and chunk c + rot / 16, so that both elements of every pair are the
+// lane's own, and its angles are inv_freq[8 j .. 8 j + 7] in either order of
+// pairs.
+template <bool E4M3>
+__global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4u + (threadIdx.x >> 6));
+    const uint32_t row = wave / a.waves_per_row;
+    if (row >= a.rows) return;
+    const uint32_t s = find_seq(a.row_starts, a.num_seqs, a.seq_rows, a.rows, row, a.error);
+    if (s >= a.num_seqs) return;
+    const uint32_t capacity = a.table_stride << a.page_shift;
+    const SeqRows sr = seq_rows(a.row_starts, a.lengths, s, a.seq_rows, a.rows, capacity);
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t L = 1u << a.lanes_log2, j = lane & (L - 1u);
+    const uint32_t head =
+        (wave % a.waves_per_row) * (64u >> a.lanes_log2) + (lane >> a.lanes_log2);
+    const uint32_t heads = a.q_heads + 2u * a.kv_heads;
+    const int32_t pos = (int32_t)sr.length - (int32_t)sr.count + (int32_t)(row - sr.first);
+    bool drop = sr.bad || pos < 0;  // nothing to append; the query row becomes zeros (NaN)
+    if (sr.bad && lane == 0) report(a.error, sr.bad);
+    uint32_t page = 0;
+    if (!drop) {
+        page = a.table[(uint64_t)s * a.table_stride + ((uint32_t)pos >> a.page_shift)];
+        if (page >= a.num_pages) {
+            drop = true;
+            if (lane == 0) report(a.error, kErrAttnPage);
+        }
+    }
+    if (head >= heads) return;
+    const bool is_q = head < a.q_heads, is_v = head >= a.q_heads + a.kv_heads;
+    const uint32_t kvh = is_q ? 0u : (is_v ? head - a.q_heads - a.kv_heads : head - a.q_heads);
+    const uint16_t* src = is_q ? a.q + (uint64_t)row * a.q_stride + head * a.dim
+                          : is_v ? a.v + (uint64_t)row * a.v_stride + kvh * a.dim
+                                 : a.k + (uint64_t)row * a.k_stride + kvh * a.dim;
+    const uint32_t chunks = a.dim / 8u, half = a.rot / 16u;
+    uint32_t c0 = 2u * j, c1 = 2u * j + 1u;
+    if (!a.interleaved && !is_v && j < half) {
+        c0 = j;
+        c1 = j + half;
+    }
+    const bool has0 = c0 < chunks, has1 = c1 < chunks;
+    float y[16];
+    unpack8(has0 ? *reinterpret_cast<const uint4*>(src + 8u * c0) : make_uint4(0, 0, 0, 0), y);
+    unpack8(has1 ? *reinterpret_cast<const uint4*>(src + 8u * c1) : make_uint4(0, 0, 0, 0), y + 8);
+
+    const uint16_t* weight = is_q ? a.q_weight : a.k_weight;
+    const bool norm = is_v ? a.normalize_v != 0 : weight != nullptr;
+    float ss = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) ss = __builtin_fmaf(y[e], y[e], ss);
+    for (uint32_t o = L >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, (int)o, 64);
+    if (norm) {
+        const float inv = 1.0f / __builtin_sqrtf(ss / (float)a.dim + a.eps);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[e] *= inv;
+        if (!is_v) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                y[e] *= has0 ? bf16_to_f32(weight[8u * c0 + e]) : 0.0f;
+                y[8 + e] *= has1 ? bf16_to_f32(weight[8u * c1 + e]) : 0.0f;
+            }
+        }
+    }
+    if (!is_v && j < half) {
+        const f4a4_t f0 = *reinterpret_cast<const f4a4_t*>(a.inv_freq + 8u * j);
+        const f4a4_t f1 = *reinterpret_cast<const f4a4_t*>(a.inv_freq + 8u * j + 4u);
+        const double turn = (double)pos * 0.15915494309189535;  // 1 / 2 pi
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            double t = turn * (double)(e < 4 ? f0[e & 3] : f1[e & 3]);
+            t -= __builtin_rint(t);
+            const float cs = __builtin_amdgcn_cosf((float)t), sn = __builtin_amdgcn_sinf((float)t);
+            const float u = a.interleaved ? y[2 * e] : y[e];
+            const float w = a.interleaved ? y[2 * e + 1] : y[e + 8];
+            const float ru = u * cs - w * sn, rw = w * cs + u * sn;
+            if (a.interleaved) {
+                y[2 * e] = ru;
+                y[2 * e + 1] = rw;
+            } else {
+                y[e] = ru;
+                y[e + 8] = rw;
+            }
+        }
+    }
+    if (is_q) {
+        if (drop) {
+            const float fill = pos < 0 && !sr.bad ? 0.0f : __builtin_nanf("");
+#pragma unroll
+            for (int e = 0; e < 16; ++e) y[e] = fill;
+        }
+        uint16_t* dst = a.q_out + (uint64_t)row * a.q_out_stride + head * a.dim;
+        if (has0) *reinterpret_cast<uint4*>(dst + 8u * c0) = pack8_f16(y);
+        if (has1) *reinterpret_cast<uint4*>(dst + 8u * c1) = pack8_f16(y + 8);
+        return;
+    }
+    if (drop) return;
+    uint8_t* dst = (is_v ? a.v_pages : a.k_pages) + page * a.page_stride + kvh * a.head_stride +
+                   (uint64_t)((uint32_t)pos & ((1u << a.page_shift) - 1u)) * a.token_stride;
+    if (E4M3) {
+        const float inv_scale = is_v ? a.v_inv_scale : a.k_inv_scale;
+        if (has0) *reinterpret_cast<uint2*>(dst + 8u * c0) = pack8_e4m3(y, inv_scale);
+        if (has1) *reinterpret_cast<uint2*>(dst + 8u * c1) = pack8_e4m3(y + 8, inv_scale);
+    } else {
+        if (has0) *reinterpret_cast<uint4*>(dst + 16u * c0) = pack8_f16(y);
+        if (has1) *reinterpret_cast<uint4*>(dst + 16u * c1) = pack8_f16(y + 8);
+    }
+}
+
+// --------------------------------------------------------------- attention
+//
+// One wave a (row, query head): the keys one after another, lanes over the
+// head's elements.
+template <bool E4M3>
+__global__ __launch_bounds__(64) void attention_kernel(AttnArgs a) {
+    const uint32_t row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
+    const uint32_t s = find_seq(a.row_starts, a.num_seqs, a.seq_rows, a.rows, row, a.error);
+    if (s >= a.num_seqs) return;
+    const uint32_t capacity = a.table_stride << a.page_shift;
+    const SeqRows sr = seq_rows(a.row_starts, a.lengths, s, a.seq_rows, a.rows, capacity);
+    const int32_t pos = (int32_t)sr.length - (int32_t)sr.count + (int32_t)(row - sr.first);
+    const uint32_t kvh = head / a.group;
+    const uint16_t* q = a.q + (uint64_t)row * a.q_stride + head * a.dim;
+    float qv[8], acc[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        qv[e] = lane + 64u * e < a.dim ? f16_to_f32(q[lane + 64u * e]) : 0.0f;
+        acc[e] = 0.0f;
+    }
+    float m = -1e30f, l = 0.0f;
+    bool bad = sr.bad;
+    if (bad && lane == 0) report(a.error, sr.bad);
+    const auto load = [&](const uint8_t* p, uint32_t i) -> float {
+        if (i >= a.dim) return 0.0f;
+        if (E4M3) {
+            const uint2 u = e4m3x4_to_f16(p[i]);
+            return f16_to_f32((uint16_t)(u.x & 0xFFFFu));
+        }
+        return f16_to_f32(reinterpret_cast<const uint16_t*>(p)[i]);
+    };
+    for (int32_t t = 0; t <= pos && !bad; ++t) {
+        if (a.window && pos - t >= (int32_t)a.window && t >= (int32_t)a.sinks) {
+            t = pos - (int32_t)a.window;  // on to the window's first key
+            continue;
+        }
+        const uint32_t page = a.table[(uint64_t)s * a.table_stride + ((uint32_t)t >> a.page_shift)];
+        if (page >= a.num_pages) {
+            bad = true;
+            if (lane == 0) report(a.error, kErrAttnPage);
+            break;
+        }
+        const uint64_t at = page * a.page_stride + kvh * a.head_stride +
+                            (uint64_t)((uint32_t)t & ((1u << a.page_shift) - 1u)) * a.token_stride;
+        float dot = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dot = __builtin_fmaf(qv[e], load(a.k + at, lane + 64u * e), dot);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
+        dot *= a.scale_log2;
+        const float mn = fmaxf(m, dot);
+        const float alpha = __builtin_amdgcn_exp2f(m - mn), p = __builtin_amdgcn_exp2f(dot - mn);
+        m = mn;
+        l = l * alpha + p;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            acc[e] = acc[e] * alpha + p * load(a.v + at, lane + 64u * e);
+    }
+    const float inv = bad ? __builtin_nanf("") : (l == 0.0f ? 0.0f : a.v_scale / l);
+    uint16_t* out = a.out + (uint64_t)row * a.out_stride + head * a.dim;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (lane + 64u * e < a.dim) out[lane + 64u * e] = f32_to_f16(acc[e] * inv);
+}
+
+tsg_status attention(tsg_attn* attn, tsg_stream stream, const tsg_kv_pages* pages,
+                     const tsg_attn_batch* batch, const uint16_t* q, uint32_t q_stride,
+                     uint16_t* out, uint32_t out_stride) {
+    AttnArgs a{};
+    if (tsg_status s = attn_args(attn, pages, batch, q, q_stride, out, out_stride, &a)) return s;
+    DeviceScope scope(attn->ctx->device);
+    TSG_HIP_TRY(scope.status);
+    const dim3 grid(a.rows, a.q_heads);
+    if (attn->cfg.kv_type == TSG_KV_E4M3)
+        hipLaunchKernelGGL(attention_kernel<true>, grid, dim3(64), 0, as_stream(stream), a);
+    else
+        hipLaunchKernelGGL(attention_kernel<false>, grid, dim3(64), 0, as_stream(stream), a);
+    return check_launch("attention");
+}
+
+}  // namespace
+}  // namespace tsg
+
+using namespace tsg;
+
+extern "C" tsg_status tsg_attn_check(const tsg_attn_config* config, const tsg_kv_pages* pages,
+                                     const tsg_attn_batch* batch) {
+    if (tsg_status s = check_attn_config(config)) return s;
+    if (pages)
+        if (tsg_status s = check_attn_pages(*config, pages)) return s;
+    if (batch)
+        if (tsg_status s = check_attn_batch(*config, batch)) return s;
+    return TSG_OK;
+}
+
+extern "C" tsg_status tsg_attn_create(tsg_ctx* ctx, const tsg_attn_config* config, tsg_attn** out) {
+    TSG_REQUIRE(out, TSG_ERR_INVALID_ARGUMENT, "out is NULL");
+    *out = nullptr;
+    if (tsg_status s = check_attn_config(config)) return s;
+    TSG_REQUIRE(ctx, TSG_ERR_INVALID_ARGUMENT, "ctx is NULL");
+    tsg_attn* attn = new (std::nothrow) tsg_attn();
+    TSG_REQUIRE(attn, TSG_ERR_OUT_OF_MEMORY, "host allocation failed");
+    attn->ctx = ctx;
+    attn->cfg = *config;
+    attn->group = config->q_heads / config->kv_heads;
+    attn->page_shift = (uint32_t)__builtin_ctz(config->page_tokens);
+    attn->cell = cell_bytes(*config);
+    *out = attn;
+    return TSG_OK;
+}
+
+extern "C" void tsg_attn_destroy(tsg_attn* attn) { delete attn; }
+
+extern "C" tsg_status tsg_attn_append(tsg_attn* attn, tsg_stream stream, const tsg_kv_pages* pages,
+                                      const tsg_attn_batch* batch, const tsg_attn_rows* rows,
+                                      const tsg_attn_norm_rope* nr, uint16_t* q_out,
+                                      uint32_t q_out_stride) {
+    TSG_REQUIRE(attn, TSG_ERR_INVALID_ARGUMENT, "attn is NULL");
+    const tsg_attn_config& c = attn->cfg;
+    if (tsg_status s = check_attn_pages(c, pages)) return s;
+    if (tsg_status s = check_attn_batch(c, batch)) return s;
+    TSG_REQUIRE(rows && nr && rows->q && rows->k && rows->v && q_out, TSG_ERR_INVALID_ARGUMENT,
+                "NULL append operand");
+    const uint32_t q_width = c.q_heads * c.head_dim, kv_width = c.kv_heads * c.head_dim;
+    TSG_REQUIRE(rows->q_stride >= q_width && q_out_stride >= q_width, TSG_ERR_INVALID_ARGUMENT,
+                "q stride is too small");
+    TSG_REQUIRE(rows->k_stride >= kv_width && rows->v_stride >= kv_width, TSG_ERR_INVALID_ARGUMENT,
+                "k or v stride is too small");
+    TSG_REQUIRE(is16(rows->q) && is16(rows->k) && is16(rows->v) && is16(q_out) &&
+                    rows->q_stride % 8u == 0 && rows->k_stride % 8u == 0 &&
+                    rows->v_stride % 8u == 0 && q_out_stride % 8u == 0,
+                TSG_ERR_ALIGNMENT, "q, k and v rows must be 16-byte aligned");
+    TSG_REQUIRE(nr->rotary_dim <= c.head_dim && nr->rotary_dim % 16u == 0, TSG_ERR_UNSUPPORTED,
+                "rotary_dim %u: a multiple of 16 up to head_dim", nr->rotary_dim);
+    TSG_REQUIRE(nr->rotary_dim == 0 || nr->inv_freq, TSG_ERR_INVALID_ARGUMENT, "inv_freq is NULL");
+    TSG_REQUIRE(is4(nr->inv_freq) && is2(nr->q_weight) && is2(nr->k_weight), TSG_ERR_ALIGNMENT,
+                "norm weights must be 2-byte and inv_freq 4-byte aligned");
+    TSG_REQUIRE(nr->eps >= 0.0f && std::isfinite(nr->eps), TSG_ERR_INVALID_ARGUMENT,
+                "eps must be finite and not negative");
+    AppendArgs a{};
+    a.q = rows->q;
+    a.k = rows->k;
+    a.v = rows->v;
+    a.q_out = q_out;
+    a.q_weight = nr->q_weight;
+    a.k_weight = nr->k_weight;
+    a.inv_freq = nr->inv_freq;
+    a.k_pages = static_cast<uint8_t*>(pages->k);
+    a.v_pages = static_cast<uint8_t*>(pages->v);
+    a.table = batch->page_table;
+    a.lengths = batch->lengths;
+    a.row_starts = batch->row_starts;
+    a.error = attn->ctx->counters + kSyncErrorWord;
+    a.page_stride = pages->page_stride * attn->cell;
+    a.head_stride = pages->head_stride * attn->cell;
+    a.token_stride = pages->token_stride * attn->cell;
+    a.q_stride = rows->q_stride;
+    a.k_stride = rows->k_stride;
+    a.v_stride = rows->v_stride;
+    a.q_out_stride = q_out_stride;
+    a.table_stride = batch->table_stride;
+    a.num_seqs = batch->num_seqs;
+    a.rows = batch->rows;
+    a.seq_rows = batch->row_starts ? 0u : batch->rows / batch->num_seqs;
+    a.num_pages = pages->num_pages;
+    a.q_heads = c.q_heads;
+    a.kv_heads = c.kv_heads;
+    a.dim = c.head_dim;
+    a.page_shift = attn->page_shift;
+    a.rot = nr->rotary_dim;
+    a.interleaved = nr->interleaved ? 1u : 0u;
+    a.normalize_v = nr->normalize_v ? 1u : 0u;
+    while ((16u << a.lanes_log2) < c.head_dim) ++a.lanes_log2;
+    const uint32_t heads = c.q_heads + 2u * c.kv_heads, per_wave = 64u >> a.lanes_log2;
+    a.waves_per_row = (heads + per_wave - 1u) / per_wave;
+    a.eps = nr->eps;
+    a.k_inv_scale = 1.0f / c.k_scale;
+    a.v_inv_scale = 1.0f / c.v_scale;
+    DeviceScope scope(attn->ctx->device);
+    TSG_HIP_TRY(scope.status);
+    const uint64_t waves = (uint64_t)a.rows * a.waves_per_row;
+    TSG_REQUIRE(waves <= 0x7fffffffu, TSG_ERR_UNSUPPORTED, "too many rows and heads for one launch");
+    const dim3 grid((uint32_t)((waves + 3u) / 4u));
+    if (c.kv_type == TSG_KV_E4M3)
+        hipLaunchKernelGGL(append_kernel<true>, grid, dim3(256), 0, as_stream(stream), a);
+    else
+        hipLaunchKernelGGL(append_kernel<false>, grid, dim3(256), 0, as_stream(stream), a);
+    return check_launch("attn_append");
+}
+
+extern "C" tsg_status tsg_attn_decode(tsg_attn* attn, tsg_stream stream, const tsg_kv_pages* pages,
+                                      const tsg_attn_batch* batch, const uint16_t* q,
+                                      uint32_t q_stride, uint16_t* out, uint32_t out_stride) {
+    if (attn && batch) {
+        TSG_REQUIRE(!batch->row_starts, TSG_ERR_INVALID_ARGUMENT,
+                    "decode takes the same 1...8 rows of every sequence (no row starts)");
+        TSG_REQUIRE(batch->num_seqs == 0 || batch->rows / batch->num_seqs <= kMaxDecodeRows,
+                    TSG_ERR_DECLINED, "more than %u rows a sequence: tsg_attn_prefill",
+                    kMaxDecodeRows);
+    }
+    return attention(attn, stream, pages, batch, q, q_stride, out, out_stride);
+}
+
+extern "C" tsg_status tsg_attn_prefill(tsg_attn* attn, tsg_stream stream,
+                                       const tsg_kv_pages* pages, const tsg_attn_batch* batch,
+                                       const uint16_t* q, uint32_t q_stride, uint16_t* out,
+                                       uint32_t out_stride) {
+    return attention(attn, stream, pages, batch, q, q_stride, out, out_stride);
+}

@@ -1,5 +1,5 @@
 // core.hip — context, errors, HBM-resident layers and synthetic generators.
-#include "tsg_internal.hpp"
+#include "attn_internal.hpp"
 
 #include <cstring>
 #include <new>
@@ -199,6 +199,16 @@ extern "C" tsg_status tsg_ctx_synchronize(tsg_ctx* ctx, tsg_stream stream) {
             return fail(TSG_ERR_INVALID_ARGUMENT,
                         "grouped GEMM: a routed block named an expert past the layer; it was "
                         "skipped and its rows were not written");
+        if (err & (kErrAttnPage | kErrAttnLength | kErrAttnRows))
+            return fail(TSG_ERR_INVALID_ARGUMENT,
+                        err & kErrAttnPage
+                            ? "attention: a page table entry past the cache's pages; the rows "
+                              "that needed it are NaN or not appended"
+                        : err & kErrAttnLength
+                            ? "attention: a sequence longer than its page table; its rows are "
+                              "NaN or not appended"
+                            : "attention: row starts that fall or pass the batch's rows; the "
+                              "rows of those sequences are NaN or not appended");
         if (err & kErrGemmWait)
             return fail(TSG_ERR_HIP, "fused grouped GEMM: a down item timed out waiting for its "
                                      "block's gate/up tiles, or an XCD queue was not drained; "
