@@ -433,11 +433,39 @@ extern "C" tsg_status tsg_attn_create(tsg_ctx* ctx, const tsg_attn_config* confi
     attn->group = config->q_heads / config->kv_heads;
     attn->page_shift = (uint32_t)__builtin_ctz(config->page_tokens);
     attn->cell = cell_bytes(*config);
+    attn->padded_dim = 64u;
+    while (attn->padded_dim < config->head_dim) attn->padded_dim *= 2u;
+    DeviceScope scope(ctx->device);
+    hipError_t e = scope.status;
+    const size_t words = (size_t)kMaxPartials * kDecodeTileRows * (attn->padded_dim + 2u);
+    if (e == hipSuccess) e = hipMalloc(&attn->partials, words * sizeof(float));
+    if (e == hipSuccess) e = hipMalloc(&attn->arrivals, kMaxPartials * sizeof(uint32_t));
+    if (e == hipSuccess) e = hipMemset(attn->arrivals, 0, kMaxPartials * sizeof(uint32_t));
+    if (e == hipSuccess) e = hipDeviceSynchronize();
+    if (e != hipSuccess) {
+        (void)hipFree(attn->partials);
+        (void)hipFree(attn->arrivals);
+        delete attn;
+        return fail(TSG_ERR_OUT_OF_MEMORY, "attention scratch: %s", hipGetErrorString(e));
+    }
+    if (tsg_status s = prepare_decode(attn)) {
+        (void)hipFree(attn->partials);
+        (void)hipFree(attn->arrivals);
+        delete attn;
+        return s;
+    }
     *out = attn;
     return TSG_OK;
 }
 
-extern "C" void tsg_attn_destroy(tsg_attn* attn) { delete attn; }
+extern "C" void tsg_attn_destroy(tsg_attn* attn) {
+    if (!attn) return;
+    DeviceScope scope(attn->ctx->device);
+    (void)hipDeviceSynchronize();
+    (void)hipFree(attn->partials);
+    (void)hipFree(attn->arrivals);
+    delete attn;
+}
 
 extern "C" tsg_status tsg_attn_append(tsg_attn* attn, tsg_stream stream, const tsg_kv_pages* pages,
                                       const tsg_attn_batch* batch, const tsg_attn_rows* rows,
@@ -519,14 +547,16 @@ extern "C" tsg_status tsg_attn_append(tsg_attn* attn, tsg_stream stream, const t
 extern "C" tsg_status tsg_attn_decode(tsg_attn* attn, tsg_stream stream, const tsg_kv_pages* pages,
                                       const tsg_attn_batch* batch, const uint16_t* q,
                                       uint32_t q_stride, uint16_t* out, uint32_t out_stride) {
-    if (attn && batch) {
-        TSG_REQUIRE(!batch->row_starts, TSG_ERR_INVALID_ARGUMENT,
-                    "decode takes the same 1...8 rows of every sequence (no row starts)");
-        TSG_REQUIRE(batch->num_seqs == 0 || batch->rows / batch->num_seqs <= kMaxDecodeRows,
-                    TSG_ERR_DECLINED, "more than %u rows a sequence: tsg_attn_prefill",
-                    kMaxDecodeRows);
-    }
-    return attention(attn, stream, pages, batch, q, q_stride, out, out_stride);
+    AttnArgs a{};
+    if (tsg_status s = attn_args(attn, pages, batch, q, q_stride, out, out_stride, &a)) return s;
+    TSG_REQUIRE(!batch->row_starts, TSG_ERR_INVALID_ARGUMENT,
+                "decode takes the same 1...%u rows of every sequence (no row starts)",
+                kMaxDecodeRows);
+    TSG_REQUIRE(a.seq_rows <= kMaxDecodeRows, TSG_ERR_DECLINED,
+                "more than %u rows a sequence: tsg_attn_prefill", kMaxDecodeRows);
+    DeviceScope scope(attn->ctx->device);
+    TSG_HIP_TRY(scope.status);
+    return launch_decode(attn, a, stream);
 }
 
 extern "C" tsg_status tsg_attn_prefill(tsg_attn* attn, tsg_stream stream,

@@ -1,0 +1,464 @@
+// attn_decode.hip — attention of 1..8 new rows of each sequence over the paged
+// cache.
+//
+// o = sum_j w_j v_j / sum_j w_j, w_j = exp(scale q.k_j): every key and value is
+// read once and used for the few rows of its head's group, so HBM bounds it
+// (4 flop a byte and row) and, for short caches, the latency of the chain
+// page table -> keys -> values -> join.
+//
+// A workgroup takes 16 rows (tokens x heads of one key head's group) and a run
+// of key tiles; its four waves take the tiles in turn, 16 keys each, with no
+// barrier between them: K goes from memory to the first operand's registers, V
+// through the wave's own LDS to be read transposed. The waves' sums are joined
+// in LDS; the workgroups of a split sequence leave partial sums in the plan's
+// scratch, and the last of them to arrive adds those up in the order of the
+// splits, so the result does not depend on which one it is.
+#include "attn_internal.hpp"
+
+namespace tsg {
+namespace {
+
+constexpr uint32_t kWaves = 4;
+constexpr uint32_t kTile = 16;  // keys of a wave's tile; never more than a page
+
+struct DecodeArgs {
+    AttnArgs a;
+    float* part_o;         // [pair][16][DP]
+    float* part_ml;        // [pair][16][2]: reference m and sum
+    uint32_t* arrivals;    // [unit]
+    uint32_t splits;       // workgroups a unit may be split over
+    uint32_t row_tiles;    // 16-row tiles of a sequence's rows and group
+    uint32_t pairs;        // sequences * key heads * splits
+    uint32_t min_tiles;    // key tiles worth a workgroup
+};
+
+// Wide heads' query fragments, the same for the four waves, are read from LDS
+// for each tile: in registers (16 x DP fp16, DP / 8 of them) they would spill.
+template <int DP>
+constexpr bool kQueryInLds = DP >= 256;
+
+template <int DP>
+constexpr uint32_t decode_lds_bytes() {
+    return kWaves * 16u * (DP + 4u) * 4u + 2u * kWaves * 16u * 4u + 16u +
+           (kQueryInLds<DP> ? 16u * DP * 2u : 0u);
+}
+
+// Place of the 32-byte pieces of key t's row in the wave's V tile: piece b lies
+// at b ^ value_swizzle(t), so that the eight keys that half a wave reads at
+// once (transposing) lie in different banks.
+template <int DP>
+__device__ __forceinline__ uint32_t value_swizzle(uint32_t t) {
+    return DP >= 128 ? t & 7u : (t >> 1) & 3u;
+}
+
+template <int DP, bool E4M3, bool FULL>
+__global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode_kernel(
+    DecodeArgs p) {
+    constexpr uint32_t NS = DP / 32, NB = DP / 16;   // key-product steps, value blocks
+    constexpr uint32_t CELL = E4M3 ? 1 : 2;
+    constexpr uint32_t KL = E4M3 ? NS / 2 : NS;      // 16-byte K loads of a lane
+    constexpr uint32_t CPR = DP * CELL / 16;         // 16-byte chunks of a cache row
+    constexpr uint32_t TPI = 64 / CPR;               // keys one V load instruction covers
+    constexpr uint32_t VL = kTile / TPI;             // V loads of a lane
+    extern __shared__ __align__(16) uint8_t smem[];
+    const AttnArgs& a = p.a;
+
+    uint32_t pair = blockIdx.x, rt = 0;
+    if (p.row_tiles > 1u) {  // the row tiles of a pair share its keys: one XCD
+        const uint32_t j = blockIdx.x >> 3;
+        rt = j % p.row_tiles;
+        pair = (j / p.row_tiles) * 8u + (blockIdx.x & 7u);
+        if (pair >= p.pairs) return;
+    }
+    const uint32_t split = pair % p.splits, unit = pair / p.splits;
+    const uint32_t kvh = unit % a.kv_heads, s = unit / a.kv_heads;
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t i16 = lane & 15u, g = lane >> 4;
+    const uint32_t capacity = a.table_stride << a.page_shift;
+    const SeqRows sr = seq_rows(nullptr, a.lengths, s, a.seq_rows, a.rows, capacity);
+
+    const uint32_t rows = sr.count * a.group, r0 = rt * kDecodeTileRows;
+    const uint32_t last = r0 + 15u < rows ? r0 + 15u : rows - 1u;
+    const int32_t base = (int32_t)sr.length - (int32_t)sr.count;
+    const int32_t p_lo = base + (int32_t)(r0 / a.group), p_hi = base + (int32_t)(last / a.group);
+    const TileSpan span = tile_span<kTile>(p_lo < 0 ? 0 : p_lo, p_hi, a.window, a.sinks);
+    uint32_t per = (span.count + p.splits - 1u) / p.splits;
+    per = per > p.min_tiles ? per : p.min_tiles;
+    uint32_t used = (span.count + per - 1u) / per;  // workgroups with keys
+    used = used > 1u ? used : 1u;
+    if (split >= used) return;
+    const uint32_t tile_end = (split + 1u) * per < span.count ? (split + 1u) * per : span.count;
+
+    // the lane's query row as the second operand of K Q^T; step s of the
+    // product takes, from lane group g, head elements qdim(s) ..
+    const auto qdim = [&](uint32_t st) {
+        return E4M3 ? 64u * (st >> 1) + 16u * g + 8u * (st & 1u) : 32u * st + 8u * g;
+    };
+    const uint32_t row = r0 + i16 < rows ? r0 + i16 : last;
+    const uint32_t tok = row / a.group;
+    const int32_t pos = base + (int32_t)tok;
+    const uint16_t* q = a.q + (uint64_t)(sr.first + tok) * a.q_stride +
+                        (uint64_t)(kvh * a.group + row % a.group) * a.dim;
+    const auto load_q = [&](uint32_t st) -> h8_t {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (FULL || qdim(st) < a.dim) u = *reinterpret_cast<const uint4*>(q + qdim(st));
+        return __builtin_bit_cast(h8_t, u);
+    };
+    constexpr bool QL = kQueryInLds<DP>;
+    h8_t* qs = reinterpret_cast<h8_t*>(smem + decode_lds_bytes<DP>() - 16u * DP * 2u) + lane;
+    h8_t qf[QL ? NS / kWaves : NS];  // QL: the steps that this wave stages
+#pragma unroll
+    for (uint32_t st = 0; st < (QL ? NS / kWaves : NS); ++st)
+        qf[st] = load_q(QL ? wave * (NS / kWaves) + st : st);
+
+    const uint32_t* table = a.table + (uint64_t)s * a.table_stride;
+    const uint32_t page_mask = (1u << a.page_shift) - 1u;
+    const uint64_t head_off = (uint64_t)kvh * a.head_stride;
+    bool bad = false;
+    // byte offset of a tile's first key in the pools
+    const auto tile_offset = [&](uint32_t idx) -> uint64_t {
+        const uint32_t t = span.key_tile(idx) * kTile;
+        uint32_t page = __builtin_amdgcn_readfirstlane(table[t >> a.page_shift]);
+        if (page >= a.num_pages) {
+            bad = true;
+            page = 0u;
+        }
+        return page * a.page_stride + head_off + (uint64_t)(t & page_mask) * a.token_stride;
+    };
+
+    const uint32_t k_lane = i16 * a.token_stride;  // lane i16 of each group holds key i16
+    const uint32_t v_chunk = lane % CPR;
+    const bool v_in = FULL || v_chunk * 16u < a.dim * CELL;
+    const uint32_t v_lane = (lane / CPR) * a.token_stride + (v_in ? v_chunk * 16u : 0u);
+    uint4 kreg[KL], vreg[VL];
+    const auto load_k = [&](uint64_t off) {
+        const uint8_t* kp = a.k + off;
+#pragma unroll
+        for (uint32_t l = 0; l < KL; ++l) {
+            const uint32_t byte = 64u * l + 16u * g;
+            const bool in = FULL || byte < a.dim * CELL;
+            const uint4 x = load16_nt(kp + (k_lane + (in ? byte : 0u)));
+            kreg[l] = in ? x : make_uint4(0, 0, 0, 0);
+        }
+    };
+    const auto load_v = [&](uint64_t off) {
+#pragma unroll
+        for (uint32_t n = 0; n < VL; ++n)
+            vreg[n] = load16_nt(a.v + (off + n * TPI * a.token_stride) + v_lane);
+    };
+    const auto k_frag = [&](uint32_t st) -> h8_t {
+        if constexpr (E4M3) {
+            const uint4 w = kreg[st >> 1];
+            const uint2 lo = e4m3x4_to_f16(st & 1u ? w.z : w.x), hi = e4m3x4_to_f16(st & 1u ? w.w : w.y);
+            return __builtin_bit_cast(h8_t, make_uint4(lo.x, lo.y, hi.x, hi.y));
+        } else {
+            return __builtin_bit_cast(h8_t, kreg[st]);
+        }
+    };
+
+    uint8_t* vs = smem + wave * (kTile * DP * 2u);
+    const uint32_t v_tok = lane / CPR;
+    const uint32_t tr_tok = 4u * g + (i16 >> 2);  // accumulator register j of group g is key 4 g + j
+    const uint32_t tr_base =
+        tr_tok * (DP * 2u) + 8u * (i16 & 3u) + 32u * value_swizzle<DP>(tr_tok);
+    const auto v_frag = [&](uint32_t b) -> h4_t {
+        return __builtin_bit_cast(h4_t, lds_read_tr(vs + (tr_base ^ (32u * b))));
+    };
+
+    f4_t o[NB];
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b) o[b] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = kNoKey, l = 0.0f;
+
+    uint32_t idx = split * per + wave;
+    if (sr.bad) idx = tile_end;
+    uint64_t off = 0;
+    if (idx < tile_end) {
+        off = tile_offset(idx);
+        load_k(off);
+        load_v(off);
+    }
+    if constexpr (QL) {
+#pragma unroll
+        for (uint32_t st = 0; st < NS / kWaves; ++st)
+            qs[(wave * (NS / kWaves) + st) * 64u] = qf[st];
+        __syncthreads();
+    }
+    for (; idx < tile_end; idx += kWaves) {
+        const uint32_t t0 = span.key_tile(idx) * kTile;
+        const bool whole = tile_seen_whole<kTile>(t0, p_lo, p_hi, a.window, a.sinks);
+        f4_t sc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (uint32_t st = 0; st < NS; ++st) {
+            const h8_t qx = QL ? qs[st * 64u] : qf[QL ? 0 : st];
+            sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k_frag(st), qx, sc, 0, 0, 0);
+            if (QL && st % 4u == 3u) __builtin_amdgcn_sched_barrier(0);  // few reads ahead: registers
+        }
+        const bool more = idx + kWaves < tile_end;
+        if (more) {
+            off = tile_offset(idx + kWaves);
+            load_k(off);
+        }
+        // V into the wave's LDS
+#pragma unroll
+        for (uint32_t n = 0; n < VL; ++n) {
+            const uint32_t t = n * TPI + v_tok;
+            if constexpr (E4M3) {
+                const uint2 x0 = e4m3x4_to_f16(vreg[n].x), x1 = e4m3x4_to_f16(vreg[n].y);
+                const uint2 x2 = e4m3x4_to_f16(vreg[n].z), x3 = e4m3x4_to_f16(vreg[n].w);
+                uint4* dst = reinterpret_cast<uint4*>(
+                    vs + t * (DP * 2u) + 32u * (v_chunk ^ value_swizzle<DP>(t)));
+                dst[0] = make_uint4(x0.x, x0.y, x1.x, x1.y);
+                dst[1] = make_uint4(x2.x, x2.y, x3.x, x3.y);
+            } else {
+                *reinterpret_cast<uint4*>(vs + t * (DP * 2u) +
+                                          16u * (v_chunk ^ (2u * value_swizzle<DP>(t)))) = vreg[n];
+            }
+        }
+        bool tainted = false;
+        uint32_t seen = 0xFu;
+        if (!whole) {
+            uint32_t found = 0;
+#pragma unroll
+            for (uint32_t n = 0; n < VL; ++n)
+                found |= not_finite<E4M3>(vreg[n].x) | not_finite<E4M3>(vreg[n].y) |
+                         not_finite<E4M3>(vreg[n].z) | not_finite<E4M3>(vreg[n].w);
+            tainted = __ballot(found != 0u) != 0;
+            seen = 0u;
+#pragma unroll
+            for (uint32_t e = 0; e < 4u; ++e)
+                seen |= (uint32_t)key_seen((int32_t)(t0 + 4u * g + e), pos, a.window, a.sinks) << e;
+        }
+        if (more) load_v(off);
+
+        float x[4];
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e)
+            x[e] = (seen >> e) & 1u ? sc[e] * a.scale_log2 : -__builtin_inff();
+        const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        if (__ballot(top > m + kMaxLag)) {
+            const float mn = fmaxf(m, max_across32(max_across16(top)));
+            const float alpha = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b) o[b] *= alpha;
+        }
+        const float shift = kWeightBias - m;
+        h4_t w;
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e) {
+            const float we = __builtin_amdgcn_exp2f(x[e] + shift);
+            l += we;
+            w[e] = (_Float16)we;
+        }
+        __builtin_amdgcn_wave_barrier();  // the wave's own LDS: its operations stay in order
+        if (!tainted) {
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b) {
+                o[b] = __builtin_amdgcn_mfma_f32_16x16x16f16(v_frag(b), w, o[b], 0, 0, 0);
+                if (QL && b % 8u == 7u) __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            h4_t ones;
+#pragma unroll
+            for (uint32_t e = 0; e < 4u; ++e) ones[e] = (_Float16)(float)((seen >> e) & 1u);
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b) {
+                // one kind at a time: registers
+                o[b] = __builtin_amdgcn_mfma_f32_16x16x16f16(finite_values(v_frag(b)), w, o[b], 0,
+                                                             0, 0);
+                const auto add = [&](uint32_t kind, float what) {
+                    const f4_t n = __builtin_amdgcn_mfma_f32_16x16x16f16(
+                        value_kind(v_frag(b), kind), ones, f4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[b][e] = n[e] > 0.0f ? o[b][e] + what : o[b][e];
+                    __builtin_amdgcn_sched_barrier(0);
+                };
+                add(kIsNan, __builtin_nanf(""));
+                add(kIsPosInf, __builtin_inff());
+                add(kIsNegInf, -__builtin_inff());
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    l = sum_across32(sum_across16(l));
+    if (bad || sr.bad) {
+        l = __builtin_nanf("");
+        if (lane == 0) report(a.error, sr.bad ? sr.bad : kErrAttnPage);
+    }
+
+    // the four waves' sums: lane (row i16, g) holds elements 16 b + 4 g .. + 3
+    float* so = reinterpret_cast<float*>(smem);
+    float* sm = so + kWaves * 16u * (DP + 4u);
+    float* sl = sm + kWaves * 16u;
+    uint32_t* flag = reinterpret_cast<uint32_t*>(sl + kWaves * 16u);
+    __syncthreads();  // every wave is done with its V
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b)
+        *reinterpret_cast<f4_t*>(so + (wave * 16u + i16) * (DP + 4u) + 16u * b + 4u * g) = o[b];
+    if (g == 0) {
+        sm[wave * 16u + i16] = m;
+        sl[wave * 16u + i16] = l;
+    }
+    __syncthreads();
+
+    constexpr uint32_t C8 = DP / 8;                      // 8-element pieces of a row
+    constexpr uint32_t PIECES = (16u * C8 + 255u) / 256u;  // of a thread
+    const uint32_t live = last - r0 + 1u;
+    const uint64_t tile = (uint64_t)unit * p.row_tiles + rt;
+    const auto emit = [&](uint32_t r, uint32_t c, const float* acc, float sum) {
+        const float inv = sum == 0.0f ? 0.0f : a.v_scale / sum;
+        uint32_t h[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            h[e] = (uint32_t)f32_to_f16(acc[2 * e] * inv) |
+                   ((uint32_t)f32_to_f16(acc[2 * e + 1] * inv) << 16);
+        const uint32_t t = (r0 + r) / a.group;
+        uint16_t* out = a.out + (uint64_t)(sr.first + t) * a.out_stride +
+                        (uint64_t)(kvh * a.group + (r0 + r) % a.group) * a.dim + 8u * c;
+        *reinterpret_cast<uint4*>(out) = make_uint4(h[0], h[1], h[2], h[3]);
+    };
+#pragma unroll 1
+    for (uint32_t n = 0; n < PIECES; ++n) {
+        const uint32_t piece = threadIdx.x + 256u * n, r = piece / C8, c = piece % C8;
+        if (r >= live || 8u * c >= a.dim) continue;
+        float mm = sm[r];
+#pragma unroll
+        for (uint32_t w = 1; w < kWaves; ++w) mm = fmaxf(mm, sm[w * 16u + r]);
+        float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0.0f;
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(sm[w * 16u + r] - mm);
+            sum += sl[w * 16u + r] * f;
+            const float* src = so + (w * 16u + r) * (DP + 4u) + 8u * c;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] += src[e] * f;
+        }
+        if (used == 1u) {
+            emit(r, c, acc, sum);
+        } else {
+            const uint64_t slot = (tile * p.splits + split) * 16u + r;
+            float* dst = p.part_o + slot * DP + 8u * c;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint64_t two = (uint64_t)__float_as_uint(acc[2 * e]) |
+                                     ((uint64_t)__float_as_uint(acc[2 * e + 1]) << 32);
+                st_coherent(reinterpret_cast<uint64_t*>(dst) + e, two);
+            }
+            if (c == 0)
+                st_coherent(reinterpret_cast<uint64_t*>(p.part_ml) + slot,
+                            (uint64_t)__float_as_uint(mm) | ((uint64_t)__float_as_uint(sum) << 32));
+        }
+    }
+    if (used == 1u) return;
+
+    // the last workgroup of the unit to arrive joins the splits
+    wait_vector_memory();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const uint32_t before = __hip_atomic_fetch_add(p.arrivals + tile, 1u, __ATOMIC_RELAXED,
+                                                       __HIP_MEMORY_SCOPE_AGENT);
+        *flag = before == used - 1u ? 1u : 0u;
+        if (before == used - 1u) st_coherent(p.arrivals + tile, 0u);
+    }
+    __syncthreads();
+    if (!*flag) return;
+    float2* ml = reinterpret_cast<float2*>(smem);  // [split][16]
+    for (uint32_t n = threadIdx.x; n < used * 16u; n += 256u) {
+        if ((n & 15u) >= live) continue;
+        const uint64_t v = ld_coherent(reinterpret_cast<const uint64_t*>(p.part_ml) +
+                                       tile * p.splits * 16u + n);
+        ml[n] = make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (uint32_t n = 0; n < PIECES; ++n) {
+        const uint32_t piece = threadIdx.x + 256u * n, r = piece / C8, c = piece % C8;
+        if (r >= live || 8u * c >= a.dim) continue;
+        float mm = ml[r].x;
+        for (uint32_t w = 1; w < used; ++w) mm = fmaxf(mm, ml[w * 16u + r].x);
+        float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0.0f;
+        const float* src = p.part_o + (tile * p.splits * 16u + r) * DP + 8u * c;
+#pragma unroll 4
+        for (uint32_t w = 0; w < used; ++w) {
+            const float2 e2 = ml[w * 16u + r];
+            const float f = __builtin_amdgcn_exp2f(e2.x - mm);
+            sum += e2.y * f;
+            const uint4 lo = ld_coherent16(src + (uint64_t)w * 16u * DP);
+            const uint4 hi = ld_coherent16(src + (uint64_t)w * 16u * DP + 4u);
+            acc[0] += __uint_as_float(lo.x) * f;
+            acc[1] += __uint_as_float(lo.y) * f;
+            acc[2] += __uint_as_float(lo.z) * f;
+            acc[3] += __uint_as_float(lo.w) * f;
+            acc[4] += __uint_as_float(hi.x) * f;
+            acc[5] += __uint_as_float(hi.y) * f;
+            acc[6] += __uint_as_float(hi.z) * f;
+            acc[7] += __uint_as_float(hi.w) * f;
+        }
+        emit(r, c, acc, sum);
+    }
+}
+
+typedef void (*DecodeKernel)(DecodeArgs);
+
+template <int DP>
+DecodeKernel kernel_of(bool e4m3, bool full) {
+    if (e4m3) return full ? decode_kernel<DP, true, true> : decode_kernel<DP, true, false>;
+    return full ? decode_kernel<DP, false, true> : decode_kernel<DP, false, false>;
+}
+
+struct Variant {
+    DecodeKernel kernel;
+    uint32_t lds;
+};
+Variant variant_of(const tsg_attn* attn) {
+    const bool e4m3 = attn->cfg.kv_type == TSG_KV_E4M3;
+    const bool full = attn->cfg.head_dim == attn->padded_dim;
+    switch (attn->padded_dim) {
+        case 64: return {kernel_of<64>(e4m3, full), decode_lds_bytes<64>()};
+        case 128: return {kernel_of<128>(e4m3, full), decode_lds_bytes<128>()};
+        case 256: return {kernel_of<256>(e4m3, full), decode_lds_bytes<256>()};
+        default: return {kernel_of<512>(e4m3, full), decode_lds_bytes<512>()};
+    }
+}
+
+}  // namespace
+
+tsg_status prepare_decode(const tsg_attn* attn) {
+    const Variant v = variant_of(attn);
+    TSG_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(v.kernel),
+                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)v.lds));
+    return TSG_OK;
+}
+
+tsg_status launch_decode(const tsg_attn* attn, const AttnArgs& a, tsg_stream stream) {
+    DecodeArgs p{};
+    p.a = a;
+    p.row_tiles = (a.seq_rows * a.group + kDecodeTileRows - 1u) / kDecodeTileRows;
+    const uint64_t units = (uint64_t)a.num_seqs * a.kv_heads, tiles = units * p.row_tiles;
+    // Workgroups of a split: enough for the card, none for fewer than min_tiles
+    // tiles of the longest sequence the table can hold.
+    const uint64_t capacity_tiles =
+        (((uint64_t)a.table_stride << a.page_shift) + kTile - 1u) / kTile;
+    p.min_tiles = kWaves;
+    uint64_t splits = 4u * (uint64_t)attn->ctx->num_cus / tiles;
+    splits = std::min(splits, (capacity_tiles + p.min_tiles - 1u) / p.min_tiles);
+    splits = std::min<uint64_t>(splits, kMaxSplits);
+    splits = std::min<uint64_t>(splits, kMaxPartials / tiles);
+    p.splits = (uint32_t)std::max<uint64_t>(splits, 1u);
+    const uint64_t pairs = units * p.splits;
+    const uint64_t blocks = p.row_tiles > 1u ? (pairs + 7u) / 8u * 8u * p.row_tiles : pairs;
+    TSG_REQUIRE(blocks <= 0x7fffffffu, TSG_ERR_UNSUPPORTED,
+                "too many sequences and heads for one launch");
+    p.pairs = (uint32_t)pairs;
+    p.part_o = attn->partials;
+    p.part_ml = attn->partials + (uint64_t)kMaxPartials * 16u * attn->padded_dim;
+    p.arrivals = attn->arrivals;
+    const Variant v = variant_of(attn);
+    hipLaunchKernelGGL(v.kernel, dim3((uint32_t)blocks), dim3(256), v.lds, as_stream(stream), p);
+    return check_launch("attn_decode");
+}
+
+}  // namespace tsg

@@ -10,6 +10,11 @@ struct tsg_attn {
     uint32_t group = 0;       // query heads a key head serves
     uint32_t page_shift = 0;  // log2(page_tokens)
     uint32_t cell = 2;        // bytes of a cache element
+    uint32_t padded_dim = 64; // the kernels' head width: 64, 128, 256 or 512
+    // scratch of the calls that split the keys: partial results and arrival
+    // counters (zeroed once, left zeroed by each call)
+    float* partials = nullptr;
+    uint32_t* arrivals = nullptr;
 };
 
 namespace tsg {
@@ -108,6 +113,131 @@ __device__ __forceinline__ uint2 e4m3x4_to_f16(uint32_t w) {
     return make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
 }
 
+// --------------------------------------------------- the attention kernels
+//
+// Both kernels work on the transposed products: S^T = K Q^T (a wave's lanes
+// are query rows, its accumulator registers are keys), so a row's running
+// maximum and sum stay in its lanes, and P^T leaves the accumulators as the
+// second operand of O^T = V^T P^T without a move between lanes: the order in
+// which that product takes the keys is free, and V is read in the order in
+// which the accumulators hold them. V^T comes out of LDS by transposing reads.
+//
+// Weights are kept as exp2(s - m + kWeightBias), m a reference at most
+// kMaxLag below the row's running maximum: a weight's rounding to fp16 is then
+// relative (half a step, 2^-11) down to 2^-25 of the largest, and at most
+// 2^15. m moves, and with it the sums, only when a logit passes it by kMaxLag.
+constexpr float kWeightBias = 11.0f;
+constexpr float kMaxLag = 4.0f;
+constexpr float kNoKey = -1e30f;  // m of a row that has seen no key
+
+// The key tiles (T keys each) that rows at positions p_lo .. p_hi see: those of
+// the sinks, then those from the first row's window on. Tile i of them starts
+// at key T * key_tile(i).
+struct TileSpan {
+    uint32_t sink_tiles, first, count;
+    __device__ __forceinline__ uint32_t key_tile(uint32_t i) const {
+        return i < sink_tiles ? i : first + (i - sink_tiles);
+    }
+};
+template <uint32_t T>
+__device__ __forceinline__ TileSpan tile_span(int32_t p_lo, int32_t p_hi, uint32_t window,
+                                              uint32_t sinks) {
+    TileSpan t{0u, 0u, 0u};
+    if (p_hi < 0) return t;
+    const uint32_t end = (uint32_t)p_hi / T + 1u;
+    if (window && p_lo >= (int32_t)window) {
+        t.first = (uint32_t)(p_lo - (int32_t)window + 1) / T;
+        const uint32_t s = (sinks + T - 1u) / T;
+        t.sink_tiles = s < t.first ? s : t.first;
+    }
+    t.count = t.sink_tiles + end - t.first;
+    return t;
+}
+
+// Whether every row at p_lo .. p_hi sees every key of [t, t + T).
+template <uint32_t T>
+__device__ __forceinline__ bool tile_seen_whole(uint32_t t, int32_t p_lo, int32_t p_hi,
+                                                uint32_t window, uint32_t sinks) {
+    return (int32_t)(t + T - 1u) <= p_lo &&
+           (window == 0u || p_hi - (int32_t)t < (int32_t)window || t + T <= sinks);
+}
+__device__ __forceinline__ bool key_seen(int32_t key, int32_t pos, uint32_t window,
+                                         uint32_t sinks) {
+    return key <= pos && (window == 0u || pos - key < (int32_t)window || key < (int32_t)sinks);
+}
+
+// The larger of a lane's value and those of the lanes 32 (and 16) from it.
+__device__ __forceinline__ float max_across32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                    false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_across16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                    false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_across32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                    false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float sum_across16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                    false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Transposing LDS read: within 16 lanes, lane i gives the address of four
+// elements of key i / 4 (elements 4 (i % 4) ..) and gets element i of the four
+// keys.
+__device__ __forceinline__ uint2 lds_read_tr(const uint8_t* p) {
+    typedef short s4_t __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4_t lds_s4_t;
+    return __builtin_bit_cast(
+        uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)(uintptr_t)p));
+}
+
+// Not zero if any element of a dword of the cache is an infinity or NaN: the
+// exponent (e4m3: all bits, it has NaN only) of all ones carries into the sign.
+template <bool E4M3>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    return E4M3 ? ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u
+                : ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+}
+
+typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+
+// The part of O^T += V^T P^T that a tile with infinities or NaN in V needs
+// where some row does not see some key: the product would make NaN of 0 times
+// them. The finite values go through the product as they are; for the others a
+// product of zeros and ones counts, for each row and element, the seen keys
+// that hold a NaN, a positive and a negative infinity.
+constexpr uint32_t kIsNan = 0, kIsPosInf = 1, kIsNegInf = 2;
+template <typename H>
+__device__ __forceinline__ H finite_values(H v) {
+#pragma unroll
+    for (uint32_t j = 0; j < sizeof(H) / 2u; ++j) {
+        const _Float16 x = v[j];  // a scalar: vector elements have no address
+        const bool bad = (__builtin_bit_cast(uint16_t, x) & 0x7C00u) == 0x7C00u;
+        v[j] = bad ? (_Float16)0.0f : x;
+    }
+    return v;
+}
+template <typename H>
+__device__ __forceinline__ H value_kind(H v, uint32_t kind) {
+#pragma unroll
+    for (uint32_t j = 0; j < sizeof(H) / 2u; ++j) {
+        const _Float16 x = v[j];
+        const uint16_t b = __builtin_bit_cast(uint16_t, x);
+        const bool is = kind == kIsNan      ? (b & 0x7FFFu) > 0x7C00u
+                        : kind == kIsPosInf ? b == 0x7C00u
+                                            : b == 0xFC00u;
+        v[j] = is ? (_Float16)1.0f : (_Float16)0.0f;
+    }
+    return v;
+}
+
 // Runs with the plan's device current; the caller's is restored on return.
 struct DeviceScope {
     int before = -1;
@@ -133,5 +263,12 @@ tsg_status check_attn_batch(const tsg_attn_config& c, const tsg_attn_batch* b);
 tsg_status attn_args(const tsg_attn* attn, const tsg_kv_pages* pages, const tsg_attn_batch* batch,
                      const uint16_t* q, uint32_t q_stride, uint16_t* out, uint32_t out_stride,
                      AttnArgs* a);
+
+// attn_decode.hip
+constexpr uint32_t kDecodeTileRows = 16;
+constexpr uint32_t kMaxPartials = 2048;  // (row tile, split) pairs of one call
+constexpr uint32_t kMaxSplits = 128;
+tsg_status prepare_decode(const tsg_attn* attn);  // once a plan, its device current
+tsg_status launch_decode(const tsg_attn* attn, const AttnArgs& a, tsg_stream stream);
 
 }  // namespace tsg
