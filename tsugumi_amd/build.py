@@ -23,7 +23,7 @@ FLOORS_LIB = os.path.join(HERE, "libtsugumi_floors.so")
 GEMM_SOURCES = ["gemm_g32_sym.hip", "gemm_g32_affine.hip", "gemm_g64_sym.hip",
                 "gemm_g64_affine.hip"]
 SOURCES = ["core.hip", "decode.hip", "prompt_router.hip", "qmv.hip", "shared.hip", "prefill.hip",
-           "tail.hip", "attn.hip", "attn_decode.hip",
+           "tail.hip", "attn.hip", "attn_decode.hip", "attn_prefill.hip",
            *GEMM_SOURCES,
            "host_routing.cpp",
            "moepack.cpp"]

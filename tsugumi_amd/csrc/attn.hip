@@ -326,86 +326,6 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     }
 }
 
-// --------------------------------------------------------------- attention
-//
-// One wave a (row, query head): the keys one after another, lanes over the
-// head's elements.
-template <bool E4M3>
-__global__ __launch_bounds__(64) void attention_kernel(AttnArgs a) {
-    const uint32_t row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
-    const uint32_t s = find_seq(a.row_starts, a.num_seqs, a.seq_rows, a.rows, row, a.error);
-    if (s >= a.num_seqs) return;
-    const uint32_t capacity = a.table_stride << a.page_shift;
-    const SeqRows sr = seq_rows(a.row_starts, a.lengths, s, a.seq_rows, a.rows, capacity);
-    const int32_t pos = (int32_t)sr.length - (int32_t)sr.count + (int32_t)(row - sr.first);
-    const uint32_t kvh = head / a.group;
-    const uint16_t* q = a.q + (uint64_t)row * a.q_stride + head * a.dim;
-    float qv[8], acc[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        qv[e] = lane + 64u * e < a.dim ? f16_to_f32(q[lane + 64u * e]) : 0.0f;
-        acc[e] = 0.0f;
-    }
-    float m = -1e30f, l = 0.0f;
-    bool bad = sr.bad;
-    if (bad && lane == 0) report(a.error, sr.bad);
-    const auto load = [&](const uint8_t* p, uint32_t i) -> float {
-        if (i >= a.dim) return 0.0f;
-        if (E4M3) {
-            const uint2 u = e4m3x4_to_f16(p[i]);
-            return f16_to_f32((uint16_t)(u.x & 0xFFFFu));
-        }
-        return f16_to_f32(reinterpret_cast<const uint16_t*>(p)[i]);
-    };
-    for (int32_t t = 0; t <= pos && !bad; ++t) {
-        if (a.window && pos - t >= (int32_t)a.window && t >= (int32_t)a.sinks) {
-            t = pos - (int32_t)a.window;  // on to the window's first key
-            continue;
-        }
-        const uint32_t page = a.table[(uint64_t)s * a.table_stride + ((uint32_t)t >> a.page_shift)];
-        if (page >= a.num_pages) {
-            bad = true;
-            if (lane == 0) report(a.error, kErrAttnPage);
-            break;
-        }
-        const uint64_t at = page * a.page_stride + kvh * a.head_stride +
-                            (uint64_t)((uint32_t)t & ((1u << a.page_shift) - 1u)) * a.token_stride;
-        float dot = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) dot = __builtin_fmaf(qv[e], load(a.k + at, lane + 64u * e), dot);
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
-        dot *= a.scale_log2;
-        const float mn = fmaxf(m, dot);
-        const float alpha = __builtin_amdgcn_exp2f(m - mn), p = __builtin_amdgcn_exp2f(dot - mn);
-        m = mn;
-        l = l * alpha + p;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            acc[e] = acc[e] * alpha + p * load(a.v + at, lane + 64u * e);
-    }
-    const float inv = bad ? __builtin_nanf("") : (l == 0.0f ? 0.0f : a.v_scale / l);
-    uint16_t* out = a.out + (uint64_t)row * a.out_stride + head * a.dim;
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (lane + 64u * e < a.dim) out[lane + 64u * e] = f32_to_f16(acc[e] * inv);
-}
-
-tsg_status attention(tsg_attn* attn, tsg_stream stream, const tsg_kv_pages* pages,
-                     const tsg_attn_batch* batch, const uint16_t* q, uint32_t q_stride,
-                     uint16_t* out, uint32_t out_stride) {
-    AttnArgs a{};
-    if (tsg_status s = attn_args(attn, pages, batch, q, q_stride, out, out_stride, &a)) return s;
-    DeviceScope scope(attn->ctx->device);
-    TSG_HIP_TRY(scope.status);
-    const dim3 grid(a.rows, a.q_heads);
-    if (attn->cfg.kv_type == TSG_KV_E4M3)
-        hipLaunchKernelGGL(attention_kernel<true>, grid, dim3(64), 0, as_stream(stream), a);
-    else
-        hipLaunchKernelGGL(attention_kernel<false>, grid, dim3(64), 0, as_stream(stream), a);
-    return check_launch("attention");
-}
-
 }  // namespace
 }  // namespace tsg
 
@@ -437,7 +357,7 @@ extern "C" tsg_status tsg_attn_create(tsg_ctx* ctx, const tsg_attn_config* confi
     while (attn->padded_dim < config->head_dim) attn->padded_dim *= 2u;
     DeviceScope scope(ctx->device);
     hipError_t e = scope.status;
-    const size_t words = (size_t)kMaxPartials * kDecodeTileRows * (attn->padded_dim + 2u);
+    const size_t words = (size_t)kPartialRows * (attn->padded_dim + 2u);
     if (e == hipSuccess) e = hipMalloc(&attn->partials, words * sizeof(float));
     if (e == hipSuccess) e = hipMalloc(&attn->arrivals, kMaxPartials * sizeof(uint32_t));
     if (e == hipSuccess) e = hipMemset(attn->arrivals, 0, kMaxPartials * sizeof(uint32_t));
@@ -448,7 +368,9 @@ extern "C" tsg_status tsg_attn_create(tsg_ctx* ctx, const tsg_attn_config* confi
         delete attn;
         return fail(TSG_ERR_OUT_OF_MEMORY, "attention scratch: %s", hipGetErrorString(e));
     }
-    if (tsg_status s = prepare_decode(attn)) {
+    tsg_status s = prepare_decode(attn);
+    if (s == TSG_OK) s = prepare_prefill(attn);
+    if (s != TSG_OK) {
         (void)hipFree(attn->partials);
         (void)hipFree(attn->arrivals);
         delete attn;
@@ -563,5 +485,9 @@ extern "C" tsg_status tsg_attn_prefill(tsg_attn* attn, tsg_stream stream,
                                        const tsg_kv_pages* pages, const tsg_attn_batch* batch,
                                        const uint16_t* q, uint32_t q_stride, uint16_t* out,
                                        uint32_t out_stride) {
-    return attention(attn, stream, pages, batch, q, q_stride, out, out_stride);
+    AttnArgs a{};
+    if (tsg_status s = attn_args(attn, pages, batch, q, q_stride, out, out_stride, &a)) return s;
+    DeviceScope scope(attn->ctx->device);
+    TSG_HIP_TRY(scope.status);
+    return launch_prefill(attn, a, stream);
 }

@@ -161,6 +161,13 @@ __device__ __forceinline__ bool tile_seen_whole(uint32_t t, int32_t p_lo, int32_
     return (int32_t)(t + T - 1u) <= p_lo &&
            (window == 0u || p_hi - (int32_t)t < (int32_t)window || t + T <= sinks);
 }
+// Whether any row at p_lo .. p_hi sees any key of [t, t + T).
+template <uint32_t T>
+__device__ __forceinline__ bool keys_seen(uint32_t t, int32_t p_lo, int32_t p_hi, uint32_t window,
+                                          uint32_t sinks) {
+    return (int32_t)t <= p_hi &&
+           (window == 0u || p_lo - (int32_t)(t + T - 1u) < (int32_t)window || t < sinks);
+}
 __device__ __forceinline__ bool key_seen(int32_t key, int32_t pos, uint32_t window,
                                          uint32_t sinks) {
     return key <= pos && (window == 0u || pos - key < (int32_t)window || key < (int32_t)sinks);
@@ -268,7 +275,15 @@ tsg_status attn_args(const tsg_attn* attn, const tsg_kv_pages* pages, const tsg_
 constexpr uint32_t kDecodeTileRows = 16;
 constexpr uint32_t kMaxPartials = 2048;  // (row tile, split) pairs of one call
 constexpr uint32_t kMaxSplits = 128;
+constexpr uint32_t kMaxPrefillPartials = 512;  // (row tile, key head, split) of one call
+constexpr uint32_t kPrefillRows = 128;
+// rows of partial results the plan's scratch holds, padded_dim + 2 floats each
+constexpr uint32_t kPartialRows = std::max(kMaxPartials * kDecodeTileRows,
+                                           kMaxPrefillPartials * kPrefillRows);
 tsg_status prepare_decode(const tsg_attn* attn);  // once a plan, its device current
 tsg_status launch_decode(const tsg_attn* attn, const AttnArgs& a, tsg_stream stream);
+// attn_prefill.hip
+tsg_status prepare_prefill(const tsg_attn* attn);
+tsg_status launch_prefill(const tsg_attn* attn, const AttnArgs& a, tsg_stream stream);
 
 }  // namespace tsg

@@ -1,0 +1,584 @@
+// attn_prefill.hip — attention of a prompt's rows, or of the next chunk of one,
+// over the paged cache.
+//
+// A workgroup takes 128 rows of a sequence and key head, the heads of the group
+// within the tokens (so a tile spans few positions and every key read serves
+// the whole group), and goes through the keys they see, TK at a time: K and V
+// tiles go from the pages into one of two LDS buffers while the other is
+// computed on. Each of the four waves holds 32 rows: S^T = K Q^T and O^T =
+// V^T P^T on 32 x 32 x 16 matrix instructions, Q, the weights and the sums in
+// registers, V read from LDS transposed. Bound by the matrix instructions (2 D
+// flop a pair each way) and, for narrow heads, by the exponentials beside them
+// (16 cycles for 64 pairs against 0.25 D of matrix work).
+//
+// Where the rows are few and the keys many, the keys are split over several
+// workgroups, and a second kernel joins their sums in the order of the splits.
+#include "attn_internal.hpp"
+
+#include <type_traits>
+
+namespace tsg {
+namespace {
+
+constexpr uint32_t kRows = kPrefillRows;  // of a workgroup
+constexpr uint32_t kWaveRows = 32;        // of a wave
+constexpr uint32_t kJoinRows = 8;         // rows a joining workgroup takes
+
+struct PrefillArgs {
+    AttnArgs a;
+    float* part_o;   // [tile block][split][128][DP]
+    float* part_ml;  // [tile block][split][128][2]
+    uint32_t splits, min_tiles;
+    uint32_t seq_tiles;  // row tiles of a sequence when its rows are uniform
+};
+
+template <int DP>
+constexpr uint32_t kTileKeys = DP <= 128 ? 64 : 32;
+template <int DP>
+constexpr uint32_t prefill_lds_bytes() {
+    return 2u * 2u * kTileKeys<DP> * DP * 2u;
+}
+
+typedef __attribute__((address_space(4))) const uint32_t const_u32_t;
+__device__ __forceinline__ uint32_t scalar_load(const uint32_t* p) {
+    return *(const_u32_t*)(uintptr_t)p;
+}
+
+// 16 bytes a lane from memory straight into LDS at `lds` + 16 x lane. Issued as
+// asm: the compiler would wait for it before any LDS read. It returns no
+// register; a wait on vector memory and a barrier come before the data is
+// read. Nothing else in this file uses m0.
+__device__ __forceinline__ void dma16(const uint8_t* base, uint32_t lane_off, uint32_t lds) {
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, %2"
+        :
+        : "s"(lds), "v"(lane_off), "s"(base)
+        : "memory");
+}
+
+// The row tile of workgroup `at`, counted from the last: sequences from the
+// last to the first, a sequence's tiles from its last (most keys first).
+// Uniform over the wave; false past the first.
+struct RowTile {
+    uint32_t seq, tile;
+};
+__device__ __forceinline__ bool find_tile(const PrefillArgs& p, uint32_t at, bool check,
+                                          RowTile* out) {
+    const AttnArgs& a = p.a;
+    if (!a.row_starts) {
+        out->seq = a.num_seqs - 1u - at / p.seq_tiles;
+        out->tile = p.seq_tiles - 1u - at % p.seq_tiles;
+        return at / p.seq_tiles < a.num_seqs;
+    }
+    const uint32_t lane = threadIdx.x & 63u;
+    bool found = false;
+    for (uint32_t base = 0; base < a.num_seqs; base += 64u) {
+        const uint32_t back = base + lane;
+        const bool live = back < a.num_seqs;
+        const uint32_t s = live ? a.num_seqs - 1u - back : 0u;
+        const uint32_t lo = live ? a.row_starts[s] : 0u, hi = live ? a.row_starts[s + 1u] : 0u;
+        if (check && __ballot(lo > hi || hi > a.rows) && lane == 0) report(a.error, kErrAttnRows);
+        if (found) continue;
+        const uint32_t end = hi < a.rows ? hi : a.rows;
+        const uint32_t n = end > lo ? end - lo : 0u;
+        const uint32_t tiles = (n * a.group + kRows - 1u) / kRows;
+        uint32_t sum = tiles;  // inclusive over the lanes
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t v = (uint32_t)__shfl_up((int)sum, (unsigned)o, 64);
+            if (lane >= (uint32_t)o) sum += v;
+        }
+        const uint64_t past = __ballot(sum > at);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            const uint32_t before = (uint32_t)__builtin_amdgcn_readlane((int)(sum - tiles), l);
+            const uint32_t count = (uint32_t)__builtin_amdgcn_readlane((int)tiles, l);
+            out->seq = a.num_seqs - 1u - (base + (uint32_t)l);
+            out->tile = count - 1u - (at - before);
+            found = true;
+            if (!check) return true;
+        } else {
+            at -= (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+        }
+    }
+    return found;
+}
+
+// What a row tile's workgroups share: positions of its rows and the part of the
+// key tiles that each split takes.
+template <int DP>
+struct TilePlan {
+    uint32_t rows, r0, live;
+    int32_t base, p_lo, p_hi;
+    TileSpan span;
+    uint32_t per, used;
+};
+template <int DP>
+__device__ __forceinline__ TilePlan<DP> tile_plan(const PrefillArgs& p, const SeqRows& sr,
+                                                  uint32_t tile) {
+    const AttnArgs& a = p.a;
+    TilePlan<DP> t;
+    t.rows = sr.count * a.group;
+    t.r0 = tile * kRows;
+    t.live = t.rows - t.r0 < kRows ? t.rows - t.r0 : kRows;
+    t.base = (int32_t)sr.length - (int32_t)sr.count;
+    t.p_lo = t.base + (int32_t)(t.r0 / a.group);
+    t.p_hi = t.base + (int32_t)((t.r0 + t.live - 1u) / a.group);
+    t.span = tile_span<kTileKeys<DP>>(t.p_lo < 0 ? 0 : t.p_lo, t.p_hi, a.window, a.sinks);
+    const uint32_t even = (t.span.count + p.splits - 1u) / p.splits;
+    t.per = even > p.min_tiles ? even : p.min_tiles;
+    const uint32_t used = (t.span.count + t.per - 1u) / t.per;
+    t.used = used > 1u ? used : 1u;
+    return t;
+}
+
+template <int DP, bool E4M3, bool FULL>
+__global__ __launch_bounds__(256, DP <= 256 ? 2 : 1) void prefill_kernel(PrefillArgs p) {
+    constexpr uint32_t TK = kTileKeys<DP>;
+    constexpr uint32_t NS = DP / 16, NB = DP / 32;  // key-product steps, value blocks
+    constexpr uint32_t ROW = DP * 2u;               // bytes of a key's row in LDS
+    constexpr uint32_t CPR = DP / 8u;               // 16-byte chunks of it
+    constexpr uint32_t TILE = TK * ROW;
+    constexpr uint32_t KW = TK / 4u;                // keys a wave stages
+    constexpr bool DMA = !E4M3 && FULL;
+    extern __shared__ __align__(16) uint8_t smem[];
+    const AttnArgs& a = p.a;
+
+    const uint32_t split = blockIdx.y;
+    const uint32_t kvh = blockIdx.x % a.kv_heads;
+    const uint32_t at = blockIdx.x / a.kv_heads;
+    RowTile rt;
+    if (!find_tile(p, at, at == 0u && split == 0u, &rt)) return;
+    const uint32_t s = rt.seq;
+    const uint32_t capacity = a.table_stride << a.page_shift;
+    const SeqRows sr = seq_rows(a.row_starts, a.lengths, s, a.seq_rows, a.rows, capacity);
+    const TilePlan<DP> t = tile_plan<DP>(p, sr, rt.tile);
+    if (split >= t.used) return;
+    const uint32_t tile_first = split * t.per;
+    uint32_t tile_end = tile_first + t.per < t.span.count ? tile_first + t.per : t.span.count;
+    if (sr.bad) tile_end = tile_first;
+
+    const uint32_t lane = threadIdx.x & 63u, i32 = lane & 31u, h = lane >> 5;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+    // the wave's rows; lane i32 of both halves holds row i32 of them
+    const uint32_t w0 = wave * kWaveRows;  // within the tile
+    const bool wave_live = w0 < t.live;
+    const uint32_t w_last = w0 + 31u < t.live ? w0 + 31u : t.live - 1u;
+    const int32_t p_lo = t.base + (int32_t)((t.r0 + (wave_live ? w0 : 0u)) / a.group);
+    const int32_t p_hi = t.base + (int32_t)((t.r0 + w_last) / a.group);
+    const uint32_t row = t.r0 + (w0 + i32 < t.live ? w0 + i32 : t.live - 1u);
+    const uint32_t tok = row / a.group;
+    const int32_t pos = t.base + (int32_t)tok;
+    const uint32_t q_head = kvh * a.group + row % a.group;
+    const uint16_t* q = a.q + (uint64_t)(sr.first + tok) * a.q_stride + (uint64_t)q_head * a.dim;
+    h8_t qf[NS];  // step st takes, from lane half h, elements 16 st + 8 h ..
+#pragma unroll
+    for (uint32_t st = 0; st < NS; ++st) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (FULL || 16u * st + 8u * h < a.dim)
+            u = *reinterpret_cast<const uint4*>(q + 16u * st + 8u * h);
+        qf[st] = __builtin_bit_cast(h8_t, u);
+    }
+
+    // ------------------------------------------------------------- staging
+    // Key t's row: chunk c of K lies at c ^ key_swizzle(t), of V at c ^ 2
+    // value_swizzle(t): 16 keys' equal chunks, and the 8 keys of a transposing
+    // read, lie in different banks.
+    const auto key_swizzle = [](uint32_t k) { return DP >= 128 ? k & 15u : (k >> 1) & 7u; };
+    const auto value_swizzle = [](uint32_t k) {
+        return DP >= 128 ? ((k & 3u) << 1) | ((k >> 2) & 1u)
+                         : (((k >> 1) & 1u) << 1) | ((k >> 2) & 1u);
+    };
+    const uint32_t* table = a.table + (uint64_t)s * a.table_stride;
+    const uint32_t page_mask = (1u << a.page_shift) - 1u;
+    const uint32_t last_page = t.p_hi < 0 ? 0u : (uint32_t)t.p_hi >> a.page_shift;
+    const uint64_t head_off = (uint64_t)kvh * a.head_stride;
+    bool bad = false;
+    // byte offset in the pools of the first key that this wave stages
+    const auto wave_offset = [&](uint32_t idx) -> uint64_t {
+        const uint32_t k0 = t.span.key_tile(idx) * TK + wave * KW;
+        const uint32_t want = k0 >> a.page_shift;
+        uint32_t page = scalar_load(table + (want < last_page ? want : last_page));
+        if (page >= a.num_pages) {
+            bad = bad || keys_seen<KW>(k0, t.p_lo, t.p_hi, a.window, a.sinks);
+            page = 0u;
+        }
+        return page * a.page_stride + head_off + (uint64_t)(k0 & page_mask) * a.token_stride;
+    };
+    constexpr uint32_t SRC = E4M3 ? CPR / 2u : CPR;  // 16-byte chunks of a cache row
+    constexpr uint32_t KPI = 64u / SRC;              // keys of one load instruction
+    constexpr uint32_t NL = KW / KPI;                // loads of K (and of V) a tile
+    static_assert(NL >= 1u && KW % KPI == 0u, "a wave's keys are whole load instructions");
+    uint4 kst[DMA ? 1 : NL], vst[DMA ? 1 : NL];
+    const uint32_t l_key = lane / SRC, l_chunk = lane % SRC;
+    const auto stage_begin = [&](uint32_t idx, uint32_t buf) {
+        const uint64_t off = wave_offset(idx);
+        if constexpr (DMA) {
+            const uint32_t lds = (uint32_t)(uintptr_t)smem + buf * 2u * TILE + wave * KW * ROW;
+#pragma unroll
+            for (uint32_t n = 0; n < NL; ++n) {
+                const uint32_t k = wave * KW + n * KPI + l_key;
+                const uint32_t at_k = (n * KPI + l_key) * a.token_stride;
+                dma16(a.k + off, at_k + 16u * (l_chunk ^ key_swizzle(k)), lds + n * KPI * ROW);
+                dma16(a.v + off, at_k + 16u * (l_chunk ^ (2u * value_swizzle(k))),
+                      lds + TILE + n * KPI * ROW);
+            }
+        } else {
+            const bool in = FULL || l_chunk * 16u < a.dim * (E4M3 ? 1u : 2u);
+#pragma unroll
+            for (uint32_t n = 0; n < NL; ++n) {
+                const uint32_t at_k =
+                    (n * KPI + l_key) * a.token_stride + (in ? 16u * l_chunk : 0u);
+                const uint4 kx = *reinterpret_cast<const uint4*>(a.k + off + at_k);
+                const uint4 vx = *reinterpret_cast<const uint4*>(a.v + off + at_k);
+                kst[n] = in ? kx : make_uint4(0, 0, 0, 0);
+                vst[n] = in ? vx : make_uint4(0, 0, 0, 0);
+            }
+        }
+    };
+    const auto stage_end = [&](uint32_t buf) {
+        if constexpr (!DMA) {
+            uint8_t* kb = smem + buf * 2u * TILE;
+#pragma unroll
+            for (uint32_t n = 0; n < NL; ++n) {
+                const uint32_t k = wave * KW + n * KPI + l_key;
+                const auto put = [&](uint8_t* to, const uint4& x, uint32_t swizzle) {
+                    if constexpr (E4M3) {
+                        const uint2 x0 = e4m3x4_to_f16(x.x), x1 = e4m3x4_to_f16(x.y);
+                        const uint2 x2 = e4m3x4_to_f16(x.z), x3 = e4m3x4_to_f16(x.w);
+                        *reinterpret_cast<uint4*>(to + k * ROW + 16u * ((2u * l_chunk) ^ swizzle)) =
+                            make_uint4(x0.x, x0.y, x1.x, x1.y);
+                        *reinterpret_cast<uint4*>(
+                            to + k * ROW + 16u * ((2u * l_chunk + 1u) ^ swizzle)) =
+                            make_uint4(x2.x, x2.y, x3.x, x3.y);
+                    } else {
+                        *reinterpret_cast<uint4*>(to + k * ROW + 16u * (l_chunk ^ swizzle)) = x;
+                    }
+                };
+                put(kb, kst[n], key_swizzle(k));
+                put(kb + TILE, vst[n], 2u * value_swizzle(k));
+            }
+        }
+    };
+
+    // ------------------------------------------------------------- compute
+    f16v_t o[NB];
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[b][e] = 0.0f;
+    float m = kNoKey, l = 0.0f;
+    // Accumulator register e of lane half h is key 8 (e / 4) + 4 h + e % 4 of 32;
+    // registers 8 ss .. 8 ss + 7 are the lane's eight of the second operand of
+    // V^T P^T's step ss, whose first operand comes in two transposing reads.
+    const uint32_t i16 = lane & 15u, tr_key = 4u * h + (i16 >> 2);
+    const uint32_t k_at = i32 * ROW, k_swz = key_swizzle(i32);
+    const uint32_t v_at = tr_key * ROW + 8u * (i16 & 3u);
+    const uint32_t v_pair = ((lane >> 4) & 1u) ^ value_swizzle(tr_key);
+
+    // N sub-tiles of 32 keys from key0 on; WHOLE: every row of the wave sees all.
+    const auto process = [&](auto n_tag, auto whole_tag, const uint8_t* kb, uint32_t sub,
+                             uint32_t key0) {
+        constexpr uint32_t N = decltype(n_tag)::value;
+        constexpr bool WHOLE = decltype(whole_tag)::value;
+        const uint8_t* vb = kb + TILE;
+        f16v_t sc[N];
+#pragma unroll
+        for (uint32_t u = 0; u < N; ++u) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sc[u][e] = 0.0f;
+#pragma unroll
+            for (uint32_t st = 0; st < NS; ++st) {
+                const h8_t kf = *reinterpret_cast<const h8_t*>(
+                    kb + (sub + u) * 32u * ROW + k_at + 16u * ((2u * st + h) ^ k_swz));
+                sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[st], sc[u], 0, 0, 0);
+            }
+        }
+        uint32_t seen = 0xFFFFu;
+        if constexpr (!WHOLE) {
+            seen = 0u;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                seen |= (uint32_t)key_seen((int32_t)(key0 + 8u * (e / 4) + 4u * h + e % 4), pos,
+                                           a.window, a.sinks)
+                        << e;
+        }
+        float x[N][16];
+        float top = -__builtin_inff();
+#pragma unroll
+        for (uint32_t u = 0; u < N; ++u)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                x[u][e] = sc[u][e] * a.scale_log2;
+                if (!WHOLE) x[u][e] = (seen >> e) & 1u ? x[u][e] : -__builtin_inff();
+                top = fmaxf(top, x[u][e]);
+            }
+        if (__ballot(top > m + kMaxLag)) {
+            const float mn = fmaxf(m, max_across32(top));
+            const float alpha = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b) o[b] *= alpha;
+        }
+        const float shift = kWeightBias - m;
+        h8_t w[N][2];
+#pragma unroll
+        for (uint32_t u = 0; u < N; ++u)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float we = __builtin_amdgcn_exp2f(x[u][e] + shift);
+                l += we;
+                w[u][e / 8][e % 8] = (_Float16)we;
+            }
+        const auto v_frag = [&](uint32_t u, uint32_t ss, uint32_t b) -> h8_t {
+            const uint8_t* at_v =
+                vb + ((sub + u) * 32u + 16u * ss) * ROW + v_at + 32u * ((2u * b) ^ v_pair);
+            const uint2 lo = lds_read_tr(at_v), hi = lds_read_tr(at_v + 8u * ROW);
+            return __builtin_bit_cast(h8_t, make_uint4(lo.x, lo.y, hi.x, hi.y));
+        };
+        bool tainted = false;
+        if constexpr (!WHOLE) {
+            uint32_t found = 0;
+#pragma unroll 1
+            for (uint32_t k = 0; k < 32u * CPR / 64u; ++k) {
+                const uint4 v = *reinterpret_cast<const uint4*>(vb + sub * 32u * ROW +
+                                                                16u * (64u * k + lane));
+                found |= not_finite<false>(v.x) | not_finite<false>(v.y) | not_finite<false>(v.z) |
+                         not_finite<false>(v.w);
+            }
+            tainted = __ballot(found != 0u) != 0;
+        }
+        if (!tainted) {
+#pragma unroll
+            for (uint32_t u = 0; u < N; ++u)
+#pragma unroll
+                for (uint32_t ss = 0; ss < 2u; ++ss)
+#pragma unroll
+                    for (uint32_t b = 0; b < NB; ++b)
+                        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_frag(u, ss, b), w[u][ss],
+                                                                      o[b], 0, 0, 0);
+        } else {
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b) {
+                const auto add = [&](uint32_t kind, float what) {
+                    f16v_t n;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) n[e] = 0.0f;
+#pragma unroll
+                    for (uint32_t ss = 0; ss < 2u; ++ss) {
+                        h8_t ones;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            ones[e] = (_Float16)(float)((seen >> (8u * ss + e)) & 1u);
+                        n = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                            value_kind(v_frag(0u, ss, b), kind), ones, n, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[b][e] = n[e] > 0.0f ? o[b][e] + what : o[b][e];
+                    __builtin_amdgcn_sched_barrier(0);
+                };
+#pragma unroll
+                for (uint32_t ss = 0; ss < 2u; ++ss)
+                    o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(finite_values(v_frag(0u, ss, b)),
+                                                                  w[0][ss], o[b], 0, 0, 0);
+                add(kIsNan, __builtin_nanf(""));
+                add(kIsPosInf, __builtin_inff());
+                add(kIsNegInf, -__builtin_inff());
+            }
+        }
+    };
+
+    if (tile_first < tile_end) {
+        stage_begin(tile_first, 0u);
+        stage_end(0u);
+    }
+    for (uint32_t idx = tile_first; idx < tile_end; ++idx) {
+        const uint32_t buf = (idx - tile_first) & 1u;
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const bool more = idx + 1u < tile_end;
+        if (more) stage_begin(idx + 1u, buf ^ 1u);
+        const uint32_t k0 = t.span.key_tile(idx) * TK;
+        const uint8_t* kb = smem + buf * 2u * TILE;
+        if (wave_live) {
+            if (tile_seen_whole<TK>(k0, p_lo, p_hi, a.window, a.sinks)) {
+                process(std::integral_constant<uint32_t, TK / 32u>{}, std::true_type{}, kb, 0u, k0);
+            } else {
+#pragma unroll 1
+                for (uint32_t sub = 0; sub < TK / 32u; ++sub)
+                    if (keys_seen<32>(k0 + 32u * sub, p_lo, p_hi, a.window, a.sinks))
+                        process(std::integral_constant<uint32_t, 1u>{}, std::false_type{}, kb, sub,
+                                k0 + 32u * sub);
+            }
+        }
+        if (more) stage_end(buf ^ 1u);
+    }
+
+    // a page past the pool: the tile's rows are NaN, whichever wave met it
+    uint32_t* flag = reinterpret_cast<uint32_t*>(smem);
+    __syncthreads();
+    if (threadIdx.x == 0) *flag = 0u;
+    __syncthreads();
+    if (lane == 0 && (bad || sr.bad)) {
+        report(a.error, sr.bad ? sr.bad : kErrAttnPage);
+        *flag = 1u;
+    }
+    __syncthreads();
+    l = sum_across32(l);
+    if (*flag) l = __builtin_nanf("");
+    if (w0 + i32 >= t.live) return;
+
+    // lane half h holds elements 32 b + 8 k + 4 h .. + 3 of its row
+    if (t.used == 1u) {
+        const float inv = l == 0.0f ? 0.0f : a.v_scale / l;
+        uint16_t* out = a.out + (uint64_t)(sr.first + tok) * a.out_stride + (uint64_t)q_head * a.dim;
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k) {
+                const uint32_t e = 32u * b + 8u * k + 4u * h;
+                if (!FULL && e >= a.dim) continue;
+                uint2 u;
+                u.x = (uint32_t)f32_to_f16(o[b][4 * k] * inv) |
+                      ((uint32_t)f32_to_f16(o[b][4 * k + 1] * inv) << 16);
+                u.y = (uint32_t)f32_to_f16(o[b][4 * k + 2] * inv) |
+                      ((uint32_t)f32_to_f16(o[b][4 * k + 3] * inv) << 16);
+                *reinterpret_cast<uint2*>(out + e) = u;
+            }
+    } else {
+        const uint64_t slot = ((uint64_t)blockIdx.x * p.splits + split) * kRows + w0 + i32;
+        float* dst = p.part_o + slot * DP;
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k)
+                *reinterpret_cast<float4*>(dst + 32u * b + 8u * k + 4u * h) = make_float4(
+                    o[b][4 * k], o[b][4 * k + 1], o[b][4 * k + 2], o[b][4 * k + 3]);
+        if (h == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2u) = make_float2(m, l);
+    }
+}
+
+// Adds up the splits' sums of a row tile, kJoinRows rows a workgroup, 8
+// elements a thread.
+template <int DP>
+__global__ __launch_bounds__(256) void prefill_join_kernel(PrefillArgs p) {
+    const AttnArgs& a = p.a;
+    const uint32_t kvh = blockIdx.x % a.kv_heads;
+    RowTile rt;
+    if (!find_tile(p, blockIdx.x / a.kv_heads, false, &rt)) return;
+    const SeqRows sr = seq_rows(a.row_starts, a.lengths, rt.seq, a.seq_rows, a.rows,
+                                a.table_stride << a.page_shift);
+    const TilePlan<DP> t = tile_plan<DP>(p, sr, rt.tile);
+    if (t.used == 1u) return;
+    for (uint32_t n = threadIdx.x; n < kJoinRows * (DP / 8u); n += 256u) {
+        const uint32_t r = blockIdx.y * kJoinRows + n / (DP / 8u), c = n % (DP / 8u);
+        if (r >= t.live || 8u * c >= a.dim) continue;
+        const uint64_t slot = (uint64_t)blockIdx.x * p.splits * kRows + r;
+        float m = kNoKey;
+        for (uint32_t w = 0; w < t.used; ++w)
+            m = fmaxf(m, p.part_ml[(slot + (uint64_t)w * kRows) * 2u]);
+        float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0.0f;
+#pragma unroll 4
+        for (uint32_t w = 0; w < t.used; ++w) {
+            const uint64_t at = slot + (uint64_t)w * kRows;
+            const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2u);
+            const float f = __builtin_amdgcn_exp2f(ml.x - m);
+            sum += ml.y * f;
+            const float4* src = reinterpret_cast<const float4*>(p.part_o + at * DP + 8u * c);
+            const float4 lo = src[0], hi = src[1];
+            acc[0] += lo.x * f;
+            acc[1] += lo.y * f;
+            acc[2] += lo.z * f;
+            acc[3] += lo.w * f;
+            acc[4] += hi.x * f;
+            acc[5] += hi.y * f;
+            acc[6] += hi.z * f;
+            acc[7] += hi.w * f;
+        }
+        const float inv = sum == 0.0f ? 0.0f : a.v_scale / sum;
+        uint32_t u[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            u[e] = (uint32_t)f32_to_f16(acc[2 * e] * inv) |
+                   ((uint32_t)f32_to_f16(acc[2 * e + 1] * inv) << 16);
+        const uint32_t tok = (t.r0 + r) / a.group;
+        *reinterpret_cast<uint4*>(a.out + (uint64_t)(sr.first + tok) * a.out_stride +
+                                  (uint64_t)(kvh * a.group + (t.r0 + r) % a.group) * a.dim +
+                                  8u * c) = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+}
+
+typedef void (*PrefillKernel)(PrefillArgs);
+
+template <int DP>
+PrefillKernel kernel_of(bool e4m3, bool full) {
+    if (e4m3) return full ? prefill_kernel<DP, true, true> : prefill_kernel<DP, true, false>;
+    return full ? prefill_kernel<DP, false, true> : prefill_kernel<DP, false, false>;
+}
+
+struct Variant {
+    PrefillKernel kernel, join;
+    uint32_t lds, tile_keys;
+};
+template <int DP>
+Variant variant(bool e4m3, bool full) {
+    return {kernel_of<DP>(e4m3, full), prefill_join_kernel<DP>, prefill_lds_bytes<DP>(),
+            kTileKeys<DP>};
+}
+Variant variant_of(const tsg_attn* attn) {
+    const bool e4m3 = attn->cfg.kv_type == TSG_KV_E4M3;
+    const bool full = attn->cfg.head_dim == attn->padded_dim;
+    switch (attn->padded_dim) {
+        case 64: return variant<64>(e4m3, full);
+        case 128: return variant<128>(e4m3, full);
+        case 256: return variant<256>(e4m3, full);
+        default: return variant<512>(e4m3, full);
+    }
+}
+
+}  // namespace
+
+tsg_status prepare_prefill(const tsg_attn* attn) {
+    const Variant v = variant_of(attn);
+    TSG_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(v.kernel),
+                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)v.lds));
+    return TSG_OK;
+}
+
+tsg_status launch_prefill(const tsg_attn* attn, const AttnArgs& a, tsg_stream stream) {
+    const Variant v = variant_of(attn);
+    PrefillArgs p{};
+    p.a = a;
+    p.seq_tiles = a.row_starts ? 0u : (uint32_t)(((uint64_t)a.seq_rows * a.group + kRows - 1u) / kRows);
+    // row starts: every sequence may end inside a tile
+    const uint64_t tiles = a.row_starts
+                               ? (uint64_t)a.rows * a.group / kRows + std::min(a.num_seqs, a.rows)
+                               : (uint64_t)a.num_seqs * p.seq_tiles;
+    const uint64_t blocks = tiles * a.kv_heads;
+    TSG_REQUIRE(blocks <= 0x7fffffffu, TSG_ERR_UNSUPPORTED, "too many rows and heads for one launch");
+    const uint64_t capacity_tiles =
+        (((uint64_t)a.table_stride << a.page_shift) + v.tile_keys - 1u) / v.tile_keys;
+    p.min_tiles = 2u;
+    uint64_t splits = 2u * (uint64_t)attn->ctx->num_cus / blocks;
+    splits = std::min(splits, (capacity_tiles + p.min_tiles - 1u) / p.min_tiles);
+    splits = std::min<uint64_t>(splits, kMaxPrefillPartials / blocks);
+    p.splits = (uint32_t)std::max<uint64_t>(splits, 1u);
+    p.part_o = attn->partials;
+    p.part_ml = attn->partials + (uint64_t)kMaxPrefillPartials * kRows * attn->padded_dim;
+    hipLaunchKernelGGL(v.kernel, dim3((uint32_t)blocks, p.splits), dim3(256), v.lds,
+                       as_stream(stream), p);
+    if (tsg_status s = check_launch("attn_prefill")) return s;
+    if (p.splits > 1u) {
+        hipLaunchKernelGGL(v.join, dim3((uint32_t)blocks, kRows / kJoinRows), dim3(256), 0,
+                           as_stream(stream), p);
+        return check_launch("attn_prefill_join");
+    }
+    return TSG_OK;
+}
+
+}  // namespace tsg
