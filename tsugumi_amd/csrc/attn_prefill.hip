@@ -15,8 +15,6 @@
 // workgroups, and a second kernel joins their sums in the order of the splits.
 #include "attn_internal.hpp"
 
-#include <type_traits>
-
 namespace tsg {
 namespace {
 
@@ -36,7 +34,7 @@ template <int DP>
 constexpr uint32_t kTileKeys = DP <= 128 ? 64 : 32;
 template <int DP>
 constexpr uint32_t prefill_lds_bytes() {
-    return 2u * 2u * kTileKeys<DP> * DP * 2u;
+    return 2u * 2u * kTileKeys<DP> * DP * 2u + kRows * DP / 4u;  // + marks
 }
 
 typedef __attribute__((address_space(4))) const uint32_t const_u32_t;
@@ -279,43 +277,40 @@ __global__ __launch_bounds__(256, DP <= 256 ? 2 : 1) void prefill_kernel(Prefill
     const uint32_t v_at = tr_key * ROW + 8u * (i16 & 3u);
     const uint32_t v_pair = ((lane >> 4) & 1u) ^ value_swizzle(tr_key);
 
-    // N sub-tiles of 32 keys from key0 on; WHOLE: every row of the wave sees all.
-    const auto process = [&](auto n_tag, auto whole_tag, const uint8_t* kb, uint32_t sub,
-                             uint32_t key0) {
-        constexpr uint32_t N = decltype(n_tag)::value;
-        constexpr bool WHOLE = decltype(whole_tag)::value;
+    // the wave's rows against the TK keys from key0 on
+    constexpr uint32_t N = TK / 32u;
+    const auto process = [&](const uint8_t* kb, uint32_t key0) {
         const uint8_t* vb = kb + TILE;
-        f16v_t sc[N];
+        f16v_t x[N];
 #pragma unroll
         for (uint32_t u = 0; u < N; ++u) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) sc[u][e] = 0.0f;
+            for (int e = 0; e < 16; ++e) x[u][e] = 0.0f;
 #pragma unroll
             for (uint32_t st = 0; st < NS; ++st) {
                 const h8_t kf = *reinterpret_cast<const h8_t*>(
-                    kb + (sub + u) * 32u * ROW + k_at + 16u * ((2u * st + h) ^ k_swz));
-                sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[st], sc[u], 0, 0, 0);
+                    kb + u * 32u * ROW + k_at + 16u * ((2u * st + h) ^ k_swz));
+                x[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[st], x[u], 0, 0, 0);
             }
         }
-        uint32_t seen = 0xFFFFu;
-        if constexpr (!WHOLE) {
-            seen = 0u;
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-                seen |= (uint32_t)key_seen((int32_t)(key0 + 8u * (e / 4) + 4u * h + e % 4), pos,
-                                           a.window, a.sinks)
-                        << e;
+        for (uint32_t u = 0; u < N; ++u)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[u][e] *= a.scale_log2;
+        if (!tile_seen_whole<TK>(key0, p_lo, p_hi, a.window, a.sinks)) {
+#pragma unroll
+            for (uint32_t u = 0; u < N; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (!key_seen((int32_t)(key0 + 32u * u + 8u * (e / 4) + 4u * h + e % 4), pos,
+                                  a.window, a.sinks))
+                        x[u][e] = -__builtin_inff();
         }
-        float x[N][16];
         float top = -__builtin_inff();
 #pragma unroll
         for (uint32_t u = 0; u < N; ++u)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                x[u][e] = sc[u][e] * a.scale_log2;
-                if (!WHOLE) x[u][e] = (seen >> e) & 1u ? x[u][e] : -__builtin_inff();
-                top = fmaxf(top, x[u][e]);
-            }
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, x[u][e]);
         if (__ballot(top > m + kMaxLag)) {
             const float mn = fmaxf(m, max_across32(top));
             const float alpha = __builtin_amdgcn_exp2f(m - mn);
@@ -334,62 +329,58 @@ __global__ __launch_bounds__(256, DP <= 256 ? 2 : 1) void prefill_kernel(Prefill
                 l += we;
                 w[u][e / 8][e % 8] = (_Float16)we;
             }
-        const auto v_frag = [&](uint32_t u, uint32_t ss, uint32_t b) -> h8_t {
-            const uint8_t* at_v =
-                vb + ((sub + u) * 32u + 16u * ss) * ROW + v_at + 32u * ((2u * b) ^ v_pair);
-            const uint2 lo = lds_read_tr(at_v), hi = lds_read_tr(at_v + 8u * ROW);
-            return __builtin_bit_cast(h8_t, make_uint4(lo.x, lo.y, hi.x, hi.y));
-        };
-        bool tainted = false;
-        if constexpr (!WHOLE) {
-            uint32_t found = 0;
+#pragma unroll
+        for (uint32_t u = 0; u < N; ++u)
+#pragma unroll
+            for (uint32_t ss = 0; ss < 2u; ++ss)
+#pragma unroll
+                for (uint32_t b = 0; b < NB; ++b) {
+                    const uint8_t* at_v =
+                        vb + (u * 32u + 16u * ss) * ROW + v_at + 32u * ((2u * b) ^ v_pair);
+                    const uint2 lo = lds_read_tr(at_v), hi = lds_read_tr(at_v + 8u * ROW);
+                    const h8_t vf = __builtin_bit_cast(h8_t, make_uint4(lo.x, lo.y, hi.x, hi.y));
+                    o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, w[u][ss], o[b], 0, 0, 0);
+                }
+    };
+
+    // A tile that some row sees a part of: an infinity or NaN in its V would
+    // make NaN of the weight 0 of a row that does not see its key. They are
+    // taken out of LDS and noted in `marks` (two bits, +inf and -inf, NaN both,
+    // for each element of the rows that see the key), which go onto the sums at
+    // the end.
+    uint32_t* marks = reinterpret_cast<uint32_t*>(smem + 4u * TILE);  // [row][DP / 16]
+    bool marked = false;
+    const auto take_out = [&](uint8_t* vb, uint32_t key0) {
+        bool found = false;
 #pragma unroll 1
-            for (uint32_t k = 0; k < 32u * CPR / 64u; ++k) {
-                const uint4 v = *reinterpret_cast<const uint4*>(vb + sub * 32u * ROW +
-                                                                16u * (64u * k + lane));
-                found |= not_finite<false>(v.x) | not_finite<false>(v.y) | not_finite<false>(v.z) |
-                         not_finite<false>(v.w);
-            }
-            tainted = __ballot(found != 0u) != 0;
+        for (uint32_t c = threadIdx.x; c < TK * CPR; c += 256u) {
+            const uint4 v = *reinterpret_cast<const uint4*>(vb + 16u * c);
+            found = found || (not_finite<false>(v.x) | not_finite<false>(v.y) |
+                              not_finite<false>(v.z) | not_finite<false>(v.w)) != 0u;
         }
-        if (!tainted) {
-#pragma unroll
-            for (uint32_t u = 0; u < N; ++u)
-#pragma unroll
-                for (uint32_t ss = 0; ss < 2u; ++ss)
-#pragma unroll
-                    for (uint32_t b = 0; b < NB; ++b)
-                        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_frag(u, ss, b), w[u][ss],
-                                                                      o[b], 0, 0, 0);
-        } else {
-#pragma unroll
-            for (uint32_t b = 0; b < NB; ++b) {
-                const auto add = [&](uint32_t kind, float what) {
-                    f16v_t n;
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) n[e] = 0.0f;
-#pragma unroll
-                    for (uint32_t ss = 0; ss < 2u; ++ss) {
-                        h8_t ones;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            ones[e] = (_Float16)(float)((seen >> (8u * ss + e)) & 1u);
-                        n = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                            value_kind(v_frag(0u, ss, b), kind), ones, n, 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) o[b][e] = n[e] > 0.0f ? o[b][e] + what : o[b][e];
-                    __builtin_amdgcn_sched_barrier(0);
-                };
-#pragma unroll
-                for (uint32_t ss = 0; ss < 2u; ++ss)
-                    o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(finite_values(v_frag(0u, ss, b)),
-                                                                  w[0][ss], o[b], 0, 0, 0);
-                add(kIsNan, __builtin_nanf(""));
-                add(kIsPosInf, __builtin_inff());
-                add(kIsNegInf, -__builtin_inff());
-            }
+        if (!__syncthreads_or(found)) return;
+        if (!marked) {
+            for (uint32_t n = threadIdx.x; n < kRows * DP / 16u; n += 256u) marks[n] = 0u;
+            marked = true;
+            __syncthreads();
         }
+#pragma unroll 1
+        for (uint32_t n = threadIdx.x; n < TK * DP; n += 256u) {
+            uint16_t* v = reinterpret_cast<uint16_t*>(vb) + n;
+            const uint32_t bits = *v;
+            if ((bits & 0x7C00u) != 0x7C00u) continue;
+            *v = 0;
+            const uint32_t k = n / DP, e = n % DP;
+            if (!keys_seen<1>(key0 + k, t.p_lo, t.p_hi, a.window, a.sinks)) continue;
+            const uint32_t dim = 8u * ((e / 8u) ^ (2u * value_swizzle(k))) + e % 8u;
+            const uint32_t mark = (bits & 0x3FFu ? 3u : bits & 0x8000u ? 2u : 1u) << (2u * (dim & 15u));
+#pragma unroll 1
+            for (uint32_t r = 0; r < t.live; ++r)
+                if (key_seen((int32_t)(key0 + k), t.base + (int32_t)((t.r0 + r) / a.group), a.window,
+                             a.sinks))
+                    atomicOr(marks + r * (DP / 16u) + dim / 16u, mark);
+        }
+        __syncthreads();
     };
 
     if (tile_first < tile_end) {
@@ -404,18 +395,9 @@ __global__ __launch_bounds__(256, DP <= 256 ? 2 : 1) void prefill_kernel(Prefill
         const bool more = idx + 1u < tile_end;
         if (more) stage_begin(idx + 1u, buf ^ 1u);
         const uint32_t k0 = t.span.key_tile(idx) * TK;
-        const uint8_t* kb = smem + buf * 2u * TILE;
-        if (wave_live) {
-            if (tile_seen_whole<TK>(k0, p_lo, p_hi, a.window, a.sinks)) {
-                process(std::integral_constant<uint32_t, TK / 32u>{}, std::true_type{}, kb, 0u, k0);
-            } else {
-#pragma unroll 1
-                for (uint32_t sub = 0; sub < TK / 32u; ++sub)
-                    if (keys_seen<32>(k0 + 32u * sub, p_lo, p_hi, a.window, a.sinks))
-                        process(std::integral_constant<uint32_t, 1u>{}, std::false_type{}, kb, sub,
-                                k0 + 32u * sub);
-            }
-        }
+        uint8_t* kb = smem + buf * 2u * TILE;
+        if (!tile_seen_whole<TK>(k0, t.p_lo, t.p_hi, a.window, a.sinks)) take_out(kb + TILE, k0);
+        if (wave_live && keys_seen<TK>(k0, p_lo, p_hi, a.window, a.sinks)) process(kb, k0);
         if (more) stage_end(buf ^ 1u);
     }
 
@@ -432,6 +414,18 @@ __global__ __launch_bounds__(256, DP <= 256 ? 2 : 1) void prefill_kernel(Prefill
     l = sum_across32(l);
     if (*flag) l = __builtin_nanf("");
     if (w0 + i32 >= t.live) return;
+    if (marked) {
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const uint32_t dim = 32u * b + 8u * (e / 4) + 4u * h + e % 4;
+                const uint32_t mark =
+                    marks[(w0 + i32) * (DP / 16u) + dim / 16u] >> (2u * (dim & 15u));
+                if (mark & 1u) o[b][e] += __builtin_inff();
+                if (mark & 2u) o[b][e] -= __builtin_inff();
+            }
+    }
 
     // lane half h holds elements 32 b + 8 k + 4 h .. + 3 of its row
     if (t.used == 1u) {
