@@ -32,6 +32,13 @@ struct PrefillArgs {
 
 template <int DP>
 constexpr uint32_t kTileKeys = DP <= 128 ? 64 : 32;
+// Head elements a wave takes. At 512 a wave's sums and queries would fill all
+// registers of a SIMD: two waves share the rows instead, each with one half of
+// the elements, and add up their halves of the key products through LDS.
+template <int DP>
+constexpr uint32_t kWaveDim = DP <= 256 ? DP : DP / 2;
+template <int DP>
+constexpr uint32_t kThreads = 256u * (DP / kWaveDim<DP>);
 template <int DP>
 constexpr uint32_t prefill_lds_bytes() {
     return 2u * 2u * kTileKeys<DP> * DP * 2u + kRows * DP / 4u;  // + marks
@@ -133,13 +140,14 @@ __device__ __forceinline__ TilePlan<DP> tile_plan(const PrefillArgs& p, const Se
 }
 
 template <int DP, bool E4M3, bool FULL>
-__global__ __launch_bounds__(256, DP <= 256 ? 2 : 1) void prefill_kernel(PrefillArgs p) {
+__global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p) {
     constexpr uint32_t TK = kTileKeys<DP>;
-    constexpr uint32_t NS = DP / 16, NB = DP / 32;  // key-product steps, value blocks
+    constexpr uint32_t DW = kWaveDim<DP>, THREADS = kThreads<DP>, SHARE = DP / DW;
+    constexpr uint32_t NS = DW / 16, NB = DW / 32;  // key-product steps, value blocks of a wave
     constexpr uint32_t ROW = DP * 2u;               // bytes of a key's row in LDS
     constexpr uint32_t CPR = DP / 8u;               // 16-byte chunks of it
     constexpr uint32_t TILE = TK * ROW;
-    constexpr uint32_t KW = TK / 4u;                // keys a wave stages
+    constexpr uint32_t KW = TK / (4u * SHARE);      // keys a wave stages
     constexpr bool DMA = !E4M3 && FULL;
     extern __shared__ __align__(16) uint8_t smem[];
     const AttnArgs& a = p.a;
@@ -162,7 +170,8 @@ __global__ __launch_bounds__(256, DP <= 256 ? 2 : 1) void prefill_kernel(Prefill
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
     // the wave's rows; lane i32 of both halves holds row i32 of them
-    const uint32_t w0 = wave * kWaveRows;  // within the tile
+    const uint32_t w0 = (wave & 3u) * kWaveRows;  // within the tile
+    const uint32_t d0 = (wave >> 2) * DW;         // its first head element
     const bool wave_live = w0 < t.live;
     const uint32_t w_last = w0 + 31u < t.live ? w0 + 31u : t.live - 1u;
     const int32_t p_lo = t.base + (int32_t)((t.r0 + (wave_live ? w0 : 0u)) / a.group);
@@ -176,8 +185,8 @@ __global__ __launch_bounds__(256, DP <= 256 ? 2 : 1) void prefill_kernel(Prefill
 #pragma unroll
     for (uint32_t st = 0; st < NS; ++st) {
         uint4 u = make_uint4(0, 0, 0, 0);
-        if (FULL || 16u * st + 8u * h < a.dim)
-            u = *reinterpret_cast<const uint4*>(q + 16u * st + 8u * h);
+        if (FULL || d0 + 16u * st + 8u * h < a.dim)
+            u = *reinterpret_cast<const uint4*>(q + d0 + 16u * st + 8u * h);
         qf[st] = __builtin_bit_cast(h8_t, u);
     }
 
@@ -273,13 +282,13 @@ __global__ __launch_bounds__(256, DP <= 256 ? 2 : 1) void prefill_kernel(Prefill
     // registers 8 ss .. 8 ss + 7 are the lane's eight of the second operand of
     // V^T P^T's step ss, whose first operand comes in two transposing reads.
     const uint32_t i16 = lane & 15u, tr_key = 4u * h + (i16 >> 2);
-    const uint32_t k_at = i32 * ROW, k_swz = key_swizzle(i32);
-    const uint32_t v_at = tr_key * ROW + 8u * (i16 & 3u);
+    const uint32_t k_at = i32 * ROW + 2u * d0, k_swz = key_swizzle(i32);
+    const uint32_t v_at = tr_key * ROW + 2u * d0 + 8u * (i16 & 3u);
     const uint32_t v_pair = ((lane >> 4) & 1u) ^ value_swizzle(tr_key);
 
     // the wave's rows against the TK keys from key0 on
     constexpr uint32_t N = TK / 32u;
-    const auto process = [&](const uint8_t* kb, uint32_t key0) {
+    const auto process = [&](uint8_t* kb, uint32_t key0) {
         const uint8_t* vb = kb + TILE;
         f16v_t x[N];
 #pragma unroll
@@ -291,6 +300,22 @@ __global__ __launch_bounds__(256, DP <= 256 ? 2 : 1) void prefill_kernel(Prefill
                 const h8_t kf = *reinterpret_cast<const h8_t*>(
                     kb + u * 32u * ROW + k_at + 16u * ((2u * st + h) ^ k_swz));
                 x[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[st], x[u], 0, 0, 0);
+            }
+        }
+        if constexpr (SHARE == 2u) {  // through the K tile, once every wave is done with it
+            static_assert(N == 1u && 2u * 4u * 64u * 64u <= TILE, "the sums fit the K tile");
+            lds_barrier();
+            f4_t* mine = reinterpret_cast<f4_t*>(kb) + wave * 256u + lane;
+            const f4_t* other = reinterpret_cast<const f4_t*>(kb) + (wave ^ 4u) * 256u + lane;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                mine[64 * k] = f4_t{x[0][4 * k], x[0][4 * k + 1], x[0][4 * k + 2], x[0][4 * k + 3]};
+            lds_barrier();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const f4_t y = other[64 * k];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[0][4 * k + e] += y[e];
             }
         }
 #pragma unroll
@@ -353,19 +378,19 @@ __global__ __launch_bounds__(256, DP <= 256 ? 2 : 1) void prefill_kernel(Prefill
     const auto take_out = [&](uint8_t* vb, uint32_t key0) {
         bool found = false;
 #pragma unroll 1
-        for (uint32_t c = threadIdx.x; c < TK * CPR; c += 256u) {
+        for (uint32_t c = threadIdx.x; c < TK * CPR; c += THREADS) {
             const uint4 v = *reinterpret_cast<const uint4*>(vb + 16u * c);
             found = found || (not_finite<false>(v.x) | not_finite<false>(v.y) |
                               not_finite<false>(v.z) | not_finite<false>(v.w)) != 0u;
         }
         if (!__syncthreads_or(found)) return;
         if (!marked) {
-            for (uint32_t n = threadIdx.x; n < kRows * DP / 16u; n += 256u) marks[n] = 0u;
+            for (uint32_t n = threadIdx.x; n < kRows * DP / 16u; n += THREADS) marks[n] = 0u;
             marked = true;
             __syncthreads();
         }
 #pragma unroll 1
-        for (uint32_t n = threadIdx.x; n < TK * DP; n += 256u) {
+        for (uint32_t n = threadIdx.x; n < TK * DP; n += THREADS) {
             uint16_t* v = reinterpret_cast<uint16_t*>(vb) + n;
             const uint32_t bits = *v;
             if ((bits & 0x7C00u) != 0x7C00u) continue;
@@ -397,7 +422,9 @@ __global__ __launch_bounds__(256, DP <= 256 ? 2 : 1) void prefill_kernel(Prefill
         const uint32_t k0 = t.span.key_tile(idx) * TK;
         uint8_t* kb = smem + buf * 2u * TILE;
         if (!tile_seen_whole<TK>(k0, t.p_lo, t.p_hi, a.window, a.sinks)) take_out(kb + TILE, k0);
-        if (wave_live && keys_seen<TK>(k0, p_lo, p_hi, a.window, a.sinks)) process(kb, k0);
+        // waves that share rows meet inside; every wave goes in
+        if (SHARE == 2u || (wave_live && keys_seen<TK>(k0, p_lo, p_hi, a.window, a.sinks)))
+            process(kb, k0);
         if (more) stage_end(buf ^ 1u);
     }
 
@@ -419,7 +446,7 @@ __global__ __launch_bounds__(256, DP <= 256 ? 2 : 1) void prefill_kernel(Prefill
         for (uint32_t b = 0; b < NB; ++b)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const uint32_t dim = 32u * b + 8u * (e / 4) + 4u * h + e % 4;
+                const uint32_t dim = d0 + 32u * b + 8u * (e / 4) + 4u * h + e % 4;
                 const uint32_t mark =
                     marks[(w0 + i32) * (DP / 16u) + dim / 16u] >> (2u * (dim & 15u));
                 if (mark & 1u) o[b][e] += __builtin_inff();
@@ -435,7 +462,7 @@ __global__ __launch_bounds__(256, DP <= 256 ? 2 : 1) void prefill_kernel(Prefill
         for (uint32_t b = 0; b < NB; ++b)
 #pragma unroll
             for (uint32_t k = 0; k < 4u; ++k) {
-                const uint32_t e = 32u * b + 8u * k + 4u * h;
+                const uint32_t e = d0 + 32u * b + 8u * k + 4u * h;
                 if (!FULL && e >= a.dim) continue;
                 uint2 u;
                 u.x = (uint32_t)f32_to_f16(o[b][4 * k] * inv) |
@@ -451,9 +478,9 @@ __global__ __launch_bounds__(256, DP <= 256 ? 2 : 1) void prefill_kernel(Prefill
         for (uint32_t b = 0; b < NB; ++b)
 #pragma unroll
             for (uint32_t k = 0; k < 4u; ++k)
-                *reinterpret_cast<float4*>(dst + 32u * b + 8u * k + 4u * h) = make_float4(
+                *reinterpret_cast<float4*>(dst + d0 + 32u * b + 8u * k + 4u * h) = make_float4(
                     o[b][4 * k], o[b][4 * k + 1], o[b][4 * k + 2], o[b][4 * k + 3]);
-        if (h == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2u) = make_float2(m, l);
+        if (h == 0 && d0 == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2u) = make_float2(m, l);
     }
 }
 
@@ -517,12 +544,12 @@ PrefillKernel kernel_of(bool e4m3, bool full) {
 
 struct Variant {
     PrefillKernel kernel, join;
-    uint32_t lds, tile_keys;
+    uint32_t threads, lds, tile_keys;
 };
 template <int DP>
 Variant variant(bool e4m3, bool full) {
-    return {kernel_of<DP>(e4m3, full), prefill_join_kernel<DP>, prefill_lds_bytes<DP>(),
-            kTileKeys<DP>};
+    return {kernel_of<DP>(e4m3, full), prefill_join_kernel<DP>, kThreads<DP>,
+            prefill_lds_bytes<DP>(), kTileKeys<DP>};
 }
 Variant variant_of(const tsg_attn* attn) {
     const bool e4m3 = attn->cfg.kv_type == TSG_KV_E4M3;
@@ -564,7 +591,7 @@ tsg_status launch_prefill(const tsg_attn* attn, const AttnArgs& a, tsg_stream st
     p.splits = (uint32_t)std::max<uint64_t>(splits, 1u);
     p.part_o = attn->partials;
     p.part_ml = attn->partials + (uint64_t)kMaxPrefillPartials * kRows * attn->padded_dim;
-    hipLaunchKernelGGL(v.kernel, dim3((uint32_t)blocks, p.splits), dim3(256), v.lds,
+    hipLaunchKernelGGL(v.kernel, dim3((uint32_t)blocks, p.splits), dim3(v.threads), v.lds,
                        as_stream(stream), p);
     if (tsg_status s = check_launch("attn_prefill")) return s;
     if (p.splits > 1u) {
