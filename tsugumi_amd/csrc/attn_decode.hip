@@ -39,6 +39,7 @@ constexpr bool kQueryInLds = DP >= 256;
 
 template <int DP>
 constexpr uint32_t decode_lds_bytes() {
+    // the waves' K and V tiles, and in their place at the end the waves' sums
     return kWaves * 16u * (DP + 4u) * 4u + 2u * kWaves * 16u * 4u + 16u +
            (kQueryInLds<DP> ? 16u * DP * 2u : 0u);
 }
@@ -51,6 +52,11 @@ __device__ __forceinline__ uint32_t value_swizzle(uint32_t t) {
     return DP >= 128 ? t & 7u : (t >> 1) & 3u;
 }
 
+template <int DP>
+__device__ __forceinline__ uint32_t key_swizzle(uint32_t t) {  // of 16-byte chunks of K
+    return DP >= 128 ? t & 15u : (t >> 1) & 7u;
+}
+
 template <int DP, bool E4M3, bool FULL>
 __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode_kernel(
     DecodeArgs p) {
@@ -60,6 +66,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
     constexpr uint32_t CPR = DP * CELL / 16;         // 16-byte chunks of a cache row
     constexpr uint32_t TPI = 64 / CPR;               // keys one V load instruction covers
     constexpr uint32_t VL = kTile / TPI;             // V loads of a lane
+    // fp16 rows go straight from memory to LDS, K as well; e4m3 codes (and rows
+    // of other widths, whose ends are zeros) pass through registers
+    constexpr bool DMA = !E4M3 && FULL;
     extern __shared__ __align__(16) uint8_t smem[];
     const AttnArgs& a = p.a;
 
@@ -119,7 +128,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
     // byte offset of a tile's first key in the pools
     const auto tile_offset = [&](uint32_t idx) -> uint64_t {
         const uint32_t t = span.key_tile(idx) * kTile;
-        uint32_t page = __builtin_amdgcn_readfirstlane(table[t >> a.page_shift]);
+        uint32_t page = scalar_load(table + (t >> a.page_shift));
         if (page >= a.num_pages) {
             bad = true;
             page = 0u;
@@ -131,8 +140,21 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
     const uint32_t v_chunk = lane % CPR;
     const bool v_in = FULL || v_chunk * 16u < a.dim * CELL;
     const uint32_t v_lane = (lane / CPR) * a.token_stride + (v_in ? v_chunk * 16u : 0u);
-    uint4 kreg[KL], vreg[VL];
+    uint8_t* vs = smem + wave * (kTile * DP * 2u * (DMA ? 2u : 1u));
+    uint8_t* ks = vs + kTile * DP * 2u;  // DMA only
+    const uint32_t v_tok = lane / CPR;
+    const uint32_t vs_lds = (uint32_t)(uintptr_t)vs, ks_lds = (uint32_t)(uintptr_t)ks;
+    uint4 kreg[DMA ? 1 : KL], vreg[DMA ? 1 : VL];
     const auto load_k = [&](uint64_t off) {
+        if constexpr (DMA) {
+#pragma unroll
+            for (uint32_t n = 0; n < VL; ++n) {
+                const uint32_t t = n * TPI + v_tok;
+                dma16(a.k + off, t * a.token_stride + 16u * (v_chunk ^ key_swizzle<DP>(t)),
+                      ks_lds + n * 1024u);
+            }
+            return;
+        }
         const uint8_t* kp = a.k + off;
 #pragma unroll
         for (uint32_t l = 0; l < KL; ++l) {
@@ -143,6 +165,15 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
         }
     };
     const auto load_v = [&](uint64_t off) {
+        if constexpr (DMA) {
+#pragma unroll
+            for (uint32_t n = 0; n < VL; ++n) {
+                const uint32_t t = n * TPI + v_tok;
+                dma16(a.v + off, t * a.token_stride + 16u * (v_chunk ^ (2u * value_swizzle<DP>(t))),
+                      vs_lds + n * 1024u);
+            }
+            return;
+        }
 #pragma unroll
         for (uint32_t n = 0; n < VL; ++n)
             vreg[n] = load16_nt(a.v + (off + n * TPI * a.token_stride) + v_lane);
@@ -152,13 +183,14 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
             const uint4 w = kreg[st >> 1];
             const uint2 lo = e4m3x4_to_f16(st & 1u ? w.z : w.x), hi = e4m3x4_to_f16(st & 1u ? w.w : w.y);
             return __builtin_bit_cast(h8_t, make_uint4(lo.x, lo.y, hi.x, hi.y));
+        } else if constexpr (DMA) {
+            return *reinterpret_cast<const h8_t*>(
+                ks + i16 * (DP * 2u) + 16u * ((4u * st + g) ^ key_swizzle<DP>(i16)));
         } else {
             return __builtin_bit_cast(h8_t, kreg[st]);
         }
     };
 
-    uint8_t* vs = smem + wave * (kTile * DP * 2u);
-    const uint32_t v_tok = lane / CPR;
     const uint32_t tr_tok = 4u * g + (i16 >> 2);  // accumulator register j of group g is key 4 g + j
     const uint32_t tr_base =
         tr_tok * (DP * 2u) + 8u * (i16 & 3u) + 32u * value_swizzle<DP>(tr_tok);
@@ -183,11 +215,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
 #pragma unroll
         for (uint32_t st = 0; st < NS / kWaves; ++st)
             qs[(wave * (NS / kWaves) + st) * 64u] = qf[st];
-        __syncthreads();
+        lds_barrier();
     }
     for (; idx < tile_end; idx += kWaves) {
         const uint32_t t0 = span.key_tile(idx) * kTile;
         const bool whole = tile_seen_whole<kTile>(t0, p_lo, p_hi, a.window, a.sinks);
+        if constexpr (DMA) wait_loads<VL>();  // K is there, V still on its way
         f4_t sc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (uint32_t st = 0; st < NS; ++st) {
@@ -198,11 +231,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
         const bool more = idx + kWaves < tile_end;
         if (more) {
             off = tile_offset(idx + kWaves);
+            if constexpr (DMA) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K was read
             load_k(off);
         }
         // V into the wave's LDS
 #pragma unroll
-        for (uint32_t n = 0; n < VL; ++n) {
+        for (uint32_t n = 0; n < (DMA ? 0u : VL); ++n) {
             const uint32_t t = n * TPI + v_tok;
             if constexpr (E4M3) {
                 const uint2 x0 = e4m3x4_to_f16(vreg[n].x), x1 = e4m3x4_to_f16(vreg[n].y);
@@ -219,18 +253,22 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
         bool tainted = false;
         uint32_t seen = 0xFu;
         if (!whole) {
+            if constexpr (DMA) wait_loads<0>();
             uint32_t found = 0;
 #pragma unroll
-            for (uint32_t n = 0; n < VL; ++n)
-                found |= not_finite<E4M3>(vreg[n].x) | not_finite<E4M3>(vreg[n].y) |
-                         not_finite<E4M3>(vreg[n].z) | not_finite<E4M3>(vreg[n].w);
+            for (uint32_t n = 0; n < VL; ++n) {
+                const uint4 x = DMA ? reinterpret_cast<const uint4*>(vs)[n * 64u + lane]
+                                    : vreg[DMA ? 0 : n];
+                found |= not_finite<E4M3>(x.x) | not_finite<E4M3>(x.y) | not_finite<E4M3>(x.z) |
+                         not_finite<E4M3>(x.w);
+            }
             tainted = __ballot(found != 0u) != 0;
             seen = 0u;
 #pragma unroll
             for (uint32_t e = 0; e < 4u; ++e)
                 seen |= (uint32_t)key_seen((int32_t)(t0 + 4u * g + e), pos, a.window, a.sinks) << e;
         }
-        if (more) load_v(off);
+        if (!DMA && more) load_v(off);
 
         float x[4];
 #pragma unroll
@@ -252,6 +290,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
             const float we = __builtin_amdgcn_exp2f(x[e] + shift);
             l += we;
             w[e] = (_Float16)we;
+        }
+        if constexpr (DMA) {  // V is there, the next K still on its way
+            if (more) wait_loads<VL>();
+            else wait_loads<0>();
         }
         __builtin_amdgcn_wave_barrier();  // the wave's own LDS: its operations stay in order
         if (!tainted) {
@@ -282,6 +324,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
             }
         }
         __builtin_amdgcn_wave_barrier();
+        if constexpr (DMA) {
+            if (more) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V was read
+                load_v(off);
+            }
+        }
     }
     l = sum_across32(sum_across16(l));
     if (bad || sr.bad) {

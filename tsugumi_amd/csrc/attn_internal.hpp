@@ -195,6 +195,33 @@ __device__ __forceinline__ float sum_across16(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+typedef __attribute__((address_space(4))) const uint32_t const_u32_t;
+__device__ __forceinline__ uint32_t scalar_load(const uint32_t* p) {
+    return *(const_u32_t*)(uintptr_t)p;
+}
+
+// 16 bytes a lane from memory straight into LDS at `lds` + 16 x lane. Issued as
+// asm: the compiler would wait for it before any LDS read. It returns no
+// register; a wait on vector memory and a barrier come before the data is
+// read. Nothing else in these kernels uses m0.
+__device__ __forceinline__ void dma16(const uint8_t* base, uint32_t lane_off, uint32_t lds) {
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, %2"
+        :
+        : "s"(lds), "v"(lane_off), "s"(base)
+        : "memory");
+}
+
+// Until at most N of the wave's loads are outstanding (they complete in order),
+// and all of its LDS accesses done.
+template <uint32_t N>
+__device__ __forceinline__ void wait_loads() {
+    static_assert(N < 64u, "vmcnt is 6 bits");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+
 // Transposing LDS read: within 16 lanes, lane i gives the address of four
 // elements of key i / 4 (elements 4 (i % 4) ..) and gets element i of the four
 // keys.

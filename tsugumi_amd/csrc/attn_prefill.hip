@@ -44,25 +44,6 @@ constexpr uint32_t prefill_lds_bytes() {
     return 2u * 2u * kTileKeys<DP> * DP * 2u + kRows * DP / 4u;  // + marks
 }
 
-typedef __attribute__((address_space(4))) const uint32_t const_u32_t;
-__device__ __forceinline__ uint32_t scalar_load(const uint32_t* p) {
-    return *(const_u32_t*)(uintptr_t)p;
-}
-
-// 16 bytes a lane from memory straight into LDS at `lds` + 16 x lane. Issued as
-// asm: the compiler would wait for it before any LDS read. It returns no
-// register; a wait on vector memory and a barrier come before the data is
-// read. Nothing else in this file uses m0.
-__device__ __forceinline__ void dma16(const uint8_t* base, uint32_t lane_off, uint32_t lds) {
-    asm volatile(
-        "s_mov_b32 m0, %0\n\t"
-        "s_nop 0\n\t"
-        "global_load_lds_dwordx4 %1, %2"
-        :
-        : "s"(lds), "v"(lane_off), "s"(base)
-        : "memory");
-}
-
 // The row tile of workgroup `at`, counted from the last: sequences from the
 // last to the first, a sequence's tiles from its last (most keys first).
 // Uniform over the wave; false past the first.
@@ -132,8 +113,17 @@ __device__ __forceinline__ TilePlan<DP> tile_plan(const PrefillArgs& p, const Se
     t.p_lo = t.base + (int32_t)(t.r0 / a.group);
     t.p_hi = t.base + (int32_t)((t.r0 + t.live - 1u) / a.group);
     t.span = tile_span<kTileKeys<DP>>(t.p_lo < 0 ? 0 : t.p_lo, t.p_hi, a.window, a.sinks);
-    const uint32_t even = (t.span.count + p.splits - 1u) / p.splits;
+    // the same run of key tiles for all of a sequence's rows: of its last rows'
+    // span, so that a prompt's early rows, which see few keys, are not split
+    const int32_t end = (int32_t)sr.length - 1;
+    const int32_t end_lo = end - (int32_t)((t.rows < kRows ? t.rows : kRows) - 1u) / (int32_t)a.group;
+    const uint32_t most =
+        tile_span<kTileKeys<DP>>(end_lo < 0 ? 0 : end_lo, end, a.window, a.sinks).count;
+    const uint32_t even = (most + p.splits - 1u) / p.splits;
     t.per = even > p.min_tiles ? even : p.min_tiles;
+    // a window's span may begin one tile earlier in it than the last rows' does
+    const uint32_t own = (t.span.count + p.splits - 1u) / p.splits;
+    t.per = own > t.per ? own : t.per;
     const uint32_t used = (t.span.count + t.per - 1u) / t.per;
     t.used = used > 1u ? used : 1u;
     return t;
@@ -585,7 +575,8 @@ tsg_status launch_prefill(const tsg_attn* attn, const AttnArgs& a, tsg_stream st
     const uint64_t capacity_tiles =
         (((uint64_t)a.table_stride << a.page_shift) + v.tile_keys - 1u) / v.tile_keys;
     p.min_tiles = 2u;
-    uint64_t splits = 2u * (uint64_t)attn->ctx->num_cus / blocks;
+    const uint64_t resident = 2u * (uint64_t)attn->ctx->num_cus * 256u / v.threads;
+    uint64_t splits = 2u * resident / blocks;
     splits = std::min(splits, (capacity_tiles + p.min_tiles - 1u) / p.min_tiles);
     splits = std::min<uint64_t>(splits, kMaxPrefillPartials / blocks);
     p.splits = (uint32_t)std::max<uint64_t>(splits, 1u);
