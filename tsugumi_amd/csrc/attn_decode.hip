@@ -491,7 +491,8 @@ tsg_status launch_decode(const tsg_attn* attn, const AttnArgs& a, tsg_stream str
     const uint64_t capacity_tiles =
         (((uint64_t)a.table_stride << a.page_shift) + kTile - 1u) / kTile;
     p.min_tiles = kWaves;
-    uint64_t splits = 4u * (uint64_t)attn->ctx->num_cus / tiles;
+    const uint64_t resident = attn->padded_dim <= 128u ? 4u : 512u / attn->padded_dim;
+    uint64_t splits = resident * (uint64_t)attn->ctx->num_cus / tiles;
     splits = std::min(splits, (capacity_tiles + p.min_tiles - 1u) / p.min_tiles);
     splits = std::min<uint64_t>(splits, kMaxSplits);
     splits = std::min<uint64_t>(splits, kMaxPartials / tiles);
