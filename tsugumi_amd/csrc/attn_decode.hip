@@ -23,14 +23,99 @@ constexpr uint32_t kTile = 16;  // keys of a wave's tile; never more than a page
 
 struct DecodeArgs {
     AttnArgs a;
-    float* part_o;         // [pair][16][DP]
-    float* part_ml;        // [pair][16][2]: reference m and sum
-    uint32_t* arrivals;    // [unit]
-    uint32_t splits;       // workgroups a unit may be split over
-    uint32_t row_tiles;    // 16-row tiles of a sequence's rows and group
-    uint32_t pairs;        // sequences * key heads * splits
-    uint32_t min_tiles;    // key tiles worth a workgroup
+    float* part_o;       // [slot][16][DP]
+    float* part_ml;      // [slot][16][2]: reference m and sum
+    uint32_t* arrivals;  // [slot]
+    uint32_t chunks;     // runs of keys wanted, a head and row tile; 0: one a sequence
+    uint32_t row_tiles;  // 16-row tiles of a sequence's rows and group
+    uint32_t pairs;      // key heads * (most runs there can be)
 };
+
+constexpr uint32_t kMinTiles = kWaves;  // key tiles worth a workgroup: one a wave
+constexpr uint32_t kMaxSplits = 128;    // partial sums one workgroup joins
+constexpr uint32_t kMaxBalanced = 256;  // sequences of a batch with runs of one length
+
+// The run of key tiles that workgroup `at` (of a head and row tile) takes. All
+// runs of a batch have about the same length, whatever the sequences' lengths:
+// the tiles of all sequences over the runs wanted.
+struct Run {
+    uint32_t seq, split, used, per;
+    uint32_t slot;    // of the sequence's first partial sum
+    uint32_t length;  // the sequence's
+};
+__device__ __forceinline__ uint32_t seq_key_tiles(const AttnArgs& a, uint32_t length) {
+    if (length > (a.table_stride << a.page_shift)) return 0u;  // reported; its rows are NaN
+    const int32_t lo = (int32_t)length - (int32_t)a.seq_rows;
+    return tile_span<kTile>(lo < 0 ? 0 : lo, (int32_t)length - 1, a.window, a.sinks).count;
+}
+__device__ __forceinline__ bool find_run(const DecodeArgs& p, uint32_t at, Run* r) {
+    const AttnArgs& a = p.a;
+    if (p.chunks == 0u) {
+        if (at >= a.num_seqs) return false;
+        *r = Run{at, 0u, 1u, 0xFFFFFFFFu, 0u, scalar_load(a.lengths + at)};
+        return true;
+    }
+    const auto runs_of = [](uint32_t tiles, uint32_t per) {
+        const uint32_t n = (tiles + per - 1u) / per;
+        return n > 1u ? n : 1u;
+    };
+    const auto run_length = [](uint32_t tiles, uint32_t per) {  // of one sequence
+        const uint32_t least = (tiles + kMaxSplits - 1u) / kMaxSplits;
+        return per > least ? per : least;
+    };
+    if (a.num_seqs == 1u) {
+        const uint32_t length = scalar_load(a.lengths);
+        const uint32_t tiles = seq_key_tiles(a, length);
+        const uint32_t even = (tiles + p.chunks - 1u) / p.chunks;
+        const uint32_t per = run_length(tiles, even > kMinTiles ? even : kMinTiles);
+        *r = Run{0u, at, runs_of(tiles, per), per, 0u, length};
+        return at < r->used;
+    }
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t first = 0, total = 0;  // the first 64 lengths are read once
+    for (uint32_t base = 0; base < a.num_seqs; base += 64u) {
+        const uint32_t length = base + lane < a.num_seqs ? a.lengths[base + lane] : 0u;
+        uint32_t n = base + lane < a.num_seqs ? seq_key_tiles(a, length) : 0u;
+        if (base == 0u) first = length;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) n += (uint32_t)__shfl_xor((int)n, o, 64);
+        total += __builtin_amdgcn_readfirstlane(n);
+    }
+    uint32_t per = (total + p.chunks - 1u) / p.chunks;
+    per = per > kMinTiles ? per : kMinTiles;
+    uint32_t slots = 0;
+    for (uint32_t base = 0; base < a.num_seqs; base += 64u) {
+        const bool live = base + lane < a.num_seqs;
+        const uint32_t length = base == 0u ? first : live ? a.lengths[base + lane] : 0u;
+        const uint32_t tiles = live ? seq_key_tiles(a, length) : 0u;
+        const uint32_t own = run_length(tiles, per);
+        const uint32_t runs = live ? runs_of(tiles, own) : 0u;
+        // runs, and above them those of split sequences: both sums stay under 2^16
+        const uint32_t both = runs | (runs > 1u ? runs << 16 : 0u);
+        uint32_t sum = both;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t v = (uint32_t)__shfl_up((int)sum, (unsigned)o, 64);
+            if (lane >= (uint32_t)o) sum += v;
+        }
+        const uint64_t past = __ballot((sum & 0xFFFFu) > at);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            const uint32_t before = (uint32_t)__builtin_amdgcn_readlane((int)(sum - both), l);
+            r->seq = base + (uint32_t)l;
+            r->split = at - (before & 0xFFFFu);
+            r->used = (uint32_t)__builtin_amdgcn_readlane((int)runs, l);
+            r->per = (uint32_t)__builtin_amdgcn_readlane((int)own, l);
+            r->slot = slots + (before >> 16);
+            r->length = (uint32_t)__builtin_amdgcn_readlane((int)length, l);
+            return true;
+        }
+        const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+        at -= all & 0xFFFFu;
+        slots += all >> 16;
+    }
+    return false;
+}
 
 // Wide heads' query fragments, the same for the four waves, are read from LDS
 // for each tile: in registers (16 x DP fp16, DP / 8 of them) they would spill.
@@ -38,10 +123,13 @@ template <int DP>
 constexpr bool kQueryInLds = DP >= 256;
 
 template <int DP>
+constexpr uint32_t kMarkBytes = kWaves * 16u * DP / 4u;
+
+template <int DP>
 constexpr uint32_t decode_lds_bytes() {
     // the waves' K and V tiles, and in their place at the end the waves' sums
-    return kWaves * 16u * (DP + 4u) * 4u + 2u * kWaves * 16u * 4u + 16u +
-           (kQueryInLds<DP> ? 16u * DP * 2u : 0u);
+    return kWaves * 16u * (DP + 4u) * 4u + 2u * kWaves * 16u * 4u + 32u +
+           (kQueryInLds<DP> ? 16u * DP * 2u : 0u) + kMarkBytes<DP>;
 }
 
 // Place of the 32-byte pieces of key t's row in the wave's V tile: piece b lies
@@ -57,18 +145,24 @@ __device__ __forceinline__ uint32_t key_swizzle(uint32_t t) {  // of 16-byte chu
     return DP >= 128 ? t & 15u : (t >> 1) & 7u;
 }
 
+// fp16 rows go straight from memory to LDS, K as well; e4m3 codes (and rows of
+// other widths, whose ends are zeros) pass through registers.
+template <bool E4M3, bool FULL>
+constexpr bool kDirect = !E4M3 && FULL;
+// Waves a SIMD's registers are shared by.
 template <int DP, bool E4M3, bool FULL>
-__global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode_kernel(
-    DecodeArgs p) {
+constexpr int kSimdWaves = kDirect<E4M3, FULL> ? (DP <= 128 ? 4 : 2)
+                                               : (DP <= 128 ? 3 : DP <= 256 ? 2 : 1);
+
+template <int DP, bool E4M3, bool FULL>
+__global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kernel(DecodeArgs p) {
     constexpr uint32_t NS = DP / 32, NB = DP / 16;   // key-product steps, value blocks
     constexpr uint32_t CELL = E4M3 ? 1 : 2;
     constexpr uint32_t KL = E4M3 ? NS / 2 : NS;      // 16-byte K loads of a lane
     constexpr uint32_t CPR = DP * CELL / 16;         // 16-byte chunks of a cache row
     constexpr uint32_t TPI = 64 / CPR;               // keys one V load instruction covers
     constexpr uint32_t VL = kTile / TPI;             // V loads of a lane
-    // fp16 rows go straight from memory to LDS, K as well; e4m3 codes (and rows
-    // of other widths, whose ends are zeros) pass through registers
-    constexpr bool DMA = !E4M3 && FULL;
+    constexpr bool DMA = kDirect<E4M3, FULL>;
     extern __shared__ __align__(16) uint8_t smem[];
     const AttnArgs& a = p.a;
 
@@ -79,25 +173,27 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
         pair = (j / p.row_tiles) * 8u + (blockIdx.x & 7u);
         if (pair >= p.pairs) return;
     }
-    const uint32_t split = pair % p.splits, unit = pair / p.splits;
-    const uint32_t kvh = unit % a.kv_heads, s = unit / a.kv_heads;
+    const uint32_t kvh = pair % a.kv_heads;
+    Run run;
+    if (!find_run(p, pair / a.kv_heads, &run)) return;
+    const uint32_t s = run.seq;
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t i16 = lane & 15u, g = lane >> 4;
     const uint32_t capacity = a.table_stride << a.page_shift;
-    const SeqRows sr = seq_rows(nullptr, a.lengths, s, a.seq_rows, a.rows, capacity);
+    const uint32_t bad_length = run.length > capacity ? kErrAttnLength : 0u;
+    const SeqRows sr{s, s * a.seq_rows, a.seq_rows, bad_length ? capacity : run.length, bad_length};
 
     const uint32_t rows = sr.count * a.group, r0 = rt * kDecodeTileRows;
     const uint32_t last = r0 + 15u < rows ? r0 + 15u : rows - 1u;
     const int32_t base = (int32_t)sr.length - (int32_t)sr.count;
-    const int32_t p_lo = base + (int32_t)(r0 / a.group), p_hi = base + (int32_t)(last / a.group);
+    // positions of all of the sequence's rows: its row tiles take the same runs
+    const int32_t p_lo = base, p_hi = (int32_t)sr.length - 1;
     const TileSpan span = tile_span<kTile>(p_lo < 0 ? 0 : p_lo, p_hi, a.window, a.sinks);
-    uint32_t per = (span.count + p.splits - 1u) / p.splits;
-    per = per > p.min_tiles ? per : p.min_tiles;
-    uint32_t used = (span.count + per - 1u) / per;  // workgroups with keys
-    used = used > 1u ? used : 1u;
-    if (split >= used) return;
-    const uint32_t tile_end = (split + 1u) * per < span.count ? (split + 1u) * per : span.count;
+    const uint32_t used = run.used;
+    const uint32_t tile_first = run.split * run.per;  // one run: split 0
+    const uint32_t tile_end =
+        used > 1u && tile_first + run.per < span.count ? tile_first + run.per : span.count;
 
     // the lane's query row as the second operand of K Q^T; step s of the
     // product takes, from lane group g, head elements qdim(s) ..
@@ -115,7 +211,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
         return __builtin_bit_cast(h8_t, u);
     };
     constexpr bool QL = kQueryInLds<DP>;
-    h8_t* qs = reinterpret_cast<h8_t*>(smem + decode_lds_bytes<DP>() - 16u * DP * 2u) + lane;
+    h8_t* qs = reinterpret_cast<h8_t*>(smem + decode_lds_bytes<DP>() - kMarkBytes<DP> - 16u * DP * 2u) + lane;
     h8_t qf[QL ? NS / kWaves : NS];  // QL: the steps that this wave stages
 #pragma unroll
     for (uint32_t st = 0; st < (QL ? NS / kWaves : NS); ++st)
@@ -142,17 +238,19 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
     const uint32_t v_lane = (lane / CPR) * a.token_stride + (v_in ? v_chunk * 16u : 0u);
     uint8_t* vs = smem + wave * (kTile * DP * 2u * (DMA ? 2u : 1u));
     uint8_t* ks = vs + kTile * DP * 2u;  // DMA only
-    const uint32_t v_tok = lane / CPR;
+    const uint32_t v_tok = lane / CPR, v_row = v_tok * a.token_stride;
     const uint32_t vs_lds = (uint32_t)(uintptr_t)vs, ks_lds = (uint32_t)(uintptr_t)ks;
     uint4 kreg[DMA ? 1 : KL], vreg[DMA ? 1 : VL];
     const auto load_k = [&](uint64_t off) {
         if constexpr (DMA) {
+            // offsets are formed here each time (opaque lane): hoisted they would be
+            // spilled, and a reload's wait would drain the loads under way
+            uint32_t c = v_chunk;
+            asm("" : "+v"(c));
 #pragma unroll
-            for (uint32_t n = 0; n < VL; ++n) {
-                const uint32_t t = n * TPI + v_tok;
-                dma16(a.k + off, t * a.token_stride + 16u * (v_chunk ^ key_swizzle<DP>(t)),
-                      ks_lds + n * 1024u);
-            }
+            for (uint32_t n = 0; n < VL; ++n)
+                dma16(a.k + (off + n * TPI * a.token_stride),
+                      v_row + 16u * (c ^ key_swizzle<DP>(n * TPI + v_tok)), ks_lds + n * 1024u);
             return;
         }
         const uint8_t* kp = a.k + off;
@@ -166,12 +264,13 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
     };
     const auto load_v = [&](uint64_t off) {
         if constexpr (DMA) {
+            uint32_t c = v_chunk;
+            asm("" : "+v"(c));
 #pragma unroll
-            for (uint32_t n = 0; n < VL; ++n) {
-                const uint32_t t = n * TPI + v_tok;
-                dma16(a.v + off, t * a.token_stride + 16u * (v_chunk ^ (2u * value_swizzle<DP>(t))),
+            for (uint32_t n = 0; n < VL; ++n)
+                dma16(a.v + (off + n * TPI * a.token_stride),
+                      v_row + 16u * (c ^ (2u * value_swizzle<DP>(n * TPI + v_tok))),
                       vs_lds + n * 1024u);
-            }
             return;
         }
 #pragma unroll
@@ -198,12 +297,43 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
         return __builtin_bit_cast(h4_t, lds_read_tr(vs + (tr_base ^ (32u * b))));
     };
 
+    // The product would make NaN of the weight 0 of a row that does not see an
+    // infinity's or NaN's key: they are taken out of the V tile and noted in
+    // `marks` (two bits, +inf and -inf, NaN both, for each element of the rows
+    // that see the key), which go onto the sums at the end.
+    uint32_t* marks =
+        reinterpret_cast<uint32_t*>(smem + decode_lds_bytes<DP>() - kMarkBytes<DP>) +
+        wave * (kMarkBytes<DP> / 4u / kWaves);  // [row][DP / 16]
+    bool marked = false;
+    const auto take_out = [&](uint32_t t0) {
+        if (!marked)
+            for (uint32_t n = lane; n < DP; n += 64u) marks[n] = 0u;
+        marked = true;
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (uint32_t n = lane; n < kTile * DP; n += 64u) {
+            uint16_t* v = reinterpret_cast<uint16_t*>(vs) + n;
+            const uint32_t bits = *v;
+            if ((bits & 0x7C00u) != 0x7C00u) continue;
+            *v = 0;
+            const uint32_t t = n / DP, e = n % DP;
+            const uint32_t dim = 8u * ((e / 8u) ^ (2u * value_swizzle<DP>(t))) + e % 8u;
+            const uint32_t mark = (bits & 0x3FFu ? 3u : bits & 0x8000u ? 2u : 1u) << (2u * (dim & 15u));
+#pragma unroll 1
+            for (uint32_t r = 0; r <= last - r0; ++r)
+                if (key_seen((int32_t)(t0 + t), base + (int32_t)((r0 + r) / a.group), a.window,
+                             a.sinks))
+                    atomicOr(marks + r * (DP / 16u) + dim / 16u, mark);
+        }
+        __builtin_amdgcn_wave_barrier();
+    };
+
     f4_t o[NB];
 #pragma unroll
     for (uint32_t b = 0; b < NB; ++b) o[b] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
     float m = kNoKey, l = 0.0f;
 
-    uint32_t idx = split * per + wave;
+    uint32_t idx = tile_first + wave;
     if (sr.bad) idx = tile_end;
     uint64_t off = 0;
     if (idx < tile_end) {
@@ -234,6 +364,31 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
             if constexpr (DMA) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K was read
             load_k(off);
         }
+        // Keys that no row sees (behind the last, before the window) may hold
+        // anything: their V becomes zeros.
+        bool tainted = false;  // an infinity or NaN that some row sees and some may not
+        uint32_t seen = 0xFu;
+        if (!whole) {
+            if constexpr (DMA) wait_loads<0>();
+            uint32_t found = 0;
+#pragma unroll
+            for (uint32_t n = 0; n < VL; ++n) {
+                uint4* at = reinterpret_cast<uint4*>(vs) + n * 64u + lane;
+                uint4 x = DMA ? *at : vreg[DMA ? 0 : n];
+                const uint32_t keep =
+                    keys_seen<1>(t0 + n * TPI + v_tok, p_lo, p_hi, a.window, a.sinks) ? ~0u : 0u;
+                x = make_uint4(x.x & keep, x.y & keep, x.z & keep, x.w & keep);
+                if constexpr (DMA) *at = x;
+                else vreg[n] = x;
+                found |= not_finite<E4M3>(x.x) | not_finite<E4M3>(x.y) | not_finite<E4M3>(x.z) |
+                         not_finite<E4M3>(x.w);
+            }
+            tainted = __ballot(found != 0u) != 0;
+            seen = 0u;
+#pragma unroll
+            for (uint32_t e = 0; e < 4u; ++e)
+                seen |= (uint32_t)key_seen((int32_t)(t0 + 4u * g + e), pos, a.window, a.sinks) << e;
+        }
         // V into the wave's LDS
 #pragma unroll
         for (uint32_t n = 0; n < (DMA ? 0u : VL); ++n) {
@@ -249,24 +404,6 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
                 *reinterpret_cast<uint4*>(vs + t * (DP * 2u) +
                                           16u * (v_chunk ^ (2u * value_swizzle<DP>(t)))) = vreg[n];
             }
-        }
-        bool tainted = false;
-        uint32_t seen = 0xFu;
-        if (!whole) {
-            if constexpr (DMA) wait_loads<0>();
-            uint32_t found = 0;
-#pragma unroll
-            for (uint32_t n = 0; n < VL; ++n) {
-                const uint4 x = DMA ? reinterpret_cast<const uint4*>(vs)[n * 64u + lane]
-                                    : vreg[DMA ? 0 : n];
-                found |= not_finite<E4M3>(x.x) | not_finite<E4M3>(x.y) | not_finite<E4M3>(x.z) |
-                         not_finite<E4M3>(x.w);
-            }
-            tainted = __ballot(found != 0u) != 0;
-            seen = 0u;
-#pragma unroll
-            for (uint32_t e = 0; e < 4u; ++e)
-                seen |= (uint32_t)key_seen((int32_t)(t0 + 4u * g + e), pos, a.window, a.sinks) << e;
         }
         if (!DMA && more) load_v(off);
 
@@ -296,32 +433,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
             else wait_loads<0>();
         }
         __builtin_amdgcn_wave_barrier();  // the wave's own LDS: its operations stay in order
-        if (!tainted) {
+        if (tainted) take_out(t0);
 #pragma unroll
-            for (uint32_t b = 0; b < NB; ++b) {
-                o[b] = __builtin_amdgcn_mfma_f32_16x16x16f16(v_frag(b), w, o[b], 0, 0, 0);
-                if (QL && b % 8u == 7u) __builtin_amdgcn_sched_barrier(0);
-            }
-        } else {
-            h4_t ones;
-#pragma unroll
-            for (uint32_t e = 0; e < 4u; ++e) ones[e] = (_Float16)(float)((seen >> e) & 1u);
-#pragma unroll
-            for (uint32_t b = 0; b < NB; ++b) {
-                // one kind at a time: registers
-                o[b] = __builtin_amdgcn_mfma_f32_16x16x16f16(finite_values(v_frag(b)), w, o[b], 0,
-                                                             0, 0);
-                const auto add = [&](uint32_t kind, float what) {
-                    const f4_t n = __builtin_amdgcn_mfma_f32_16x16x16f16(
-                        value_kind(v_frag(b), kind), ones, f4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[b][e] = n[e] > 0.0f ? o[b][e] + what : o[b][e];
-                    __builtin_amdgcn_sched_barrier(0);
-                };
-                add(kIsNan, __builtin_nanf(""));
-                add(kIsPosInf, __builtin_inff());
-                add(kIsNegInf, -__builtin_inff());
-            }
+        for (uint32_t b = 0; b < NB; ++b) {
+            o[b] = __builtin_amdgcn_mfma_f32_16x16x16f16(v_frag(b), w, o[b], 0, 0, 0);
+            if (QL && b % 8u == 7u) __builtin_amdgcn_sched_barrier(0);
         }
         __builtin_amdgcn_wave_barrier();
         if constexpr (DMA) {
@@ -341,7 +457,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
     float* so = reinterpret_cast<float*>(smem);
     float* sm = so + kWaves * 16u * (DP + 4u);
     float* sl = sm + kWaves * 16u;
-    uint32_t* flag = reinterpret_cast<uint32_t*>(sl + kWaves * 16u);
+    uint32_t* sx = reinterpret_cast<uint32_t*>(sl + kWaves * 16u);  // which waves have marks
+    uint32_t* flag = sx + kWaves;
     __syncthreads();  // every wave is done with its V
 #pragma unroll
     for (uint32_t b = 0; b < NB; ++b)
@@ -350,12 +467,15 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
         sm[wave * 16u + i16] = m;
         sl[wave * 16u + i16] = l;
     }
+    if (lane == 0) sx[wave] = marked ? 1u : 0u;
     __syncthreads();
 
     constexpr uint32_t C8 = DP / 8;                      // 8-element pieces of a row
     constexpr uint32_t PIECES = (16u * C8 + 255u) / 256u;  // of a thread
     const uint32_t live = last - r0 + 1u;
-    const uint64_t tile = (uint64_t)unit * p.row_tiles + rt;
+    const auto slot_of = [&](uint32_t split) {  // its place among the partial sums
+        return ((uint64_t)(run.slot + split) * a.kv_heads + kvh) * p.row_tiles + rt;
+    };
     const auto emit = [&](uint32_t r, uint32_t c, const float* acc, float sum) {
         const float inv = sum == 0.0f ? 0.0f : a.v_scale / sum;
         uint32_t h[4];
@@ -384,10 +504,20 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
 #pragma unroll
             for (int e = 0; e < 8; ++e) acc[e] += src[e] * f;
         }
+        for (uint32_t w = 0; w < kWaves; ++w) {
+            if (!sx[w]) continue;
+            const uint32_t mark = reinterpret_cast<const uint16_t*>(
+                smem + decode_lds_bytes<DP>() - kMarkBytes<DP>)[(w * 16u + r) * (DP / 8u) + c];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (mark >> (2 * e) & 1u) acc[e] += __builtin_inff();
+                if (mark >> (2 * e) & 2u) acc[e] -= __builtin_inff();
+            }
+        }
         if (used == 1u) {
             emit(r, c, acc, sum);
         } else {
-            const uint64_t slot = (tile * p.splits + split) * 16u + r;
+            const uint64_t slot = slot_of(run.split) * 16u + r;
             float* dst = p.part_o + slot * DP + 8u * c;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -402,50 +532,83 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : DP <= 256 ? 2 : 1) void decode
     }
     if (used == 1u) return;
 
-    // the last workgroup of the unit to arrive joins the splits
+    // The last workgroup of the sequence, head and row tile to arrive joins the
+    // splits: `ways` threads share an 8-element piece, each adds up every
+    // ways-th split, in order, from loads that all go out at once; their sums
+    // are added in LDS.
     wait_vector_memory();
     __syncthreads();
     if (threadIdx.x == 0) {
-        const uint32_t before = __hip_atomic_fetch_add(p.arrivals + tile, 1u, __ATOMIC_RELAXED,
-                                                       __HIP_MEMORY_SCOPE_AGENT);
+        uint32_t* count = p.arrivals + slot_of(0);
+        const uint32_t before =
+            __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         *flag = before == used - 1u ? 1u : 0u;
-        if (before == used - 1u) st_coherent(p.arrivals + tile, 0u);
+        if (before == used - 1u) st_coherent(count, 0u);
     }
     __syncthreads();
     if (!*flag) return;
-    float2* ml = reinterpret_cast<float2*>(smem);  // [split][16]
-    for (uint32_t n = threadIdx.x; n < used * 16u; n += 256u) {
-        if ((n & 15u) >= live) continue;
-        const uint64_t v = ld_coherent(reinterpret_cast<const uint64_t*>(p.part_ml) +
-                                       tile * p.splits * 16u + n);
-        ml[n] = make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
-    }
-    __syncthreads();
+    const uint32_t pieces = live * C8;
+    uint32_t ways_log2 = 0;
+    while ((pieces << (ways_log2 + 1u)) <= 256u && (2u << ways_log2) <= used) ++ways_log2;
+    const uint32_t ways = 1u << ways_log2;
+    float* sums = reinterpret_cast<float*>(smem);  // [way][piece][10]
+    const uint64_t step = (uint64_t)a.kv_heads * p.row_tiles * 16u;
 #pragma unroll 1
-    for (uint32_t n = 0; n < PIECES; ++n) {
-        const uint32_t piece = threadIdx.x + 256u * n, r = piece / C8, c = piece % C8;
-        if (r >= live || 8u * c >= a.dim) continue;
-        float mm = ml[r].x;
-        for (uint32_t w = 1; w < used; ++w) mm = fmaxf(mm, ml[w * 16u + r].x);
-        float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0.0f;
-        const float* src = p.part_o + (tile * p.splits * 16u + r) * DP + 8u * c;
-#pragma unroll 4
-        for (uint32_t w = 0; w < used; ++w) {
-            const float2 e2 = ml[w * 16u + r];
-            const float f = __builtin_amdgcn_exp2f(e2.x - mm);
-            sum += e2.y * f;
-            const uint4 lo = ld_coherent16(src + (uint64_t)w * 16u * DP);
-            const uint4 hi = ld_coherent16(src + (uint64_t)w * 16u * DP + 4u);
-            acc[0] += __uint_as_float(lo.x) * f;
-            acc[1] += __uint_as_float(lo.y) * f;
-            acc[2] += __uint_as_float(lo.z) * f;
-            acc[3] += __uint_as_float(lo.w) * f;
-            acc[4] += __uint_as_float(hi.x) * f;
-            acc[5] += __uint_as_float(hi.y) * f;
-            acc[6] += __uint_as_float(hi.z) * f;
-            acc[7] += __uint_as_float(hi.w) * f;
+    for (uint32_t n = 0; n < pieces; n += 256u >> ways_log2) {
+        const uint32_t piece = n + (threadIdx.x >> ways_log2), way = threadIdx.x & (ways - 1u);
+        const uint32_t r = piece / C8, c = piece % C8;
+        const bool in = piece < pieces && 8u * c < a.dim;
+        float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0.0f, mm = kNoKey;
+        const uint64_t first = slot_of(0) * 16u + r;
+        for (uint32_t w0 = way; in && w0 < used; w0 += 4u * ways) {
+            uint4 lo[4], hi[4];
+            uint64_t ml[4];
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k) {
+                const uint32_t w = w0 + k * ways < used ? w0 + k * ways : w0;
+                const uint64_t at = first + w * step;
+                ml[k] = ld_coherent(reinterpret_cast<const uint64_t*>(p.part_ml) + at);
+                lo[k] = ld_coherent16(p.part_o + at * DP + 8u * c);
+                hi[k] = ld_coherent16(p.part_o + at * DP + 8u * c + 4u);
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k) {
+                if (w0 + k * ways >= used) continue;
+                const float mk = __uint_as_float((uint32_t)ml[k]);
+                const float mn = fmaxf(mm, mk);
+                const float f0 = __builtin_amdgcn_exp2f(mm - mn);
+                const float f1 = __builtin_amdgcn_exp2f(mk - mn);
+                mm = mn;
+                sum = sum * f0 + __uint_as_float((uint32_t)(ml[k] >> 32)) * f1;
+                const uint32_t u[8] = {lo[k].x, lo[k].y, lo[k].z, lo[k].w,
+                                       hi[k].x, hi[k].y, hi[k].z, hi[k].w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[e] = acc[e] * f0 + __uint_as_float(u[e]) * f1;
+            }
         }
-        emit(r, c, acc, sum);
+        if (ways > 1u) {
+            float* mine = sums + threadIdx.x * 10u;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mine[e] = acc[e];
+            mine[8] = sum;
+            mine[9] = mm;
+            __syncthreads();
+            if (in && way == 0u) {
+                for (uint32_t w = 1; w < ways; ++w) mm = fmaxf(mm, mine[w * 10u + 9u]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
+                sum = 0.0f;
+                for (uint32_t w = 0; w < ways; ++w) {
+                    const float* part = mine + w * 10u;
+                    const float f = __builtin_amdgcn_exp2f(part[9] - mm);
+                    sum += part[8] * f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) acc[e] += part[e] * f;
+                }
+            }
+            __syncthreads();
+        }
+        if (in && way == 0u) emit(r, c, acc, sum);
     }
 }
 
@@ -485,19 +648,18 @@ tsg_status launch_decode(const tsg_attn* attn, const AttnArgs& a, tsg_stream str
     DecodeArgs p{};
     p.a = a;
     p.row_tiles = (a.seq_rows * a.group + kDecodeTileRows - 1u) / kDecodeTileRows;
-    const uint64_t units = (uint64_t)a.num_seqs * a.kv_heads, tiles = units * p.row_tiles;
-    // Workgroups of a split: enough for the card, none for fewer than min_tiles
-    // tiles of the longest sequence the table can hold.
-    const uint64_t capacity_tiles =
-        (((uint64_t)a.table_stride << a.page_shift) + kTile - 1u) / kTile;
-    p.min_tiles = kWaves;
-    const uint64_t resident = attn->padded_dim <= 128u ? 4u : 512u / attn->padded_dim;
-    uint64_t splits = resident * (uint64_t)attn->ctx->num_cus / tiles;
-    splits = std::min(splits, (capacity_tiles + p.min_tiles - 1u) / p.min_tiles);
-    splits = std::min<uint64_t>(splits, kMaxSplits);
-    splits = std::min<uint64_t>(splits, kMaxPartials / tiles);
-    p.splits = (uint32_t)std::max<uint64_t>(splits, 1u);
-    const uint64_t pairs = units * p.splits;
+    // As many runs as workgroups fit the card at once (LDS: four a CU up to
+    // heads of 128, then two and one); a batch of so many sequences that its
+    // workgroups' search for their run would cost more than even runs gain has
+    // one run each.
+    const uint64_t resident = (attn->padded_dim <= 128u ? 4u : 512u / attn->padded_dim) *
+                              (uint64_t)attn->ctx->num_cus;
+    const uint64_t heads = (uint64_t)a.kv_heads * p.row_tiles;
+    uint64_t chunks = std::min<uint64_t>(resident, kMaxPartials / 2u) / heads;
+    // each sequence ends in a shorter run: on the average half a run more
+    chunks = std::max(chunks - std::min<uint64_t>(chunks, a.num_seqs / 2u), chunks / 2u);
+    p.chunks = a.num_seqs <= kMaxBalanced && chunks > 1u ? (uint32_t)chunks : 0u;
+    const uint64_t pairs = a.kv_heads * ((uint64_t)p.chunks + a.num_seqs);
     const uint64_t blocks = p.row_tiles > 1u ? (pairs + 7u) / 8u * 8u * p.row_tiles : pairs;
     TSG_REQUIRE(blocks <= 0x7fffffffu, TSG_ERR_UNSUPPORTED,
                 "too many sequences and heads for one launch");

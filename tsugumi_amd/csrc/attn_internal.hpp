@@ -48,6 +48,13 @@ struct AttnArgs {
     float v_scale;
 };
 
+// A word that no kernel writes meanwhile, at an address that is the same for
+// the wave, by a scalar load.
+typedef __attribute__((address_space(4))) const uint32_t const_u32_t;
+__device__ __forceinline__ uint32_t scalar_load(const uint32_t* p) {
+    return *(const_u32_t*)(uintptr_t)p;
+}
+
 struct SeqRows {
     uint32_t seq, first, count;  // its rows are first .. first + count - 1
     uint32_t length;             // tokens in the cache
@@ -63,7 +70,7 @@ __device__ __forceinline__ SeqRows seq_rows(const uint32_t* row_starts, const ui
     r.seq = s;
     r.bad = 0u;
     if (row_starts) {
-        const uint32_t lo = row_starts[s], hi = row_starts[s + 1];
+        const uint32_t lo = scalar_load(row_starts + s), hi = scalar_load(row_starts + s + 1u);
         if (lo > hi || hi > rows) r.bad = kErrAttnRows;
         r.first = lo < rows ? lo : rows;
         const uint32_t end = hi < rows ? hi : rows;
@@ -72,7 +79,7 @@ __device__ __forceinline__ SeqRows seq_rows(const uint32_t* row_starts, const ui
         r.first = s * uniform;
         r.count = uniform;
     }
-    const uint32_t n = lengths[s];
+    const uint32_t n = scalar_load(lengths + s);
     if (n > capacity) r.bad = kErrAttnLength;
     r.length = n > capacity ? capacity : n;
     return r;
@@ -195,11 +202,6 @@ __device__ __forceinline__ float sum_across16(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-typedef __attribute__((address_space(4))) const uint32_t const_u32_t;
-__device__ __forceinline__ uint32_t scalar_load(const uint32_t* p) {
-    return *(const_u32_t*)(uintptr_t)p;
-}
-
 // 16 bytes a lane from memory straight into LDS at `lds` + 16 x lane. Issued as
 // asm: the compiler would wait for it before any LDS read. It returns no
 // register; a wait on vector memory and a barrier come before the data is
@@ -242,36 +244,6 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
 
 typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
 
-// The part of O^T += V^T P^T that a tile with infinities or NaN in V needs
-// where some row does not see some key: the product would make NaN of 0 times
-// them. The finite values go through the product as they are; for the others a
-// product of zeros and ones counts, for each row and element, the seen keys
-// that hold a NaN, a positive and a negative infinity.
-constexpr uint32_t kIsNan = 0, kIsPosInf = 1, kIsNegInf = 2;
-template <typename H>
-__device__ __forceinline__ H finite_values(H v) {
-#pragma unroll
-    for (uint32_t j = 0; j < sizeof(H) / 2u; ++j) {
-        const _Float16 x = v[j];  // a scalar: vector elements have no address
-        const bool bad = (__builtin_bit_cast(uint16_t, x) & 0x7C00u) == 0x7C00u;
-        v[j] = bad ? (_Float16)0.0f : x;
-    }
-    return v;
-}
-template <typename H>
-__device__ __forceinline__ H value_kind(H v, uint32_t kind) {
-#pragma unroll
-    for (uint32_t j = 0; j < sizeof(H) / 2u; ++j) {
-        const _Float16 x = v[j];
-        const uint16_t b = __builtin_bit_cast(uint16_t, x);
-        const bool is = kind == kIsNan      ? (b & 0x7FFFu) > 0x7C00u
-                        : kind == kIsPosInf ? b == 0x7C00u
-                                            : b == 0xFC00u;
-        v[j] = is ? (_Float16)1.0f : (_Float16)0.0f;
-    }
-    return v;
-}
-
 // Runs with the plan's device current; the caller's is restored on return.
 struct DeviceScope {
     int before = -1;
@@ -300,8 +272,7 @@ tsg_status attn_args(const tsg_attn* attn, const tsg_kv_pages* pages, const tsg_
 
 // attn_decode.hip
 constexpr uint32_t kDecodeTileRows = 16;
-constexpr uint32_t kMaxPartials = 2048;  // (row tile, split) pairs of one call
-constexpr uint32_t kMaxSplits = 128;
+constexpr uint32_t kMaxPartials = 2048;  // partial sums (of a 16-row tile) of one call
 constexpr uint32_t kMaxPrefillPartials = 512;  // (row tile, key head, split) of one call
 constexpr uint32_t kPrefillRows = 128;
 // rows of partial results the plan's scratch holds, padded_dim + 2 floats each
