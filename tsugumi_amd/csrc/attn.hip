@@ -136,7 +136,9 @@ tsg_status attn_args(const tsg_attn* attn, const tsg_kv_pages* pages, const tsg_
     a->page_shift = attn->page_shift;
     a->window = c.window;
     a->sinks = c.sinks;
-    a->scale_log2 = (float)((double)c.scale * c.k_scale * 1.4426950408889634);
+    const double scale = std::fabs((double)c.scale) * c.k_scale * 1.4426950408889634;
+    a->scale_log2 = scale > 1e-30 ? (float)scale : 1e-30f;
+    a->q_sign = c.scale < 0.0f ? 0x80008000u : 0u;
     a->v_scale = c.v_scale;
     return TSG_OK;
 }

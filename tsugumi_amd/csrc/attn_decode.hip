@@ -207,7 +207,7 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
                         (uint64_t)(kvh * a.group + row % a.group) * a.dim;
     const auto load_q = [&](uint32_t st) -> h8_t {
         uint4 u = make_uint4(0, 0, 0, 0);
-        if (FULL || qdim(st) < a.dim) u = *reinterpret_cast<const uint4*>(q + qdim(st));
+        if (FULL || qdim(st) < a.dim) u = load_query(q + qdim(st), a.q_sign);
         return __builtin_bit_cast(h8_t, u);
     };
     constexpr bool QL = kQueryInLds<DP>;
@@ -410,10 +410,10 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
         float x[4];
 #pragma unroll
         for (uint32_t e = 0; e < 4u; ++e)
-            x[e] = (seen >> e) & 1u ? sc[e] * a.scale_log2 : -__builtin_inff();
+            x[e] = (seen >> e) & 1u ? sc[e] : -__builtin_inff();
         const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-        if (__ballot(top > m + kMaxLag)) {
-            const float mn = fmaxf(m, max_across32(max_across16(top)));
+        if (__ballot(top * a.scale_log2 > m + kMaxLag)) {
+            const float mn = fmaxf(m, max_across32(max_across16(top)) * a.scale_log2);
             const float alpha = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= alpha;
@@ -424,7 +424,7 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
         h4_t w;
 #pragma unroll
         for (uint32_t e = 0; e < 4u; ++e) {
-            const float we = __builtin_amdgcn_exp2f(x[e] + shift);
+            const float we = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale_log2, shift));
             l += we;
             w[e] = (_Float16)we;
         }

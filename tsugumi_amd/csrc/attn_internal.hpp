@@ -44,7 +44,10 @@ struct AttnArgs {
     uint32_t table_stride, num_seqs, rows, seq_rows, num_pages;
     uint32_t q_heads, kv_heads, group, dim, page_shift;
     uint32_t window, sinks;
-    float scale_log2;  // logits to powers of two: scale * k_scale * log2(e)
+    // q . k to logits in powers of two: |scale| k_scale log2(e), at least 1e-30
+    // so that a masked product of -inf stays -inf; a negative scale turns q
+    float scale_log2;
+    uint32_t q_sign;  // 0x80008000 where the scale is negative
     float v_scale;
 };
 
@@ -118,6 +121,12 @@ __device__ __forceinline__ uint2 e4m3x4_to_f16(uint32_t w) {
     const h2_t lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false);
     const h2_t hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true);
     return make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
+}
+
+// Eight query elements, their signs turned by q_sign.
+__device__ __forceinline__ uint4 load_query(const uint16_t* p, uint32_t q_sign) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    return make_uint4(u.x ^ q_sign, u.y ^ q_sign, u.z ^ q_sign, u.w ^ q_sign);
 }
 
 // --------------------------------------------------- the attention kernels

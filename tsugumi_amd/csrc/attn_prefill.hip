@@ -176,7 +176,7 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
     for (uint32_t st = 0; st < NS; ++st) {
         uint4 u = make_uint4(0, 0, 0, 0);
         if (FULL || d0 + 16u * st + 8u * h < a.dim)
-            u = *reinterpret_cast<const uint4*>(q + d0 + 16u * st + 8u * h);
+            u = load_query(q + d0 + 16u * st + 8u * h, a.q_sign);
         qf[st] = __builtin_bit_cast(h8_t, u);
     }
 
@@ -308,10 +308,6 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
                 for (int e = 0; e < 4; ++e) x[0][4 * k + e] += y[e];
             }
         }
-#pragma unroll
-        for (uint32_t u = 0; u < N; ++u)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) x[u][e] *= a.scale_log2;
         if (!tile_seen_whole<TK>(key0, p_lo, p_hi, a.window, a.sinks)) {
 #pragma unroll
             for (uint32_t u = 0; u < N; ++u)
@@ -326,8 +322,8 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
         for (uint32_t u = 0; u < N; ++u)
 #pragma unroll
             for (int e = 0; e < 16; ++e) top = fmaxf(top, x[u][e]);
-        if (__ballot(top > m + kMaxLag)) {
-            const float mn = fmaxf(m, max_across32(top));
+        if (__ballot(top * a.scale_log2 > m + kMaxLag)) {
+            const float mn = fmaxf(m, max_across32(top) * a.scale_log2);
             const float alpha = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= alpha;
@@ -340,7 +336,8 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
         for (uint32_t u = 0; u < N; ++u)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const float we = __builtin_amdgcn_exp2f(x[u][e] + shift);
+                const float we =
+                    __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][e], a.scale_log2, shift));
                 l += we;
                 w[u][e / 8][e % 8] = (_Float16)we;
             }
