@@ -181,13 +181,13 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
     }
 
     // ------------------------------------------------------------- staging
-    // Key t's row: chunk c of K lies at c ^ key_swizzle(t), of V at c ^ 2
+    // Key t's row: chunk c of K lies at c ^ key_swizzle(t), of V at c ^
     // value_swizzle(t): 16 keys' equal chunks, and the 8 keys of a transposing
     // read, lie in different banks.
     const auto key_swizzle = [](uint32_t k) { return DP >= 128 ? k & 15u : (k >> 1) & 7u; };
     const auto value_swizzle = [](uint32_t k) {
-        return DP >= 128 ? ((k & 3u) << 1) | ((k >> 2) & 1u)
-                         : (((k >> 1) & 1u) << 1) | ((k >> 2) & 1u);
+        return 2u * (DP >= 128 ? ((k & 3u) << 1) | ((k >> 2) & 1u)
+                               : (((k >> 1) & 1u) << 1) | ((k >> 2) & 1u));
     };
     const uint32_t* table = a.table + (uint64_t)s * a.table_stride;
     const uint32_t page_mask = (1u << a.page_shift) - 1u;
@@ -209,56 +209,65 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
     constexpr uint32_t KPI = 64u / SRC;              // keys of one load instruction
     constexpr uint32_t NL = KW / KPI;                // loads of K (and of V) a tile
     static_assert(NL >= 1u && KW % KPI == 0u, "a wave's keys are whole load instructions");
+    const uint32_t l_key = lane / SRC, l_chunk = lane % SRC, l_row = l_key * a.token_stride;
+    const auto k_tile = [&](uint32_t buf) { return smem + buf * 2u * TILE; };
+    const auto v_tile = [&](uint32_t buf) { return smem + buf * 2u * TILE + TILE; };
     uint4 kst[DMA ? 1 : NL], vst[DMA ? 1 : NL];
-    const uint32_t l_key = lane / SRC, l_chunk = lane % SRC;
-    const auto stage_begin = [&](uint32_t idx, uint32_t buf) {
-        const uint64_t off = wave_offset(idx);
+    // The wave's keys of a tile, from byte `off` of a pool: to LDS at once, or to
+    // registers (begin) and from there, as fp16, to LDS (end).
+    const auto stage_begin = [&](const uint8_t* pool, uint64_t off, uint8_t* to, auto swizzle,
+                                 uint4* regs) {
         if constexpr (DMA) {
-            const uint32_t lds = (uint32_t)(uintptr_t)smem + buf * 2u * TILE + wave * KW * ROW;
+            const uint32_t lds = (uint32_t)(uintptr_t)to + wave * KW * ROW;
+            // offsets are formed here each time (opaque lane): hoisted they would be
+            // spilled, and a reload's wait would drain the loads under way
+            uint32_t c = l_chunk;
+            asm("" : "+v"(c));
 #pragma unroll
-            for (uint32_t n = 0; n < NL; ++n) {
-                const uint32_t k = wave * KW + n * KPI + l_key;
-                const uint32_t at_k = (n * KPI + l_key) * a.token_stride;
-                dma16(a.k + off, at_k + 16u * (l_chunk ^ key_swizzle(k)), lds + n * KPI * ROW);
-                dma16(a.v + off, at_k + 16u * (l_chunk ^ (2u * value_swizzle(k))),
-                      lds + TILE + n * KPI * ROW);
-            }
+            for (uint32_t n = 0; n < NL; ++n)
+                dma16(pool + (off + n * KPI * a.token_stride),
+                      l_row + 16u * (c ^ swizzle(wave * KW + n * KPI + l_key)), lds + n * KPI * ROW);
         } else {
             const bool in = FULL || l_chunk * 16u < a.dim * (E4M3 ? 1u : 2u);
 #pragma unroll
             for (uint32_t n = 0; n < NL; ++n) {
-                const uint32_t at_k =
-                    (n * KPI + l_key) * a.token_stride + (in ? 16u * l_chunk : 0u);
-                const uint4 kx = *reinterpret_cast<const uint4*>(a.k + off + at_k);
-                const uint4 vx = *reinterpret_cast<const uint4*>(a.v + off + at_k);
-                kst[n] = in ? kx : make_uint4(0, 0, 0, 0);
-                vst[n] = in ? vx : make_uint4(0, 0, 0, 0);
+                const uint4 x = *reinterpret_cast<const uint4*>(
+                    pool + (off + n * KPI * a.token_stride) + (l_row + (in ? 16u * l_chunk : 0u)));
+                regs[n] = in ? x : make_uint4(0, 0, 0, 0);
             }
         }
     };
-    const auto stage_end = [&](uint32_t buf) {
+    const auto stage_end = [&](uint8_t* to, auto swizzle, const uint4* regs) {
         if constexpr (!DMA) {
-            uint8_t* kb = smem + buf * 2u * TILE;
 #pragma unroll
             for (uint32_t n = 0; n < NL; ++n) {
-                const uint32_t k = wave * KW + n * KPI + l_key;
-                const auto put = [&](uint8_t* to, const uint4& x, uint32_t swizzle) {
-                    if constexpr (E4M3) {
-                        const uint2 x0 = e4m3x4_to_f16(x.x), x1 = e4m3x4_to_f16(x.y);
-                        const uint2 x2 = e4m3x4_to_f16(x.z), x3 = e4m3x4_to_f16(x.w);
-                        *reinterpret_cast<uint4*>(to + k * ROW + 16u * ((2u * l_chunk) ^ swizzle)) =
-                            make_uint4(x0.x, x0.y, x1.x, x1.y);
-                        *reinterpret_cast<uint4*>(
-                            to + k * ROW + 16u * ((2u * l_chunk + 1u) ^ swizzle)) =
-                            make_uint4(x2.x, x2.y, x3.x, x3.y);
-                    } else {
-                        *reinterpret_cast<uint4*>(to + k * ROW + 16u * (l_chunk ^ swizzle)) = x;
-                    }
-                };
-                put(kb, kst[n], key_swizzle(k));
-                put(kb + TILE, vst[n], 2u * value_swizzle(k));
+                const uint32_t k = wave * KW + n * KPI + l_key, z = swizzle(k);
+                if constexpr (E4M3) {
+                    const uint2 x0 = e4m3x4_to_f16(regs[n].x), x1 = e4m3x4_to_f16(regs[n].y);
+                    const uint2 x2 = e4m3x4_to_f16(regs[n].z), x3 = e4m3x4_to_f16(regs[n].w);
+                    *reinterpret_cast<uint4*>(to + k * ROW + 16u * ((2u * l_chunk) ^ z)) =
+                        make_uint4(x0.x, x0.y, x1.x, x1.y);
+                    *reinterpret_cast<uint4*>(to + k * ROW + 16u * ((2u * l_chunk + 1u) ^ z)) =
+                        make_uint4(x2.x, x2.y, x3.x, x3.y);
+                } else {
+                    *reinterpret_cast<uint4*>(to + k * ROW + 16u * (l_chunk ^ z)) = regs[n];
+                }
             }
         }
+    };
+    const auto k_begin = [&](uint64_t off, uint32_t buf) {
+        stage_begin(a.k, off, k_tile(buf), key_swizzle, kst);
+    };
+    const auto v_begin = [&](uint64_t off, uint32_t buf) {
+        stage_begin(a.v, off, v_tile(buf), value_swizzle, vst);
+    };
+    const auto k_end = [&](uint32_t buf) { stage_end(k_tile(buf), key_swizzle, kst); };
+    const auto v_end = [&](uint32_t buf) { stage_end(v_tile(buf), value_swizzle, vst); };
+    // every wave's part of the tiles is in LDS, and every wave done with the last
+    const auto staged = [&] {
+        wait_loads<0>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
     };
 
     // ------------------------------------------------------------- compute
@@ -274,24 +283,23 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
     const uint32_t i16 = lane & 15u, tr_key = 4u * h + (i16 >> 2);
     const uint32_t k_at = i32 * ROW + 2u * d0, k_swz = key_swizzle(i32);
     const uint32_t v_at = tr_key * ROW + 2u * d0 + 8u * (i16 & 3u);
-    const uint32_t v_pair = ((lane >> 4) & 1u) ^ value_swizzle(tr_key);
+    const uint32_t v_chunk = (2u * ((lane >> 4) & 1u)) ^ value_swizzle(tr_key);
 
-    // the wave's rows against the TK keys from key0 on
+    // the wave's rows against a tile's keys, in steps
     constexpr uint32_t N = TK / 32u;
-    const auto process = [&](uint8_t* kb, uint32_t key0) {
-        const uint8_t* vb = kb + TILE;
-        f16v_t x[N];
+    const auto products = [&](uint8_t* kb, f16v_t (&x)[N]) {
 #pragma unroll
-        for (uint32_t u = 0; u < N; ++u) {
+        for (uint32_t u = 0; u < N; ++u)
 #pragma unroll
             for (int e = 0; e < 16; ++e) x[u][e] = 0.0f;
 #pragma unroll
-            for (uint32_t st = 0; st < NS; ++st) {
+        for (uint32_t st = 0; st < NS; ++st)
+#pragma unroll
+            for (uint32_t u = 0; u < N; ++u) {
                 const h8_t kf = *reinterpret_cast<const h8_t*>(
                     kb + u * 32u * ROW + k_at + 16u * ((2u * st + h) ^ k_swz));
                 x[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[st], x[u], 0, 0, 0);
             }
-        }
         if constexpr (SHARE == 2u) {  // through the K tile, once every wave is done with it
             static_assert(N == 1u && 2u * 4u * 64u * 64u <= TILE, "the sums fit the K tile");
             lds_barrier();
@@ -308,15 +316,18 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
                 for (int e = 0; e < 4; ++e) x[0][4 * k + e] += y[e];
             }
         }
-        if (!tile_seen_whole<TK>(key0, p_lo, p_hi, a.window, a.sinks)) {
+    };
+    const auto mask = [&](f16v_t (&x)[N], uint32_t key0) {
+        if (tile_seen_whole<TK>(key0, p_lo, p_hi, a.window, a.sinks)) return;
 #pragma unroll
-            for (uint32_t u = 0; u < N; ++u)
+        for (uint32_t u = 0; u < N; ++u)
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (!key_seen((int32_t)(key0 + 32u * u + 8u * (e / 4) + 4u * h + e % 4), pos,
-                                  a.window, a.sinks))
-                        x[u][e] = -__builtin_inff();
-        }
+            for (int e = 0; e < 16; ++e)
+                if (!key_seen((int32_t)(key0 + 32u * u + 8u * (e / 4) + 4u * h + e % 4), pos,
+                              a.window, a.sinks))
+                    x[u][e] = -__builtin_inff();
+    };
+    const auto move_reference = [&](const f16v_t (&x)[N]) {
         float top = -__builtin_inff();
 #pragma unroll
         for (uint32_t u = 0; u < N; ++u)
@@ -330,8 +341,9 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b) o[b] *= alpha;
         }
+    };
+    const auto weights = [&](const f16v_t (&x)[N], h8_t (&w)[N][2]) {
         const float shift = kWeightBias - m;
-        h8_t w[N][2];
 #pragma unroll
         for (uint32_t u = 0; u < N; ++u)
 #pragma unroll
@@ -341,6 +353,8 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
                 l += we;
                 w[u][e / 8][e % 8] = (_Float16)we;
             }
+    };
+    const auto add_values = [&](const h8_t (&w)[N][2], const uint8_t* vb) {
 #pragma unroll
         for (uint32_t u = 0; u < N; ++u)
 #pragma unroll
@@ -348,7 +362,7 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
 #pragma unroll
                 for (uint32_t b = 0; b < NB; ++b) {
                     const uint8_t* at_v =
-                        vb + (u * 32u + 16u * ss) * ROW + v_at + 32u * ((2u * b) ^ v_pair);
+                        vb + (u * 32u + 16u * ss) * ROW + v_at + 16u * ((4u * b) ^ v_chunk);
                     const uint2 lo = lds_read_tr(at_v), hi = lds_read_tr(at_v + 8u * ROW);
                     const h8_t vf = __builtin_bit_cast(h8_t, make_uint4(lo.x, lo.y, hi.x, hi.y));
                     o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, w[u][ss], o[b], 0, 0, 0);
@@ -384,7 +398,7 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
             *v = 0;
             const uint32_t k = n / DP, e = n % DP;
             if (!keys_seen<1>(key0 + k, t.p_lo, t.p_hi, a.window, a.sinks)) continue;
-            const uint32_t dim = 8u * ((e / 8u) ^ (2u * value_swizzle(k))) + e % 8u;
+            const uint32_t dim = 8u * ((e / 8u) ^ value_swizzle(k)) + e % 8u;
             const uint32_t mark = (bits & 0x3FFu ? 3u : bits & 0x8000u ? 2u : 1u) << (2u * (dim & 15u));
 #pragma unroll 1
             for (uint32_t r = 0; r < t.live; ++r)
@@ -395,24 +409,44 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
         __syncthreads();
     };
 
+    const auto key0_of = [&](uint32_t idx) { return t.span.key_tile(idx) * TK; };
+    // a tile that not all rows of the workgroup see whole
+    const auto clean_values = [&](uint32_t idx, uint8_t* vb) {
+        if (!tile_seen_whole<TK>(key0_of(idx), t.p_lo, t.p_hi, a.window, a.sinks))
+            take_out(vb, key0_of(idx));
+    };
     if (tile_first < tile_end) {
-        stage_begin(tile_first, 0u);
-        stage_end(0u);
+        const uint64_t off = wave_offset(tile_first);
+        k_begin(off, 0u);
+        v_begin(off, 0u);
+        k_end(0u);
+        v_end(0u);
     }
     for (uint32_t idx = tile_first; idx < tile_end; ++idx) {
         const uint32_t buf = (idx - tile_first) & 1u;
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
         const bool more = idx + 1u < tile_end;
-        if (more) stage_begin(idx + 1u, buf ^ 1u);
-        const uint32_t k0 = t.span.key_tile(idx) * TK;
-        uint8_t* kb = smem + buf * 2u * TILE;
-        if (!tile_seen_whole<TK>(k0, t.p_lo, t.p_hi, a.window, a.sinks)) take_out(kb + TILE, k0);
+        staged();
+        if (more) {
+            const uint64_t off = wave_offset(idx + 1u);
+            k_begin(off, buf ^ 1u);
+            v_begin(off, buf ^ 1u);
+        }
+        clean_values(idx, v_tile(buf));
+        const uint32_t key0 = key0_of(idx);
         // waves that share rows meet inside; every wave goes in
-        if (SHARE == 2u || (wave_live && keys_seen<TK>(k0, p_lo, p_hi, a.window, a.sinks)))
-            process(kb, k0);
-        if (more) stage_end(buf ^ 1u);
+        if (SHARE == 2u || (wave_live && keys_seen<TK>(key0, p_lo, p_hi, a.window, a.sinks))) {
+            f16v_t x[N];
+            h8_t w[N][2];
+            products(k_tile(buf), x);
+            mask(x, key0);
+            move_reference(x);
+            weights(x, w);
+            add_values(w, v_tile(buf));
+        }
+        if (more) {
+            k_end(buf ^ 1u);
+            v_end(buf ^ 1u);
+        }
     }
 
     // a page past the pool: the tile's rows are NaN, whichever wave met it
