@@ -173,9 +173,9 @@ struct AppendArgs {
     uint32_t q_stride, k_stride, v_stride, q_out_stride;
     uint32_t table_stride, num_seqs, rows, seq_rows, num_pages;
     uint32_t q_heads, kv_heads, dim, page_shift;
-    uint32_t rot, interleaved, normalize_v;
-    uint32_t lanes_log2;     // lanes a head row takes, 16 elements each
-    uint32_t waves_per_row;
+    uint32_t rot, normalize_v, weights16;
+    uint32_t lanes_log2;  // lanes a head row takes, 16 elements each
+    uint32_t groups, waves_per_row;
     float eps, k_inv_scale, v_inv_scale;
 };
 
@@ -218,113 +218,153 @@ __device__ __forceinline__ uint2 pack8_e4m3(const float* y, float inv_scale) {
     return make_uint2(w[0], w[1]);
 }
 
-// A wave takes one row's heads, 64 >> lanes_log2 of them: queries, then keys,
-// then values. Lane j of a head holds two 8-element chunks; for split pairs
-// chunk c and chunk c + rot / 16, so that both elements of every pair are the
-// lane's own, and its angles are inv_freq[8 j .. 8 j + 7] in either order of
-// pairs.
-template <bool E4M3>
+// A wave takes `groups` groups of one row's heads, 64 >> lanes_log2 heads each:
+// queries, then keys, then values. Lane j of a head holds two 8-element chunks;
+// for split pairs chunk j and chunk j + rot / 16, so that both elements of every
+// pair are the lane's own, and its angles are inv_freq[8 j .. 8 j + 7] in either
+// order of pairs, the same for all of the wave's heads.
+template <bool E4M3, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4u + (threadIdx.x >> 6));
     const uint32_t row = wave / a.waves_per_row;
     if (row >= a.rows) return;
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t L = 1u << a.lanes_log2, j = lane & (L - 1u), per = 64u >> a.lanes_log2;
+    const uint32_t heads = a.q_heads + 2u * a.kv_heads;
+    const uint32_t chunks = a.dim / 8u, half = a.rot / 16u;
+    const bool turns = j < half;
+    const uint32_t q0 = !INTERLEAVED && turns ? j : 2u * j;  // the lane's chunks of q and k
+    const uint32_t q1 = !INTERLEAVED && turns ? j + half : 2u * j + 1u;
+
+    struct Head {
+        uint32_t head, c0, c1;
+        uint4 x0, x1;
+    };
+    const auto load = [&](uint32_t group) {
+        Head t;
+        t.head = group * per + (lane >> a.lanes_log2);
+        const bool is_q = t.head < a.q_heads, is_v = t.head >= a.q_heads + a.kv_heads;
+        t.c0 = is_v ? 2u * j : q0;
+        t.c1 = is_v ? 2u * j + 1u : q1;
+        const uint16_t* src =
+            is_q   ? a.q + (uint64_t)row * a.q_stride + t.head * a.dim
+            : is_v ? a.v + (uint64_t)row * a.v_stride + (t.head - a.q_heads - a.kv_heads) * a.dim
+                   : a.k + (uint64_t)row * a.k_stride + (t.head - a.q_heads) * a.dim;
+        t.x0 = t.x1 = make_uint4(0, 0, 0, 0);
+        if (t.head < heads && t.c0 < chunks) t.x0 = *reinterpret_cast<const uint4*>(src + 8u * t.c0);
+        if (t.head < heads && t.c1 < chunks) t.x1 = *reinterpret_cast<const uint4*>(src + 8u * t.c1);
+        return t;
+    };
+    const uint32_t first = (wave % a.waves_per_row) * a.groups;
+    const uint32_t all = (heads + per - 1u) / per;
+    const uint32_t end = first + a.groups < all ? first + a.groups : all;
+    Head next = load(first);
+
+    // the norms' weights at the lane's chunks (8 bf16 each) and its frequencies
+    const auto weights = [&](const uint16_t* w, uint32_t c) {
+        if (!w || c >= chunks) return make_uint4(0, 0, 0, 0);
+        if (a.weights16) return *reinterpret_cast<const uint4*>(w + 8u * c);
+        uint32_t u[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            u[e] = (uint32_t)w[8u * c + 2 * e] | ((uint32_t)w[8u * c + 2 * e + 1] << 16);
+        return make_uint4(u[0], u[1], u[2], u[3]);
+    };
+    const uint4 qw0 = weights(a.q_weight, q0), qw1 = weights(a.q_weight, q1);
+    const uint4 kw0 = weights(a.k_weight, q0), kw1 = weights(a.k_weight, q1);
+    f4a4_t f0 = {0, 0, 0, 0}, f1 = {0, 0, 0, 0};
+    if (turns) {
+        f0 = *reinterpret_cast<const f4a4_t*>(a.inv_freq + 8u * j);
+        f1 = *reinterpret_cast<const f4a4_t*>(a.inv_freq + 8u * j + 4u);
+    }
+
     const uint32_t s = find_seq(a.row_starts, a.num_seqs, a.seq_rows, a.rows, row, a.error);
     if (s >= a.num_seqs) return;
     const uint32_t capacity = a.table_stride << a.page_shift;
     const SeqRows sr = seq_rows(a.row_starts, a.lengths, s, a.seq_rows, a.rows, capacity);
-    const uint32_t lane = threadIdx.x & 63u;
-    const uint32_t L = 1u << a.lanes_log2, j = lane & (L - 1u);
-    const uint32_t head =
-        (wave % a.waves_per_row) * (64u >> a.lanes_log2) + (lane >> a.lanes_log2);
-    const uint32_t heads = a.q_heads + 2u * a.kv_heads;
     const int32_t pos = (int32_t)sr.length - (int32_t)sr.count + (int32_t)(row - sr.first);
     bool drop = sr.bad || pos < 0;  // nothing to append; the query row becomes zeros (NaN)
     if (sr.bad && lane == 0) report(a.error, sr.bad);
     uint32_t page = 0;
     if (!drop) {
-        page = a.table[(uint64_t)s * a.table_stride + ((uint32_t)pos >> a.page_shift)];
+        page = scalar_load(a.table + ((uint64_t)s * a.table_stride + ((uint32_t)pos >> a.page_shift)));
         if (page >= a.num_pages) {
             drop = true;
             if (lane == 0) report(a.error, kErrAttnPage);
         }
     }
-    if (head >= heads) return;
-    const bool is_q = head < a.q_heads, is_v = head >= a.q_heads + a.kv_heads;
-    const uint32_t kvh = is_q ? 0u : (is_v ? head - a.q_heads - a.kv_heads : head - a.q_heads);
-    const uint16_t* src = is_q ? a.q + (uint64_t)row * a.q_stride + head * a.dim
-                          : is_v ? a.v + (uint64_t)row * a.v_stride + kvh * a.dim
-                                 : a.k + (uint64_t)row * a.k_stride + kvh * a.dim;
-    const uint32_t chunks = a.dim / 8u, half = a.rot / 16u;
-    uint32_t c0 = 2u * j, c1 = 2u * j + 1u;
-    if (!a.interleaved && !is_v && j < half) {
-        c0 = j;
-        c1 = j + half;
-    }
-    const bool has0 = c0 < chunks, has1 = c1 < chunks;
-    float y[16];
-    unpack8(has0 ? *reinterpret_cast<const uint4*>(src + 8u * c0) : make_uint4(0, 0, 0, 0), y);
-    unpack8(has1 ? *reinterpret_cast<const uint4*>(src + 8u * c1) : make_uint4(0, 0, 0, 0), y + 8);
+    const uint64_t slot = page * a.page_stride +
+                          (uint64_t)((uint32_t)pos & ((1u << a.page_shift) - 1u)) * a.token_stride;
 
-    const uint16_t* weight = is_q ? a.q_weight : a.k_weight;
-    const bool norm = is_v ? a.normalize_v != 0 : weight != nullptr;
-    float ss = 0.0f;
+    float cs[8], sn[8];
+    const double turn = (double)pos * 0.15915494309189535;  // 1 / 2 pi
 #pragma unroll
-    for (int e = 0; e < 16; ++e) ss = __builtin_fmaf(y[e], y[e], ss);
-    for (uint32_t o = L >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, (int)o, 64);
-    if (norm) {
-        const float inv = 1.0f / __builtin_sqrtf(ss / (float)a.dim + a.eps);
+    for (int e = 0; e < 8; ++e) {
+        double t = turn * (double)(e < 4 ? f0[e & 3] : f1[e & 3]);
+        t -= __builtin_rint(t);
+        cs[e] = __builtin_amdgcn_cosf((float)t);
+        sn[e] = __builtin_amdgcn_sinf((float)t);
+    }
+
+    for (uint32_t group = first; group < end; ++group) {
+        const Head t = next;
+        if (group + 1u < end) next = load(group + 1u);
+        const bool is_q = t.head < a.q_heads, is_v = t.head >= a.q_heads + a.kv_heads;
+        float y[16];
+        unpack8(t.x0, y);
+        unpack8(t.x1, y + 8);
+        float ss = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) y[e] *= inv;
-        if (!is_v) {
+        for (int e = 0; e < 16; ++e) ss = __builtin_fmaf(y[e], y[e], ss);
+        for (uint32_t o = L >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, (int)o, 64);
+        if (is_v ? a.normalize_v != 0 : (is_q ? a.q_weight : a.k_weight) != nullptr) {
+            const float inv = 1.0f / __builtin_sqrtf(ss / (float)a.dim + a.eps);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) y[e] *= inv;
+            if (!is_v) {
+                const uint32_t w[8] = {is_q ? qw0.x : kw0.x, is_q ? qw0.y : kw0.y,
+                                       is_q ? qw0.z : kw0.z, is_q ? qw0.w : kw0.w,
+                                       is_q ? qw1.x : kw1.x, is_q ? qw1.y : kw1.y,
+                                       is_q ? qw1.z : kw1.z, is_q ? qw1.w : kw1.w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    y[2 * e] *= __uint_as_float(w[e] << 16);
+                    y[2 * e + 1] *= __uint_as_float(w[e] & 0xFFFF0000u);
+                }
+            }
+        }
+        if (!is_v && turns) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                y[e] *= has0 ? bf16_to_f32(weight[8u * c0 + e]) : 0.0f;
-                y[8 + e] *= has1 ? bf16_to_f32(weight[8u * c1 + e]) : 0.0f;
+                const int i = INTERLEAVED ? 2 * e : e, k = INTERLEAVED ? 2 * e + 1 : e + 8;
+                const float u = y[i], w = y[k];
+                y[i] = u * cs[e] - w * sn[e];
+                y[k] = w * cs[e] + u * sn[e];
             }
         }
-    }
-    if (!is_v && j < half) {
-        const f4a4_t f0 = *reinterpret_cast<const f4a4_t*>(a.inv_freq + 8u * j);
-        const f4a4_t f1 = *reinterpret_cast<const f4a4_t*>(a.inv_freq + 8u * j + 4u);
-        const double turn = (double)pos * 0.15915494309189535;  // 1 / 2 pi
+        if (t.head >= heads) continue;
+        const bool has0 = t.c0 < chunks, has1 = t.c1 < chunks;
+        if (is_q) {
+            if (drop) {
+                const float fill = pos < 0 && !sr.bad ? 0.0f : __builtin_nanf("");
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            double t = turn * (double)(e < 4 ? f0[e & 3] : f1[e & 3]);
-            t -= __builtin_rint(t);
-            const float cs = __builtin_amdgcn_cosf((float)t), sn = __builtin_amdgcn_sinf((float)t);
-            const float u = a.interleaved ? y[2 * e] : y[e];
-            const float w = a.interleaved ? y[2 * e + 1] : y[e + 8];
-            const float ru = u * cs - w * sn, rw = w * cs + u * sn;
-            if (a.interleaved) {
-                y[2 * e] = ru;
-                y[2 * e + 1] = rw;
+                for (int e = 0; e < 16; ++e) y[e] = fill;
+            }
+            uint16_t* dst = a.q_out + (uint64_t)row * a.q_out_stride + t.head * a.dim;
+            if (has0) *reinterpret_cast<uint4*>(dst + 8u * t.c0) = pack8_f16(y);
+            if (has1) *reinterpret_cast<uint4*>(dst + 8u * t.c1) = pack8_f16(y + 8);
+        } else if (!drop) {
+            const uint32_t kvh = is_v ? t.head - a.q_heads - a.kv_heads : t.head - a.q_heads;
+            uint8_t* dst = (is_v ? a.v_pages : a.k_pages) + slot + kvh * a.head_stride;
+            if (E4M3) {
+                const float inv_scale = is_v ? a.v_inv_scale : a.k_inv_scale;
+                if (has0) *reinterpret_cast<uint2*>(dst + 8u * t.c0) = pack8_e4m3(y, inv_scale);
+                if (has1) *reinterpret_cast<uint2*>(dst + 8u * t.c1) = pack8_e4m3(y + 8, inv_scale);
             } else {
-                y[e] = ru;
-                y[e + 8] = rw;
+                if (has0) *reinterpret_cast<uint4*>(dst + 16u * t.c0) = pack8_f16(y);
+                if (has1) *reinterpret_cast<uint4*>(dst + 16u * t.c1) = pack8_f16(y + 8);
             }
         }
-    }
-    if (is_q) {
-        if (drop) {
-            const float fill = pos < 0 && !sr.bad ? 0.0f : __builtin_nanf("");
-#pragma unroll
-            for (int e = 0; e < 16; ++e) y[e] = fill;
-        }
-        uint16_t* dst = a.q_out + (uint64_t)row * a.q_out_stride + head * a.dim;
-        if (has0) *reinterpret_cast<uint4*>(dst + 8u * c0) = pack8_f16(y);
-        if (has1) *reinterpret_cast<uint4*>(dst + 8u * c1) = pack8_f16(y + 8);
-        return;
-    }
-    if (drop) return;
-    uint8_t* dst = (is_v ? a.v_pages : a.k_pages) + page * a.page_stride + kvh * a.head_stride +
-                   (uint64_t)((uint32_t)pos & ((1u << a.page_shift) - 1u)) * a.token_stride;
-    if (E4M3) {
-        const float inv_scale = is_v ? a.v_inv_scale : a.k_inv_scale;
-        if (has0) *reinterpret_cast<uint2*>(dst + 8u * c0) = pack8_e4m3(y, inv_scale);
-        if (has1) *reinterpret_cast<uint2*>(dst + 8u * c1) = pack8_e4m3(y + 8, inv_scale);
-    } else {
-        if (has0) *reinterpret_cast<uint4*>(dst + 16u * c0) = pack8_f16(y);
-        if (has1) *reinterpret_cast<uint4*>(dst + 16u * c1) = pack8_f16(y + 8);
     }
 }
 
@@ -448,11 +488,16 @@ extern "C" tsg_status tsg_attn_append(tsg_attn* attn, tsg_stream stream, const t
     a.dim = c.head_dim;
     a.page_shift = attn->page_shift;
     a.rot = nr->rotary_dim;
-    a.interleaved = nr->interleaved ? 1u : 0u;
+    a.weights16 = is16(nr->q_weight) && is16(nr->k_weight) ? 1u : 0u;
     a.normalize_v = nr->normalize_v ? 1u : 0u;
     while ((16u << a.lanes_log2) < c.head_dim) ++a.lanes_log2;
     const uint32_t heads = c.q_heads + 2u * c.kv_heads, per_wave = 64u >> a.lanes_log2;
-    a.waves_per_row = (heads + per_wave - 1u) / per_wave;
+    // A wave takes all of a row (its sequence, page and angles found once) when
+    // the rows alone give every SIMD eight waves; few rows spread out.
+    const uint32_t groups = (heads + per_wave - 1u) / per_wave;
+    const uint32_t spread = 32u * (uint32_t)attn->ctx->num_cus / a.rows;
+    a.groups = spread >= groups ? 1u : groups / (spread > 1u ? spread : 1u);
+    a.waves_per_row = (groups + a.groups - 1u) / a.groups;
     a.eps = nr->eps;
     a.k_inv_scale = 1.0f / c.k_scale;
     a.v_inv_scale = 1.0f / c.v_scale;
@@ -461,10 +506,10 @@ extern "C" tsg_status tsg_attn_append(tsg_attn* attn, tsg_stream stream, const t
     const uint64_t waves = (uint64_t)a.rows * a.waves_per_row;
     TSG_REQUIRE(waves <= 0x7fffffffu, TSG_ERR_UNSUPPORTED, "too many rows and heads for one launch");
     const dim3 grid((uint32_t)((waves + 3u) / 4u));
-    if (c.kv_type == TSG_KV_E4M3)
-        hipLaunchKernelGGL(append_kernel<true>, grid, dim3(256), 0, as_stream(stream), a);
-    else
-        hipLaunchKernelGGL(append_kernel<false>, grid, dim3(256), 0, as_stream(stream), a);
+    const bool e4m3 = c.kv_type == TSG_KV_E4M3;
+    const auto kernel = nr->interleaved ? (e4m3 ? append_kernel<true, true> : append_kernel<false, true>)
+                                        : (e4m3 ? append_kernel<true, false> : append_kernel<false, false>);
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, as_stream(stream), a);
     return check_launch("attn_append");
 }
 
