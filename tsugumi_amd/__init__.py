@@ -93,13 +93,19 @@ def _stream(stream) -> int | None:
     return _current_stream()
 
 
+_raw_stream = None
+
+
 def _current_stream_of(device: int) -> int:
     """torch's current stream on `device`, which need not be the current one."""
-    import torch
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    if raw is not None and torch.cuda.is_initialized():
-        return raw(device)
-    return torch.cuda.current_stream(device).cuda_stream
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+        if not torch.cuda.is_initialized():
+            torch.cuda.init()
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return _raw_stream(device)
 
 
 def _np_ptr(a: np.ndarray):
@@ -919,7 +925,10 @@ class HeadNormRope:
         for t, types in ((q_weight, bits), (k_weight, bits), (inv_freq, _types("float32"))):
             if t is not None and (t.dim() != 1 or t.dtype not in types):
                 _refuse("norm weights are bf16 [head_dim], inv_freq is fp32 [rotary_dim / 2]")
-        self.widths = {int(t.shape[0]) for t in (q_weight, k_weight) if t is not None}
+        widths = {int(t.shape[0]) for t in (q_weight, k_weight) if t is not None}
+        if len(widths) > 1:
+            _refuse("norm weights of two lengths")
+        self.width = widths.pop() if widths else None
         self._keep = (q_weight, k_weight, inv_freq)
         self.norm_rope = _abi.AttnNormRope(
             _ptr(q_weight), _ptr(k_weight), _ptr(inv_freq),
@@ -951,8 +960,11 @@ class Attention:
         h = C.c_void_p()
         check(self.lib.tsg_attn_create(ctx.handle, C.addressof(self.config), C.byref(h)))
         self.handle = h
-        self._half = _types("float16", "int16", "uint16")
-        self._q_width, self._kv_width = q_heads * head_dim, kv_heads * head_dim
+        # what the calls look at each time
+        self._half, self._device = _types("float16", "int16", "uint16"), ctx.device
+        self._layout = (q_heads, kv_heads, head_dim, q_heads * head_dim, kv_heads * head_dim)
+        self._append, self._decode, self._prefill = (
+            self.lib.tsg_attn_append, self.lib.tsg_attn_decode, self.lib.tsg_attn_prefill)
 
     def cache(self, k, v) -> PagedKVCache:
         return PagedKVCache(self, k, v)
@@ -963,50 +975,55 @@ class Attention:
     def _rows(self, t, rows: int, heads: int, width: int):
         """Address and row stride of a row operand."""
         shape, strides = t.shape, t.stride()
-        if t.dtype not in self._half or not t.is_cuda or t.get_device() != self.ctx.device:
-            _refuse("row operands must be fp16 tensors on the context's device")
         if len(shape) == 2:
             fits = shape[1] == width and strides[1] == 1
         else:
-            fits = (len(shape) == 3 and shape[1] == heads and shape[1] * shape[2] == width
+            fits = (len(shape) == 3 and shape[1] == heads and heads * shape[2] == width
                     and strides[2] == 1 and (heads == 1 or strides[1] == shape[2]))
-        if not fits or shape[0] < rows:
+        n = shape[0] if fits else 0
+        if n < rows:
             _refuse(f"row operand of shape {tuple(shape)}, strides {strides}: not {rows} rows of "
                     f"{width}")
-        return t.data_ptr(), strides[0] if shape[0] > 1 else width
+        if t.dtype not in self._half or t.get_device() != self._device:
+            _refuse("row operands must be fp16 tensors on the context's device")
+        return t.data_ptr(), strides[0] if n > 1 else width
 
     def _on(self, stream):
         if stream is not None:
             return stream if isinstance(stream, int) else stream.cuda_stream
-        return _current_stream_of(self.ctx.device)
+        return _current_stream_of(self._device)
 
     def encode_append(self, cache, batch, q, k, v, norm_rope, q_out, stream=None):
         """Norms, rotation and cache write of the batch's rows; q_out gets the
         query heads (it may be q)."""
-        c, n = self.config, batch.rows
-        if norm_rope.widths - {c.head_dim}:
+        n, hq, hk, dim, q_width, kv_width = batch.rows, *self._layout
+        if norm_rope.width is not None and norm_rope.width != dim:
             _refuse("norm weights must be [head_dim]")
-        q, qs = self._rows(q, n, c.q_heads, self._q_width)
-        k, ks = self._rows(k, n, c.kv_heads, self._kv_width)
-        v, vs = self._rows(v, n, c.kv_heads, self._kv_width)
-        out, os = self._rows(q_out, n, c.q_heads, self._q_width)
+        q, qs = self._rows(q, n, hq, q_width)
+        k, ks = self._rows(k, n, hk, kv_width)
+        v, vs = self._rows(v, n, hk, kv_width)
+        out, os = self._rows(q_out, n, hq, q_width)
         rows = _abi.AttnRows(q, k, v, qs, ks, vs)
-        check(self.lib.tsg_attn_append(self.handle, self._on(stream), cache._ref, batch._ref,
-                                       C.addressof(rows), norm_rope._ref, out, os))
+        status = self._append(self.handle, self._on(stream), cache._ref, batch._ref,
+                              C.addressof(rows), norm_rope._ref, out, os)
+        if status:
+            check(status)
 
     def _attend(self, call, cache, batch, q, out, stream):
-        c, n = self.config, batch.rows
-        q, qs = self._rows(q, n, c.q_heads, self._q_width)
-        out, os = self._rows(out, n, c.q_heads, self._q_width)
-        check(call(self.handle, self._on(stream), cache._ref, batch._ref, q, qs, out, os))
+        n, hq, _, _, width, _ = batch.rows, *self._layout
+        q, qs = self._rows(q, n, hq, width)
+        out, os = self._rows(out, n, hq, width)
+        status = call(self.handle, self._on(stream), cache._ref, batch._ref, q, qs, out, os)
+        if status:
+            check(status)
 
     def encode_decode(self, cache, batch, q, out, stream=None):
         """Attention of 1..8 new tokens of every sequence."""
-        self._attend(self.lib.tsg_attn_decode, cache, batch, q, out, stream)
+        self._attend(self._decode, cache, batch, q, out, stream)
 
     def encode_prefill(self, cache, batch, q, out, stream=None):
         """Attention of a prompt's rows, or of the next chunk of one."""
-        self._attend(self.lib.tsg_attn_prefill, cache, batch, q, out, stream)
+        self._attend(self._prefill, cache, batch, q, out, stream)
 
     def close(self) -> None:
         if getattr(self, "handle", None) and getattr(self.ctx, "handle", None):
