@@ -476,16 +476,18 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
     const auto slot_of = [&](uint32_t split) {  // its place among the partial sums
         return ((uint64_t)(run.slot + split) * a.kv_heads + kvh) * p.row_tiles + rt;
     };
-    const auto emit = [&](uint32_t r, uint32_t c, const float* acc, float sum) {
+    const auto out_at = [&](uint32_t r, uint32_t c) {
+        const uint32_t t = (r0 + r) / a.group;
+        return a.out + (uint64_t)(sr.first + t) * a.out_stride +
+               (uint64_t)(kvh * a.group + (r0 + r - t * a.group)) * a.dim + 8u * c;
+    };
+    const auto emit = [&](uint16_t* out, const float* acc, float sum) {
         const float inv = sum == 0.0f ? 0.0f : a.v_scale / sum;
         uint32_t h[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             h[e] = (uint32_t)f32_to_f16(acc[2 * e] * inv) |
                    ((uint32_t)f32_to_f16(acc[2 * e + 1] * inv) << 16);
-        const uint32_t t = (r0 + r) / a.group;
-        uint16_t* out = a.out + (uint64_t)(sr.first + t) * a.out_stride +
-                        (uint64_t)(kvh * a.group + (r0 + r) % a.group) * a.dim + 8u * c;
         *reinterpret_cast<uint4*>(out) = make_uint4(h[0], h[1], h[2], h[3]);
     };
 #pragma unroll 1
@@ -515,7 +517,7 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
             }
         }
         if (used == 1u) {
-            emit(r, c, acc, sum);
+            emit(out_at(r, c), acc, sum);
         } else {
             const uint64_t slot = slot_of(run.split) * 16u + r;
             float* dst = p.part_o + slot * DP + 8u * c;
@@ -533,83 +535,78 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
     if (used == 1u) return;
 
     // The last workgroup of the sequence, head and row tile to arrive joins the
-    // splits: `ways` threads share an 8-element piece, each adds up every
-    // ways-th split, in order, from loads that all go out at once; their sums
-    // are added in LDS.
-    wait_vector_memory();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        uint32_t* count = p.arrivals + slot_of(0);
-        const uint32_t before =
-            __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        *flag = before == used - 1u ? 1u : 0u;
-        if (before == used - 1u) st_coherent(count, 0u);
-    }
-    __syncthreads();
-    if (!*flag) return;
+    // splits: `ways` neighbouring lanes share an 8-element piece, each adds up
+    // every ways-th split, in order, four at a time from loads that go out
+    // together; then the lanes' sums are added in a fixed order.
     const uint32_t pieces = live * C8;
-    uint32_t ways_log2 = 0;
+    uint32_t ways_log2 = 0;  // at most 5: a row has at least eight pieces
     while ((pieces << (ways_log2 + 1u)) <= 256u && (2u << ways_log2) <= used) ++ways_log2;
-    const uint32_t ways = 1u << ways_log2;
-    float* sums = reinterpret_cast<float*>(smem);  // [way][piece][10]
-    const uint64_t step = (uint64_t)a.kv_heads * p.row_tiles * 16u;
+    const uint32_t ways = 1u << ways_log2, way = threadIdx.x & (ways - 1u);
+    const uint32_t slot0 = (uint32_t)slot_of(0);
+    wait_vector_memory();
+    lds_barrier();
+    if (threadIdx.x == 0) {
+        const uint32_t before = __hip_atomic_fetch_add(p.arrivals + slot0, 1u, __ATOMIC_RELAXED,
+                                                       __HIP_MEMORY_SCOPE_AGENT);
+        *flag = before == used - 1u ? 1u : 0u;
+    }
+    lds_barrier();
+    if (!*flag) return;
+    const uint32_t step = a.kv_heads * p.row_tiles * 16u;
 #pragma unroll 1
     for (uint32_t n = 0; n < pieces; n += 256u >> ways_log2) {
-        const uint32_t piece = n + (threadIdx.x >> ways_log2), way = threadIdx.x & (ways - 1u);
-        const uint32_t r = piece / C8, c = piece % C8;
+        const uint32_t piece = n + (threadIdx.x >> ways_log2), r = piece / C8, c = piece % C8;
         const bool in = piece < pieces && 8u * c < a.dim;
         float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0.0f, mm = kNoKey;
-        const uint64_t first = slot_of(0) * 16u + r;
-        for (uint32_t w0 = way; in && w0 < used; w0 += 4u * ways) {
+        uint32_t at = slot0 * 16u + (in ? r : 0u) + way * step;  // the scratch is under 4 GiB
+#pragma unroll 1
+        for (uint32_t w0 = way; w0 < used; w0 += 4u * ways, at += 4u * ways * step) {
             uint4 lo[4], hi[4];
             uint64_t ml[4];
 #pragma unroll
             for (uint32_t k = 0; k < 4u; ++k) {
-                const uint32_t w = w0 + k * ways < used ? w0 + k * ways : w0;
-                const uint64_t at = first + w * step;
-                ml[k] = ld_coherent(reinterpret_cast<const uint64_t*>(p.part_ml) + at);
-                lo[k] = ld_coherent16(p.part_o + at * DP + 8u * c);
-                hi[k] = ld_coherent16(p.part_o + at * DP + 8u * c + 4u);
+                const uint32_t at_k = w0 + k * ways < used ? at + k * ways * step : at;
+                const uint32_t byte = (at_k * (uint32_t)DP + 8u * c) * 4u;
+                ml[k] = ld_coherent(reinterpret_cast<const uint64_t*>(
+                    reinterpret_cast<const uint8_t*>(p.part_ml) + at_k * 8u));
+                lo[k] = ld_coherent16(reinterpret_cast<const uint8_t*>(p.part_o) + byte);
+                hi[k] = ld_coherent16(reinterpret_cast<const uint8_t*>(p.part_o) + byte + 16u);
             }
+            float mk[4], mn = mm;
 #pragma unroll
             for (uint32_t k = 0; k < 4u; ++k) {
-                if (w0 + k * ways >= used) continue;
-                const float mk = __uint_as_float((uint32_t)ml[k]);
-                const float mn = fmaxf(mm, mk);
-                const float f0 = __builtin_amdgcn_exp2f(mm - mn);
-                const float f1 = __builtin_amdgcn_exp2f(mk - mn);
-                mm = mn;
-                sum = sum * f0 + __uint_as_float((uint32_t)(ml[k] >> 32)) * f1;
+                mk[k] = __uint_as_float((uint32_t)ml[k]);
+                mn = fmaxf(mn, mk[k]);
+            }
+            const float f0 = __builtin_amdgcn_exp2f(mm - mn);
+            mm = mn;
+            sum *= f0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] *= f0;
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k) {
+                const bool have = w0 + k * ways < used;
+                const float f = have ? __builtin_amdgcn_exp2f(mk[k] - mn) : 0.0f;
                 const uint32_t u[8] = {lo[k].x, lo[k].y, lo[k].z, lo[k].w,
                                        hi[k].x, hi[k].y, hi[k].z, hi[k].w};
+                if (have) {
+                    sum += __uint_as_float((uint32_t)(ml[k] >> 32)) * f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) acc[e] = acc[e] * f0 + __uint_as_float(u[e]) * f1;
-            }
-        }
-        if (ways > 1u) {
-            float* mine = sums + threadIdx.x * 10u;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) mine[e] = acc[e];
-            mine[8] = sum;
-            mine[9] = mm;
-            __syncthreads();
-            if (in && way == 0u) {
-                for (uint32_t w = 1; w < ways; ++w) mm = fmaxf(mm, mine[w * 10u + 9u]);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
-                sum = 0.0f;
-                for (uint32_t w = 0; w < ways; ++w) {
-                    const float* part = mine + w * 10u;
-                    const float f = __builtin_amdgcn_exp2f(part[9] - mm);
-                    sum += part[8] * f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) acc[e] += part[e] * f;
+                    for (int e = 0; e < 8; ++e) acc[e] += __uint_as_float(u[e]) * f;
                 }
             }
-            __syncthreads();
         }
-        if (in && way == 0u) emit(r, c, acc, sum);
+        for (uint32_t o = 1; o < ways; o <<= 1) {
+            const float m2 = __shfl_xor(mm, (int)o, 64), mn = fmaxf(mm, m2);
+            const float f0 = __builtin_amdgcn_exp2f(mm - mn), f1 = __builtin_amdgcn_exp2f(m2 - mn);
+            mm = mn;
+            sum = sum * f0 + __shfl_xor(sum, (int)o, 64) * f1;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] = acc[e] * f0 + __shfl_xor(acc[e], (int)o, 64) * f1;
+        }
+        if (in && way == 0u) emit(out_at(r, c), acc, sum);
     }
+    if (threadIdx.x == 0) st_coherent(p.arrivals + slot0, 0u);  // for the next call
 }
 
 typedef void (*DecodeKernel)(DecodeArgs);
