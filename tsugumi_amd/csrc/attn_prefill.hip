@@ -380,7 +380,12 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
         bool found = false;
 #pragma unroll 1
         for (uint32_t c = threadIdx.x; c < TK * CPR; c += THREADS) {
-            const uint4 v = *reinterpret_cast<const uint4*>(vb + 16u * c);
+            uint4* at = reinterpret_cast<uint4*>(vb + 16u * c);
+            if (!keys_seen<1>(key0 + c / CPR, t.p_lo, t.p_hi, a.window, a.sinks)) {
+                *at = make_uint4(0, 0, 0, 0);  // no row's: it may hold anything
+                continue;
+            }
+            const uint4 v = *at;
             found = found || (not_finite<false>(v.x) | not_finite<false>(v.y) |
                               not_finite<false>(v.z) | not_finite<false>(v.w)) != 0u;
         }
@@ -397,7 +402,6 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
             if ((bits & 0x7C00u) != 0x7C00u) continue;
             *v = 0;
             const uint32_t k = n / DP, e = n % DP;
-            if (!keys_seen<1>(key0 + k, t.p_lo, t.p_hi, a.window, a.sinks)) continue;
             const uint32_t dim = 8u * ((e / 8u) ^ value_swizzle(k)) + e % 8u;
             const uint32_t mark = (bits & 0x3FFu ? 3u : bits & 0x8000u ? 2u : 1u) << (2u * (dim & 15u));
 #pragma unroll 1
@@ -505,10 +509,12 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
     }
 }
 
-// Adds up the splits' sums of a row tile, kJoinRows rows a workgroup, 8
-// elements a thread.
+// Adds up the splits' sums of a row tile, kJoinRows rows a workgroup: `ways`
+// neighbouring lanes share an 8-element piece, each takes every ways-th split,
+// in order, from loads that go out together.
 template <int DP>
 __global__ __launch_bounds__(256) void prefill_join_kernel(PrefillArgs p) {
+    constexpr uint32_t C8 = DP / 8u, PIECES = kJoinRows * C8;
     const AttnArgs& a = p.a;
     const uint32_t kvh = blockIdx.x % a.kv_heads;
     RowTile rt;
@@ -516,32 +522,38 @@ __global__ __launch_bounds__(256) void prefill_join_kernel(PrefillArgs p) {
     const SeqRows sr = seq_rows(a.row_starts, a.lengths, rt.seq, a.seq_rows, a.rows,
                                 a.table_stride << a.page_shift);
     const TilePlan<DP> t = tile_plan<DP>(p, sr, rt.tile);
-    if (t.used == 1u) return;
-    for (uint32_t n = threadIdx.x; n < kJoinRows * (DP / 8u); n += 256u) {
-        const uint32_t r = blockIdx.y * kJoinRows + n / (DP / 8u), c = n % (DP / 8u);
-        if (r >= t.live || 8u * c >= a.dim) continue;
-        const uint64_t slot = (uint64_t)blockIdx.x * p.splits * kRows + r;
-        float m = kNoKey;
-        for (uint32_t w = 0; w < t.used; ++w)
-            m = fmaxf(m, p.part_ml[(slot + (uint64_t)w * kRows) * 2u]);
-        float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0.0f;
+    if (t.used == 1u || blockIdx.y * kJoinRows >= t.live) return;
+    uint32_t ways = 1u;
+    while (ways < t.used && 2u * ways * PIECES <= 256u) ways *= 2u;
+    const uint32_t way = threadIdx.x & (ways - 1u);
+    for (uint32_t n = 0; n < PIECES; n += 256u / ways) {
+        const uint32_t piece = n + threadIdx.x / ways;
+        const uint32_t r = blockIdx.y * kJoinRows + piece / C8, c = piece % C8;
+        const bool in = piece < PIECES && r < t.live && 8u * c < a.dim;
+        const uint64_t slot = (uint64_t)blockIdx.x * p.splits * kRows + (in ? r : 0u);
+        float m = kNoKey, acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0.0f;
 #pragma unroll 4
-        for (uint32_t w = 0; w < t.used; ++w) {
+        for (uint32_t w = way; w < t.used; w += ways) {
             const uint64_t at = slot + (uint64_t)w * kRows;
             const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2u);
-            const float f = __builtin_amdgcn_exp2f(ml.x - m);
-            sum += ml.y * f;
-            const float4* src = reinterpret_cast<const float4*>(p.part_o + at * DP + 8u * c);
-            const float4 lo = src[0], hi = src[1];
-            acc[0] += lo.x * f;
-            acc[1] += lo.y * f;
-            acc[2] += lo.z * f;
-            acc[3] += lo.w * f;
-            acc[4] += hi.x * f;
-            acc[5] += hi.y * f;
-            acc[6] += hi.z * f;
-            acc[7] += hi.w * f;
+            const f4_t* src = reinterpret_cast<const f4_t*>(p.part_o + at * DP + 8u * c);
+            const f4_t lo = src[0], hi = src[1];
+            const float mn = fmaxf(m, ml.x);
+            const float f0 = __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(ml.x - mn);
+            m = mn;
+            sum = sum * f0 + ml.y * f1;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] = acc[e] * f0 + (e < 4 ? lo[e & 3] : hi[e & 3]) * f1;
         }
+        for (uint32_t o = 1; o < ways; o <<= 1) {
+            const float m2 = __shfl_xor(m, (int)o, 64), mn = fmaxf(m, m2);
+            const float f0 = __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(m2 - mn);
+            m = mn;
+            sum = sum * f0 + __shfl_xor(sum, (int)o, 64) * f1;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] = acc[e] * f0 + __shfl_xor(acc[e], (int)o, 64) * f1;
+        }
+        if (!in || way != 0u) continue;
         const float inv = sum == 0.0f ? 0.0f : a.v_scale / sum;
         uint32_t u[4];
 #pragma unroll
@@ -605,7 +617,7 @@ tsg_status launch_prefill(const tsg_attn* attn, const AttnArgs& a, tsg_stream st
     TSG_REQUIRE(blocks <= 0x7fffffffu, TSG_ERR_UNSUPPORTED, "too many rows and heads for one launch");
     const uint64_t capacity_tiles =
         (((uint64_t)a.table_stride << a.page_shift) + v.tile_keys - 1u) / v.tile_keys;
-    p.min_tiles = 2u;
+    p.min_tiles = 4u;
     const uint64_t resident = 2u * (uint64_t)attn->ctx->num_cus * 256u / v.threads;
     uint64_t splits = 2u * resident / blocks;
     splits = std::min(splits, (capacity_tiles + p.min_tiles - 1u) / p.min_tiles);
