@@ -769,8 +769,10 @@ typedef struct tsg_attn tsg_attn; /* one kind of attention layer and its scratch
  * (pages and batch may be NULL: not checked). */
 tsg_status tsg_attn_check(const tsg_attn_config* config, const tsg_kv_pages* pages,
                           const tsg_attn_batch* batch);
-/* Calls on one tsg_attn run in stream order (they share its scratch); two
- * tsg_attn may run beside each other. Destroyed before its context. */
+/* Calls on one tsg_attn run in stream order (they share its scratch: 17, 34, 68 or
+ * 135 MB for head sizes up to 64, 128, 256, 512); two tsg_attn may run beside each
+ * other. Not while a stream is captured (it allocates). The context outlives
+ * the calls. */
 tsg_status tsg_attn_create(tsg_ctx* ctx, const tsg_attn_config* config, tsg_attn** out);
 void tsg_attn_destroy(tsg_attn* attn);
 
@@ -790,8 +792,8 @@ tsg_status tsg_attn_append(tsg_attn* attn, tsg_stream stream, const tsg_kv_pages
  * every sequence (a decoded token, a speculative block). What lies in the
  * cache at keys a row does not see, NaN and infinities among it, does not
  * reach the row. Returns TSG_ERR_DECLINED for more than 8 rows a sequence;
- * row_starts must be NULL. q and out rows on 16 bytes; out must not share an
- * element with q. */
+ * row_starts must be NULL. q and out rows on 16 bytes; out may be q itself (same
+ * address and stride) and otherwise shares no element with it. */
 tsg_status tsg_attn_decode(tsg_attn* attn, tsg_stream stream, const tsg_kv_pages* pages,
                            const tsg_attn_batch* batch, const uint16_t* q, uint32_t q_stride,
                            uint16_t* out, uint32_t out_stride);

@@ -348,6 +348,85 @@ def test_bad_row_starts_are_reported(tsg, ctx, starts):
     assert e.value.status == 1 and "row starts" in str(e.value)
 
 
+# ------------------------------------------------- larger batches, refusals
+
+@pytest.mark.parametrize("seqs,rows", [(70, 1), (130, 3), (256, 1), (300, 1)])
+def test_decode_many_sequences(tsg, ctx, seqs, rows):
+    """Runs found over several scans of the lengths, and (past 256) one run a sequence."""
+    rng = np.random.default_rng(seqs)
+    lengths = np.where(rng.random(seqs) < 0.1, rng.integers(rows, 900, seqs),
+                       rng.integers(0, 60, seqs))
+    lengths = np.maximum(lengths, np.where(rng.random(seqs) < 0.05, 0, rows)).tolist()
+    check_attention(tsg, ctx, Case([rows] * seqs, lengths, 6, 2, 32, seed=seqs), "decode")
+
+
+def test_decode_rows_past_one_tile_over_splits(tsg, ctx):
+    """Eight rows of groups of five: three row tiles of each head, split and joined."""
+    c = Case([8] * 3, [3000, 40, 1500], 10, 2, 256, seed=50, window=2500, sinks=3)
+    check_attention(tsg, ctx, c, "decode")
+
+
+def test_prefill_ragged_splits_with_window(tsg, ctx):
+    c = Case([12, 3, 40, 0, 1], [5000, 900, 2100, 9, 1], 6, 2, 64, page=32, window=1800, sinks=5,
+             seed=51, spare=4)
+    check_attention(tsg, ctx, c, "prefill")
+
+
+@pytest.mark.parametrize("dim", [256, 512])
+def test_prefill_wide_heads_over_splits(tsg, ctx, dim):
+    check_attention(tsg, ctx, Case([33], [1500], 4, 1, dim, seed=dim), "prefill")
+
+
+@pytest.mark.parametrize("op,lengths", [("decode", [50, 3000]), ("prefill", [50, 3000])])
+def test_in_place(tsg, ctx, op, lengths):
+    c = Case([3, 3], lengths, 8, 2, 128, seed=52)
+    d = c.to_device()
+    launch(tsg, ctx, c, op, d=d, out=d["q"])
+    ctx.synchronize()
+    want, tol = c.attention()
+    assert_near(d["q"], want, tol, op)
+
+
+def test_call_refusals(tsg, ctx):
+    """Nothing is launched: the outputs keep their marks."""
+    c = Case([9, 9], [30, 40], 4, 2, 64, seed=53)
+    d = c.to_device()
+    attn = plan(tsg, ctx, c)
+    cache = attn.cache(d["k"], d["v"])
+    uniform = attn.batch(d["table"], d["lengths"], 18)
+    ragged = attn.batch(d["table"], d["lengths"], 18, d["starts"])
+    out = torch.full_like(d["q"], -77.0)
+
+    def refused(status, call, *args):
+        with pytest.raises(tsg.TsgError) as e:
+            call(*args)
+        assert e.value.status == status
+
+    refused(4, attn.encode_decode, cache, uniform, d["q"], out)  # nine rows: declined
+    refused(1, attn.encode_decode, cache, ragged, d["q"], out)
+    refused(1, attn.encode_prefill, cache, ragged, d["q"][:5], out)
+    refused(1, attn.encode_prefill, cache, ragged, d["q"].float(), out)
+    refused(1, attn.encode_prefill, cache, ragged, d["q"].cpu(), out)
+    refused(1, attn.encode_prefill, cache, ragged, d["q"].transpose(1, 2), out)
+    off = torch.zeros(18 * 256 + 8, dtype=torch.float16, device="cuda")[2:18 * 256 + 2].view(18, 256)
+    refused(2, attn.encode_prefill, cache, ragged, off, out)
+    refused(2, attn.encode_prefill, cache, ragged, d["q"], off)
+    rope = tsg.HeadNormRope(inv_freq=torch.ones(20, device="cuda"))
+    kv = torch.zeros(18, 2, 64, dtype=torch.float16, device="cuda")
+    refused(3, attn.encode_append, cache, ragged, d["q"], kv, kv, rope, out)  # 40 of 64
+    wide = tsg.HeadNormRope(torch.ones(32, device="cuda").bfloat16())
+    refused(1, attn.encode_append, cache, ragged, d["q"], kv, kv, wide, out)
+    refused(1, tsg.HeadNormRope, torch.ones(64, device="cuda"))
+    refused(1, attn.cache, d["k"], d["v"].float())
+    refused(1, attn.cache, d["k"][:, :1], d["v"][:, :1])
+    refused(1, attn.batch, d["table"], d["lengths"].long(), 18)
+    refused(1, attn.batch, d["table"], d["lengths"], 17)
+    refused(1, tsg.Attention, ctx, 4, 2, 64, 16, "f32")
+    refused(3, tsg.Attention, ctx, 4, 2, 60, 16)
+    ctx.synchronize()
+    assert bool((out == -77).all())
+
+
 # -------------------------------------------------------------------- append
 
 def append_case(tsg, ctx, c, rot, interleaved=False, normalize_v=False, weights=True, seed=0,

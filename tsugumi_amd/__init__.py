@@ -1026,9 +1026,9 @@ class Attention:
         self._attend(self._prefill, cache, batch, q, out, stream)
 
     def close(self) -> None:
-        if getattr(self, "handle", None) and getattr(self.ctx, "handle", None):
+        if getattr(self, "handle", None):
             self.lib.tsg_attn_destroy(self.handle)
-        self.handle = None
+            self.handle = None
 
     def __del__(self):
         try:

@@ -6,6 +6,7 @@
 
 struct tsg_attn {
     tsg_ctx* ctx = nullptr;
+    int device = 0;  // the context's
     tsg_attn_config cfg{};
     uint32_t group = 0;       // query heads a key head serves
     uint32_t page_shift = 0;  // log2(page_tokens)
@@ -269,6 +270,8 @@ struct DeviceScope {
         if (before >= 0) (void)hipSetDevice(before);
     }
 };
+
+constexpr uint64_t kMaxBlocks = (1u << 24) - 1u;  // 256 threads each, under 2^32 in all
 
 // The argument checks every entry point makes, without a device (attn.hip).
 tsg_status check_attn_config(const tsg_attn_config* c);
