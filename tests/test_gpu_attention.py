@@ -238,6 +238,16 @@ def test_prefill_uniform_equals_ragged(tsg, ctx):
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("kv", ["f16", "e4m3"])
+@pytest.mark.parametrize("dim,heads,rows", [(256, (4, 2), 1), (256, (4, 2), 32), (256, (4, 2), 33),
+                                            (512, (8, 1), 31), (512, (8, 1), 33), (272, (2, 1), 128),
+                                            (272, (2, 1), 130)])
+def test_prefill_uniform_few_rows_of_wide_heads(tsg, ctx, dim, heads, rows, kv):
+    """On both sides of the sizes at which the kernels change."""
+    c = Case([rows] * 2, [rows + 300, rows], *heads, dim, kv=kv, window=170, sinks=3, seed=rows)
+    check_attention(tsg, ctx, c, "prefill", uniform=True)
+
+
 def test_prefill_few_rows_over_a_long_cache(tsg, ctx):
     c = Case([12], [9001], 8, 2, 64, page=64, seed=9)
     check_attention(tsg, ctx, c, "prefill")

@@ -34,10 +34,12 @@ struct DecodeArgs {
     uint32_t chunks;     // runs of keys wanted, a head and row tile; 0: one a sequence
     uint32_t row_tiles;  // 16-row tiles of a sequence's rows and group
     uint32_t pairs;      // key heads * (most runs there can be)
+    float join_cost;     // of a split in the join, against a tile's of its run
 };
 
 constexpr uint32_t kMinTiles = kWaves;  // key tiles worth a workgroup: one a wave
 constexpr uint32_t kMaxSplits = 128;    // partial sums one workgroup joins
+constexpr uint32_t kJoinLoads = 4;      // splits whose loads go out together
 constexpr uint32_t kMaxBalanced = 256;  // sequences of a batch with runs of one length
 
 // The run of key tiles that workgroup `at` (of a head and row tile) takes. All
@@ -64,8 +66,14 @@ __device__ __forceinline__ bool find_run(const DecodeArgs& p, uint32_t at, Run* 
         const uint32_t n = (tiles + per - 1u) / per;
         return n > 1u ? n : 1u;
     };
-    const auto run_length = [](uint32_t tiles, uint32_t per) {  // of one sequence
-        const uint32_t least = (tiles + kMaxSplits - 1u) / kMaxSplits;
+    // Of one sequence: a longer run takes longer, more runs are longer to join;
+    // runs of r tiles and tiles / r splits cost the least together at r =
+    // sqrt(tiles * join_cost). (4000 keys, 16 rows of 128: 30 us with 63 runs of
+    // 4 tiles, 17 with longer ones; 32,000 keys 63 and 43.)
+    const auto run_length = [&](uint32_t tiles, uint32_t per) {
+        const uint32_t cap = (tiles + kMaxSplits - 1u) / kMaxSplits;
+        const uint32_t even = (uint32_t)__builtin_sqrtf((float)tiles * p.join_cost) + 1u;
+        const uint32_t least = cap > even ? cap : even;
         return per > least ? per : least;
     };
     if (a.num_seqs == 1u) {
@@ -565,11 +573,11 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
         float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0.0f, mm = kNoKey;
         uint32_t at = slot0 * 16u + (in ? r : 0u) + way * step;  // the scratch is under 4 GiB
 #pragma unroll 1
-        for (uint32_t w0 = way; w0 < used; w0 += 4u * ways, at += 4u * ways * step) {
-            uint4 lo[4], hi[4];
-            uint64_t ml[4];
+        for (uint32_t w0 = way; w0 < used; w0 += kJoinLoads * ways, at += kJoinLoads * ways * step) {
+            uint4 lo[kJoinLoads], hi[kJoinLoads];
+            uint64_t ml[kJoinLoads];
 #pragma unroll
-            for (uint32_t k = 0; k < 4u; ++k) {
+            for (uint32_t k = 0; k < kJoinLoads; ++k) {
                 const uint32_t at_k = w0 + k * ways < used ? at + k * ways * step : at;
                 const uint32_t byte = (at_k * (uint32_t)DP + 8u * c) * 4u;
                 ml[k] = ld_coherent(reinterpret_cast<const uint64_t*>(
@@ -577,9 +585,9 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
                 lo[k] = ld_coherent16(reinterpret_cast<const uint8_t*>(p.part_o) + byte);
                 hi[k] = ld_coherent16(reinterpret_cast<const uint8_t*>(p.part_o) + byte + 16u);
             }
-            float mk[4], mn = mm;
+            float mk[kJoinLoads], mn = mm;
 #pragma unroll
-            for (uint32_t k = 0; k < 4u; ++k) {
+            for (uint32_t k = 0; k < kJoinLoads; ++k) {
                 mk[k] = __uint_as_float((uint32_t)ml[k]);
                 mn = fmaxf(mn, mk[k]);
             }
@@ -589,7 +597,7 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
 #pragma unroll
             for (int e = 0; e < 8; ++e) acc[e] *= f0;
 #pragma unroll
-            for (uint32_t k = 0; k < 4u; ++k) {
+            for (uint32_t k = 0; k < kJoinLoads; ++k) {
                 const bool have = w0 + k * ways < used;
                 const float f = have ? __builtin_amdgcn_exp2f(mk[k] - mn) : 0.0f;
                 const uint32_t u[8] = {lo[k].x, lo[k].y, lo[k].z, lo[k].w,
@@ -666,6 +674,11 @@ tsg_status launch_decode(const tsg_attn* attn, const AttnArgs& a, tsg_stream str
     TSG_REQUIRE(blocks <= kMaxBlocks, TSG_ERR_UNSUPPORTED,
                 "too many sequences and heads for one launch");
     p.pairs = (uint32_t)pairs;
+    // the join's passes over a split's live rows, kJoinLoads splits a pass and way;
+    // a tile of a run is done by one of the four waves
+    const uint32_t pieces =
+        std::min(a.seq_rows * a.group, kDecodeTileRows) * (attn->padded_dim / 8u);
+    p.join_cost = (float)kWaves * (float)pieces / 256.0f / (float)kJoinLoads;
     p.part_o = attn->partials;
     p.part_ml = attn->partials + (uint64_t)kMaxPartials * 16u * attn->padded_dim;
     p.arrivals = attn->arrivals;
