@@ -1,5 +1,5 @@
-// attn_decode.hip — attention of 1..8 new rows of each sequence over the paged
-// cache.
+// attn_decode.hip — attention of a few new rows of each sequence (1..8, or a
+// prefill call's few rows of wide heads) over the paged cache.
 //
 // o = sum_j w_j v_j / sum_j w_j, w_j = exp(scale q.k_j): every key and value is
 // read once and used for the few rows of its head's group, so HBM bounds it
@@ -8,9 +8,10 @@
 //
 // A workgroup takes 16 rows (tokens x heads of one key head's group) and a run
 // of key tiles; its four waves take the tiles in turn, 16 keys each, with no
-// barrier between them: K goes from memory to the first operand's registers, V
-// through the wave's own LDS to be read transposed. The waves' sums are joined
-// in LDS; the workgroups of a split sequence leave partial sums in the plan's
+// barrier between them: K and V go to the wave's own LDS (e4m3: K to the first
+// operand's registers, V through registers), V to be read transposed, and the
+// next tile's K is under way while this one's V is used. The waves' sums are
+// joined in LDS; the workgroups of a split sequence leave partial sums in the plan's
 // scratch, and the last of them to arrive adds those up in the order of the
 // splits, so the result does not depend on which one it is.
 //

@@ -618,7 +618,12 @@ tsg_status launch_prefill(const tsg_attn* attn, const AttnArgs& a, tsg_stream st
                                ? (uint64_t)a.rows * a.group / kRows + std::min(a.num_seqs, a.rows)
                                : (uint64_t)a.num_seqs * p.seq_tiles;
     const uint64_t blocks = tiles * a.kv_heads;
-    TSG_REQUIRE(blocks * (v.threads / 256u) <= kMaxBlocks, TSG_ERR_UNSUPPORTED, "too many rows and heads for one launch");
+    TSG_REQUIRE(blocks * (v.threads / 256u) <= kMaxBlocks, TSG_ERR_UNSUPPORTED,
+                "too many rows and heads for one launch");
+    // Splits where the row tiles are fewer than the workgroups the card holds:
+    // up to twice as many, since a prompt's tiles are uneven (2011 rows of 512-wide
+    // heads in 252 workgroups 167 us, in up to 504 147), of at least four key
+    // tiles (67 rows over 967 keys 24.0 us, of at least two 25.1).
     const uint64_t capacity_tiles =
         (((uint64_t)a.table_stride << a.page_shift) + v.tile_keys - 1u) / v.tile_keys;
     p.min_tiles = 4u;
