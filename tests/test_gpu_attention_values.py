@@ -1,0 +1,75 @@
+"""Attention at the edges of its values' ranges: logits far from zero, rows whose
+result is one value, infinities that some rows see, in every kernel's width."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.attention_ref import Case, assert_near
+from tests.test_gpu_attention import ctx, launch, tsg  # noqa: F401 (fixtures)
+
+pytestmark = pytest.mark.gpu
+
+
+def set_products(c, base, steps):
+    """Queries and keys of small whole numbers with q . k = base + steps[j] for key j of
+    every sequence and head, exact in fp32 in any order (every partial sum is below 2^24)."""
+    half = c.dim // 2
+    c.q[:] = 0
+    c.q[..., :half] = 1024.0
+    c.q[..., half] = 1.0
+    for s, length in enumerate(c.lengths):
+        for t in range(length):
+            i, j = c.slot(s, t)
+            row = torch.zeros(c.dim)
+            row[:half] = base / (1024.0 * half) / c.k_scale
+            row[half] = float(steps[t % len(steps)]) / c.k_scale
+            assert torch.equal(row.to(c.k.dtype).float(), row)
+            c.k[i, :, j] = row.to(c.k.dtype)
+
+
+def products_tolerance(c, out):
+    """Products are exact here, so a weight is off by its rounding to fp16 (half a step, 2^-11),
+    by its exponent (at most 40 powers of two matter; scale log2(e) in fp32 and two roundings of
+    the multiply-add: 3 x 40 x 2^-24, under 2^-16), and by the sums in fp32; the result by its
+    own rounding."""
+    size = torch.zeros_like(out)
+    for s, n in enumerate(c.rows):
+        first = int(c.starts[s])
+        size[first:first + n] = c.tokens("v", s).abs().amax((0, 2))[
+            torch.arange(c.q_heads) // (c.q_heads // c.kv_heads)][:, None]
+    return (2.0 ** -11 * out.abs()
+            + size * (2.0 ** -11 + 2.0 ** -16 + (max(c.lengths) + 64) * 2.0 ** -23) + 2.0 ** -24)
+
+
+@pytest.mark.parametrize("op", ["decode", "prefill"])
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+@pytest.mark.parametrize("base", [1 << 21, -(1 << 21)])
+@pytest.mark.parametrize("scale", [0.5, 37.0, 1e4])
+def test_logits_far_from_zero(tsg, ctx, op, dim, base, scale):  # noqa: F811
+    """Logits of 10^6 to 2 10^10 whose differences are exact: the weights are those of the
+    differences, and a row that sees one key returns its value. The maximum comes step by
+    step, and (3001 keys, split) lies in one split only."""
+    steps = [-9.0, -8.0, -7.0, -7.0, -8.0, -6.0, -9.0]
+    c = Case([2, 2, 2], [2, 150, 3001], 4, 2, dim, page=64, scale=scale, seed=dim)
+    set_products(c, base, steps)
+    for length, t in ((150, 77), (3001, 40), (3001, 2000)):
+        i, j = c.slot(c.lengths.index(length), t)
+        c.k[i, :, j, dim // 2] = -4.0 if t != 2000 else 0.0
+    got = launch(tsg, ctx, c, op, uniform=True)
+    ctx.synchronize()
+    want, _ = c.attention()
+    assert bool(torch.isfinite(want).all())
+    assert_near(got, want, products_tolerance(c, want), op)
+    assert_near(got[:1], want[:1], 2.0 ** -11 * want[:1].abs(), "a single key")
+
+
+@pytest.mark.parametrize("op", ["decode", "prefill"])
+@pytest.mark.parametrize("scale", [40.0, 3e5])
+def test_logits_far_from_zero_e4m3(tsg, ctx, op, scale):  # noqa: F811
+    c = Case([1, 1], [1, 700], 4, 2, 128, kv="e4m3", scale=scale, seed=1)
+    set_products(c, 4.0 * 1024 * 64, [-0.125, -0.25, 0.0, -0.125])
+    got = launch(tsg, ctx, c, op, uniform=True)
+    ctx.synchronize()
+    want, _ = c.attention()
+    assert_near(got, want, products_tolerance(c, want), op)

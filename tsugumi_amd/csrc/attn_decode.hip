@@ -426,19 +426,18 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
         for (uint32_t e = 0; e < 4u; ++e)
             x[e] = (seen >> e) & 1u ? sc[e] : -__builtin_inff();
         const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-        if (__ballot(top * a.scale_log2 > m + kMaxLag)) {
-            const float mn = fmaxf(m, max_across32(max_across16(top)) * a.scale_log2);
-            const float alpha = __builtin_amdgcn_exp2f(m - mn);
+        if (__ballot((top - m) * a.scale_log2 > kMaxLag)) {
+            const float mn = fmaxf(m, max_across32(max_across16(top)));
+            const float alpha = __builtin_amdgcn_exp2f((m - mn) * a.scale_log2);
             m = mn;
             l *= alpha;
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b) o[b] *= alpha;
         }
-        const float shift = kWeightBias - m;
         h4_t w;
 #pragma unroll
         for (uint32_t e = 0; e < 4u; ++e) {
-            const float we = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale_log2, shift));
+            const float we = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e] - m, a.scale_log2, kWeightBias));
             l += we;
             w[e] = (_Float16)we;
         }
@@ -514,7 +513,7 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
         float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0.0f;
 #pragma unroll
         for (uint32_t w = 0; w < kWaves; ++w) {
-            const float f = __builtin_amdgcn_exp2f(sm[w * 16u + r] - mm);
+            const float f = __builtin_amdgcn_exp2f((sm[w * 16u + r] - mm) * a.scale_log2);
             sum += sl[w * 16u + r] * f;
             const float* src = so + (w * 16u + r) * (DP + 4u) + 8u * c;
 #pragma unroll
@@ -592,7 +591,7 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
                 mk[k] = __uint_as_float((uint32_t)ml[k]);
                 mn = fmaxf(mn, mk[k]);
             }
-            const float f0 = __builtin_amdgcn_exp2f(mm - mn);
+            const float f0 = __builtin_amdgcn_exp2f((mm - mn) * a.scale_log2);
             mm = mn;
             sum *= f0;
 #pragma unroll
@@ -600,7 +599,7 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
 #pragma unroll
             for (uint32_t k = 0; k < kJoinLoads; ++k) {
                 const bool have = w0 + k * ways < used;
-                const float f = have ? __builtin_amdgcn_exp2f(mk[k] - mn) : 0.0f;
+                const float f = have ? __builtin_amdgcn_exp2f((mk[k] - mn) * a.scale_log2) : 0.0f;
                 const uint32_t u[8] = {lo[k].x, lo[k].y, lo[k].z, lo[k].w,
                                        hi[k].x, hi[k].y, hi[k].z, hi[k].w};
                 if (have) {
@@ -612,7 +611,8 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
         }
         for (uint32_t o = 1; o < ways; o <<= 1) {
             const float m2 = __shfl_xor(mm, (int)o, 64), mn = fmaxf(mm, m2);
-            const float f0 = __builtin_amdgcn_exp2f(mm - mn), f1 = __builtin_amdgcn_exp2f(m2 - mn);
+            const float f0 = __builtin_amdgcn_exp2f((mm - mn) * a.scale_log2);
+            const float f1 = __builtin_amdgcn_exp2f((m2 - mn) * a.scale_log2);
             mm = mn;
             sum = sum * f0 + __shfl_xor(sum, (int)o, 64) * f1;
 #pragma unroll

@@ -139,13 +139,18 @@ __device__ __forceinline__ uint4 load_query(const uint16_t* p, uint32_t q_sign) 
 // which that product takes the keys is free, and V is read in the order in
 // which the accumulators hold them. V^T comes out of LDS by transposing reads.
 //
-// Weights are kept as exp2(s - m + kWeightBias), m a reference at most
-// kMaxLag below the row's running maximum: a weight's rounding to fp16 is then
-// relative (half a step, 2^-11) down to 2^-25 of the largest, and at most
-// 2^15. m moves, and with it the sums, only when a logit passes it by kMaxLag.
+// Weights are kept as exp2((x - m) scale_log2 + kWeightBias), x the product q.k
+// and m a reference at most kMaxLag powers of two below the row's running
+// maximum: a weight's rounding to fp16 is then relative (half a step, 2^-11)
+// down to 2^-25 of the largest, and at most 2^15. m moves, and with it the sums,
+// only when a logit passes it by kMaxLag. It is a product, not a logit: a
+// rounded logit would be off by whole powers of two from 2^24 on, and the
+// weight of the very key that it came from with it.
 constexpr float kWeightBias = 11.0f;
 constexpr float kMaxLag = 4.0f;
-constexpr float kNoKey = -1e30f;  // m of a row that has seen no key
+// m of a row that has seen no key: below all products (512 x 65504^2), and
+// finite times any scale_log2
+constexpr float kNoKey = -1e25f;
 
 // The key tiles (T keys each) that rows at positions p_lo .. p_hi see: those of
 // the sinks, then those from the first row's window on. Tile i of them starts

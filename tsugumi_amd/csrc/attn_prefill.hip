@@ -25,6 +25,7 @@ namespace {
 constexpr uint32_t kRows = kPrefillRows;  // of a workgroup
 constexpr uint32_t kWaveRows = 32;        // of a wave
 constexpr uint32_t kJoinRows = 8;         // rows a joining workgroup takes
+constexpr float kFar = 1024.0f;           // a reference's logit in powers of two
 
 struct PrefillArgs {
     AttnArgs a;
@@ -281,6 +282,10 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[b][e] = 0.0f;
     float m = kNoKey, l = 0.0f;
+    // (x - m) scale_log2 + bias as one multiply-add, with m's part rounded by
+    // itself (by 2^-14 at most), or, far from zero, of the difference
+    float shift = __builtin_fmaf(-kNoKey, a.scale_log2, kWeightBias);
+    bool far = false;  // some row of the wave's is
     // Accumulator register e of lane half h is key 8 (e / 4) + 4 h + e % 4 of 32;
     // registers 8 ss .. 8 ss + 7 are the lane's eight of the second operand of
     // V^T P^T's step ss, whose first operand comes in two transposing reads.
@@ -337,17 +342,26 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
         for (uint32_t u = 0; u < N; ++u)
 #pragma unroll
             for (int e = 0; e < 16; ++e) top = fmaxf(top, x[u][e]);
-        if (__ballot(top * a.scale_log2 > m + kMaxLag)) {
-            const float mn = fmaxf(m, max_across32(top) * a.scale_log2);
-            const float alpha = __builtin_amdgcn_exp2f(m - mn);
+        if (__ballot((top - m) * a.scale_log2 > kMaxLag)) {
+            const float mn = fmaxf(m, max_across32(top));
+            const float alpha = __builtin_amdgcn_exp2f((m - mn) * a.scale_log2);
             m = mn;
+            const bool row_far = fabsf(m * a.scale_log2) >= kFar && m != kNoKey;
+            shift = row_far ? kWeightBias : __builtin_fmaf(-m, a.scale_log2, kWeightBias);
+            far = __ballot(row_far) != 0;
             l *= alpha;
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b) o[b] *= alpha;
         }
     };
-    const auto weights = [&](const f16v_t (&x)[N], h8_t (&w)[N][2]) {
-        const float shift = kWeightBias - m;
+    const auto weights = [&](f16v_t (&x)[N], h8_t (&w)[N][2]) {
+        if (far) {
+            const float sub = shift == kWeightBias ? m : 0.0f;
+#pragma unroll
+            for (uint32_t u = 0; u < N; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[u][e] -= sub;
+        }
 #pragma unroll
         for (uint32_t u = 0; u < N; ++u)
 #pragma unroll
@@ -543,7 +557,8 @@ __global__ __launch_bounds__(256) void prefill_join_kernel(PrefillArgs p) {
             const f4_t* src = reinterpret_cast<const f4_t*>(p.part_o + at * DP + 8u * c);
             const f4_t lo = src[0], hi = src[1];
             const float mn = fmaxf(m, ml.x);
-            const float f0 = __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(ml.x - mn);
+            const float f0 = __builtin_amdgcn_exp2f((m - mn) * a.scale_log2);
+            const float f1 = __builtin_amdgcn_exp2f((ml.x - mn) * a.scale_log2);
             m = mn;
             sum = sum * f0 + ml.y * f1;
 #pragma unroll
@@ -551,7 +566,8 @@ __global__ __launch_bounds__(256) void prefill_join_kernel(PrefillArgs p) {
         }
         for (uint32_t o = 1; o < ways; o <<= 1) {
             const float m2 = __shfl_xor(m, (int)o, 64), mn = fmaxf(m, m2);
-            const float f0 = __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(m2 - mn);
+            const float f0 = __builtin_amdgcn_exp2f((m - mn) * a.scale_log2);
+            const float f1 = __builtin_amdgcn_exp2f((m2 - mn) * a.scale_log2);
             m = mn;
             sum = sum * f0 + __shfl_xor(sum, (int)o, 64) * f1;
 #pragma unroll
