@@ -73,3 +73,26 @@ def test_logits_far_from_zero_e4m3(tsg, ctx, op, scale):  # noqa: F811
     ctx.synchronize()
     want, _ = c.attention()
     assert_near(got, want, products_tolerance(c, want), op)
+
+
+@pytest.mark.parametrize("op", ["decode", "prefill"])
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+def test_equal_values_come_back(tsg, ctx, op, dim):  # noqa: F811
+    """Where all keys have one value the result is that value, whatever the weights: their
+    rounding to fp16 is in the sum as well. Two keys count, the later one 3.4 .. 4 powers of two
+    above the earlier, so that the reference lags behind it."""
+    n = 300  # so many that the keys are not split
+    c = Case([1] * n, [80] * n, 2, 1, dim, page=64, scale=1.0, seed=dim)
+    c.q[:] = 0
+    c.q[..., 0] = 1.0
+    c.k[:] = 0
+    c.k[..., 0] = -100.0
+    c.v[:] = 1.9990234375  # half a step is 2^-12 of it
+    for s in range(n):
+        i, j = c.slot(s, 4)
+        c.k[i, :, j, 0] = 0.0
+        i, j = c.slot(s, 68)  # another tile of the same wave, in decode too
+        c.k[i, :, j, 0] = (3.4 + 0.6 * s / n) * 0.6931
+    got = launch(tsg, ctx, c, op, uniform=True)
+    ctx.synchronize()
+    assert bool((got == 1.9990234375).all())

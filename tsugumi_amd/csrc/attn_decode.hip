@@ -436,10 +436,12 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
         }
         h4_t w;
 #pragma unroll
-        for (uint32_t e = 0; e < 4u; ++e) {
-            const float we = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e] - m, a.scale_log2, kWeightBias));
-            l += we;
-            w[e] = (_Float16)we;
+        for (uint32_t e = 0; e < 4u; e += 2u) {
+            const h2_t two = weight_pair(__builtin_fmaf(x[e] - m, a.scale_log2, kWeightBias),
+                                         __builtin_fmaf(x[e + 1] - m, a.scale_log2, kWeightBias));
+            l = dot2(two, h2_t{1, 1}, l);
+            w[e] = two[0];
+            w[e + 1] = two[1];
         }
         if constexpr (DMA) {  // V is there, the next K still on its way
             if (more) wait_loads<VL>();

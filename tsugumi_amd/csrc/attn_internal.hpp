@@ -152,6 +152,13 @@ constexpr float kMaxLag = 4.0f;
 // finite times any scale_log2
 constexpr float kNoKey = -1e25f;
 
+// Two weights of these exponents, rounded to fp16 for the matrix product. A row's
+// sum takes the rounded weights (in fp32): the result is then a mean of the
+// values, with the weights off by their rounding, and exact where they are equal.
+__device__ __forceinline__ h2_t weight_pair(float x, float y) {
+    return h2_t{(_Float16)__builtin_amdgcn_exp2f(x), (_Float16)__builtin_amdgcn_exp2f(y)};
+}
+
 // The key tiles (T keys each) that rows at positions p_lo .. p_hi see: those of
 // the sinks, then those from the first row's window on. Tile i of them starts
 // at key T * key_tile(i).

@@ -365,11 +365,12 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
 #pragma unroll
         for (uint32_t u = 0; u < N; ++u)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float we =
-                    __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][e], a.scale_log2, shift));
-                l += we;
-                w[u][e / 8][e % 8] = (_Float16)we;
+            for (int e = 0; e < 16; e += 2) {
+                const h2_t two = weight_pair(__builtin_fmaf(x[u][e], a.scale_log2, shift),
+                                             __builtin_fmaf(x[u][e + 1], a.scale_log2, shift));
+                l = dot2(two, h2_t{1, 1}, l);
+                w[u][e / 8][e % 8] = two[0];
+                w[u][e / 8][e % 8 + 1] = two[1];
             }
     };
     const auto add_values = [&](const h8_t (&w)[N][2], const uint8_t* vb) {
