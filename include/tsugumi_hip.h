@@ -788,9 +788,11 @@ tsg_status tsg_attn_append(tsg_attn* attn, tsg_stream stream, const tsg_kv_pages
                            const tsg_attn_norm_rope* norm_rope, uint16_t* q_out,
                            uint32_t q_out_stride);
 /* out[row, head] = sum_j softmax_j(scale * q . k_j) v_j over the visible keys
- * (zeros where there are none), softmax and sums in fp32, for 1...8 rows of
- * every sequence (a decoded token, a speculative block). What lies in the
- * cache at keys a row does not see, NaN and infinities among it, does not
+ * (zeros where there are none, NaN where all logits are -inf), for 1...8 rows of
+ * every sequence (a decoded token, a speculative block). Softmax and sums are in
+ * fp32; the weights are rounded to fp16 (half a step, 2^-11 of each, down to
+ * 2^-25 of the largest), in the row's sum as in the product with v. What lies in
+ * the cache at keys a row does not see, NaN and infinities among it, does not
  * reach the row. Returns TSG_ERR_DECLINED for more than 8 rows a sequence;
  * row_starts must be NULL. q and out rows on 16 bytes; out may be q itself (same
  * address and stride) and otherwise shares no element with it. */

@@ -96,3 +96,31 @@ def test_equal_values_come_back(tsg, ctx, op, dim):  # noqa: F811
     got = launch(tsg, ctx, c, op, uniform=True)
     ctx.synchronize()
     assert bool((got == 1.9990234375).all())
+
+
+@pytest.mark.parametrize("op", ["decode", "prefill"])
+@pytest.mark.parametrize("length", [40, 3000])
+def test_logits_of_minus_infinity(tsg, ctx, op, length):  # noqa: F811
+    """Weight 0 beside finite logits; a row that sees no others is 0 / 0; rows
+    without a token stay zeros."""
+    c = Case([4, 4, 4], [length, length, 2], 4, 2, 64, window=30, seed=60)
+    c.q[..., 0] = c.q[..., 0].abs() + 0.5
+    for t in range(length - 33, length):
+        for s in (0, 1):
+            i, j = c.slot(s, t)
+            if s == 0 or t % 3 == 0:
+                c.k[i, 0, j, 0] = -float("inf")
+    got = launch(tsg, ctx, c, op, uniform=True)
+    ctx.synchronize()
+    want, tol = c.attention()
+    assert bool(torch.isnan(want[:4, :2]).all()) and int(torch.isnan(want).sum()) == 4 * 2 * 64
+    # the tolerance of attention_ref, its logits' sizes those of the finite keys
+    k, v = c.tokens("k", 1), c.tokens("v", 1)
+    k[torch.isinf(k)] = 0.0
+    size = torch.einsum("jhd,rhgd->rhg", k.abs().amax(0, keepdim=True),
+                        c.q[4:8].view(4, 2, 2, 64).abs().double()).reshape(4, 4, 1) * c.scale
+    rel = 2.0 ** -11 + 2 * size * 72 * 2.0 ** -24 + (length + 64) * 2.0 ** -23
+    tol[:4, :2] = 0.0
+    tol[4:8] = 2.0 ** -11 * want[4:8].abs() + v.abs().max() * rel + 2.0 ** -24
+    assert_near(got, want, tol, op)
+    assert bool((got[8:10] == 0).all())

@@ -496,8 +496,9 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
         return a.out + (uint64_t)(sr.first + t) * a.out_stride +
                (uint64_t)(kvh * a.group + (r0 + r - t * a.group)) * a.dim + 8u * c;
     };
-    const auto emit = [&](uint16_t* out, const float* acc, float sum) {
-        const float inv = sum == 0.0f ? 0.0f : a.v_scale / sum;
+    const auto emit = [&](uint32_t r, uint32_t c, const float* acc, float sum) {
+        uint16_t* out = out_at(r, c);
+        const float inv = row_inverse(sum, base + (int32_t)((r0 + r) / a.group), a.v_scale);
         uint32_t h[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -532,7 +533,7 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
             }
         }
         if (used == 1u) {
-            emit(out_at(r, c), acc, sum);
+            emit(r, c, acc, sum);
         } else {
             const uint64_t slot = slot_of(run.split) * 16u + r;
             float* dst = p.part_o + slot * DP + 8u * c;
@@ -620,7 +621,7 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
 #pragma unroll
             for (int e = 0; e < 8; ++e) acc[e] = acc[e] * f0 + __shfl_xor(acc[e], (int)o, 64) * f1;
         }
-        if (in && way == 0u) emit(out_at(r, c), acc, sum);
+        if (in && way == 0u) emit(r, c, acc, sum);
     }
     if (threadIdx.x == 0) st_coherent(p.arrivals + slot0, 0u);  // for the next call
 }

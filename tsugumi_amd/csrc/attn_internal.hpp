@@ -202,6 +202,13 @@ __device__ __forceinline__ bool key_seen(int32_t key, int32_t pos, uint32_t wind
     return key <= pos && (window == 0u || pos - key < (int32_t)window || key < (int32_t)sinks);
 }
 
+// What a row's sums are multiplied by. A row at a position before 0 is no token,
+// sees no key and becomes zeros; any other sees its own key at least, and a sum
+// of 0 (all logits -inf) makes it NaN, as 0 / 0.
+__device__ __forceinline__ float row_inverse(float sum, int32_t pos, float v_scale) {
+    return sum == 0.0f && pos < 0 ? 0.0f : v_scale / sum;
+}
+
 // The larger of a lane's value and those of the lanes 32 (and 16) from it.
 __device__ __forceinline__ float max_across32(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,

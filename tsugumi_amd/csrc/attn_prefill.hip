@@ -500,7 +500,7 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
 
     // lane half h holds elements 32 b + 8 k + 4 h .. + 3 of its row
     if (t.used == 1u) {
-        const float inv = l == 0.0f ? 0.0f : a.v_scale / l;
+        const float inv = row_inverse(l, pos, a.v_scale);
         uint16_t* out = a.out + (uint64_t)(sr.first + tok) * a.out_stride + (uint64_t)q_head * a.dim;
 #pragma unroll
         for (uint32_t b = 0; b < NB; ++b)
@@ -575,13 +575,13 @@ __global__ __launch_bounds__(256) void prefill_join_kernel(PrefillArgs p) {
             for (int e = 0; e < 8; ++e) acc[e] = acc[e] * f0 + __shfl_xor(acc[e], (int)o, 64) * f1;
         }
         if (!in || way != 0u) continue;
-        const float inv = sum == 0.0f ? 0.0f : a.v_scale / sum;
+        const uint32_t tok = (t.r0 + r) / a.group;
+        const float inv = row_inverse(sum, t.base + (int32_t)tok, a.v_scale);
         uint32_t u[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             u[e] = (uint32_t)f32_to_f16(acc[2 * e] * inv) |
                    ((uint32_t)f32_to_f16(acc[2 * e + 1] * inv) << 16);
-        const uint32_t tok = (t.r0 + r) / a.group;
         *reinterpret_cast<uint4*>(a.out + (uint64_t)(sr.first + tok) * a.out_stride +
                                   (uint64_t)(kvh * a.group + (t.r0 + r) % a.group) * a.dim +
                                   8u * c) = make_uint4(u[0], u[1], u[2], u[3]);
