@@ -124,3 +124,18 @@ def test_logits_of_minus_infinity(tsg, ctx, op, length):  # noqa: F811
     tol[4:8] = 2.0 ** -11 * want[4:8].abs() + v.abs().max() * rel + 2.0 ** -24
     assert_near(got, want, tol, op)
     assert bool((got[8:10] == 0).all())
+
+
+def test_decode_more_key_tiles_than_32_bits_count(tsg, ctx):  # noqa: F811
+    """64 sequences of 2^30 tokens, all on one shared page: 2^32 tiles of 16 keys. Keys of 0
+    and values of 1 give sums that fp32 holds exactly (multiples of a power of two)."""
+    seqs, page = 64, 4096
+    attn = tsg.Attention(ctx, 1, 1, 8, page)
+    k = torch.zeros(1, 1, page, 8, dtype=torch.float16, device="cuda")
+    table = torch.zeros(seqs, (1 << 30) // page, dtype=torch.int32, device="cuda")
+    lengths = torch.full((seqs,), 1 << 30, dtype=torch.int32, device="cuda")
+    q = torch.ones(seqs, 1, 8, dtype=torch.float16, device="cuda")
+    out = torch.full_like(q, -77.0)
+    attn.encode_decode(attn.cache(k, torch.ones_like(k)), attn.batch(table, lengths, seqs), q, out)
+    ctx.synchronize()
+    assert bool((out == 1).all())

@@ -86,16 +86,21 @@ __device__ __forceinline__ bool find_run(const DecodeArgs& p, uint32_t at, Run* 
         return at < r->used;
     }
     const uint32_t lane = threadIdx.x & 63u;
-    uint32_t first = 0, total = 0;  // the first 64 lengths are read once
+    uint32_t first = 0;  // the first 64 lengths are read once
+    uint64_t total = 0;  // of 256 sequences of up to 2^26 tiles each
     for (uint32_t base = 0; base < a.num_seqs; base += 64u) {
         const uint32_t length = base + lane < a.num_seqs ? a.lengths[base + lane] : 0u;
         uint32_t n = base + lane < a.num_seqs ? seq_key_tiles(a, length) : 0u;
         if (base == 0u) first = length;
+        n -= n >> 26;  // 64 of them stay under 2^32
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) n += (uint32_t)__shfl_xor((int)n, o, 64);
-        total += __builtin_amdgcn_readfirstlane(n);
+        total += (uint32_t)__builtin_amdgcn_readfirstlane((int)n);
     }
-    uint32_t per = (total + p.chunks - 1u) / p.chunks;
+    // at least total / chunks: no more runs then than chunks + sequences (the grid), and
+    // fewer than 2 chunks of split sequences (the scratch)
+    uint32_t per = total >> 31 ? ((uint32_t)(total >> 8) / p.chunks + 1u) << 8
+                               : ((uint32_t)total + p.chunks - 1u) / p.chunks;
     per = per > kMinTiles ? per : kMinTiles;
     uint32_t slots = 0;
     for (uint32_t base = 0; base < a.num_seqs; base += 64u) {
