@@ -134,6 +134,9 @@ void tsg_ctx_destroy(tsg_ctx* ctx);
  * Group sizes {32, 64}; defaults are 64 and TSG_AFFINE, as in the reference. */
 tsg_status tsg_ctx_set_affine_group_size(tsg_ctx* ctx, uint32_t group_size);
 tsg_status tsg_ctx_set_affine_scheme(tsg_ctx* ctx, tsg_affine_scheme scheme);
+/* Waits for the stream, then returns and clears what the context's launches have
+ * reported from the device up to then, on any stream: TSG_OK or the first
+ * error's status, with every one of them in tsg_last_error(). */
 tsg_status tsg_ctx_synchronize(tsg_ctx* ctx, tsg_stream stream);
 
 /* ------------------------------------------------- HBM-resident layers ---

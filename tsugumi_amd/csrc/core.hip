@@ -9,7 +9,7 @@ namespace tsg {
 static thread_local std::string g_last_error;
 
 void set_error(const char* fmt, ...) {
-    char buf[1024];
+    char buf[2048];
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(buf, sizeof(buf), fmt, ap);
@@ -18,7 +18,7 @@ void set_error(const char* fmt, ...) {
 }
 
 tsg_status fail(tsg_status status, const char* fmt, ...) {
-    char buf[1024];
+    char buf[2048];
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(buf, sizeof(buf), fmt, ap);
@@ -164,6 +164,55 @@ extern "C" tsg_status tsg_ctx_set_affine_scheme(tsg_ctx* ctx, tsg_affine_scheme 
     return TSG_OK;
 }
 
+// What the bits of the error word say, causes before what they may cause (the
+// NaN rows of an attention call can leave a router without eligible logits).
+namespace {
+struct DeviceError {
+    uint32_t bit;
+    tsg_status status;
+    const char* text;
+};
+constexpr DeviceError kDeviceErrors[] = {
+    {kErrAttnPage, TSG_ERR_INVALID_ARGUMENT,
+     "attention: a page table entry past the cache's pages; the rows that needed it are NaN or "
+     "not appended"},
+    {kErrAttnLength, TSG_ERR_INVALID_ARGUMENT,
+     "attention: a sequence longer than its page table; its rows are NaN or not appended"},
+    {kErrAttnRows, TSG_ERR_INVALID_ARGUMENT,
+     "attention: row starts that fall or pass the batch's rows; the rows of those sequences are "
+     "NaN or not appended"},
+    {kErrGroupExpertRange, TSG_ERR_GROUPING_EXPERT_OUT_OF_RANGE,
+     "expertOutOfRange: the device grouping met a route expert id >= numExperts; those pairs were "
+     "not grouped"},
+    {kErrGroupBlocks, TSG_ERR_INVALID_ARGUMENT,
+     "the device grouping's work list exceeded max_blocks"},
+    {kErrRowsBlock, TSG_ERR_INVALID_ARGUMENT,
+     "rows path: a device block had no rows, more than 8, or an expert past the layer; it was "
+     "skipped"},
+    {kErrVerifyRouting, TSG_ERR_INVALID_ARGUMENT,
+     "verify layer: a token had fewer than 8 eligible router logits (NaN or -inf scores); the "
+     "layer's outputs are NaN"},
+    {kErrRouterWait, TSG_ERR_HIP,
+     "staged router: the selecting block timed out waiting for the other blocks' logits; the "
+     "routing is invalid"},
+    {kErrGemmBlock, TSG_ERR_INVALID_ARGUMENT,
+     "grouped GEMM: a routed block named an expert past the layer; it was skipped and its rows "
+     "were not written"},
+    {kErrGemmWait, TSG_ERR_HIP,
+     "fused grouped GEMM: a down item timed out waiting for its block's gate/up tiles, or an XCD "
+     "queue was not drained; the layer's outputs are invalid"},
+    {kErrDecodeTimeout, TSG_ERR_HIP,
+     "fused decode layer: a block timed out waiting for the others; outputs of the affected "
+     "launch are invalid"},
+};
+
+// Reads and clears the error word in one step: a bit that a call on another
+// stream sets meanwhile is in this report or stays for the next.
+__global__ void take_errors_kernel(uint32_t* word) {
+    word[1] = __hip_atomic_exchange(word, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+}  // namespace
+
 extern "C" tsg_status tsg_ctx_synchronize(tsg_ctx* ctx, tsg_stream stream) {
     TSG_REQUIRE(ctx, TSG_ERR_INVALID_ARGUMENT, "ctx is NULL");
     TSG_HIP_TRY(hipStreamSynchronize(as_stream(stream)));
@@ -172,51 +221,29 @@ extern "C" tsg_status tsg_ctx_synchronize(tsg_ctx* ctx, tsg_stream stream) {
     // an out-of-range expert id or an overfull work list, the device-list rows
     // path on a block it cannot take); the outputs of the affected launches
     // are invalid. Reading clears it.
+    uint32_t* word = ctx->counters + kSyncErrorWord;
     uint32_t err = 0;
-    TSG_HIP_TRY(hipMemcpy(&err, ctx->counters + kSyncErrorWord, sizeof(err),
-                          hipMemcpyDeviceToHost));
-    if (err) {
-        TSG_HIP_TRY(hipMemset(ctx->counters + kSyncErrorWord, 0, sizeof(err)));
-        if (err & kErrGroupExpertRange)
-            return fail(TSG_ERR_GROUPING_EXPERT_OUT_OF_RANGE,
-                        "expertOutOfRange: the device grouping met a route expert id >= "
-                        "numExperts; those pairs were not grouped");
-        if (err & kErrGroupBlocks)
-            return fail(TSG_ERR_INVALID_ARGUMENT,
-                        "the device grouping's work list exceeded max_blocks");
-        if (err & kErrRowsBlock)
-            return fail(TSG_ERR_INVALID_ARGUMENT,
-                        "rows path: a device block had no rows, more than 8, or an expert past "
-                        "the layer; it was skipped");
-        if (err & kErrVerifyRouting)
-            return fail(TSG_ERR_INVALID_ARGUMENT,
-                        "verify layer: a token had fewer than 8 eligible router logits (NaN or "
-                        "-inf scores); the layer's outputs are NaN");
-        if (err & kErrRouterWait)
-            return fail(TSG_ERR_HIP, "staged router: the selecting block timed out waiting for "
-                                     "the other blocks' logits; the routing is invalid");
-        if (err & kErrGemmBlock)
-            return fail(TSG_ERR_INVALID_ARGUMENT,
-                        "grouped GEMM: a routed block named an expert past the layer; it was "
-                        "skipped and its rows were not written");
-        if (err & (kErrAttnPage | kErrAttnLength | kErrAttnRows))
-            return fail(TSG_ERR_INVALID_ARGUMENT,
-                        err & kErrAttnPage
-                            ? "attention: a page table entry past the cache's pages; the rows "
-                              "that needed it are NaN or not appended"
-                        : err & kErrAttnLength
-                            ? "attention: a sequence longer than its page table; its rows are "
-                              "NaN or not appended"
-                            : "attention: row starts that fall or pass the batch's rows; the "
-                              "rows of those sequences are NaN or not appended");
-        if (err & kErrGemmWait)
-            return fail(TSG_ERR_HIP, "fused grouped GEMM: a down item timed out waiting for its "
-                                     "block's gate/up tiles, or an XCD queue was not drained; "
-                                     "the layer's outputs are invalid");
-        return fail(TSG_ERR_HIP, "fused decode layer: a block timed out waiting for the "
-                                 "others; outputs of the affected launch are invalid");
+    TSG_HIP_TRY(hipMemcpy(&err, word, sizeof(err), hipMemcpyDeviceToHost));
+    if (!err) return TSG_OK;
+    {
+        const std::lock_guard<std::mutex> lock(ctx->error_mutex);  // word[1] is one call's
+        DeviceScope scope(ctx->device);
+        TSG_HIP_TRY(scope.status);
+        hipLaunchKernelGGL(take_errors_kernel, dim3(1), dim3(1), 0, as_stream(stream), word);
+        if (tsg_status s = check_launch("take_errors")) return s;
+        TSG_HIP_TRY(hipStreamSynchronize(as_stream(stream)));
+        TSG_HIP_TRY(hipMemcpy(&err, word + 1, sizeof(err), hipMemcpyDeviceToHost));
     }
-    return TSG_OK;
+    tsg_status status = TSG_OK;
+    char text[2048] = "";  // all of them are 1200 characters
+    size_t at = 0;
+    for (const DeviceError& e : kDeviceErrors) {
+        if (!(err & e.bit)) continue;
+        const int n = snprintf(text + at, sizeof(text) - at, "%s%s", at ? "; also " : "", e.text);
+        at = std::min(at + (size_t)std::max(n, 0), sizeof(text) - 1u);
+        if (status == TSG_OK) status = e.status;
+    }
+    return status == TSG_OK ? TSG_OK : fail(status, "%s", text);
 }
 
 // ---------------------------------------------------------------- layers

@@ -8,6 +8,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <mutex>
 #include <string>
 
 #include "../../include/tsugumi_hip.h"
@@ -60,6 +61,7 @@ struct tsg_ctx {
     // one-partition mode) when that is a power of two of at most 8, else 0
     // (the fused launch is not used)
     uint32_t gemm_queues = 0;
+    std::mutex error_mutex;  // tsg_ctx_synchronize's taking of the error word
 };
 
 struct tsg_moe {
@@ -111,7 +113,8 @@ constexpr uint32_t kDecodeGroups = 8;      // one expert slot per group
 constexpr uint32_t kGroupMembers = 32;     // blocks per group
 constexpr uint32_t kDecodeBlocks = kDecodeGroups * kGroupMembers;
 constexpr uint32_t kSyncEpochWord = 1024;  // launch epoch
-constexpr uint32_t kSyncErrorWord = 1056;  // device-side error bits (kErr*), read by tsg_ctx_synchronize
+constexpr uint32_t kSyncErrorWord = 1056;  // device-side error bits (kErr*), read by tsg_ctx_synchronize;
+                                           // the next word: what its last call took
 // Bits of the error word: a one-launch decode layer whose hand-off wait timed
 // out; a device grouping that met an expert id >= num_experts (its pairs are
 // not grouped); a device grouping whose work list did not fit max_blocks; a
