@@ -45,3 +45,31 @@ def test_every_error_is_reported(tsg, ctx):  # noqa: F811
                                            "row starts", "expertOutOfRange")]
     assert -1 not in places and places == sorted(places)
     ctx.synchronize()  # reported once
+
+
+def refused(tsg, call, *args, text=""):  # noqa: F811
+    with pytest.raises(tsg.TsgError) as e:
+        call(*args)
+    assert e.value.status == 1 and text in str(e.value)
+
+
+def test_closed_context_and_plan(tsg):  # noqa: F811
+    """A plan points into its context: after the context's end its calls are refused."""
+    c = Case([1], [20], 2, 1, 64, seed=71)
+    d = c.to_device()
+    own = tsg.Context(0)
+    attn, other = plan(tsg, own, c), plan(tsg, own, c)
+    cache, batch = attn.cache(d["k"], d["v"]), attn.batch(d["table"], d["lengths"], 1)
+    out = torch.full_like(d["q"], -77.0)
+    rows = torch.zeros(1, 64, dtype=torch.float16, device="cuda")
+    calls = [(attn.encode_decode, cache, batch, d["q"], out),
+             (attn.encode_prefill, cache, batch, d["q"], out),
+             (attn.encode_append, cache, batch, d["q"], rows, rows, tsg.HeadNormRope(), out)]
+    other.close()
+    refused(tsg, other.encode_decode, cache, batch, d["q"], out)
+    own.close()
+    for call in calls:
+        refused(tsg, *call, text="closed")
+    torch.cuda.synchronize()
+    assert bool((out == -77).all())
+    attn.close()  # needs no context

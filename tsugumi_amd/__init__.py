@@ -989,6 +989,8 @@ class Attention:
         return t.data_ptr(), strides[0] if n > 1 else width
 
     def _on(self, stream):
+        if not self.ctx.handle:  # the plan points into it
+            _refuse("the attention's context is closed")
         if stream is not None:
             return stream if isinstance(stream, int) else stream.cuda_stream
         return _current_stream_of(self._device)
