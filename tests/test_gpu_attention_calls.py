@@ -73,3 +73,46 @@ def test_closed_context_and_plan(tsg):  # noqa: F811
     torch.cuda.synchronize()
     assert bool((out == -77).all())
     attn.close()  # needs no context
+
+
+def test_caches_and_batches_of_another_kind(tsg, ctx):  # noqa: F811
+    """A cache of another type, head or page size is refused (its bytes would be read as the
+    plan's own), as is a batch whose table counts other pages; those of a plan that differs in
+    window or query heads only are taken."""
+    c = Case([2], [40], 4, 2, 64, kv="e4m3", seed=72)
+    d = c.to_device()
+    codes = plan(tsg, ctx, c)
+    cache, batch = codes.cache(d["k"], d["v"]), codes.batch(d["table"], d["lengths"], 2)
+    out = torch.full_like(d["q"], -77.0)
+    rows = torch.zeros(2, 128, dtype=torch.float16, device="cuda")
+    pool = torch.zeros(4, 2, 32, 64, dtype=torch.float16, device="cuda")
+    half, wide_pages = tsg.Attention(ctx, 4, 2, 64, 16), tsg.Attention(ctx, 4, 2, 64, 32)
+    one_head = tsg.Attention(ctx, 4, 1, 64, 16, "e4m3")
+    for attn in (half, one_head):
+        refused(tsg, attn.encode_decode, cache, batch, d["q"], out, text="a cache of")
+        refused(tsg, attn.encode_prefill, cache, batch, d["q"], out, text="a cache of")
+    refused(tsg, half.encode_append, cache, batch, d["q"], rows, rows, tsg.HeadNormRope(), out,
+            text="a cache of")
+    refused(tsg, wide_pages.encode_decode, wide_pages.cache(pool, pool), batch, d["q"], out,
+            text="a batch of")
+    torch.cuda.synchronize()
+    assert bool((out == -77).all())
+    again = tsg.Attention(ctx, 4, 2, 64, 16, "e4m3", window=40, scale=c.scale, k_scale=c.k_scale,
+                          v_scale=c.v_scale)
+    again.encode_decode(cache, batch, d["q"], out)
+    ctx.synchronize()
+    want, tol = c.attention()
+    assert_near(out, want, tol)
+
+
+def test_norm_weights_on_another_device(tsg, ctx):  # noqa: F811
+    weight, inv = torch.ones(64, device="cuda").bfloat16(), torch.ones(32)
+    refused(tsg, tsg.HeadNormRope, weight, weight, inv, text="two devices")
+    c = Case([1], [20], 2, 1, 64, seed=73)
+    d = c.to_device()
+    attn, rope = plan(tsg, ctx, c), tsg.HeadNormRope(weight, weight)
+    rope.device = 1  # as of weights on a second card
+    rows = torch.zeros(1, 64, dtype=torch.float16, device="cuda")
+    refused(tsg, attn.encode_append, attn.cache(d["k"], d["v"]),
+            attn.batch(d["table"], d["lengths"], 1), d["q"], rows, rows, rope, d["q"],
+            text="context's device")

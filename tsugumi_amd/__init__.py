@@ -862,7 +862,8 @@ def _types(*names):
 class PagedKVCache:
     """A layer's key and value pools (tsg_kv_pages) on torch CUDA tensors of
     shape [pages, kv_heads, page_tokens, head_dim], contiguous or views with
-    the heads inside the tokens (the last dimension contiguous)."""
+    the heads inside the tokens (the last dimension contiguous). For calls of
+    any Attention of these sizes, this cache type and this device."""
 
     def __init__(self, attn: "Attention", k, v):
         c = attn.config
@@ -887,11 +888,13 @@ class PagedKVCache:
                                   head if shape[0] > 1 else 0, page if k.shape[0] > 1 else 0)
         self._ref = C.addressof(self.pages)
         check(attn.lib.tsg_attn_check(C.addressof(c), self._ref, None))
+        self.kind = attn.cache_kind
 
 
 class AttentionBatch:
     """The sequences of one call (tsg_attn_batch): page_table [seqs, pages] and
-    lengths [seqs] of 32-bit integers; row_starts [seqs + 1] for ragged rows."""
+    lengths [seqs] of 32-bit integers; row_starts [seqs + 1] for ragged rows.
+    For calls of any Attention of this page size and device."""
 
     def __init__(self, attn: "Attention", page_table, lengths, rows: int, row_starts=None):
         for t in (page_table, lengths, row_starts):
@@ -913,6 +916,7 @@ class AttentionBatch:
                                     page_table.shape[1], seqs, self.rows)
         self._ref = C.addressof(self.batch)
         check(attn.lib.tsg_attn_check(C.addressof(attn.config), None, self._ref))
+        self.kind = attn.batch_kind
 
 
 class HeadNormRope:
@@ -929,6 +933,10 @@ class HeadNormRope:
         if len(widths) > 1:
             _refuse("norm weights of two lengths")
         self.width = widths.pop() if widths else None
+        devices = {t.get_device() for t in (q_weight, k_weight, inv_freq) if t is not None}
+        if len(devices) > 1:
+            _refuse("norm weights and inv_freq on two devices")
+        self.device = devices.pop() if devices else None
         self._keep = (q_weight, k_weight, inv_freq)
         self.norm_rope = _abi.AttnNormRope(
             _ptr(q_weight), _ptr(k_weight), _ptr(inv_freq),
@@ -963,6 +971,8 @@ class Attention:
         # what the calls look at each time
         self._half, self._device = _types("float16", "int16", "uint16"), ctx.device
         self._layout = (q_heads, kv_heads, head_dim, q_heads * head_dim, kv_heads * head_dim)
+        self.batch_kind = (page_tokens, ctx.device)
+        self.cache_kind = (kv_heads, head_dim, kv_type, *self.batch_kind)
         self._append, self._decode, self._prefill = (
             self.lib.tsg_attn_append, self.lib.tsg_attn_decode, self.lib.tsg_attn_prefill)
 
@@ -988,6 +998,13 @@ class Attention:
             _refuse("row operands must be fp16 tensors on the context's device")
         return t.data_ptr(), strides[0] if n > 1 else width
 
+    def _fits(self, cache, batch):
+        if cache.kind != self.cache_kind:
+            _refuse(f"a cache of {cache.kind} (key heads, head_dim, type, page_tokens, device), "
+                    f"not of {self.cache_kind}")
+        if batch.kind != self.batch_kind:
+            _refuse(f"a batch of {batch.kind} (page_tokens, device), not of {self.batch_kind}")
+
     def _on(self, stream):
         if not self.ctx.handle:  # the plan points into it
             _refuse("the attention's context is closed")
@@ -999,8 +1016,12 @@ class Attention:
         """Norms, rotation and cache write of the batch's rows; q_out gets the
         query heads (it may be q)."""
         n, hq, hk, dim, q_width, kv_width = batch.rows, *self._layout
+        if cache.kind is not self.cache_kind or batch.kind is not self.batch_kind:
+            self._fits(cache, batch)  # made by another plan
         if norm_rope.width is not None and norm_rope.width != dim:
             _refuse("norm weights must be [head_dim]")
+        if norm_rope.device != self._device and norm_rope.device is not None:
+            _refuse("norm weights and inv_freq must be on the context's device")
         q, qs = self._rows(q, n, hq, q_width)
         k, ks = self._rows(k, n, hk, kv_width)
         v, vs = self._rows(v, n, hk, kv_width)
@@ -1013,6 +1034,8 @@ class Attention:
 
     def _attend(self, call, cache, batch, q, out, stream):
         n, hq, _, _, width, _ = batch.rows, *self._layout
+        if cache.kind is not self.cache_kind or batch.kind is not self.batch_kind:
+            self._fits(cache, batch)  # made by another plan
         q, qs = self._rows(q, n, hq, width)
         out, os = self._rows(out, n, hq, width)
         status = call(self.handle, self._on(stream), cache._ref, batch._ref, q, qs, out, os)
