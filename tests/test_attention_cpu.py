@@ -153,3 +153,36 @@ def test_reference_rotation_is_by_relative_position():
                                              interleaved, 0.0, False)
             dots.append(float((qr * kr).sum()))
         assert abs(dots[0] - dots[1]) < 1e-9
+
+
+# ------------------------------------------- what the Python classes refuse
+
+def bare_plan(tsg):
+    """An Attention of 8 query and 2 key heads of 64 without a device behind it."""
+    attn = tsg.Attention.__new__(tsg.Attention)
+    attn.handle, attn._half, attn._device = None, (torch.float16,), -1  # as of meta tensors
+    return attn
+
+
+def test_python_refuses_values_past_32_bits():
+    """What ctypes would cut off to 32 bits: 2^32 sinks are none, 2^32 + 8 heads are eight."""
+    import tsugumi_amd as tsg
+
+    class NoContext:
+        lib, handle, device = tsg.load(), None, 0
+
+    fine = dict(q_heads=8, kv_heads=2, head_dim=64, page_tokens=16, window=64, sinks=1)
+    for name in fine:
+        for value in (fine[name] + (1 << 32), -1):
+            with pytest.raises(tsg.TsgError) as e:
+                tsg.Attention(NoContext(), **{**fine, name: value})
+            assert e.value.status == INVALID and name in str(e.value)
+    attn = bare_plan(tsg)
+    for stride, status in ((512, None), ((1 << 32) + 512, INVALID)):
+        rows = torch.empty_strided((2, 512), (stride, 1), dtype=torch.float16, device="meta")
+        if status is None:
+            assert attn._rows(rows, 2, 8, 512) == (0, 512)
+            continue
+        with pytest.raises(tsg.TsgError) as e:
+            attn._rows(rows, 2, 8, 512)
+        assert e.value.status == status

@@ -853,6 +853,13 @@ def _refuse(text: str):
     raise TsgError(TSG_ERR_INVALID_ARGUMENT, text)
 
 
+def _words(**values):
+    """Refuses what a 32-bit argument cannot hold (ctypes would cut it off)."""
+    for name, value in values.items():
+        if not 0 <= value < 1 << 32:
+            _refuse(f"{name} {value} does not fit 32 bits")
+
+
 def _types(*names):
     """torch's types of these names (bit patterns travel as 16-bit integers too)."""
     import torch
@@ -882,6 +889,7 @@ class PagedKVCache:
         if k.shape != v.shape or k.stride() != v.stride():
             _refuse("key and value pages differ in shape or strides")
         page, head, token, _ = k.stride()
+        _words(token_stride=token)
         # a stride over one element is any number in torch; the library wants a real one
         self._keep = (k, v)
         self.pages = _abi.KVPages(k.data_ptr(), v.data_ptr(), k.shape[0], token,
@@ -912,6 +920,7 @@ class AttentionBatch:
             _refuse("row_starts must be [seqs + 1]")
         self._keep = (page_table, lengths, row_starts)
         self.rows = int(rows)
+        _words(rows=self.rows, num_seqs=seqs, table_stride=page_table.shape[1])
         self.batch = _abi.AttnBatch(_ptr(page_table), _ptr(lengths), _ptr(row_starts),
                                     page_table.shape[1], seqs, self.rows)
         self._ref = C.addressof(self.batch)
@@ -961,6 +970,8 @@ class Attention:
         types = {"f16": TSG_KV_F16, "e4m3": TSG_KV_E4M3}
         if kv_type not in types:
             _refuse(f"unknown cache type {kv_type!r}")
+        _words(q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim, page_tokens=page_tokens,
+               window=window, sinks=sinks)
         if scale is None:
             scale = float(head_dim) ** -0.5 if head_dim > 0 else 1.0
         self.config = _abi.AttnConfig(q_heads, kv_heads, head_dim, page_tokens, types[kv_type],
@@ -991,7 +1002,7 @@ class Attention:
             fits = (len(shape) == 3 and shape[1] == heads and heads * shape[2] == width
                     and strides[2] == 1 and (heads == 1 or strides[1] == shape[2]))
         n = shape[0] if fits else 0
-        if n < rows:
+        if n < rows or (n > 1 and strides[0] >> 32):
             _refuse(f"row operand of shape {tuple(shape)}, strides {strides}: not {rows} rows of "
                     f"{width}")
         if t.dtype not in self._half or t.get_device() != self._device:
