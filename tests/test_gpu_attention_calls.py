@@ -116,3 +116,54 @@ def test_norm_weights_on_another_device(tsg, ctx):  # noqa: F811
     refused(tsg, attn.encode_append, attn.cache(d["k"], d["v"]),
             attn.batch(d["table"], d["lengths"], 1), d["q"], rows, rows, rope, d["q"],
             text="context's device")
+
+
+@pytest.mark.parametrize("op", ["decode", "prefill"])
+def test_one_plan_on_two_streams(tsg, ctx, op):  # noqa: F811
+    """Calls of one plan on streams in turn, with no event between: they share its scratch,
+    and each waits for the last. The long call comes first, so that the next would overlap it."""
+    cases = [Case([1, 1], [20000, 30000], 8, 2, 128, page=64, seed=74),
+             Case([1] * 3, [900, 4000, 777], 8, 2, 128, page=64, seed=75)]
+    devices = [c.to_device() for c in cases]
+    want = [launch(tsg, ctx, c, op, d=d, uniform=True) for c, d in zip(cases, devices)]
+    attn = plan(tsg, ctx, cases[0])
+    calls = [(attn.cache(d["k"], d["v"]), attn.batch(d["table"], d["lengths"], c.total), d["q"])
+             for c, d in zip(cases, devices)]
+    call = attn.encode_decode if op == "decode" else attn.encode_prefill
+    outs = [[torch.full_like(w, -77.0) for w in want] for _ in range(10)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for pair in outs:
+        call(*calls[0], pair[0])  # on the default stream
+        for args, out, stream in zip(calls, pair, streams):
+            call(*args, out, stream=stream)
+    torch.cuda.synchronize()
+    ctx.synchronize()
+    for pair in outs:
+        assert all(torch.equal(out, w) for out, w in zip(pair, want))
+
+
+def test_plan_captured_between_eager_calls(tsg, ctx):  # noqa: F811
+    """A capture takes no event of the eager stream, and the eager calls after it none of its
+    stream; replays and eager calls in turn on one stream agree."""
+    c = Case([1, 1], [3000, 5000], 8, 2, 64, page=64, seed=76)
+    d = c.to_device()
+    attn = plan(tsg, ctx, c)
+    cache, batch = attn.cache(d["k"], d["v"]), attn.batch(d["table"], d["lengths"], 2)
+    outs = [torch.full_like(d["q"], -77.0) for _ in range(3)]
+    attn.encode_decode(cache, batch, d["q"], outs[0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attn.encode_decode(cache, batch, d["q"], outs[1])
+    for _ in range(3):
+        outs[1].fill_(-77.0)
+        graph.replay()
+        attn.encode_prefill(cache, batch, d["q"], outs[2])
+        attn.encode_decode(cache, batch, d["q"], outs[0])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], outs[1])
+    ctx.synchronize()
+    want, tol = c.attention()
+    for out in outs:
+        assert_near(out, want, tol)

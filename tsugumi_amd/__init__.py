@@ -959,7 +959,9 @@ class Attention:
     paged cache. scale defaults to head_dim ** -0.5. Row operands are fp16
     tensors [rows, heads, head_dim] or [rows, heads * head_dim], rows any
     16-byte multiple apart. Work goes to `stream`, or to torch's current stream
-    of the context's device."""
+    of the context's device. Decode and prefill calls share the plan's scratch:
+    one on another torch stream than the last waits for that one's work (raw
+    stream addresses and graphs are the caller's to keep in order)."""
 
     def __init__(self, ctx: Context, q_heads: int, kv_heads: int, head_dim: int,
                  page_tokens: int, kv_type: str = "f16", window: int = 0, sinks: int = 0,
@@ -979,6 +981,7 @@ class Attention:
         h = C.c_void_p()
         check(self.lib.tsg_attn_create(ctx.handle, C.addressof(self.config), C.byref(h)))
         self.handle = h
+        self._last = None  # torch's stream of the last decode or prefill call
         # what the calls look at each time
         self._half, self._device = _types("float16", "int16", "uint16"), ctx.device
         self._layout = (q_heads, kv_heads, head_dim, q_heads * head_dim, kv_heads * head_dim)
@@ -1023,6 +1026,21 @@ class Attention:
             return stream if isinstance(stream, int) else stream.cuda_stream
         return _current_stream_of(self._device)
 
+    def _after_last(self, stream):
+        """The stream of a call that uses the plan's scratch: where torch's stream has changed
+        since the last such call, it waits for the old one. Calls being captured run where their
+        graph is replayed, and raw addresses may outlive their streams: the caller's to order."""
+        raw = self._on(stream)
+        if raw != self._last and not isinstance(stream, int):
+            import torch
+            if not torch.cuda.is_current_stream_capturing():
+                if self._last is not None:
+                    old, new = (torch.cuda.ExternalStream(s, self._device)
+                                for s in (self._last, raw))
+                    new.wait_event(old.record_event())
+                self._last = raw
+        return raw
+
     def encode_append(self, cache, batch, q, k, v, norm_rope, q_out, stream=None):
         """Norms, rotation and cache write of the batch's rows; q_out gets the
         query heads (it may be q)."""
@@ -1049,7 +1067,8 @@ class Attention:
             self._fits(cache, batch)  # made by another plan
         q, qs = self._rows(q, n, hq, width)
         out, os = self._rows(out, n, hq, width)
-        status = call(self.handle, self._on(stream), cache._ref, batch._ref, q, qs, out, os)
+        status = call(self.handle, self._after_last(stream), cache._ref, batch._ref, q, qs, out,
+                      os)
         if status:
             check(status)
 
