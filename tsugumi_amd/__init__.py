@@ -1035,7 +1035,9 @@ class Attention:
             import torch
             if not torch.cuda.is_current_stream_capturing():
                 if self._last is not None:
-                    old, new = (torch.cuda.ExternalStream(s, self._device)
+                    # (torch makes a new stream of address 0)
+                    old, new = (torch.cuda.ExternalStream(s, self._device) if s
+                                else torch.cuda.default_stream(self._device)
                                 for s in (self._last, raw))
                     new.wait_event(old.record_event())
                 self._last = raw
