@@ -697,15 +697,16 @@ tsg_status tsg_prefill_int4_qmm(tsg_ctx* ctx, tsg_stream stream, const uint8_t* 
  * among them: row i of its n rows is at position p = lengths[s] - n + i. Its
  * token t lies in slot t % page_tokens of page page_table[s * table_stride +
  * t / page_tokens]. A row with p < 0 (a padded row, a sequence of length 0) is
- * no token: nothing of it is appended and its outputs are zeros. Rows behind
- * the last sequence's (row_starts) are left as they were.
+ * no token: nothing of it is appended and its outputs are zeros. Rows before
+ * the first sequence's and behind the last's (row_starts) are left as they were.
  *
  * page_table, lengths and row_starts are read on the device, so a captured
- * graph replays with what they then hold. A page id past the cache's pages, a
- * sequence longer than its table, or row starts that fall or pass `rows` leave
- * NaN in the rows concerned (query rows of an append included; nothing of them
- * goes to the cache) and tsg_ctx_synchronize reports TSG_ERR_INVALID_ARGUMENT;
- * the rows that share a kernel tile with them may be NaN as well. */
+ * graph replays with what they then hold. A page id past the cache's pages or a
+ * sequence longer than its table leave NaN in the rows concerned, row starts
+ * that fall or pass `rows` in every row before the sequences behind the last
+ * such one (query rows of an append included; nothing of them goes to the cache),
+ * and tsg_ctx_synchronize reports TSG_ERR_INVALID_ARGUMENT; the rows that share
+ * a kernel tile with rows concerned may be NaN as well. */
 
 /* What the cache holds: fp16, or OCP e4m3 codes c standing for c * scale. */
 typedef enum tsg_kv_type { TSG_KV_F16 = 0, TSG_KV_E4M3 = 1 } tsg_kv_type;

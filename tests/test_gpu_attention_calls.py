@@ -167,3 +167,81 @@ def test_plan_captured_between_eager_calls(tsg, ctx):  # noqa: F811
     want, tol = c.attention()
     for out in outs:
         assert_near(out, want, tol)
+
+
+# rows of each sequence as the right starts have them, starts as given, the first sequence
+# behind the last wrong one
+BAD_STARTS = [([5, 4], [0, 9, 5], 2), ([5, 4], [0, 5, 99], 2), ([5, 4], [0, -1, 9], 2),
+              ([8, 3, 4], [0, 8, 4, 15], 2), ([8, 2, 3, 4], [0, 8, 2, 5, 15], 2),
+              ([300, 40, 200, 8], [0, 300, 280, 540, 548], 2), ([3, 4, 2], [7, 3, 7, 8], 1)]
+
+
+@pytest.mark.parametrize("rows,starts,good", BAD_STARTS)
+@pytest.mark.parametrize("op", ["prefill", "append"])
+def test_bad_row_starts(tsg, ctx, op, rows, starts, good):  # noqa: F811
+    """Starts that fall or pass the rows, two sequences that claim a row among them: the
+    sequences behind the last such one are right, every row before them is NaN, and appending
+    writes nothing of them to the cache."""
+    c = Case(rows, [r + 9 * i for i, r in enumerate(rows)], 4, 2, 64, seed=77)
+    c.k.nan_to_num_(0.5)  # recycled pages, comparable
+    c.v.nan_to_num_(0.5)
+    d = c.to_device()
+    before = d["k"].clone(), d["v"].clone()
+    d["starts"] = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    lo, end = (starts[good], starts[-1]) if good < len(rows) else (c.total, c.total)
+    counts = [0] * good + [starts[i + 1] - starts[i] for i in range(good, len(rows))]
+    out = torch.full((c.total, 4, 64), -77.0, dtype=torch.float16, device="cuda")
+    if op == "prefill":
+        launch(tsg, ctx, c, op, d=d, out=out, uniform=False)
+    else:
+        attn = plan(tsg, ctx, c)
+        kv = torch.randn(c.total, 2, 64, device="cuda").half()
+        attn.encode_append(attn.cache(d["k"], d["v"]),
+                           attn.batch(d["table"], d["lengths"], c.total, d["starts"]), d["q"], kv, kv,
+                           tsg.HeadNormRope(), out)
+    with pytest.raises(tsg.TsgError) as e:
+        ctx.synchronize()
+    assert e.value.status == 1 and "row starts" in str(e.value)
+    ctx.synchronize()
+    assert bool(torch.isnan(out[:lo]).all())
+    assert bool((out[end:] == -77).all())
+    if op == "prefill":
+        c.rows, c.starts = counts, torch.tensor(starts)
+        want, tol = c.attention()
+        assert_near(out[lo:end], want[lo:end], tol[lo:end])
+        return
+    same = torch.ones(before[0].shape[0], 16, dtype=torch.bool)
+    for s, n in enumerate(counts):
+        for i in range(n):
+            row, pos = starts[s] + i, c.lengths[s] - n + i
+            assert torch.equal(out[row], d["q"][row] if pos >= 0 else torch.zeros_like(out[row]))
+            if pos >= 0:
+                page, slot = c.slot(s, pos)
+                same[page, slot] = False
+                assert torch.equal(d["k"][page, :, slot], kv[row])
+    where = same.cuda()[:, None, :, None].expand_as(before[0])
+    assert torch.equal(d["k"][where], before[0][where])
+    assert torch.equal(d["v"][where], before[1][where])
+
+
+@pytest.mark.parametrize("op", ["prefill", "append"])
+def test_bad_row_starts_far_back(tsg, ctx, op):  # noqa: F811
+    """The fall lies more than 64 sequences before the last; a row behind that belongs to none."""
+    c = Case([1] * 200, [4] * 200, 2, 1, 32, seed=78)
+    d = c.to_device()
+    d["starts"] = torch.arange(0, 201, dtype=torch.int32, device="cuda").clamp(max=199)
+    d["starts"][50] = 48
+    out = torch.full((200, 2, 32), -77.0, dtype=torch.float16, device="cuda")
+    if op == "prefill":
+        launch(tsg, ctx, c, op, d=d, out=out, uniform=False)
+    else:
+        attn = plan(tsg, ctx, c)
+        kv = torch.zeros(200, 32, dtype=torch.float16, device="cuda")
+        attn.encode_append(attn.cache(d["k"], d["v"]),
+                           attn.batch(d["table"], d["lengths"], 200, d["starts"]), d["q"], kv, kv,
+                           tsg.HeadNormRope(), out)
+    with pytest.raises(tsg.TsgError) as e:
+        ctx.synchronize()
+    assert "row starts" in str(e.value)
+    assert bool((out[199] == -77).all()) and bool(torch.isfinite(out[48:199]).all())
+    assert bool(torch.isnan(out[:48]).all())

@@ -282,10 +282,13 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
         f1 = *reinterpret_cast<const f4a4_t*>(a.inv_freq + 8u * j + 4u);
     }
 
-    const uint32_t s = find_seq(a.row_starts, a.num_seqs, a.seq_rows, a.rows, row, a.error);
-    if (s >= a.num_seqs) return;
+    bool broken;
+    const uint32_t s =
+        find_seq(a.row_starts, a.num_seqs, a.seq_rows, a.rows, row, a.error, &broken);
+    if (s >= a.num_seqs && !broken) return;
     const uint32_t capacity = a.table_stride << a.page_shift;
-    const SeqRows sr = seq_rows(a.row_starts, a.lengths, s, a.seq_rows, a.rows, capacity);
+    const SeqRows sr = broken ? SeqRows{0u, row, 1u, 0u, kErrAttnRows}
+                              : seq_rows(a.row_starts, a.lengths, s, a.seq_rows, a.rows, capacity);
     const int32_t pos = (int32_t)sr.length - (int32_t)sr.count + (int32_t)(row - sr.first);
     bool drop = sr.bad || pos < 0;  // nothing to append; the query row becomes zeros (NaN)
     if (sr.bad && lane == 0) report(a.error, sr.bad);

@@ -92,27 +92,33 @@ __device__ __forceinline__ SeqRows seq_rows(const uint32_t* row_starts, const ui
 __device__ __forceinline__ void report(uint32_t* error, uint32_t bit) { atomicOr(error, bit); }
 
 // The sequence that holds `row` (uniform over the wave), or num_seqs: with row
-// starts the first s whose end lies past the row, 64 of them at a time. The
-// waves of row 0 look at all of them and report starts that fall or pass the
-// batch's rows.
+// starts the last s that starts at or before the row, 64 of them at a time from
+// the last. Starts that fall or pass the batch's rows make those before them
+// meaningless: a row before the sequences behind the last such one is `broken`.
+// The waves of row 0 look at all starts and report.
 __device__ __forceinline__ uint32_t find_seq(const uint32_t* row_starts, uint32_t num_seqs,
                                              uint32_t uniform, uint32_t rows, uint32_t row,
-                                             uint32_t* error) {
+                                             uint32_t* error, bool* broken) {
+    *broken = false;
     if (!row_starts) return row / uniform;
     const uint32_t lane = threadIdx.x & 63u;
     uint32_t found = num_seqs;
+    bool done = false;
     for (uint32_t base = 0; base < num_seqs; base += 64u) {
-        const uint32_t s = base + lane;
-        const bool live = s < num_seqs;
+        const bool live = base + lane < num_seqs;
+        const uint32_t s = live ? num_seqs - 1u - (base + lane) : 0u;
         const uint32_t lo = live ? row_starts[s] : 0u, hi = live ? row_starts[s + 1u] : 0u;
-        const uint64_t past = __ballot(live && hi > row);
-        if (row == 0u && __ballot(lo > hi || hi > rows) && lane == 0) report(error, kErrAttnRows);
-        if (past && found == num_seqs) {
-            const int at = __builtin_ctzll(past);
-            found = base + (uint32_t)at;
-            if ((uint32_t)__builtin_amdgcn_readlane((int)lo, at) > row) return num_seqs;
-            if (row != 0u) break;
+        const uint64_t wrong = __ballot(lo > hi || hi > rows);
+        const uint64_t from = __ballot(live && lo <= row);
+        if (row == 0u && wrong && lane == 0) report(error, kErrAttnRows);
+        if (!done && (from | wrong)) {
+            done = true;
+            const int at = __builtin_ctzll(from | wrong);
+            *broken = wrong >> at & 1u;
+            if (!*broken && (uint32_t)__builtin_amdgcn_readlane((int)hi, at) > row)
+                found = num_seqs - 1u - (base + (uint32_t)at);
         }
+        if (done && row != 0u) break;
     }
     return found;
 }

@@ -49,52 +49,70 @@ constexpr uint32_t prefill_lds_bytes() {
     return 2u * 2u * kTileKeys<DP> * DP * 2u + kRows * DP / 4u;  // + marks
 }
 
-// The row tile of workgroup `at`, counted from the last: sequences from the
-// last to the first, a sequence's tiles from its last (most keys first).
-// Uniform over the wave; false past the first.
+// The row tile of workgroup `at` of a key head, counted from the last: sequences
+// from the last to the first, a sequence's tiles from its last (most keys first).
+// Uniform over the wave; kind 0 past the first. Starts that fall or pass the
+// batch's rows make those before them meaningless: the workgroups after the tiles
+// of the sequences behind the last such one leave NaN in all rows before those
+// (kind 2; workgroup `tile` of `count`, rows under `seq`). Workgroup 0 looks at
+// all starts and reports.
 struct RowTile {
-    uint32_t seq, tile;
+    uint32_t kind, seq, tile, count;
 };
-__device__ __forceinline__ bool find_tile(const PrefillArgs& p, uint32_t at, bool check,
-                                          RowTile* out) {
+__device__ __forceinline__ RowTile find_tile(const PrefillArgs& p, uint32_t at, uint32_t blocks,
+                                             bool check) {
     const AttnArgs& a = p.a;
-    if (!a.row_starts) {
-        out->seq = a.num_seqs - 1u - at / p.seq_tiles;
-        out->tile = p.seq_tiles - 1u - at % p.seq_tiles;
-        return at / p.seq_tiles < a.num_seqs;
-    }
+    if (!a.row_starts)
+        return RowTile{at / p.seq_tiles < a.num_seqs ? 1u : 0u, a.num_seqs - 1u - at / p.seq_tiles,
+                       p.seq_tiles - 1u - at % p.seq_tiles, 0u};
     const uint32_t lane = threadIdx.x & 63u;
-    bool found = false;
+    uint32_t behind = 0;  // tiles of the sequences behind these 64
+    RowTile r{0u, 0u, 0u, 0u};
     for (uint32_t base = 0; base < a.num_seqs; base += 64u) {
-        const uint32_t back = base + lane;
-        const bool live = back < a.num_seqs;
-        const uint32_t s = live ? a.num_seqs - 1u - back : 0u;
+        const bool live = base + lane < a.num_seqs;
+        const uint32_t s = live ? a.num_seqs - 1u - (base + lane) : 0u;
         const uint32_t lo = live ? a.row_starts[s] : 0u, hi = live ? a.row_starts[s + 1u] : 0u;
-        if (check && __ballot(lo > hi || hi > a.rows) && lane == 0) report(a.error, kErrAttnRows);
-        if (found) continue;
-        const uint32_t end = hi < a.rows ? hi : a.rows;
-        const uint32_t n = end > lo ? end - lo : 0u;
-        const uint32_t tiles = (n * a.group + kRows - 1u) / kRows;
+        const uint64_t wrong = __ballot(lo > hi || hi > a.rows);
+        if (check && wrong && lane == 0) report(a.error, kErrAttnRows);
+        if (r.kind) continue;
+        const int last_wrong = wrong ? __builtin_ctzll(wrong) : 64;
+        const uint32_t tiles =
+            (int)lane < last_wrong ? ((hi - lo) * a.group + kRows - 1u) / kRows : 0u;
         uint32_t sum = tiles;  // inclusive over the lanes
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const uint32_t v = (uint32_t)__shfl_up((int)sum, (unsigned)o, 64);
             if (lane >= (uint32_t)o) sum += v;
         }
-        const uint64_t past = __ballot(sum > at);
+        const uint64_t past = __ballot(behind + sum > at);
         if (past) {
             const int l = __builtin_ctzll(past);
-            const uint32_t before = (uint32_t)__builtin_amdgcn_readlane((int)(sum - tiles), l);
-            const uint32_t count = (uint32_t)__builtin_amdgcn_readlane((int)tiles, l);
-            out->seq = a.num_seqs - 1u - (base + (uint32_t)l);
-            out->tile = count - 1u - (at - before);
-            found = true;
-            if (!check) return true;
+            const uint32_t end = behind + (uint32_t)__builtin_amdgcn_readlane((int)sum, l);
+            r = RowTile{1u, a.num_seqs - 1u - (base + (uint32_t)l), end - 1u - at, 0u};
         } else {
-            at -= (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+            behind += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+            if (wrong)  // its end is where the next, right one starts
+                r = RowTile{2u,
+                            base == 0u && last_wrong == 0
+                                ? a.rows
+                                : (uint32_t)__builtin_amdgcn_readlane((int)hi, last_wrong),
+                            at - behind, blocks - behind};
         }
+        if (r.kind && !check) break;
     }
-    return found;
+    return r;
+}
+
+// NaN in a key head's part of rows `first`, `first` + step, .. under `end`.
+__device__ __forceinline__ void poison_rows(const AttnArgs& a, uint32_t kvh, uint32_t first,
+                                            uint32_t step, uint32_t end) {
+    const uint32_t pieces = a.group * a.dim / 8u;
+    const uint32_t nan2 = 0x7E007E00u;
+    for (uint64_t row = first; row < end; row += step)
+        for (uint32_t n = threadIdx.x; n < pieces; n += blockDim.x)
+            *reinterpret_cast<uint4*>(a.out + row * a.out_stride +
+                                      (uint64_t)kvh * a.group * a.dim + 8u * n) =
+                make_uint4(nan2, nan2, nan2, nan2);
 }
 
 // What a row tile's workgroups share: positions of its rows and the part of the
@@ -150,8 +168,11 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
     const uint32_t split = blockIdx.y;
     const uint32_t kvh = blockIdx.x % a.kv_heads;
     const uint32_t at = blockIdx.x / a.kv_heads;
-    RowTile rt;
-    if (!find_tile(p, at, at == 0u && split == 0u, &rt)) return;
+    const RowTile rt = find_tile(p, at, gridDim.x / a.kv_heads, at == 0u && split == 0u);
+    if (rt.kind != 1u) {
+        if (rt.kind == 2u && split == 0u) poison_rows(a, kvh, rt.tile, rt.count, rt.seq);
+        return;
+    }
     const uint32_t s = rt.seq;
     const uint32_t capacity = a.table_stride << a.page_shift;
     const SeqRows sr = seq_rows(a.row_starts, a.lengths, s, a.seq_rows, a.rows, capacity);
@@ -536,8 +557,8 @@ __global__ __launch_bounds__(256) void prefill_join_kernel(PrefillArgs p) {
     constexpr uint32_t C8 = DP / 8u, PIECES = kJoinRows * C8;
     const AttnArgs& a = p.a;
     const uint32_t kvh = blockIdx.x % a.kv_heads;
-    RowTile rt;
-    if (!find_tile(p, blockIdx.x / a.kv_heads, false, &rt)) return;
+    const RowTile rt = find_tile(p, blockIdx.x / a.kv_heads, gridDim.x / a.kv_heads, false);
+    if (rt.kind != 1u) return;
     const SeqRows sr = seq_rows(a.row_starts, a.lengths, rt.seq, a.seq_rows, a.rows,
                                 a.table_stride << a.page_shift);
     const TilePlan<DP> t = tile_plan<DP>(p, sr, rt.tile);

@@ -179,8 +179,8 @@ constexpr DeviceError kDeviceErrors[] = {
     {kErrAttnLength, TSG_ERR_INVALID_ARGUMENT,
      "attention: a sequence longer than its page table; its rows are NaN or not appended"},
     {kErrAttnRows, TSG_ERR_INVALID_ARGUMENT,
-     "attention: row starts that fall or pass the batch's rows; the rows of those sequences are "
-     "NaN or not appended"},
+     "attention: row starts that fall or pass the batch's rows; the rows before the sequences "
+     "behind the last such one are NaN and not appended"},
     {kErrGroupExpertRange, TSG_ERR_GROUPING_EXPERT_OUT_OF_RANGE,
      "expertOutOfRange: the device grouping met a route expert id >= numExperts; those pairs were "
      "not grouped"},
