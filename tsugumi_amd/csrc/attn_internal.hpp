@@ -239,7 +239,8 @@ __device__ __forceinline__ float sum_across16(float v) {
 
 // 16 bytes a lane from memory straight into LDS at `lds` + 16 x lane. Issued as
 // asm: the compiler would wait for it before any LDS read. It returns no
-// register; a wait on vector memory and a barrier come before the data is read.
+// register; a wait on vector memory and a barrier come before the data is
+// read. Nothing else in these kernels uses m0.
 __device__ __forceinline__ void dma16(const uint8_t* base, uint32_t lane_off, uint32_t lds) {
     asm volatile(
         "s_mov_b32 m0, %0\n\t"
@@ -247,7 +248,7 @@ __device__ __forceinline__ void dma16(const uint8_t* base, uint32_t lane_off, ui
         "global_load_lds_dwordx4 %1, %2"
         :
         : "s"(lds), "v"(lane_off), "s"(base)
-        : "memory", "m0");
+        : "memory");
 }
 
 // Until at most N of the wave's loads are outstanding (they complete in order),
