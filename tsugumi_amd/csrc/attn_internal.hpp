@@ -240,7 +240,9 @@ __device__ __forceinline__ float sum_across16(float v) {
 // 16 bytes a lane from memory straight into LDS at `lds` + 16 x lane. Issued as
 // asm: the compiler would wait for it before any LDS read. It returns no
 // register; a wait on vector memory and a barrier come before the data is
-// read. Nothing else in these kernels uses m0.
+// read. m0 is reserved to single instructions (the compiler holds no value in it
+// and takes it in no clobber list), and no other here reads it: LDS accesses
+// do not from gfx9 on.
 __device__ __forceinline__ void dma16(const uint8_t* base, uint32_t lane_off, uint32_t lds) {
     asm volatile(
         "s_mov_b32 m0, %0\n\t"
