@@ -139,3 +139,40 @@ def test_decode_more_key_tiles_than_32_bits_count(tsg, ctx):  # noqa: F811
     attn.encode_decode(attn.cache(k, torch.ones_like(k)), attn.batch(table, lengths, seqs), q, out)
     ctx.synchronize()
     assert bool((out == 1).all())
+
+
+@pytest.mark.parametrize("op", ["decode", "prefill"])
+@pytest.mark.parametrize("dim", [64, 80, 128, 256, 512])
+@pytest.mark.parametrize("kv", ["f16", "e4m3"])
+@pytest.mark.parametrize("window", [0, 45])
+def test_single_elements_that_a_row_does_not_see(tsg, ctx, op, dim, kv, window):  # noqa: F811
+    """+inf, -inf and NaN in one element each of tokens that some of the rows see (e4m3 has NaN
+    only), in a short sequence and in one that is split: they reach their element of the rows
+    that see them and nothing else. 140 rows of two heads take the prefill kernel at any width."""
+    rows = 4 if op == "decode" else 140
+    c = Case([rows] * 2, [rows + 90, 1500], 2, 1, dim, kv=kv, page=64, window=window, seed=dim)
+    bad = [float("inf"), -float("inf"), float("nan")]
+    places = [(2, dim - 1), (rows // 2, dim // 2 + 5), (rows // 2 + 44, 3)]  # before the last row
+    for s, length in enumerate(c.lengths):
+        for value, (back, element) in zip(bad, places):
+            i, j = c.slot(s, length - back)
+            if kv == "e4m3":
+                c.v.view(torch.uint8)[i, 0, j, element] = 0x7F
+            else:
+                c.v[i, 0, j, element] = value
+    got = launch(tsg, ctx, c, op, uniform=True)
+    ctx.synchronize()
+    want, tol = c.attention()
+    seen = ~torch.isfinite(want)
+    assert bool(seen.any()) and int(seen.sum(-1).max()) <= 3 and int(seen.sum(-1).min()) < 3
+    assert_near(got, want, tol, op)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+@pytest.mark.parametrize("dim", [64, 512])
+def test_prefill_scales(tsg, ctx, scale, dim):  # noqa: F811
+    c = Case([270], [300], 2, 1, dim, page=64, seed=61, scale=scale)
+    got = launch(tsg, ctx, c, "prefill", uniform=True)
+    ctx.synchronize()
+    want, tol = c.attention()
+    assert_near(got, want, tol)
