@@ -539,17 +539,21 @@ extern "C" tsg_status tsg_attn_decode(tsg_attn* attn, tsg_stream stream, const t
 // Few rows of wide heads, and so few tiles of them that most of the card would
 // idle: the decode kernel splits the keys finer. One sequence, heads of 512 (16
 // query, 2 key heads), decode against prefill kernel: 32 rows of the group over 4000
-// keys 35 and 38 us, 256 rows 42 and 50, 32 over 32,000 keys 79 and 203, 256 144 and
-// 164, but 512 rows 667 and 175; heads of 256 (16, 8): 8 rows over 4000 keys 17
-// and 24, 64 rows 26 and 29, over 32,000 75 and 73, but 256 rows 181 and 110.
-// Narrower heads gain only under about 1000 keys (10 and 13) and lose beyond.
+// keys 36 and 39 us, 256 rows 42 and 50, 32 over 32,000 keys 84 and 192, 256 162 and
+// 163, but 512 rows 667 and 175; heads of 256 (16, 8): 8 rows over 4000 keys 18
+// and 24, 64 rows 26 and 29, over 32,000 62 and 73, 73 and 74, but 256 rows 181
+// and 110. More sequences, heads of 512, 32 rows over 32,000 keys: 4 (16 tiles) 123 and
+// 161, 16 (64) 401 and 442; 256 rows: 4 (128) 670 and 268. Heads of 256: 4 of 8 rows
+// (32) 196 and 197, 4 of 64 (128) 321 and 205, 16 of 8 (128) 694 and 701, over 1000
+// keys 29 and 31. Narrower heads gain only under about 1000 keys (10 and 13) and lose
+// beyond.
 static bool decode_takes(const tsg_attn* attn, const AttnArgs& a) {
     if (a.row_starts || attn->padded_dim < 256u) return false;
     const uint64_t rows = (uint64_t)a.seq_rows * a.group;
     const uint64_t tiles =
         a.num_seqs * (uint64_t)a.kv_heads * ((rows + kDecodeTileRows - 1u) / kDecodeTileRows);
     return rows <= (attn->padded_dim == 256u ? 64u : 256u) &&
-           tiles <= (uint64_t)attn->ctx->num_cus / 2u;
+           tiles <= (uint64_t)attn->ctx->num_cus / 4u;
 }
 
 extern "C" tsg_status tsg_attn_prefill(tsg_attn* attn, tsg_stream stream,
