@@ -245,3 +245,31 @@ def test_bad_row_starts_far_back(tsg, ctx, op):  # noqa: F811
     assert "row starts" in str(e.value)
     assert bool((out[199] == -77).all()) and bool(torch.isfinite(out[48:199]).all())
     assert bool(torch.isnan(out[:48]).all())
+
+
+def test_outputs_that_share_elements_with_inputs(tsg, ctx):  # noqa: F811
+    """q itself is taken; q at another stride, its later rows, columns that reach into it and,
+    appending, the keys' or values' columns are refused. Columns beside q are not shared."""
+    c = Case([3], [60], 4, 2, 64, seed=79)
+    d = c.to_device()
+    attn = plan(tsg, ctx, c)
+    cache, batch = attn.cache(d["k"], d["v"]), attn.batch(d["table"], d["lengths"], 3)
+    wide = torch.zeros(8, 1024, dtype=torch.float16, device="cuda")
+    wide[:3, 256:512] = d["q"].view(3, 256)
+    q, k, v = wide[:3, 256:512], wide[:3, 512:640], wide[:3, 640:768]
+    other_stride = wide.view(-1)[256:].as_strided((3, 256), (512, 1))
+    for call in (attn.encode_decode, attn.encode_prefill):
+        for out in (wide[1:4, 256:512], wide[:3, 8:264], wide[:3, 504:760], other_stride):
+            refused(tsg, call, cache, batch, q, out, text="shares elements")
+    for out in (wide[1:4, 256:512], wide[:3, 384:640], wide[:3, 752:1008], other_stride):
+        refused(tsg, attn.encode_append, cache, batch, q, k, v, tsg.HeadNormRope(), out,
+                text="shares elements")
+    before = wide.clone()
+    torch.cuda.synchronize()
+    want, tol = c.attention()
+    for out in (wide[:3, :256], wide[:3, 768:], wide[3:6, 512:768], q):
+        for call in (attn.encode_decode, attn.encode_prefill)[out is q:]:
+            call(cache, batch, q, out)
+            ctx.synchronize()
+            assert_near(out.reshape(3, 4, 64), want, tol)
+    assert torch.equal(wide[:3, 512:768], before[:3, 512:768])

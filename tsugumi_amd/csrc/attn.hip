@@ -97,6 +97,21 @@ tsg_status check_attn_batch(const tsg_attn_config& c, const tsg_attn_batch* b) {
     return TSG_OK;
 }
 
+// Whether rows of `a` and of `b` share an element, where that is plain: rows of
+// one stride, single rows, or one address.
+static bool rows_share(const uint16_t* a, uint64_t a_stride, uint64_t a_width, const uint16_t* b,
+                       uint64_t b_stride, uint64_t b_width, uint64_t rows) {
+    const uintptr_t pa = reinterpret_cast<uintptr_t>(a) / 2u, pb = reinterpret_cast<uintptr_t>(b) / 2u;
+    if (pa == pb) return true;
+    const bool a_first = pa < pb;
+    const uint64_t apart = a_first ? pb - pa : pa - pb;
+    const uint64_t width = a_first ? a_width : b_width, other = a_first ? b_width : a_width;
+    if (rows == 1u) return apart < width;
+    if (a_stride != b_stride || apart >= (rows - 1u) * a_stride + width) return false;
+    const uint64_t off = apart % a_stride;  // of the other's row in the first's
+    return off < width || off + other > a_stride;
+}
+
 tsg_status attn_args(const tsg_attn* attn, const tsg_kv_pages* pages, const tsg_attn_batch* batch,
                      const uint16_t* q, uint32_t q_stride, uint16_t* out, uint32_t out_stride,
                      AttnArgs* a) {
@@ -113,6 +128,10 @@ tsg_status attn_args(const tsg_attn* attn, const tsg_kv_pages* pages, const tsg_
                 "out stride is too small");
     TSG_REQUIRE(is16(q) && is16(out) && q_stride % 8u == 0 && out_stride % 8u == 0,
                 TSG_ERR_ALIGNMENT, "q and out rows must be 16-byte aligned");
+    const uint32_t width = c.q_heads * c.head_dim;
+    TSG_REQUIRE((q == out && q_stride == out_stride) ||
+                    !rows_share(q, q_stride, width, out, out_stride, width, batch->rows),
+                TSG_ERR_INVALID_ARGUMENT, "out shares elements with q and is not q itself");
     a->q = q;
     a->out = out;
     a->k = static_cast<const uint8_t*>(pages->k);
@@ -458,6 +477,15 @@ extern "C" tsg_status tsg_attn_append(tsg_attn* attn, tsg_stream stream, const t
                     rows->q_stride % 8u == 0 && rows->k_stride % 8u == 0 &&
                     rows->v_stride % 8u == 0 && q_out_stride % 8u == 0,
                 TSG_ERR_ALIGNMENT, "q, k and v rows must be 16-byte aligned");
+    TSG_REQUIRE((rows->q == q_out && rows->q_stride == q_out_stride) ||
+                    !rows_share(rows->q, rows->q_stride, q_width, q_out, q_out_stride, q_width,
+                                batch->rows),
+                TSG_ERR_INVALID_ARGUMENT, "q_out shares elements with q and is not q itself");
+    TSG_REQUIRE(!rows_share(rows->k, rows->k_stride, kv_width, q_out, q_out_stride, q_width,
+                            batch->rows) &&
+                    !rows_share(rows->v, rows->v_stride, kv_width, q_out, q_out_stride, q_width,
+                                batch->rows),
+                TSG_ERR_INVALID_ARGUMENT, "q_out shares elements with k or v");
     TSG_REQUIRE(nr->rotary_dim <= c.head_dim && nr->rotary_dim % 16u == 0, TSG_ERR_UNSUPPORTED,
                 "rotary_dim %u: a multiple of 16 up to head_dim", nr->rotary_dim);
     TSG_REQUIRE(nr->rotary_dim == 0 || nr->inv_freq, TSG_ERR_INVALID_ARGUMENT, "inv_freq is NULL");
