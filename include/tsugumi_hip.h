@@ -774,9 +774,11 @@ typedef struct tsg_attn tsg_attn; /* one kind of attention layer and its scratch
 tsg_status tsg_attn_check(const tsg_attn_config* config, const tsg_kv_pages* pages,
                           const tsg_attn_batch* batch);
 /* Calls on one tsg_attn run in stream order (they share its scratch: 17, 34, 68 or
- * 135 MB for head sizes up to 64, 128, 256, 512); two tsg_attn may run beside each
- * other. Not while a stream is captured (it allocates). The context outlives
- * the calls. */
+ * 135 MB for head sizes up to 64, 128, 256, 512; two that overlap leave it unfit
+ * for later ones); two tsg_attn may run beside each other. Graphs captured with one
+ * are replayed one after the other, beside no other call of it, and before its
+ * end. Not while a stream is captured (it allocates). The context outlives the
+ * calls. */
 tsg_status tsg_attn_create(tsg_ctx* ctx, const tsg_attn_config* config, tsg_attn** out);
 void tsg_attn_destroy(tsg_attn* attn);
 
@@ -797,9 +799,11 @@ tsg_status tsg_attn_append(tsg_attn* attn, tsg_stream stream, const tsg_kv_pages
  * fp32; the weights are rounded to fp16 (half a step, 2^-11 of each, down to
  * 2^-25 of the largest), in the row's sum as in the product with v. What lies in
  * the cache at keys a row does not see, NaN and infinities among it, does not
- * reach the row. Returns TSG_ERR_DECLINED for more than 8 rows a sequence;
- * row_starts must be NULL. q and out rows on 16 bytes; out may be q itself (same
- * address and stride) and otherwise shares no element with it. */
+ * reach the row; an infinity among the values it sees makes its element that
+ * infinity or, where the key's weight rounds to 0, NaN. Returns TSG_ERR_DECLINED
+ * for more than 8 rows a sequence; row_starts must be NULL. q and out rows on 16
+ * bytes; out may be q itself (same address and stride) and otherwise shares no
+ * element with it. */
 tsg_status tsg_attn_decode(tsg_attn* attn, tsg_stream stream, const tsg_kv_pages* pages,
                            const tsg_attn_batch* batch, const uint16_t* q, uint32_t q_stride,
                            uint16_t* out, uint32_t out_stride);

@@ -16,8 +16,8 @@
 // splits, so the result does not depend on which one it is.
 //
 // Measured on an MI355X: one sequence of 131,001 keys, 8 key heads of 128 (537
-// MB) 117 us, 4.6 TB/s; 64 ragged sequences of up to 16,001 e4m3 keys (1.07 GB)
-// 211 us, 5.1 TB/s (a large copy: 4.9); 1001 keys, 8 heads of 256: 10.3 us, of
+// MB) 116 us, 4.6 TB/s; 64 ragged sequences of up to 16,001 e4m3 keys (1.07 GB)
+// 212 us, 5.0 TB/s (a large copy: 4.9); 1001 keys, 8 heads of 256: 10.6 us, of
 // which the join takes 3.5 and the way to the first product 3.
 #include "attn_internal.hpp"
 

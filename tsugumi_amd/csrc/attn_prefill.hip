@@ -11,9 +11,9 @@
 // flop a pair each way) and, for narrow heads, by the exponentials beside them
 // (16 cycles for 64 pairs against 0.25 D of matrix work).
 //
-// Measured on an MI355X: 8192 rows x 32 heads of 128 560-607 us over boxes, 906-984
-// TFLOP/s (a large fp16 matrix product: 1146); the matrix and the vector units
-// are each busy 46 % of the time, without bank conflicts.
+// Measured on an MI355X: 8192 rows x 32 heads of 128 574-594 us over boxes, 926-958
+// TFLOP/s (a large fp16 matrix product: 1306); the matrix units are busy 47 % of
+// the time and the vector units 41 %, without bank conflicts.
 //
 // Where the rows are few and the keys many, the keys are split over several
 // workgroups, and a second kernel joins their sums in the order of the splits.
