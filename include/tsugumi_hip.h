@@ -786,9 +786,9 @@ void tsg_attn_destroy(tsg_attn* attn);
  * q_out (fp16), k heads -> the cache, v heads -> the cache (not rotated):
  *   y = x * w / sqrt(mean(x^2) + eps), then (a cos t - b sin t, b cos t + a sin t)
  * in fp32 (the angle t in fp64) with one rounding at the end; e4m3 codes are of
- * y / scale, clamped to +-448. k and v may be the same rows. q_out may be q
- * itself (same address and stride) and otherwise shares no element with the
- * inputs. q, k, v, q_out rows on 16 bytes. */
+ * y / scale, clamped to +-448. k and v may be the same rows, the pools not the
+ * same. q_out may be q itself (same address and stride) and otherwise shares no
+ * element with the inputs. q, k, v, q_out rows on 16 bytes. */
 tsg_status tsg_attn_append(tsg_attn* attn, tsg_stream stream, const tsg_kv_pages* pages,
                            const tsg_attn_batch* batch, const tsg_attn_rows* rows,
                            const tsg_attn_norm_rope* norm_rope, uint16_t* q_out,

@@ -273,3 +273,20 @@ def test_outputs_that_share_elements_with_inputs(tsg, ctx):  # noqa: F811
             ctx.synchronize()
             assert_near(out.reshape(3, 4, 64), want, tol)
     assert torch.equal(wide[:3, 512:768], before[:3, 512:768])
+
+
+def test_append_to_one_pool_for_both(tsg, ctx):  # noqa: F811
+    """Rotated keys and plain values would go to the same slots; reading it as both is fine."""
+    c = Case([1], [40], 2, 1, 64, seed=80)
+    c.v = c.k
+    d = c.to_device()
+    attn = plan(tsg, ctx, c)
+    cache, batch = attn.cache(d["k"], d["k"]), attn.batch(d["table"], d["lengths"], 1)
+    out = torch.empty_like(d["q"])
+    attn.encode_decode(cache, batch, d["q"], out)
+    ctx.synchronize()
+    want, tol = c.attention()
+    assert_near(out, want, tol)
+    rows = torch.zeros(1, 64, dtype=torch.float16, device="cuda")
+    refused(tsg, attn.encode_append, cache, batch, d["q"], rows, rows, tsg.HeadNormRope(), out,
+            text="two pools")

@@ -466,6 +466,8 @@ extern "C" tsg_status tsg_attn_append(tsg_attn* attn, tsg_stream stream, const t
     const tsg_attn_config& c = attn->cfg;
     if (tsg_status s = check_attn_pages(c, pages)) return s;
     if (tsg_status s = check_attn_batch(c, batch)) return s;
+    TSG_REQUIRE(pages->k != pages->v, TSG_ERR_INVALID_ARGUMENT,
+                "append writes two pools: keys and values have one address");
     TSG_REQUIRE(rows && nr && rows->q && rows->k && rows->v && q_out, TSG_ERR_INVALID_ARGUMENT,
                 "NULL append operand");
     const uint32_t q_width = c.q_heads * c.head_dim, kv_width = c.kv_heads * c.head_dim;
