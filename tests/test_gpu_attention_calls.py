@@ -290,3 +290,18 @@ def test_append_to_one_pool_for_both(tsg, ctx):  # noqa: F811
     rows = torch.zeros(1, 64, dtype=torch.float16, device="cuda")
     refused(tsg, attn.encode_append, cache, batch, d["q"], rows, rows, tsg.HeadNormRope(), out,
             text="two pools")
+
+
+def test_one_row_in_place_at_two_strides(tsg, ctx):  # noqa: F811
+    """A single row has no second one that its stride could place in q."""
+    c = Case([1], [60], 4, 2, 64, seed=81)
+    d = c.to_device()
+    attn = plan(tsg, ctx, c)
+    cache, batch = attn.cache(d["k"], d["v"]), attn.batch(d["table"], d["lengths"], 1)
+    want, tol = c.attention()
+    wide = torch.zeros(4, 1024, dtype=torch.float16, device="cuda")
+    for call in (attn.encode_decode, attn.encode_prefill):
+        wide[0, :256] = d["q"].view(256)
+        call(cache, batch, wide[:, :256], wide.view(-1)[:512].view(2, 256))
+        ctx.synchronize()
+        assert_near(wide[:1, :256].reshape(1, 4, 64), want, tol)

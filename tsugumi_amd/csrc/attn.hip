@@ -129,7 +129,7 @@ tsg_status attn_args(const tsg_attn* attn, const tsg_kv_pages* pages, const tsg_
     TSG_REQUIRE(is16(q) && is16(out) && q_stride % 8u == 0 && out_stride % 8u == 0,
                 TSG_ERR_ALIGNMENT, "q and out rows must be 16-byte aligned");
     const uint32_t width = c.q_heads * c.head_dim;
-    TSG_REQUIRE((q == out && q_stride == out_stride) ||
+    TSG_REQUIRE((q == out && (q_stride == out_stride || batch->rows == 1u)) ||
                     !rows_share(q, q_stride, width, out, out_stride, width, batch->rows),
                 TSG_ERR_INVALID_ARGUMENT, "out shares elements with q and is not q itself");
     a->q = q;
@@ -479,7 +479,7 @@ extern "C" tsg_status tsg_attn_append(tsg_attn* attn, tsg_stream stream, const t
                     rows->q_stride % 8u == 0 && rows->k_stride % 8u == 0 &&
                     rows->v_stride % 8u == 0 && q_out_stride % 8u == 0,
                 TSG_ERR_ALIGNMENT, "q, k and v rows must be 16-byte aligned");
-    TSG_REQUIRE((rows->q == q_out && rows->q_stride == q_out_stride) ||
+    TSG_REQUIRE((rows->q == q_out && (rows->q_stride == q_out_stride || batch->rows == 1u)) ||
                     !rows_share(rows->q, rows->q_stride, q_width, q_out, q_out_stride, q_width,
                                 batch->rows),
                 TSG_ERR_INVALID_ARGUMENT, "q_out shares elements with q and is not q itself");
