@@ -813,6 +813,115 @@ tsg_status tsg_attn_prefill(tsg_attn* attn, tsg_stream stream, const tsg_kv_page
                             const tsg_attn_batch* batch, const uint16_t* q, uint32_t q_stride,
                             uint16_t* out, uint32_t out_stride);
 
+/* ----------------------------------------------------- gated delta rule ---
+ * The token mixer of a layer that keeps a state instead of a key/value cache,
+ * between the layer's projections: a short causal convolution with SiLU, whose
+ * output rows hold the queries, keys and values, and the gated delta rule. No
+ * counterpart entries: the reference's own are outside this library's path.
+ *
+ * For every value head, with its key head's q and k,
+ *   q^ = scale q / sqrt(sum q^2 + eps), k^ = k / sqrt(sum k^2 + eps),
+ *   e = exp(-exp(a_log) softplus(a + dt_bias)), beta = sigmoid(b):
+ *   S <- e S;  u = beta (v - S^T k^);  S <- S + k^ u^T;  out = S^T q^
+ * row after row of a sequence, S [key_dim, value_dim] in fp32.
+ *
+ * A sequence's state is read from slot in_slots[s] of the caller's pool
+ * (TSG_NO_SLOT: zeros) and written to out_slots[s] (TSG_NO_SLOT: not kept); the
+ * two may be the same slot, and several sequences may read one (a prefix's state
+ * from which they go on). A sequence without rows hands its state on as it is.
+ *
+ * in_slots, out_slots and row_starts are read on the device, so a captured graph
+ * replays with what they then hold. Of a sequence with a slot past the pool, or
+ * whose out slot is another sequence's in or out slot, the rows are NaN and no
+ * state is written; row starts that fall or pass `rows` make all rows of the
+ * call NaN, and nothing is written to the pool; tsg_ctx_synchronize reports
+ * TSG_ERR_INVALID_ARGUMENT. Rows before the first sequence's and behind the
+ * last's are left as they were. An infinity or NaN in a row reaches no row before
+ * it and no other sequence; where the rule would spread it over part of the
+ * elements of its head, more of them may be NaN. */
+#define TSG_NO_SLOT 0xFFFFFFFFu
+
+/* One kind of layer. value_heads a multiple of key_heads (value head h reads key
+ * head h / (value_heads / key_heads)), at most 256; key_dim a multiple of 16 up to
+ * 256, value_dim of 16 up to 512; conv_width, the inputs of one output, 2...8.
+ * channels = 2 key_heads key_dim + value_heads value_dim. |scale| up to 1e6; eps
+ * 1e-12...1. */
+typedef struct tsg_delta_config {
+    uint32_t key_heads, value_heads, key_dim, value_dim, conv_width;
+    float scale, eps;
+} tsg_delta_config;
+
+/* The state pools, caller-owned. Element (i, j) of value head h of slot n is at
+ * s + n * slot_stride + (h * key_dim + i) * value_dim + j, fp32; input j (the oldest
+ * first) of channel c at conv + n * conv_stride + j * channels + c, fp16, of
+ * conv_width - 1 inputs. Strides in elements, multiples of 16 bytes. Either pool
+ * may be NULL where no call reads it. */
+typedef struct tsg_delta_states {
+    float* s;
+    uint16_t* conv;
+    uint64_t slot_stride, conv_stride;
+    uint32_t num_slots;
+} tsg_delta_states;
+
+/* The sequences of one call: as in tsg_attn_batch, with up to 65,536 of them.
+ * kept: 1, the state behind a sequence's last row goes to out_slots[s]; or, of up to 8
+ * rows of every sequence (no row starts), their number: the state behind row i goes
+ * to out_slots[s * kept + i] (a speculative block that may be taken in part). A
+ * slot twice in one sequence's list holds the later row's. */
+typedef struct tsg_delta_batch {
+    const uint32_t* row_starts;
+    const uint32_t* in_slots;
+    const uint32_t* out_slots;
+    uint32_t num_seqs, rows, kept;
+} tsg_delta_batch;
+
+/* Rows, fp16: row r of q at q + r * q_stride (elements), heads key_dim (v:
+ * value_dim) apart; a and b have value_heads elements a row. q, k, v may lie in the
+ * convolution's output, a and b in one buffer. */
+typedef struct tsg_delta_rows {
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    const uint16_t* a;
+    const uint16_t* b;
+    uint32_t q_stride, k_stride, v_stride, a_stride, b_stride;
+} tsg_delta_rows;
+
+typedef struct tsg_delta tsg_delta; /* one kind of layer */
+
+/* The checks the entry points below make of these arguments, without a device (all
+ * but the config may be NULL: not checked). */
+tsg_status tsg_delta_check(const tsg_delta_config* config, const tsg_delta_states* states,
+                           const tsg_delta_batch* batch, const tsg_delta_rows* rows);
+/* Holds no device memory: calls of one tsg_delta may run beside each other, if
+ * their slots and scratch differ. The context outlives the calls. */
+tsg_status tsg_delta_create(tsg_ctx* ctx, const tsg_delta_config* config, tsg_delta** out);
+void tsg_delta_destroy(tsg_delta* delta);
+
+/* out[t, c] = silu(sum_j w[c, j] x[t - conv_width + 1 + j, c]), inputs before the
+ * call's rows from the slot; the slot gets the last conv_width - 1 inputs. x, out
+ * [rows, channels] fp16, rows on 16 bytes, sharing no element; weight [channels,
+ * conv_width] bf16 on 16 bytes. Sums in fp32. */
+tsg_status tsg_delta_conv(tsg_delta* delta, tsg_stream stream, const tsg_delta_states* states,
+                          const tsg_delta_batch* batch, const uint16_t* x, uint32_t x_stride,
+                          const uint16_t* weight, uint16_t* out, uint32_t out_stride);
+/* The rule for 1...8 rows of every sequence (a decoded token, a speculative
+ * block); TSG_ERR_DECLINED for more; row_starts must be NULL. a_log, dt_bias
+ * [value_heads] fp32. out [rows, value_heads * value_dim] fp16 shares no element
+ * with the rows. q, k, v, out rows on 16 bytes. All in fp32. */
+tsg_status tsg_delta_decode(tsg_delta* delta, tsg_stream stream, const tsg_delta_states* states,
+                            const tsg_delta_batch* batch, const tsg_delta_rows* rows,
+                            const float* a_log, const float* dt_bias, uint16_t* out,
+                            uint32_t out_stride);
+/* The same for any number of rows of each sequence, ragged or uniform (kept is
+ * 1). scratch: tsg_delta_prefill_scratch_bytes of device memory on 256 bytes,
+ * for this call alone until it has run. */
+size_t tsg_delta_prefill_scratch_bytes(const tsg_delta* delta, uint32_t rows, uint32_t num_seqs);
+tsg_status tsg_delta_prefill(tsg_delta* delta, tsg_stream stream, const tsg_delta_states* states,
+                             const tsg_delta_batch* batch, const tsg_delta_rows* rows,
+                             const float* a_log, const float* dt_bias, uint16_t* out,
+                             uint32_t out_stride, void* scratch, size_t scratch_bytes);
+
 /* ----------------------------------------------------------- layer tail ----
  * The Gemma decoder-layer tail after the MoE FFN, per row (fp16 h2, h1,
  * hidden; bf16 norm weights):

@@ -16,7 +16,9 @@ include/tsugumi_hip.h (libtsugumi_hip.so). Names follow the reference:
     SharedExpertInt4        -> SharedExpertInt4 (Gemma's dense int4 MLP)
 
 The attention half of the layer (Attention, PagedKVCache, AttentionBatch,
-HeadNormRope) is this library's own.
+HeadNormRope) and the gated delta rule of the layers that keep a state
+instead of a cache (GatedDelta, DeltaStates, DeltaBatch, DeltaGates) are this
+library's own.
 
 Device buffers are torch CUDA tensors (plumbing only); `stream` defaults to
 torch's current stream. Every call raises TsgError on a non-OK status; there
@@ -39,6 +41,7 @@ __all__ = [
     "PrefillRoutedGEMMPlanner", "PrefillGroupedRoutedMoE", "PrefillMoE", "ResidentLayer",
     "MoEPack", "SharedExpertInt4", "PrefillLayerTail", "FusedLayerTail", "PrefillInt4QMM",
     "Attention", "PagedKVCache", "AttentionBatch", "HeadNormRope",
+    "GatedDelta", "DeltaStates", "DeltaBatch", "DeltaGates",
     "ExpertOffsets", "TsgError", "PAIR_DTYPE", "BLOCK_DTYPE", "GROUP_DTYPE", "TILE_DTYPE",
     "generators", "load",
 ]
@@ -61,6 +64,11 @@ def _ptr(t) -> int | None:
     assert t.is_cuda, "device buffers must be CUDA (HIP) tensors"
     assert t.is_contiguous(), "device buffers must be contiguous"
     return t.data_ptr()
+
+
+def _addr(t) -> int | None:
+    """Device address of a torch tensor of any strides (None passes NULL)."""
+    return None if t is None else t.data_ptr()
 
 
 def _stream_reader():
@@ -1085,6 +1093,201 @@ class Attention:
     def close(self) -> None:
         if getattr(self, "handle", None):
             self.lib.tsg_attn_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class DeltaStates:
+    """A layer's state pools (tsg_delta_states): s of shape [slots, value_heads, key_dim,
+    value_dim] in fp32 and conv of [slots, conv_width - 1, channels] in fp16, each contiguous
+    within a slot; one may be None where no call reads it. For calls of any GatedDelta of
+    these sizes and this device."""
+
+    def __init__(self, delta: "GatedDelta", s=None, conv=None):
+        c = delta.config
+        shapes = ((s, (c.value_heads, c.key_dim, c.value_dim), _types("float32")),
+                  (conv, (c.conv_width - 1, delta.channels), delta._half))
+        slots = {int(t.shape[0]) for t, _, _ in shapes if t is not None and t.dim()}
+        if len(slots) != 1:
+            _refuse("state pools of one number of slots")
+        strides = []
+        for t, shape, types in shapes:
+            if t is None:
+                strides.append(0)
+                continue
+            if not t.is_cuda or t.device.index != delta.ctx.device:
+                _refuse("state pools must be on the context's device")
+            if t.dim() != len(shape) + 1 or tuple(t.shape[1:]) != shape or t.dtype not in types:
+                _refuse(f"a state pool of {t.dtype} {tuple(t.shape)}, not {types[0]} [slots, "
+                        f"{shape}]")
+            if t.shape[0] and not t[0].is_contiguous():
+                _refuse("a slot's elements must be contiguous")
+            strides.append(t.stride(0) if t.shape[0] > 1 else 0)
+        slots = slots.pop()
+        _words(num_slots=slots)
+        self._keep = (s, conv)
+        self.states = _abi.DeltaStates(_addr(s), _addr(conv), *strides, slots)
+        self._ref = C.addressof(self.states)
+        check(delta.lib.tsg_delta_check(C.addressof(c), self._ref, None, None))
+        self.kind = delta.state_kind
+
+
+class DeltaBatch:
+    """The sequences of one call (tsg_delta_batch): in_slots [seqs] of 32-bit integers (-1: no
+    state) and out_slots [seqs] (-1: not kept), or, for the state behind every one of a few
+    rows, [seqs * rows of one] (in any shape); row_starts [seqs + 1] for ragged rows. For calls
+    of any GatedDelta of this device."""
+
+    def __init__(self, delta: "GatedDelta", in_slots, out_slots, rows: int, row_starts=None):
+        for t in (in_slots, out_slots, row_starts):
+            if t is None:
+                continue
+            if not t.is_cuda or t.device.index != delta.ctx.device:
+                _refuse("batch tensors must be on the context's device")
+            if t.dtype not in _types("int32", "uint32") or not t.is_contiguous():
+                _refuse("batch tensors must be contiguous 32-bit integers")
+        seqs = int(in_slots.numel())
+        if in_slots.dim() != 1 or not seqs or out_slots.numel() % seqs:
+            _refuse("in_slots must be [seqs] and out_slots [seqs] or [seqs * rows]")
+        if row_starts is not None and tuple(row_starts.shape) != (seqs + 1,):
+            _refuse("row_starts must be [seqs + 1]")
+        self._keep = (in_slots, out_slots, row_starts)
+        self.rows = int(rows)
+        _words(rows=self.rows, num_seqs=seqs, kept=out_slots.numel() // seqs)
+        self.batch = _abi.DeltaBatch(_ptr(row_starts), _ptr(in_slots), _ptr(out_slots), seqs,
+                                     self.rows, out_slots.numel() // seqs)
+        self._ref = C.addressof(self.batch)
+        check(delta.lib.tsg_delta_check(C.addressof(delta.config), None, self._ref, None))
+        self.kind = ("delta", delta.ctx.device)
+
+
+class DeltaGates:
+    """A layer's decay parameters: a_log and dt_bias, fp32 [value_heads]."""
+
+    def __init__(self, a_log, dt_bias):
+        for t in (a_log, dt_bias):
+            if not t.is_cuda or t.dim() != 1 or t.dtype not in _types("float32") or \
+                    not t.is_contiguous() or t.shape != a_log.shape or t.device != a_log.device:
+                _refuse("a_log and dt_bias are fp32 [value_heads] on one device")
+        self._keep = (a_log, dt_bias)
+        self.pointers = (a_log.data_ptr(), dt_bias.data_ptr())
+        self.kind = (int(a_log.shape[0]), a_log.device.index)
+
+
+class GatedDelta:
+    """One kind of gated delta rule layer (tsg_delta): the causal convolution, decode and
+    prefill over a pool of states. scale defaults to key_dim ** -0.5. Row operands are fp16
+    tensors [rows, heads, dim] or [rows, heads * dim], rows any 16-byte multiple apart (a and
+    b, [rows, value_heads], at any stride). Work goes to `stream`, or to torch's current
+    stream of the context's device. Calls hold nothing of the plan's; those that share
+    slots or scratch are the caller's to order."""
+
+    def __init__(self, ctx: Context, key_heads: int, value_heads: int, key_dim: int,
+                 value_dim: int, conv_width: int = 4, scale: float | None = None,
+                 eps: float = 1e-6):
+        self.handle = None
+        self.ctx = ctx
+        self.lib = ctx.lib
+        _words(key_heads=key_heads, value_heads=value_heads, key_dim=key_dim,
+               value_dim=value_dim, conv_width=conv_width)
+        if scale is None:
+            scale = float(key_dim) ** -0.5 if key_dim > 0 else 1.0
+        self.config = _abi.DeltaConfig(key_heads, value_heads, key_dim, value_dim, conv_width,
+                                       scale, eps)
+        h = C.c_void_p()
+        check(self.lib.tsg_delta_create(ctx.handle, C.addressof(self.config), C.byref(h)))
+        self.handle = h
+        self.channels = 2 * key_heads * key_dim + value_heads * value_dim
+        self._half, self._device = _types("float16", "int16", "uint16"), ctx.device
+        self._layout = (key_heads, key_heads * key_dim, value_heads, value_heads * value_dim)
+        self.state_kind = (value_heads, key_dim, value_dim, conv_width, self.channels, ctx.device)
+        self._conv, self._decode, self._prefill = (
+            self.lib.tsg_delta_conv, self.lib.tsg_delta_decode, self.lib.tsg_delta_prefill)
+
+    def states(self, s=None, conv=None) -> DeltaStates:
+        return DeltaStates(self, s, conv)
+
+    def batch(self, in_slots, out_slots, rows, row_starts=None) -> DeltaBatch:
+        return DeltaBatch(self, in_slots, out_slots, rows, row_starts)
+
+    def scratch_bytes(self, rows: int, num_seqs: int) -> int:
+        """Bytes of device memory that encode_prefill needs for such a call."""
+        _words(rows=rows, num_seqs=num_seqs)
+        return int(self.lib.tsg_delta_prefill_scratch_bytes(self.handle, rows, num_seqs))
+
+    _rows = Attention._rows
+
+    def _on(self, stream):
+        if not self.ctx.handle:  # the plan points into it
+            _refuse("the layer's context is closed")
+        if stream is not None:
+            return stream if isinstance(stream, int) else stream.cuda_stream
+        return _current_stream_of(self._device)
+
+    def _fits(self, states, batch):
+        if states.kind != self.state_kind:
+            _refuse(f"states of {states.kind} (value heads, key_dim, value_dim, conv_width, "
+                    f"channels, device), not of {self.state_kind}")
+        if batch.kind != ("delta", self._device):
+            _refuse(f"a batch of {batch.kind}, not of {('delta', self._device)}")
+
+    def encode_conv(self, states, batch, x, weight, out, stream=None):
+        """The causal convolution of the batch's rows with SiLU: x [rows, channels] to out;
+        weight bf16 [channels, conv_width]."""
+        self._fits(states, batch)
+        n, width = batch.rows, self.channels
+        x, xs = self._rows(x, n, 1, width)
+        out, os = self._rows(out, n, 1, width)
+        if tuple(weight.shape) != (width, self.config.conv_width) or not weight.is_contiguous() \
+                or weight.dtype not in _types("bfloat16", "int16", "uint16") \
+                or weight.get_device() != self._device:
+            _refuse("the weight must be bf16 [channels, conv_width] on the context's device")
+        status = self._conv(self.handle, self._on(stream), states._ref, batch._ref, x, xs,
+                            weight.data_ptr(), out, os)
+        if status:
+            check(status)
+
+    def _operands(self, states, batch, q, k, v, a, b, gates, out):
+        self._fits(states, batch)
+        n, hk, kw, hv, vw = batch.rows, *self._layout
+        if gates.kind != (hv, self._device):
+            _refuse("gates must be [value_heads] on the context's device")
+        (q, qs), (k, ks) = self._rows(q, n, hk, kw), self._rows(k, n, hk, kw)
+        v, vs = self._rows(v, n, hv, vw)
+        (a, as_), (b, bs) = self._rows(a, n, hv, hv), self._rows(b, n, hv, hv)
+        out, os = self._rows(out, n, hv, vw)
+        rows = _abi.DeltaRows(q, k, v, a, b, qs, ks, vs, as_, bs)
+        return rows, (*gates.pointers, out, os)
+
+    def encode_decode(self, states, batch, q, k, v, a, b, gates, out, stream=None):
+        """The rule for 1..8 new tokens of every sequence."""
+        rows, rest = self._operands(states, batch, q, k, v, a, b, gates, out)
+        status = self._decode(self.handle, self._on(stream), states._ref, batch._ref,
+                              C.addressof(rows), *rest)
+        if status:
+            check(status)
+
+    def encode_prefill(self, states, batch, q, k, v, a, b, gates, out, scratch, stream=None):
+        """The rule for a prompt's rows, or the next chunk's. scratch: a contiguous tensor of
+        scratch_bytes(rows, seqs) bytes, this call's alone until it has run."""
+        rows, rest = self._operands(states, batch, q, k, v, a, b, gates, out)
+        if not scratch.is_cuda or scratch.get_device() != self._device or \
+                not scratch.is_contiguous():
+            _refuse("the scratch must be a contiguous tensor on the context's device")
+        status = self._prefill(self.handle, self._on(stream), states._ref, batch._ref,
+                               C.addressof(rows), *rest, scratch.data_ptr(),
+                               scratch.numel() * scratch.element_size())
+        if status:
+            check(status)
+
+    def close(self) -> None:
+        if getattr(self, "handle", None):
+            self.lib.tsg_delta_destroy(self.handle)
             self.handle = None
 
     def __del__(self):

@@ -31,6 +31,7 @@ GROUPING_ERRORS = {
 TSG_AFFINE, TSG_SYM = 0, 1
 TSG_ACT_GELU_TANH, TSG_ACT_SILU = 0, 1
 TSG_KV_F16, TSG_KV_E4M3 = 0, 1
+TSG_NO_SLOT = 0xFFFFFFFF
 
 
 class ExpertOffsets(C.Structure):
@@ -121,6 +122,30 @@ class AttnNormRope(C.Structure):
                 ("normalize_v", C.c_uint32), ("eps", C.c_float)]
 
 
+class DeltaConfig(C.Structure):
+    """tsg_delta_config: one kind of gated delta rule layer."""
+    _fields_ = [("key_heads", C.c_uint32), ("value_heads", C.c_uint32), ("key_dim", C.c_uint32),
+                ("value_dim", C.c_uint32), ("conv_width", C.c_uint32), ("scale", C.c_float),
+                ("eps", C.c_float)]
+
+
+class DeltaStates(C.Structure):
+    """tsg_delta_states: the state pools, strides in elements."""
+    _fields_ = [("s", C.c_void_p), ("conv", C.c_void_p), ("slot_stride", C.c_uint64),
+                ("conv_stride", C.c_uint64), ("num_slots", C.c_uint32)]
+
+
+class DeltaBatch(C.Structure):
+    """tsg_delta_batch: the sequences of one call."""
+    _fields_ = [("row_starts", C.c_void_p), ("in_slots", C.c_void_p), ("out_slots", C.c_void_p),
+                ("num_seqs", C.c_uint32), ("rows", C.c_uint32), ("kept", C.c_uint32)]
+
+
+class DeltaRows(C.Structure):
+    """tsg_delta_rows: query, key, value and gate rows."""
+    _fields_ = [(n, C.c_void_p) for n in "qkvab"] + [(n + "_stride", C.c_uint32) for n in "qkvab"]
+
+
 P = C.c_void_p
 U32 = C.c_uint32
 U64 = C.c_uint64
@@ -205,6 +230,13 @@ SIGNATURES = {
     "tsg_attn_append": (C.c_int, [P, P, P, P, P, P, P, U32]),
     "tsg_attn_decode": (C.c_int, [P, P, P, P, P, U32, P, U32]),
     "tsg_attn_prefill": (C.c_int, [P, P, P, P, P, U32, P, U32]),
+    "tsg_delta_check": (C.c_int, [P, P, P, P]),
+    "tsg_delta_create": (C.c_int, [P, P, C.POINTER(P)]),
+    "tsg_delta_destroy": (None, [P]),
+    "tsg_delta_conv": (C.c_int, [P, P, P, P, P, U32, P, P, U32]),
+    "tsg_delta_decode": (C.c_int, [P, P, P, P, P, P, P, P, U32]),
+    "tsg_delta_prefill_scratch_bytes": (C.c_size_t, [P, U32, U32]),
+    "tsg_delta_prefill": (C.c_int, [P, P, P, P, P, P, P, P, U32, P, C.c_size_t]),
     "tsg_prefill_layer_tail": (C.c_int, [P, P, P, P, P, P, P, U32, U32, U32, U32, U32,
                                          C.c_float, C.c_float]),
     "tsg_fused_layer_tail": (C.c_int, [P, P, P, P, P, P, P, U32, C.c_float, C.c_float]),

@@ -27,6 +27,10 @@ namespace tsg {
 constexpr uint32_t kErrAttnPage = 256u;
 constexpr uint32_t kErrAttnLength = 512u;
 constexpr uint32_t kErrAttnRows = 1024u;
+// The delta rule's: a slot past the pool or an out slot that is another
+// sequence's; wrong row starts.
+constexpr uint32_t kErrDeltaSlot = 2048u;
+constexpr uint32_t kErrDeltaRows = 4096u;
 
 constexpr uint32_t kMaxDecodeRows = 8;  // rows a sequence in a decode call (a speculative block)
 

@@ -181,6 +181,12 @@ constexpr DeviceError kDeviceErrors[] = {
     {kErrAttnRows, TSG_ERR_INVALID_ARGUMENT,
      "attention: row starts that fall or pass the batch's rows; the rows before the sequences "
      "behind the last such one are NaN and not appended"},
+    {kErrDeltaSlot, TSG_ERR_INVALID_ARGUMENT,
+     "delta rule: a slot past the pool, or a sequence's out slot that is another's in or out slot; "
+     "its rows are NaN and its state was not written"},
+    {kErrDeltaRows, TSG_ERR_INVALID_ARGUMENT,
+     "delta rule: row starts that fall or pass the batch's rows; all rows are NaN and no state was "
+     "written"},
     {kErrGroupExpertRange, TSG_ERR_GROUPING_EXPERT_OUT_OF_RANGE,
      "expertOutOfRange: the device grouping met a route expert id >= numExperts; those pairs were "
      "not grouped"},
@@ -235,7 +241,7 @@ extern "C" tsg_status tsg_ctx_synchronize(tsg_ctx* ctx, tsg_stream stream) {
         TSG_HIP_TRY(hipMemcpy(&err, word + 1, sizeof(err), hipMemcpyDeviceToHost));
     }
     tsg_status status = TSG_OK;
-    char text[2048] = "";  // all of them are 1200 characters
+    char text[2048] = "";  // all of them are under 1600 characters
     size_t at = 0;
     for (const DeviceError& e : kDeviceErrors) {
         if (!(err & e.bit)) continue;
