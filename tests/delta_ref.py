@@ -112,13 +112,13 @@ class Case:
             m = torch.zeros(self.hv, dk, self.dv, dtype=torch.float64) \
                 if self.ins[i] == NONE else self.s[self.ins[i]].double()
             err = torch.zeros(self.hv, self.dv, dtype=torch.float64)
+            bound = m.abs().amax(1)
             for j in range(rows):
                 r = first + j
                 if chunked and j % CHUNK == 0:
                     span = slice(r, first + min(rows, j + CHUNK))
-                    state_err, out_err = self._chunk_error(q[span], k[span], v[span],
-                                                           decay[span], beta[span], m)
-                    err = err + state_err
+                    state_err, out_err, bound = self._chunk_error(
+                        q[span], k[span], v[span], decay[span], beta[span], m, bound)
                 e = decay[r].exp()
                 before = m.norm(dim=1)
                 m = m * e[:, None, None]
@@ -134,6 +134,8 @@ class Case:
                     + HALF * out[r].abs() + TINY
                 if chunked:
                     tol[r] += abs(self.scale) * out_err[:, j % CHUNK]
+                    if j % CHUNK == CHUNK - 1 or j == rows - 1:  # the chunk's state is formed
+                        err = err + state_err
                 if self.every:
                     self._put(pool, pool_tol, self.outs[i * self.kept + j], m, err)
             if not self.every:
@@ -147,14 +149,19 @@ class Case:
             pool[slot] = m
             pool_tol[slot] = (err[:, None] + E24 * m.abs()).expand_as(m)
 
-    def _chunk_error(self, q, k, v, decay, beta, m):
+    def _chunk_error(self, q, k, v, decay, beta, m, bound):
         """What a chunk of rows adds to the error of a state's columns (2-norm) and of its
         outputs, per head. With A_ij = beta_i e^(Gi - Gj) k_i.k_j below the diagonal, T = (1 + A)^-1
         and u = T r, r = beta (v - e^G K S): the products over the key elements are sums in
         fp32 of operands split in two halves of fp16 (2^-21 of the sizes' products); T is off
         by |T| |A| |T| times the roundings of A (dk + 24) and of the substitution (64 + 16);
         u by |T| times r's error, T's times |r| and its own sum's. The state's columns take K^T u,
-        the outputs the weights e^(Gi - Gj) q_i.k_j, rounded to fp16 as u may be for them."""
+        the outputs the weights e^(Gi - Gj) q_i.k_j, rounded to fp16 as u may be for them.
+
+        Halves of fp16 end at steps of 2^-24, half of one off at most: S, r and u, scaled so
+        that a bound on their column lies in 2^13 ... 2^14, by `step` = 2^-25 2^-14 2 bound
+        (`before` for S, by the last chunk's bound); T and the weights, at 1024 for 1, by 2^-35;
+        u times the rows' factors by step, times keys kept with norms under 4."""
         dk = self.dk
         q, k, v = q.transpose(0, 1), k.transpose(0, 1), v.transpose(0, 1)
         beta, total = beta.T, decay.clamp(min=-1000).T.cumsum(1)
@@ -169,19 +176,27 @@ class Case:
         since = total.exp()
         r = beta[:, :, None] * (v - since[:, :, None] * (k @ m))
         split = 2.0 ** -21
+        before = bound * 2.0 ** -38
+        bound = 1.01 * dk ** 0.5 * m.abs().amax(1) + 65 * v.abs().amax(1)
+        step = (bound * 2.0 ** -38)[:, None]
+        low = torch.ones_like(lower).tril()
+        ds = dk ** 0.5 * before[:, None]
         dr = beta[:, :, None] * (4 * E24 * v.abs() + ((dk + 32) * E24 + split)
-                                 * since[:, :, None] * kn[:, :, None] * sn[:, None])
+                                 * since[:, :, None] * kn[:, :, None] * sn[:, None]
+                                 + since[:, :, None] * kn[:, :, None] * ds) + step
         ta = t.abs()
         dt = ta @ (pa.tril(-1) * (dk + 24) * E24 + a.abs() * (80 * E24)) @ ta
         u = t @ r
-        du = ta @ dr + dt @ r.abs() + (ta @ r.abs()) * (72 * E24 + 2 * split)
+        du = ta @ dr + dt @ r.abs() + (ta @ r.abs()) * (72 * E24 + 2 * split) \
+            + (low @ r.abs()) * 2.0 ** -35
         until = torch.exp(total[:, -1:] - total)[:, :, None] * kn[:, :, None]
         state = (until * du + until * u.abs() * (72 * E24 + 2 * split + 32 * E24)).sum(1) \
-            + sn * 8 * E24
-        outs = p.abs() @ du + (p.abs() @ u.abs()) * (2 * HALF + 72 * E24) + u.abs() * 2.0 ** -35 \
+            + sn * 8 * E24 + 4 * k.shape[1] * step[:, 0]
+        outs = p.abs() @ du + (p.abs() @ u.abs()) * (2 * HALF + 72 * E24) + (low @ u.abs()) * 2.0 ** -35 \
             + (lower * qn[:, :, None] * kn[:, None, :] * (dk + 24) * E24) @ u.abs() \
-            + ((dk + 32) * E24 + split) * (since * qn)[:, :, None] * sn[:, None]
-        return state, outs
+            + ((dk + 32) * E24 + split) * (since * qn)[:, :, None] * sn[:, None] \
+            + (since * qn)[:, :, None] * ds + p.abs().sum(2, keepdim=True) * step
+        return state, outs, bound
 
     def to_device(self):
         ints = lambda t: torch.tensor(t, dtype=torch.int32, device="cuda")  # noqa: E731

@@ -24,7 +24,7 @@ GEMM_SOURCES = ["gemm_g32_sym.hip", "gemm_g32_affine.hip", "gemm_g64_sym.hip",
                 "gemm_g64_affine.hip"]
 SOURCES = ["core.hip", "decode.hip", "prompt_router.hip", "qmv.hip", "shared.hip", "prefill.hip",
            "tail.hip", "attn.hip", "attn_decode.hip", "attn_prefill.hip",
-           "delta.hip",
+           "delta.hip", "delta_prefill.hip",
            *GEMM_SOURCES,
            "host_routing.cpp",
            "moepack.cpp"]

@@ -494,6 +494,14 @@ extern "C" tsg_status tsg_delta_create(tsg_ctx* ctx, const tsg_delta_config* con
     delta->group = config->value_heads / config->key_heads;
     delta->channels = channels_of(*config);
     delta->padded_key = config->key_dim <= 64u ? 64u : config->key_dim <= 128u ? 128u : 256u;
+    DeviceScope scope(ctx->device);
+    tsg_status s = scope.status == hipSuccess
+                       ? prepare_delta(delta)
+                       : fail(TSG_ERR_HIP, "device: %s", hipGetErrorString(scope.status));
+    if (s != TSG_OK) {
+        delete delta;
+        return s;
+    }
     *out = delta;
     return TSG_OK;
 }
@@ -564,7 +572,7 @@ extern "C" tsg_status tsg_delta_decode(tsg_delta* delta, tsg_stream stream,
 
 extern "C" size_t tsg_delta_prefill_scratch_bytes(const tsg_delta* delta, uint32_t rows,
                                                   uint32_t num_seqs) {
-    return delta && rows && num_seqs ? 256u : 0u;
+    return delta && rows && num_seqs ? delta_scratch_bytes(delta, rows, num_seqs) : 0u;
 }
 
 extern "C" tsg_status tsg_delta_prefill(tsg_delta* delta, tsg_stream stream,
@@ -583,5 +591,5 @@ extern "C" tsg_status tsg_delta_prefill(tsg_delta* delta, tsg_stream stream,
                 "the scratch must be 256-byte aligned");
     DeviceScope scope(delta->device);
     TSG_HIP_TRY(scope.status);
-    return launch_recurrent(delta, a, stream);
+    return launch_chunked(delta, a, scratch, stream);
 }

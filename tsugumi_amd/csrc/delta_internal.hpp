@@ -149,5 +149,10 @@ __device__ __forceinline__ DeltaTile delta_tile(const DeltaSeqs& d, uint32_t id)
 // delta.hip
 constexpr uint32_t kDeltaNan2 = 0x7E007E00u;  // two fp16 NaN
 tsg_status launch_recurrent(const tsg_delta* delta, const DeltaArgs& a, tsg_stream stream);
+// delta_prefill.hip
+tsg_status prepare_delta(const tsg_delta* delta);  // once a plan, its device current
+uint64_t delta_scratch_bytes(const tsg_delta* delta, uint32_t rows, uint32_t num_seqs);
+tsg_status launch_chunked(const tsg_delta* delta, const DeltaArgs& a, void* scratch,
+                          tsg_stream stream);
 
 }  // namespace tsg

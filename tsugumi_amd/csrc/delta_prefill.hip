@@ -1,0 +1,731 @@
+// delta_prefill.hip — the gated delta rule over a prompt's rows, 64 at a time.
+//
+// With G the decays' exponents summed from the chunk's first row, of its rows
+//   A_ij = beta_i e^(Gi - Gj) k^i.k^j (j < i),   T = (1 + A)^-1,
+//   U = T (beta (V - e^G K^ S)),
+//   O = e^G Q^ S + (e^(Gi - Gj) q^i.k^j)_(j <= i) U,   S <- e^(G_end) S + (e^(G_end - G) K^)^T U.
+// What does not need the state (T, the weights of O, the rows' factors, K^T in the
+// order of the matrix unit) a first kernel forms for all chunks at once into the
+// scratch; a second takes the state from chunk to chunk.
+//
+// The state and what goes into it keep fp32's precision: q and k are fp16 as they are
+// (their norms are factors of rows), every other operand is split into two halves of
+// fp16 (22 bits; three products where both are split), T is formed in fp32, and all
+// sums are in fp32. Only the weights of O are rounded to fp16 once, half a step of
+// 2^-11 each as O itself. fp16's range is no limit: a state's columns and U are
+// scaled by a power of two from bounds on them. |k^| <= 1, beta <= 1 and decays <= 1, so
+// a row does not lengthen a column of the state beyond |v|: columns and U stay
+// within B = sqrt(key_dim) max|S| + 65 max|v|. |T| and the weights are at most 1. What a
+// half's least step leaves out is under 2^-38 B: a state that a chunk all but forgets
+// is off by that, where row by row it would keep its 24 bits.
+#include "delta_internal.hpp"
+
+namespace tsg {
+namespace {
+
+constexpr uint32_t kChunk = 64;
+constexpr float kUnit = 1024.0f;  // T and the weights are kept times this: far from fp16's least
+
+// A chunk and value head's record: T's operand pieces (two planes) and the weights', 64
+// lanes x 16 bytes each; the rows' factors; e^G_end and how many rows count.
+// Pieces (16 rows, 32 columns) of the lower triangle: row tiles 0 and 1 need the first
+// column half, 2 and 3 both.
+constexpr uint32_t kPieces = 6, kPieceBytes = 1024;
+constexpr uint32_t kWeightsAt = 2u * kPieces * kPieceBytes;
+constexpr uint32_t kFactorsAt = kWeightsAt + kPieces * kPieceBytes;
+constexpr uint32_t kEndAt = kFactorsAt + 4u * kChunk * 4u;
+constexpr uint32_t kRecord = kEndAt + 256u;
+__device__ __forceinline__ uint32_t piece_of(uint32_t mt, uint32_t half) {
+    return mt < 2u ? mt : 2u * mt - 2u + half;
+}
+// K^T's pieces of a chunk and key head.
+template <uint32_t DKP>
+constexpr uint32_t kKeyRecord = DKP / 16u * 2u * kPieceBytes;
+
+struct ChunkArgs {
+    DeltaArgs d;
+    uint8_t* records;  // [chunk][value head]
+    uint8_t* keys;     // [chunk][key head]
+    uint32_t key_heads;
+    uint32_t slices;   // of the value elements, a head
+    uint32_t spread;   // heads' workgroups in order, not an XCD each
+};
+
+// Lane (i, g)'s eight elements of the matrix unit's operands, i = lane % 16, g = lane
+// / 16. Where an accumulator becomes the second operand of the next product, its
+// register e of the first and second 16 rows are rows 4 g + e and 16 + 4 g + e of 32:
+// the first operand takes its columns in the same order.
+__device__ __forceinline__ f4_t mfma(h8_t a, h8_t b, f4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ h8_t as_h8(uint4 u) { return __builtin_bit_cast(h8_t, u); }
+
+// x = hi + lo to 22 bits. The empty asm keeps the product that x came from out of the
+// conversion: rounded once from the exact product in one use and twice in the other, the two
+// hi would differ near ties, and lo be what is missing to another hi.
+__device__ __forceinline__ void split4(f4_t x, h4_t& hi, h4_t& lo) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float y = x[e];
+        asm("" : "+v"(y));
+        hi[e] = (_Float16)y;
+        lo[e] = (_Float16)(y - (float)hi[e]);
+    }
+}
+
+// ------------------------------------------------------- what needs no state
+
+constexpr uint32_t kLd = 68;  // floats of a row of A and T in LDS
+
+template <uint32_t DKP>
+constexpr uint32_t prepare_lds_bytes() {
+    return kChunk * (DKP + 8u) * 2u + 2u * kChunk * kLd * 4u + kChunk * (8u + 5u * 4u) + 16u;
+}
+
+template <uint32_t DKP>
+__global__ __launch_bounds__(256) void prepare_kernel(ChunkArgs p) {
+    constexpr uint32_t KS = DKP + 8u;  // halves of a key row in LDS
+    constexpr uint32_t NK = DKP / 32u;
+    extern __shared__ __align__(16) uint8_t smem[];
+    uint16_t* keys = reinterpret_cast<uint16_t*>(smem);
+    float* am = reinterpret_cast<float*>(smem + kChunk * KS * 2u);
+    float* tm = am + kChunk * kLd;
+    uint16_t* pm = reinterpret_cast<uint16_t*>(tm);  // the weights, before T is there
+    double* gs = reinterpret_cast<double*>(tm + kChunk * kLd);
+    float* g_hi = reinterpret_cast<float*>(gs + kChunk);
+    float *g_lo = g_hi + kChunk, *rk = g_lo + kChunk, *rq = rk + kChunk, *bs = rq + kChunk;
+    uint32_t* valid_at = reinterpret_cast<uint32_t*>(bs + kChunk);
+
+    const DeltaArgs& d = p.d;
+    const uint32_t head = blockIdx.y, kh = head / d.group;
+    const DeltaTile t = delta_tile<kChunk>(d.seqs, blockIdx.x);
+    const uint32_t tid = threadIdx.x, lane = tid & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t i16 = lane & 15u, g = lane >> 4;
+    if (t.kind == 2u) {
+        if (blockIdx.x == 0u && head == 0u && tid == 0u) report(d.seqs.error, kErrDeltaRows);
+        const uint32_t pieces = d.value_dim / 8u;
+        for (uint32_t n = tid; n < t.count * pieces; n += 256u)
+            *reinterpret_cast<uint4*>(d.out + (uint64_t)(t.first + n / pieces) * d.out_stride +
+                                      head * d.value_dim + n % pieces * 8u) =
+                make_uint4(kDeltaNan2, kDeltaNan2, kDeltaNan2, kDeltaNan2);
+        return;
+    }
+    if (t.count == 0u) return;
+    uint8_t* record = p.records + ((uint64_t)blockIdx.x * d.value_heads + head) * kRecord;
+
+    // rows: four threads each; norms, gates, keys to LDS
+    if (tid == 0u) *valid_at = t.count;
+    __syncthreads();
+    const uint32_t r = tid >> 2, part = tid & 3u;
+    const uint32_t row = t.first + (r < t.count ? r : t.count - 1u);
+    {
+        const uint16_t* k = d.k + (uint64_t)row * d.k_stride + kh * d.key_dim;
+        const uint16_t* q = d.q + (uint64_t)row * d.q_stride + kh * d.key_dim;
+        float kk = 0.0f, qq = 0.0f;
+        uint32_t wrong = 0;
+#pragma unroll
+        for (uint32_t n = 0; n < DKP / 32u; ++n) {
+            const uint32_t c = 8u * (part + 4u * n);
+            uint4 u = make_uint4(0, 0, 0, 0), w = u;
+            if (c < d.key_dim) {
+                u = *reinterpret_cast<const uint4*>(k + c);
+                w = *reinterpret_cast<const uint4*>(q + c);
+            }
+            if (r >= t.count) u = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(keys + r * KS + c) = u;
+            const uint32_t us[4] = {u.x, u.y, u.z, u.w}, ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                wrong |= not_finite<false>(us[e]);
+                const h2_t a = __builtin_bit_cast(h2_t, us[e]), b = __builtin_bit_cast(h2_t, ws[e]);
+                kk = __builtin_fmaf((float)a[0], (float)a[0], kk);
+                kk = __builtin_fmaf((float)a[1], (float)a[1], kk);
+                qq = __builtin_fmaf((float)b[0], (float)b[0], qq);
+                qq = __builtin_fmaf((float)b[1], (float)b[1], qq);
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            kk += __shfl_xor(kk, o, 64);
+            qq += __shfl_xor(qq, o, 64);
+            wrong |= (uint32_t)__shfl_xor((int)wrong, o, 64);
+        }
+        if (part == 0u) {
+            // far rows lose their decays to cancellation in 32 bits: exponents (of two) in 64
+            const double av = (double)f16_to_f32(d.a[(uint64_t)row * d.a_stride + head]) +
+                              (double)d.dt_bias[head];
+            const float bv = f16_to_f32(d.b[(uint64_t)row * d.b_stride + head]);
+            const double soft = (av > 0.0 ? av : 0.0) + log1p(exp(-fabs(av)));
+            double x = -exp((double)d.a_log[head]) * soft * 1.4426950408889634;
+            const float beta = 1.0f / (1.0f + expf(-bv));
+            if (av != av || x != x || beta != beta || wrong) {
+                if (r < t.count) atomicMin(valid_at, r);
+            }
+            // a decay of 2^-1500 is 0, and sums of 64 stay exact to 2^-35
+            if (x < -1500.0) x = -1500.0;
+            gs[r] = x;
+            bs[r] = beta;
+            rk[r] = 1.0f / sqrtf(kk + d.eps);
+            rq[r] = 1.0f / sqrtf(qq + d.eps);
+        }
+    }
+    __syncthreads();
+    const uint32_t valid = *valid_at;
+    if (r >= valid)
+        for (uint32_t n = 0; n < DKP / 32u; ++n)
+            *reinterpret_cast<uint4*>(keys + r * KS + 8u * (part + 4u * n)) = make_uint4(0, 0, 0, 0);
+    if (wave == 0u) {
+        const bool in = lane < valid;
+        double sum = in ? gs[lane] : 0.0;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const double up = __shfl_up(sum, (unsigned)o, 64);
+            if ((int)lane >= o) sum += up;
+        }
+        const double end = __shfl(sum, 63, 64);
+        g_hi[lane] = (float)sum;
+        g_lo[lane] = (float)(sum - (double)(float)sum);
+        float* f = reinterpret_cast<float*>(record + kFactorsAt) + lane;
+        const float since = exp2f((float)sum), until = exp2f((float)(end - sum));
+        const float beta = bs[lane], k1 = rk[lane];
+        // K^T is kept with norms of 2 ... 4, so that U times this stays in fp16's range, and
+        // neither's elements near its least
+        const int e = __builtin_amdgcn_frexp_expf(1.0f / k1);
+        f[0] = in ? beta : 0.0f;
+        f[64] = in ? beta * since * k1 : 0.0f;
+        f[128] = in ? since * rq[lane] * d.scale : 0.0f;
+        f[192] = in ? until * __builtin_amdgcn_ldexpf(k1, e - 2) : 0.0f;
+        if (!in) bs[lane] = rk[lane] = rq[lane] = 0.0f;  // no NaN into the triangles
+        if (lane == 0u) {
+            float* last = reinterpret_cast<float*>(record + kEndAt);
+            last[0] = exp2f((float)end);
+            last[1] = __uint_as_float(valid);
+        }
+    }
+    __syncthreads();
+
+    // products of the rows' 16-row tiles: K K^T and Q K^T on and below the diagonal
+    {
+        f4_t kk[4], qk[4];
+#pragma unroll
+        for (uint32_t n = 0; n < 4u; ++n) kk[n] = qk[n] = f4_t{0, 0, 0, 0};
+        const uint32_t mine = 16u * wave + i16;
+        const uint32_t q_row = t.first + (mine < t.count ? mine : t.count - 1u);
+        const uint16_t* q = d.q + (uint64_t)q_row * d.q_stride + kh * d.key_dim;
+#pragma unroll
+        for (uint32_t st = 0; st < NK; ++st) {
+            const uint32_t c = 32u * st + 8u * g;
+            uint4 qu = make_uint4(0, 0, 0, 0);
+            if (c < d.key_dim) qu = *reinterpret_cast<const uint4*>(q + c);
+            const h8_t ka = *reinterpret_cast<const h8_t*>(keys + mine * KS + c), qa = as_h8(qu);
+#pragma unroll
+            for (uint32_t n = 0; n < 4u; ++n) {
+                if (n > wave) continue;
+                const h8_t kb = *reinterpret_cast<const h8_t*>(keys + (16u * n + i16) * KS + c);
+                kk[n] = mfma(ka, kb, kk[n]);
+                qk[n] = mfma(qa, kb, qk[n]);
+            }
+        }
+#pragma unroll
+        for (uint32_t n = 0; n < 4u; ++n) {
+            const uint32_t j = 16u * n + i16;
+            if (n > wave) {
+                if ((n ^ 1u) != wave) continue;  // the other half of a piece
+#pragma unroll
+                for (uint32_t e = 0; e < 4u; ++e) pm[(16u * wave + 4u * g + e) * 72u + j] = 0;
+                continue;
+            }
+            const float hj = g_hi[j], lj = g_lo[j], kj = rk[j];
+#pragma unroll
+            for (uint32_t e = 0; e < 4u; ++e) {
+                const uint32_t i = 16u * wave + 4u * g + e;
+                const float apart = (g_hi[i] - hj) + (g_lo[i] - lj);
+                const float w = exp2f(i >= j ? apart : 0.0f) * kj;
+                am[i * kLd + j] = i > j ? bs[i] * rk[i] * w * kk[n][e] : 0.0f;
+                const float x = i >= j && i < valid ? rq[i] * w * kUnit * qk[n][e] : 0.0f;
+                pm[i * 72u + j] = f32_to_f16(x);
+            }
+        }
+    }
+    __syncthreads();
+    for (uint32_t n = wave; n < kPieces; n += 4u) {
+        const uint32_t mt = n < 2u ? n : 2u + (n - 2u) / 2u, half = n < 2u ? 0u : n % 2u;
+        const uint16_t* src = pm + (16u * mt + i16) * 72u + 32u * half + 4u * g;
+        const uint2 lo = *reinterpret_cast<const uint2*>(src), hi = *reinterpret_cast<const uint2*>(src + 16);
+        *reinterpret_cast<uint4*>(record + kWeightsAt + n * kPieceBytes + lane * 16u) =
+            make_uint4(lo.x, lo.y, hi.x, hi.y);
+    }
+    if (head % d.group == 0u) {
+        uint8_t* to = p.keys + ((uint64_t)blockIdx.x * p.key_heads + kh) * kKeyRecord<DKP>;
+        for (uint32_t n = wave; n < DKP / 8u; n += 4u) {
+            const uint32_t c = 16u * (n / 2u) + i16;
+            h8_t x;
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e) {
+                const uint32_t at = 32u * (n % 2u) + 16u * (e / 4u) + 4u * g + e % 4u;
+                const int ex = __builtin_amdgcn_frexp_expf(1.0f / rk[at]);
+                x[e] = (_Float16)__builtin_amdgcn_ldexpf(
+                    f16_to_f32(keys[at * KS + c]), 2 - ex);
+            }
+            *reinterpret_cast<h8_t*>(to + n * kPieceBytes + lane * 16u) = x;
+        }
+    }
+    __syncthreads();
+
+    // T: the diagonal tiles by substitution, a column a lane, ...
+    {
+        float x[16];
+#pragma unroll
+        for (uint32_t i = 0; i < 16u; ++i) {
+            float y = i == i16 ? 1.0f : 0.0f;
+            const float* a = am + (16u * wave + i) * kLd + 16u * wave;
+#pragma unroll
+            for (uint32_t j = 0; j < i; ++j) y = __builtin_fmaf(-a[j], x[j], y);
+            x[i] = y;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 16u; ++i)
+            if (i / 4u == g) tm[(16u * wave + i) * kLd + 16u * wave + i16] = x[i];
+        if (wave == 0u || wave == 2u) {  // beside them zeros, the other half of a piece
+#pragma unroll
+            for (uint32_t e = 0; e < 4u; ++e)
+                tm[(16u * wave + 4u * g + e) * kLd + 16u * wave + 16u + i16] = 0.0f;
+        }
+    }
+    __syncthreads();
+    // ... then T_21 = -T_22 A_21 T_11, of tiles of 16 and of 32. Tile products in fp32.
+    const auto first4 = [&](const float* m, uint32_t mt, uint32_t kt) {
+        return *reinterpret_cast<const f4_t*>(m + (16u * mt + i16) * kLd + 16u * kt + 4u * g);
+    };
+    const auto from_lds = [&](f4_t c, const float* a, uint32_t mt, uint32_t kt, const float* b,
+                              uint32_t nt) {
+        const f4_t x = first4(a, mt, kt);
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e)
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                x[e], b[(16u * kt + 4u * g + e) * kLd + 16u * nt + i16], c, 0, 0, 0);
+        return c;
+    };
+    const auto from_regs = [&](f4_t c, const float* a, uint32_t mt, uint32_t kt, f4_t b) {
+        const f4_t x = first4(a, mt, kt);
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e)
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], b[e], c, 0, 0, 0);
+        return c;
+    };
+    const auto put = [&](f4_t y, uint32_t mt, uint32_t nt) {
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e) tm[(16u * mt + 4u * g + e) * kLd + 16u * nt + i16] = -y[e];
+    };
+    const f4_t none = f4_t{0, 0, 0, 0};
+    if (wave < 2u) {
+        const uint32_t b = 2u * wave;
+        put(from_regs(none, tm, b + 1u, b + 1u, from_lds(none, am, b + 1u, b, tm, b)), b + 1u, b);
+    }
+    __syncthreads();
+    {
+        const uint32_t mt = 2u + (wave >> 1), nt = wave & 1u;
+        f4_t x2 = from_lds(none, am, 2u, 1u, tm, nt), x3 = from_lds(none, am, 3u, 1u, tm, nt);
+        if (nt == 0u) {
+            x2 = from_lds(x2, am, 2u, 0u, tm, 0u);
+            x3 = from_lds(x3, am, 3u, 0u, tm, 0u);
+        }
+        f4_t y = from_regs(none, tm, mt, 2u, x2);
+        if (mt == 3u) y = from_regs(y, tm, 3u, 3u, x3);
+        put(y, mt, nt);
+    }
+    __syncthreads();
+    for (uint32_t n = wave; n < kPieces; n += 4u) {
+        const uint32_t mt = n < 2u ? n : 2u + (n - 2u) / 2u, half = n < 2u ? 0u : n % 2u;
+        const float* src = tm + (16u * mt + i16) * kLd + 32u * half + 4u * g;
+        h4_t hi[2], lo[2];
+#pragma unroll
+        for (uint32_t e = 0; e < 2u; ++e)
+            split4(*reinterpret_cast<const f4_t*>(src + 16u * e) * kUnit, hi[e], lo[e]);
+        h4_t* to = reinterpret_cast<h4_t*>(record + n * kPieceBytes + lane * 16u);
+        to[0] = hi[0];
+        to[1] = hi[1];
+        to += kPieces * kPieceBytes / 8u;
+        to[0] = lo[0];
+        to[1] = lo[1];
+    }
+}
+
+// ------------------------------------------------------- from chunk to chunk
+//
+// A workgroup takes 16 value elements of a sequence and head, its four waves 16 of a
+// chunk's rows and a quarter of the state's key rows each: the state stays in their
+// registers, and what one wave's products need of the others' goes through LDS as
+// operands of the matrix unit, three exchanges a chunk: S, then R = beta (V - e^G K^ S),
+// then U. Operands of the next chunk are loaded as soon as this one's are used.
+
+template <uint32_t DKP>
+__global__ __launch_bounds__(256) void scan_kernel(ChunkArgs p) {
+    constexpr uint32_t NK = DKP / 32u, TW = DKP / 64u;  // key steps, state tiles of a wave
+    constexpr uint32_t SHARE = 2u * kPieceBytes;        // two planes of a piece
+    __shared__ __align__(16) uint8_t s_at[NK * SHARE];
+    __shared__ __align__(16) uint8_t r_at[2u * SHARE];
+    __shared__ __align__(16) uint8_t u_at[2u * SHARE];   // U, for the outputs
+    __shared__ __align__(16) uint8_t w_at[2u * SHARE];   // U times the rows' factors, for the state
+    __shared__ __align__(16) float most[16][8];          // [column][wave]: |S|; |v|
+    __shared__ float rare[16][8];
+
+    const DeltaArgs& d = p.d;
+    const uint32_t lane = threadIdx.x & 63u, i16 = lane & 15u, g = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // Workgroups go to the XCDs in turn: those of one key head share its rows there.
+    const uint32_t inner = d.group * p.slices;
+    uint32_t unit = blockIdx.x / inner, at = blockIdx.x % inner;
+    if (!p.spread) {
+        const uint32_t j = blockIdx.x >> 3;
+        unit = j / inner * 8u + (blockIdx.x & 7u);
+        at = j % inner;
+    }
+    const uint32_t s = unit / p.key_heads, kh = unit % p.key_heads;
+    if (s >= d.seqs.num_seqs) return;
+    const uint32_t head = kh * d.group + at / p.slices, c0 = at % p.slices * 16u;
+    if (starts_wrong(d.seqs)) return;  // reported, and the rows made NaN, by the first kernel
+    const DeltaSeq sq = delta_seq(d.seqs, s);
+    const bool bad = out_slots_clash(d.seqs, s) || sq.bad;
+    const uint32_t col = head * d.value_dim + c0 + i16;
+    if (bad) {
+        if (at == 0u && kh == 0u && threadIdx.x == 0u) report(d.seqs.error, kErrDeltaSlot);
+        for (uint32_t r = threadIdx.x >> 4; r < sq.count; r += 16u)
+            d.out[(uint64_t)(sq.first + r) * d.out_stride + col] = (uint16_t)kDeltaNan2;
+        return;
+    }
+
+    // the state: tile t of the wave's, register e is key row 16 (TW wave + t) + 4 g + e
+    const uint64_t place = (uint64_t)head * d.key_dim * d.value_dim + c0 + i16;
+    f4_t st[TW];
+#pragma unroll
+    for (uint32_t t = 0; t < TW; ++t)
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e) {
+            const uint32_t kr = 16u * (TW * wave + t) + 4u * g + e;
+            st[t][e] = !sq.fresh && kr < d.key_dim
+                           ? d.s[(uint64_t)sq.in * d.slot_stride + place + kr * d.value_dim]
+                           : 0.0f;
+        }
+    const auto column_most = [&] {
+        float m = 0.0f;
+#pragma unroll
+        for (uint32_t t = 0; t < TW; ++t)
+#pragma unroll
+            for (uint32_t e = 0; e < 4u; ++e) m = fmaxf(m, fabsf(st[t][e]));
+        return max_across32(max_across16(m));
+    };
+
+    const uint32_t chunks = (sq.count + kChunk - 1u) / kChunk;
+    const uint32_t chunk0 = delta_tile_base<kChunk>(d.seqs, sq, s);
+    const auto record = [&](uint32_t c) {
+        return p.records + ((uint64_t)(chunk0 + c) * d.value_heads + head) * kRecord;
+    };
+    const bool two = wave >= 2u;  // the wave's rows see both halves of the chunk's
+
+    h8_t kf[NK], qf[NK], th[2], tl[2], pf[2], kt[TW][2];
+    f4_t f_v, f_s, f_q, f_u;  // the rows' factors: of v, of K S, of Q S, of U
+    uint32_t vb[4];
+    float end_decay = 0.0f, end_next = 0.0f;
+    uint32_t valid = 0, valid_next = 0;
+    const auto load_rows = [&](uint32_t c) {
+        const uint32_t r = kChunk * c + 16u * wave + i16;
+        const uint32_t row = sq.first + (r < sq.count ? r : sq.count - 1u);
+        const uint16_t* k = d.k + (uint64_t)row * d.k_stride + kh * d.key_dim + 4u * g;
+        const uint16_t* q = d.q + (uint64_t)row * d.q_stride + kh * d.key_dim + 4u * g;
+#pragma unroll
+        for (uint32_t st_ = 0; st_ < NK; ++st_) {
+            uint2 a[4];
+#pragma unroll
+            for (uint32_t h = 0; h < 2u; ++h) {
+                const bool in = 32u * st_ + 16u * h < d.key_dim;
+                const uint32_t o = in ? 32u * st_ + 16u * h : 0u;
+                a[h] = *reinterpret_cast<const uint2*>(k + o);
+                a[2u + h] = *reinterpret_cast<const uint2*>(q + o);
+                // the state has zeros there, but K and Q may have infinities where they wrap
+                if (!in) a[h] = a[2u + h] = make_uint2(0, 0);
+            }
+            kf[st_] = as_h8(make_uint4(a[0].x, a[0].y, a[1].x, a[1].y));
+            qf[st_] = as_h8(make_uint4(a[2].x, a[2].y, a[3].x, a[3].y));
+        }
+    };
+    const auto load_t = [&](uint32_t c) {
+        const uint8_t* r = record(c) + lane * 16u;
+#pragma unroll
+        for (uint32_t h = 0; h < 2u; ++h) {
+            if (h && !two) continue;
+            const uint8_t* x = r + piece_of(wave, h) * kPieceBytes;
+            th[h] = *reinterpret_cast<const h8_t*>(x);
+            tl[h] = *reinterpret_cast<const h8_t*>(x + kPieces * kPieceBytes);
+        }
+    };
+    const auto load_p = [&](uint32_t c) {
+        const uint8_t* r = record(c) + kWeightsAt + lane * 16u;
+#pragma unroll
+        for (uint32_t h = 0; h < 2u; ++h)
+            if (!h || two) pf[h] = *reinterpret_cast<const h8_t*>(r + piece_of(wave, h) * kPieceBytes);
+        const uint8_t* k = p.keys + ((uint64_t)(chunk0 + c) * p.key_heads + kh) * kKeyRecord<DKP> +
+                           lane * 16u;
+#pragma unroll
+        for (uint32_t t = 0; t < TW; ++t)
+#pragma unroll
+            for (uint32_t h = 0; h < 2u; ++h)
+                kt[t][h] = *reinterpret_cast<const h8_t*>(
+                    k + ((TW * wave + t) * 2u + h) * kPieceBytes);
+        const float* f = reinterpret_cast<const float*>(record(c) + kFactorsAt) + 16u * wave + 4u * g;
+        f_q = *reinterpret_cast<const f4_t*>(f + 128);
+        f_u = *reinterpret_cast<const f4_t*>(f + 192);
+    };
+    const auto load_v = [&](uint32_t c) {
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e) {
+            const uint32_t r = kChunk * c + 16u * wave + 4u * g + e;
+            const uint32_t row = sq.first + (r < sq.count ? r : sq.count - 1u);
+            vb[e] = d.v[(uint64_t)row * d.v_stride + col];
+        }
+        const float* f = reinterpret_cast<const float*>(record(c) + kFactorsAt) + 16u * wave + 4u * g;
+        f_v = *reinterpret_cast<const f4_t*>(f);
+        f_s = *reinterpret_cast<const f4_t*>(f + 64);
+        const float* last = reinterpret_cast<const float*>(record(c) + kEndAt);
+        end_next = last[0];
+        valid_next = __float_as_uint(last[1]);
+    };
+    // a split value's planes as the second operand: the wave's tile of 16 rows
+    const auto share = [&](uint8_t* to, uint32_t tile, f4_t x) {
+        h4_t hi, lo;
+        split4(x, hi, lo);
+        uint8_t* o = to + tile / 2u * SHARE + lane * 16u + tile % 2u * 8u;
+        *reinterpret_cast<h4_t*>(o) = hi;
+        *reinterpret_cast<h4_t*>(o + kPieceBytes) = lo;
+    };
+    const auto shared_piece = [&](const uint8_t* from, uint32_t step, uint32_t plane) {
+        return *reinterpret_cast<const h8_t*>(from + step * SHARE + plane * kPieceBytes + lane * 16u);
+    };
+
+    // a column's scale: a power of two that takes its bound to 2^14 at most
+    int exponent = 0;
+    const float reach = sqrtf((float)d.key_dim) * 1.01f;
+    if (chunks) {
+        load_rows(0u);
+        load_t(0u);
+        load_p(0u);
+        load_v(0u);
+        const float m = column_most();
+        if (g == 0u) most[i16][wave] = m;
+        lds_barrier();
+        const f4_t a = *reinterpret_cast<const f4_t*>(&most[i16][0]);
+        exponent = __builtin_amdgcn_frexp_expf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])));
+        exponent = exponent > -100 ? exponent : -100;
+        lds_barrier();
+    }
+#pragma unroll 1
+    for (uint32_t c = 0; c < chunks; ++c) {
+        const uint32_t next = c + 1u < chunks ? c + 1u : c;
+        end_decay = end_next;
+        valid = valid_next;
+        const uint32_t r0 = 16u * wave + 4u * g;  // the lane's rows of the chunk: r0 .. r0 + 3
+        const uint32_t rows = sq.count - kChunk * c;
+
+        // S, and the sizes of its columns and of the values
+        const float to_s = __builtin_amdgcn_ldexpf(1.0f, 14 - exponent);
+        const float from_s = __builtin_amdgcn_ldexpf(1.0f, exponent - 14);
+#pragma unroll
+        for (uint32_t t = 0; t < TW; ++t) share(s_at, TW * wave + t, st[t] * to_s);
+        {
+            uint32_t bits = 0;
+#pragma unroll
+            for (uint32_t e = 0; e < 4u; ++e) {
+                const uint32_t b = r0 + e < rows ? vb[e] & 0x7FFFu : 0u;
+                bits = bits > b ? bits : b;
+            }
+            // infinities and NaN count as infinity
+            const float mv = max_across32(max_across16(
+                bits < 0x7C00u ? f16_to_f32((uint16_t)bits) : __builtin_inff()));
+            const float ms = column_most();
+            if (g == 0u) {
+                most[i16][wave] = ms;
+                most[i16][4u + wave] = mv;
+            }
+        }
+        lds_barrier();
+        f4_t ks = {0, 0, 0, 0}, qs = {0, 0, 0, 0};
+        const f4_t ma = *reinterpret_cast<const f4_t*>(&most[i16][0]);
+        const f4_t mb = *reinterpret_cast<const f4_t*>(&most[i16][4]);
+#pragma unroll
+        for (uint32_t n = 0; n < NK; ++n) {
+            const h8_t hi = shared_piece(s_at, n, 0u), lo = shared_piece(s_at, n, 1u);
+            ks = mfma(kf[n], hi, ks);
+            qs = mfma(qf[n], hi, qs);
+            ks = mfma(kf[n], lo, ks);
+            qs = mfma(qf[n], lo, qs);
+        }
+        load_rows(next);
+        float v_most = fmaxf(fmaxf(mb[0], mb[1]), fmaxf(mb[2], mb[3]));
+        uint32_t first_bad = kChunk;  // row of the column's first infinity or NaN
+        if (__ballot(v_most == __builtin_inff())) {  // the same in all waves
+            uint32_t from = kChunk;
+            float fine = 0.0f;
+#pragma unroll
+            for (uint32_t e = 0; e < 4u; ++e) {
+                if (r0 + e >= rows) continue;
+                const uint32_t b = vb[e] & 0x7FFFu;
+                if (b >= 0x7C00u) from = from < r0 + e ? from : r0 + e;
+                else fine = fmaxf(fine, f16_to_f32((uint16_t)b));
+            }
+            fine = max_across32(max_across16(fine));
+            const float first = -max_across32(max_across16(-(float)from));
+            if (g == 0u) {
+                rare[i16][wave] = first;
+                rare[i16][4u + wave] = fine;
+            }
+            lds_barrier();
+            v_most = 0.0f;
+#pragma unroll
+            for (uint32_t w = 0; w < 4u; ++w) {
+                const uint32_t b = (uint32_t)rare[i16][w];
+                first_bad = first_bad < b ? first_bad : b;
+                v_most = fmaxf(v_most, rare[i16][4u + w]);
+            }
+            lds_barrier();
+        }
+        const uint32_t good = valid < first_bad ? valid : first_bad;
+        const float bound = fmaxf(fmaxf(ma[0], ma[1]), fmaxf(ma[2], ma[3])) * reach + 65.0f * v_most;
+        exponent = __builtin_amdgcn_frexp_expf(bound);
+        exponent = exponent > -100 ? exponent : -100;
+        const float to_u = __builtin_amdgcn_ldexpf(1.0f, 14 - exponent);
+        const float from_u = __builtin_amdgcn_ldexpf(1.0f, exponent - 14);
+
+        f4_t x;
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e)
+            x[e] = r0 + e < good ? (f_v[e] * f16_to_f32((uint16_t)vb[e]) - f_s[e] * (ks[e] * from_s)) * to_u
+                                 : 0.0f;
+        share(r_at, wave, x);
+        load_v(next);
+        lds_barrier();
+        f4_t u = {0, 0, 0, 0}, u2 = {0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t h = 0; h < 2u; ++h) {
+            if (h && !two) continue;
+            const h8_t hi = shared_piece(r_at, h, 0u), lo = shared_piece(r_at, h, 1u);
+            u = mfma(th[h], hi, u);
+            u2 = mfma(tl[h], hi, u2);
+            u2 = mfma(th[h], lo, u2);
+        }
+        load_t(next);
+        u = (u + u2) * (1.0f / kUnit);
+        share(u_at, wave, u);
+        share(w_at, wave, u * f_u);
+        lds_barrier();
+        f4_t o = {0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t h = 0; h < 2u; ++h) {
+            if (h && !two) continue;
+            o = mfma(pf[h], shared_piece(u_at, h, 0u), o);
+            o = mfma(pf[h], shared_piece(u_at, h, 1u), o);
+        }
+        f4_t more[TW];
+#pragma unroll
+        for (uint32_t t = 0; t < TW; ++t) more[t] = f4_t{0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t h = 0; h < 2u; ++h) {
+            const h8_t hi = shared_piece(w_at, h, 0u), lo = shared_piece(w_at, h, 1u);
+#pragma unroll
+            for (uint32_t t = 0; t < TW; ++t) {
+                more[t] = mfma(kt[t][h], hi, more[t]);
+                more[t] = mfma(kt[t][h], lo, more[t]);
+            }
+        }
+        const float o_u = d.scale * (1.0f / kUnit) * from_u;
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e) {
+            if (r0 + e >= rows) continue;
+            const float y = f_q[e] * (qs[e] * from_s) + o[e] * o_u;
+            d.out[(uint64_t)(sq.first + kChunk * c + r0 + e) * d.out_stride + col] =
+                r0 + e < good ? f32_to_f16(y) : (uint16_t)kDeltaNan2;
+        }
+        const bool lost = first_bad < kChunk || valid < (rows < kChunk ? rows : kChunk);
+#pragma unroll
+        for (uint32_t t = 0; t < TW; ++t)
+#pragma unroll
+            for (uint32_t e = 0; e < 4u; ++e) {
+                st[t][e] = end_decay * st[t][e] + more[t][e] * from_u;
+                if (lost) st[t][e] = __builtin_nanf("");
+            }
+        load_p(next);
+    }
+    const uint32_t slot = scalar_load(d.seqs.out_slots + s);
+    if (slot == TSG_NO_SLOT) return;
+#pragma unroll
+    for (uint32_t t = 0; t < TW; ++t)
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e) {
+            const uint32_t kr = 16u * (TW * wave + t) + 4u * g + e;
+            if (kr < d.key_dim)
+                d.s[(uint64_t)slot * d.slot_stride + place + kr * d.value_dim] = st[t][e];
+        }
+}
+
+template <uint32_t DKP>
+constexpr uint64_t chunk_bytes(uint64_t value_heads, uint64_t key_heads) {
+    return value_heads * kRecord + key_heads * kKeyRecord<DKP>;
+}
+
+template <uint32_t DKP>
+tsg_status launch(const tsg_delta* delta, ChunkArgs p, uint32_t chunks, tsg_stream stream) {
+    p.keys = p.records + (uint64_t)chunks * p.d.value_heads * kRecord;
+    hipLaunchKernelGGL(prepare_kernel<DKP>, dim3(chunks, p.d.value_heads), dim3(256),
+                       prepare_lds_bytes<DKP>(), as_stream(stream), p);
+    if (tsg_status s = check_launch("delta_prepare")) return s;
+    const uint64_t units = (uint64_t)p.d.seqs.num_seqs * p.key_heads;
+    const uint64_t inner = (uint64_t)p.d.group * p.slices;
+    p.spread = units % 8u && units < 64u ? 1u : 0u;
+    const uint64_t blocks = p.spread ? units * inner : (units + 7u) / 8u * 8u * inner;
+    TSG_REQUIRE(blocks <= kMaxBlocks, TSG_ERR_UNSUPPORTED,
+                "too many sequences and heads for one launch");
+    hipLaunchKernelGGL(scan_kernel<DKP>, dim3((uint32_t)blocks), dim3(256), 0, as_stream(stream), p);
+    return check_launch("delta_scan");
+}
+
+}  // namespace
+
+uint64_t delta_scratch_bytes(const tsg_delta* delta, uint32_t rows, uint32_t num_seqs) {
+    const uint64_t chunks = (uint64_t)rows / kChunk + num_seqs;
+    const uint64_t hv = delta->cfg.value_heads, hk = delta->cfg.key_heads;
+    return chunks * (delta->padded_key == 64u    ? chunk_bytes<64>(hv, hk)
+                     : delta->padded_key == 128u ? chunk_bytes<128>(hv, hk)
+                                                 : chunk_bytes<256>(hv, hk));
+}
+
+tsg_status prepare_delta(const tsg_delta* delta) {
+    const auto kernel = delta->padded_key == 64u    ? prepare_kernel<64>
+                        : delta->padded_key == 128u ? prepare_kernel<128>
+                                                    : prepare_kernel<256>;
+    const uint32_t lds = delta->padded_key == 64u    ? prepare_lds_bytes<64>()
+                         : delta->padded_key == 128u ? prepare_lds_bytes<128>()
+                                                     : prepare_lds_bytes<256>();
+    TSG_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    return TSG_OK;
+}
+
+tsg_status launch_chunked(const tsg_delta* delta, const DeltaArgs& a, void* scratch,
+                          tsg_stream stream) {
+    ChunkArgs p{};
+    p.d = a;
+    p.records = static_cast<uint8_t*>(scratch);
+    p.key_heads = delta->cfg.key_heads;
+    p.slices = a.value_dim / 16u;
+    const uint32_t chunks = delta_tiles<kChunk>(a.seqs.rows, a.seqs.num_seqs, a.seqs.seq_rows,
+                                                a.seqs.row_starts != nullptr);
+    TSG_REQUIRE((uint64_t)chunks * a.value_heads <= kMaxBlocks, TSG_ERR_UNSUPPORTED,
+                "too many rows and heads for one launch");
+    switch (delta->padded_key) {
+        case 64: return launch<64>(delta, p, chunks, stream);
+        case 128: return launch<128>(delta, p, chunks, stream);
+        default: return launch<256>(delta, p, chunks, stream);
+    }
+}
+
+}  // namespace tsg
