@@ -38,9 +38,13 @@ constexpr uint32_t kRecord = kEndAt + 256u;
 __device__ __forceinline__ uint32_t piece_of(uint32_t mt, uint32_t half) {
     return mt < 2u ? mt : 2u * mt - 2u + half;
 }
-// K^T's pieces of a chunk and key head.
+// Pieces of a chunk and key head: K^T's, then K's and Q's (16 rows, 32 elements). In this
+// order a wave's load is 1 KiB in a row; the rows as they lie, in 32-byte parts, took the
+// address unit three times as long as all else together (8192 rows x 32 heads: 405 us for 230).
 template <uint32_t DKP>
-constexpr uint32_t kKeyRecord = DKP / 16u * 2u * kPieceBytes;
+constexpr uint32_t kRowsAt = DKP / 16u * 2u * kPieceBytes;
+template <uint32_t DKP>
+constexpr uint32_t kKeyRecord = kRowsAt<DKP> + 2u * 4u * (DKP / 32u) * kPieceBytes;
 
 struct ChunkArgs {
     DeltaArgs d;
@@ -270,6 +274,25 @@ __global__ __launch_bounds__(256) void prepare_kernel(ChunkArgs p) {
             }
             *reinterpret_cast<h8_t*>(to + n * kPieceBytes + lane * 16u) = x;
         }
+        to += kRowsAt<DKP> + lane * 16u;
+        const uint32_t mine = 16u * wave + i16;
+        const uint32_t q_row = t.first + (mine < t.count ? mine : t.count - 1u);
+        const uint16_t* q = d.q + (uint64_t)q_row * d.q_stride + kh * d.key_dim;
+#pragma unroll
+        for (uint32_t st = 0; st < NK; ++st) {
+            uint2 a[4];
+#pragma unroll
+            for (uint32_t h = 0; h < 2u; ++h) {
+                const uint32_t c = 32u * st + 16u * h + 4u * g;
+                a[h] = *reinterpret_cast<const uint2*>(keys + mine * KS + c);
+                a[2u + h] = make_uint2(0, 0);
+                if (c < d.key_dim) a[2u + h] = *reinterpret_cast<const uint2*>(q + c);
+            }
+            uint8_t* at = to + (wave * NK + st) * kPieceBytes;
+            *reinterpret_cast<uint4*>(at) = make_uint4(a[0].x, a[0].y, a[1].x, a[1].y);
+            *reinterpret_cast<uint4*>(at + 4u * NK * kPieceBytes) =
+                make_uint4(a[2].x, a[2].y, a[3].x, a[3].y);
+        }
     }
     __syncthreads();
 
@@ -370,6 +393,9 @@ __global__ __launch_bounds__(256) void scan_kernel(ChunkArgs p) {
     __shared__ __align__(16) uint8_t w_at[2u * SHARE];   // U times the rows' factors, for the state
     __shared__ __align__(16) float most[16][8];          // [column][wave]: |S|; |v|
     __shared__ float rare[16][8];
+    // The wave's 16 rows and columns of V or O, between the lane's place in memory (four
+    // elements of row lane / 4) and in the matrix unit: one access of 8 bytes a lane for four of 2.
+    __shared__ __align__(16) uint16_t turned_[4][16][20];
 
     const DeltaArgs& d = p.d;
     const uint32_t lane = threadIdx.x & 63u, i16 = lane & 15u, g = lane >> 4;
@@ -389,6 +415,7 @@ __global__ __launch_bounds__(256) void scan_kernel(ChunkArgs p) {
     const DeltaSeq sq = delta_seq(d.seqs, s);
     const bool bad = out_slots_clash(d.seqs, s) || sq.bad;
     const uint32_t col = head * d.value_dim + c0 + i16;
+    const uint32_t col4 = head * d.value_dim + c0 + 4u * (lane & 3u);
     if (bad) {
         if (at == 0u && kh == 0u && threadIdx.x == 0u) report(d.seqs.error, kErrDeltaSlot);
         for (uint32_t r = threadIdx.x >> 4; r < sq.count; r += 16u)
@@ -399,15 +426,6 @@ __global__ __launch_bounds__(256) void scan_kernel(ChunkArgs p) {
     // the state: tile t of the wave's, register e is key row 16 (TW wave + t) + 4 g + e
     const uint64_t place = (uint64_t)head * d.key_dim * d.value_dim + c0 + i16;
     f4_t st[TW];
-#pragma unroll
-    for (uint32_t t = 0; t < TW; ++t)
-#pragma unroll
-        for (uint32_t e = 0; e < 4u; ++e) {
-            const uint32_t kr = 16u * (TW * wave + t) + 4u * g + e;
-            st[t][e] = !sq.fresh && kr < d.key_dim
-                           ? d.s[(uint64_t)sq.in * d.slot_stride + place + kr * d.value_dim]
-                           : 0.0f;
-        }
     const auto column_most = [&] {
         float m = 0.0f;
 #pragma unroll
@@ -422,40 +440,29 @@ __global__ __launch_bounds__(256) void scan_kernel(ChunkArgs p) {
     const auto record = [&](uint32_t c) {
         return p.records + ((uint64_t)(chunk0 + c) * d.value_heads + head) * kRecord;
     };
+    uint16_t(*turned)[20] = turned_[wave];
     const bool two = wave >= 2u;  // the wave's rows see both halves of the chunk's
 
     h8_t kf[NK], qf[NK], th[2], tl[2], pf[2], kt[TW][2];
     f4_t f_v, f_s, f_q, f_u;  // the rows' factors: of v, of K S, of Q S, of U
+    uint2 v_row;
     uint32_t vb[4];
-    float end_decay = 0.0f, end_next = 0.0f;
-    uint32_t valid = 0, valid_next = 0;
+    float end_decay = 0.0f;
+    uint32_t valid = 0;
     const auto load_rows = [&](uint32_t c) {
-        const uint32_t r = kChunk * c + 16u * wave + i16;
-        const uint32_t row = sq.first + (r < sq.count ? r : sq.count - 1u);
-        const uint16_t* k = d.k + (uint64_t)row * d.k_stride + kh * d.key_dim + 4u * g;
-        const uint16_t* q = d.q + (uint64_t)row * d.q_stride + kh * d.key_dim + 4u * g;
+        const uint8_t* k = p.keys + ((uint64_t)(chunk0 + c) * p.key_heads + kh) * kKeyRecord<DKP> +
+                           kRowsAt<DKP> + wave * NK * kPieceBytes + lane * 16u;
 #pragma unroll
-        for (uint32_t st_ = 0; st_ < NK; ++st_) {
-            uint2 a[4];
-#pragma unroll
-            for (uint32_t h = 0; h < 2u; ++h) {
-                const bool in = 32u * st_ + 16u * h < d.key_dim;
-                const uint32_t o = in ? 32u * st_ + 16u * h : 0u;
-                a[h] = *reinterpret_cast<const uint2*>(k + o);
-                a[2u + h] = *reinterpret_cast<const uint2*>(q + o);
-                // the state has zeros there, but K and Q may have infinities where they wrap
-                if (!in) a[h] = a[2u + h] = make_uint2(0, 0);
-            }
-            kf[st_] = as_h8(make_uint4(a[0].x, a[0].y, a[1].x, a[1].y));
-            qf[st_] = as_h8(make_uint4(a[2].x, a[2].y, a[3].x, a[3].y));
+        for (uint32_t n = 0; n < NK; ++n) {
+            kf[n] = *reinterpret_cast<const h8_t*>(k + n * kPieceBytes);
+            qf[n] = *reinterpret_cast<const h8_t*>(k + (4u * NK + n) * kPieceBytes);
         }
     };
     const auto load_t = [&](uint32_t c) {
         const uint8_t* r = record(c) + lane * 16u;
 #pragma unroll
         for (uint32_t h = 0; h < 2u; ++h) {
-            if (h && !two) continue;
-            const uint8_t* x = r + piece_of(wave, h) * kPieceBytes;
+            const uint8_t* x = r + piece_of(wave, two ? h : 0u) * kPieceBytes;
             th[h] = *reinterpret_cast<const h8_t*>(x);
             tl[h] = *reinterpret_cast<const h8_t*>(x + kPieces * kPieceBytes);
         }
@@ -464,7 +471,7 @@ __global__ __launch_bounds__(256) void scan_kernel(ChunkArgs p) {
         const uint8_t* r = record(c) + kWeightsAt + lane * 16u;
 #pragma unroll
         for (uint32_t h = 0; h < 2u; ++h)
-            if (!h || two) pf[h] = *reinterpret_cast<const h8_t*>(r + piece_of(wave, h) * kPieceBytes);
+            pf[h] = *reinterpret_cast<const h8_t*>(r + piece_of(wave, two ? h : 0u) * kPieceBytes);
         const uint8_t* k = p.keys + ((uint64_t)(chunk0 + c) * p.key_heads + kh) * kKeyRecord<DKP> +
                            lane * 16u;
 #pragma unroll
@@ -478,18 +485,12 @@ __global__ __launch_bounds__(256) void scan_kernel(ChunkArgs p) {
         f_u = *reinterpret_cast<const f4_t*>(f + 192);
     };
     const auto load_v = [&](uint32_t c) {
-#pragma unroll
-        for (uint32_t e = 0; e < 4u; ++e) {
-            const uint32_t r = kChunk * c + 16u * wave + 4u * g + e;
-            const uint32_t row = sq.first + (r < sq.count ? r : sq.count - 1u);
-            vb[e] = d.v[(uint64_t)row * d.v_stride + col];
-        }
+        const uint32_t r = kChunk * c + 16u * wave + (lane >> 2);
+        const uint32_t row = sq.first + (r < sq.count ? r : sq.count - 1u);
+        v_row = *reinterpret_cast<const uint2*>(d.v + (uint64_t)row * d.v_stride + col4);
         const float* f = reinterpret_cast<const float*>(record(c) + kFactorsAt) + 16u * wave + 4u * g;
         f_v = *reinterpret_cast<const f4_t*>(f);
         f_s = *reinterpret_cast<const f4_t*>(f + 64);
-        const float* last = reinterpret_cast<const float*>(record(c) + kEndAt);
-        end_next = last[0];
-        valid_next = __float_as_uint(last[1]);
     };
     // a split value's planes as the second operand: the wave's tile of 16 rows
     const auto share = [&](uint8_t* to, uint32_t tile, f4_t x) {
@@ -504,28 +505,45 @@ __global__ __launch_bounds__(256) void scan_kernel(ChunkArgs p) {
     };
 
     // a column's scale: a power of two that takes its bound to 2^14 at most
-    int exponent = 0;
     const float reach = sqrtf((float)d.key_dim) * 1.01f;
     if (chunks) {
         load_rows(0u);
+        load_v(0u);
         load_t(0u);
         load_p(0u);
-        load_v(0u);
-        const float m = column_most();
-        if (g == 0u) most[i16][wave] = m;
-        lds_barrier();
-        const f4_t a = *reinterpret_cast<const f4_t*>(&most[i16][0]);
-        exponent = __builtin_amdgcn_frexp_expf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])));
-        exponent = exponent > -100 ? exponent : -100;
-        lds_barrier();
     }
+#pragma unroll
+    for (uint32_t t = 0; t < TW; ++t)
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e) {
+            const uint32_t kr = 16u * (TW * wave + t) + 4u * g + e;
+            st[t][e] = !sq.fresh && kr < d.key_dim
+                           ? d.s[(uint64_t)sq.in * d.slot_stride + place + kr * d.value_dim]
+                           : 0.0f;
+        }
+    const float m_first = column_most();
+    if (g == 0u) most[i16][wave] = m_first;
+    lds_barrier();
+    const f4_t m4 = *reinterpret_cast<const f4_t*>(&most[i16][0]);
+    int exponent = __builtin_amdgcn_frexp_expf(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+    exponent = exponent > -100 ? exponent : -100;
+    lds_barrier();
+    // all loads are there: a wait in the loop counts the loop's own
+    __builtin_amdgcn_s_waitcnt(0x0F70);
 #pragma unroll 1
     for (uint32_t c = 0; c < chunks; ++c) {
         const uint32_t next = c + 1u < chunks ? c + 1u : c;
-        end_decay = end_next;
-        valid = valid_next;
+        {
+            const float* last = reinterpret_cast<const float*>(record(c) + kEndAt);
+            end_decay = last[0];
+            valid = __float_as_uint(last[1]);
+        }
         const uint32_t r0 = 16u * wave + 4u * g;  // the lane's rows of the chunk: r0 .. r0 + 3
         const uint32_t rows = sq.count - kChunk * c;
+        *reinterpret_cast<uint2*>(&turned[lane >> 2][4u * (lane & 3u)]) = v_row;
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e) vb[e] = turned[4u * g + e][i16];
 
         // S, and the sizes of its columns and of the values
         const float to_s = __builtin_amdgcn_ldexpf(1.0f, 14 - exponent);
@@ -638,13 +656,18 @@ __global__ __launch_bounds__(256) void scan_kernel(ChunkArgs p) {
             }
         }
         const float o_u = d.scale * (1.0f / kUnit) * from_u;
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (uint32_t e = 0; e < 4u; ++e) {
-            if (r0 + e >= rows) continue;
-            const float y = f_q[e] * (qs[e] * from_s) + o[e] * o_u;
-            d.out[(uint64_t)(sq.first + kChunk * c + r0 + e) * d.out_stride + col] =
-                r0 + e < good ? f32_to_f16(y) : (uint16_t)kDeltaNan2;
-        }
+        for (uint32_t e = 0; e < 4u; ++e)
+            turned[4u * g + e][i16] = r0 + e < good ? f32_to_f16(f_q[e] * (qs[e] * from_s) + o[e] * o_u)
+                                                    : (uint16_t)kDeltaNan2;
+        __builtin_amdgcn_wave_barrier();
+        const uint32_t mine = 16u * wave + (lane >> 2);
+        if (mine < rows)
+            *reinterpret_cast<uint2*>(d.out + (uint64_t)(sq.first + kChunk * c + mine) * d.out_stride +
+                                      col4) =
+                *reinterpret_cast<const uint2*>(&turned[lane >> 2][4u * (lane & 3u)]);
+        __builtin_amdgcn_wave_barrier();
         const bool lost = first_bad < kChunk || valid < (rows < kChunk ? rows : kChunk);
 #pragma unroll
         for (uint32_t t = 0; t < TW; ++t)
