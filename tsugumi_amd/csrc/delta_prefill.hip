@@ -40,7 +40,7 @@ __device__ __forceinline__ uint32_t piece_of(uint32_t mt, uint32_t half) {
 }
 // Pieces of a chunk and key head: K^T's, then K's and Q's (16 rows, 32 elements). In this
 // order a wave's load is 1 KiB in a row; the rows as they lie, in 32-byte parts, took the
-// address unit three times as long as all else together (8192 rows x 32 heads: 405 us for 230).
+// address unit three times as long as all else together (8192 rows x 32 heads: 405 us for 260).
 template <uint32_t DKP>
 constexpr uint32_t kRowsAt = DKP / 16u * 2u * kPieceBytes;
 template <uint32_t DKP>
@@ -81,9 +81,32 @@ __device__ __forceinline__ void split4(f4_t x, h4_t& hi, h4_t& lo) {
 
 constexpr uint32_t kLd = 68;  // floats of a row of A and T in LDS
 
+// Keys, and in their place T once nobody reads them; A; the weights; what is one a row.
+template <uint32_t DKP>
+constexpr uint32_t kKeysBytes = std::max(kChunk * (DKP + 8u) * 2u, kChunk * kLd * 4u);
 template <uint32_t DKP>
 constexpr uint32_t prepare_lds_bytes() {
-    return kChunk * (DKP + 8u) * 2u + 2u * kChunk * kLd * 4u + kChunk * (8u + 5u * 4u) + 16u;
+    return kKeysBytes<DKP> + kChunk * kLd * 4u + kChunk * 72u * 2u + 6u * kChunk * 4u + 16u;
+}
+
+// x and that of the lane that the DPP control names (0 where there is none).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double add_dpp(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xF, false);
+    const uint32_t hi =
+        (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xF, false);
+    return x + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// The sum of the lanes up to this one: from 1, 2, 4 and 8 lanes before within 16, then from
+// the last lane of the 16 and of the 32 before.
+__device__ __forceinline__ double wave_scan(double x) {
+    x = add_dpp<0x111, 0xF>(x);
+    x = add_dpp<0x112, 0xF>(x);
+    x = add_dpp<0x114, 0xF>(x);
+    x = add_dpp<0x118, 0xF>(x);
+    x = add_dpp<0x142, 0xA>(x);
+    return add_dpp<0x143, 0xC>(x);
 }
 
 template <uint32_t DKP>
@@ -92,12 +115,12 @@ __global__ __launch_bounds__(256) void prepare_kernel(ChunkArgs p) {
     constexpr uint32_t NK = DKP / 32u;
     extern __shared__ __align__(16) uint8_t smem[];
     uint16_t* keys = reinterpret_cast<uint16_t*>(smem);
-    float* am = reinterpret_cast<float*>(smem + kChunk * KS * 2u);
-    float* tm = am + kChunk * kLd;
-    uint16_t* pm = reinterpret_cast<uint16_t*>(tm);  // the weights, before T is there
-    double* gs = reinterpret_cast<double*>(tm + kChunk * kLd);
-    float* g_hi = reinterpret_cast<float*>(gs + kChunk);
-    float *g_lo = g_hi + kChunk, *rk = g_lo + kChunk, *rq = rk + kChunk, *bs = rq + kChunk;
+    float* tm = reinterpret_cast<float*>(smem);
+    float* am = reinterpret_cast<float*>(smem + kKeysBytes<DKP>);
+    uint16_t* pm = reinterpret_cast<uint16_t*>(am + kChunk * kLd);
+    float* gs = reinterpret_cast<float*>(pm + kChunk * 72u);
+    float *g_hi = gs + kChunk, *g_lo = g_hi + kChunk, *rk = g_lo + kChunk, *rq = rk + kChunk,
+          *bs = rq + kChunk;
     uint32_t* valid_at = reinterpret_cast<uint32_t*>(bs + kChunk);
 
     const DeltaArgs& d = p.d;
@@ -126,6 +149,9 @@ __global__ __launch_bounds__(256) void prepare_kernel(ChunkArgs p) {
     {
         const uint16_t* k = d.k + (uint64_t)row * d.k_stride + kh * d.key_dim;
         const uint16_t* q = d.q + (uint64_t)row * d.q_stride + kh * d.key_dim;
+        const uint16_t ab = d.a[(uint64_t)row * d.a_stride + head];
+        const uint16_t bb = d.b[(uint64_t)row * d.b_stride + head];
+        const float bias = d.dt_bias[head], rate = expf(d.a_log[head]) * 1.44269504f;
         float kk = 0.0f, qq = 0.0f;
         uint32_t wrong = 0;
 #pragma unroll
@@ -156,19 +182,14 @@ __global__ __launch_bounds__(256) void prepare_kernel(ChunkArgs p) {
             wrong |= (uint32_t)__shfl_xor((int)wrong, o, 64);
         }
         if (part == 0u) {
-            // far rows lose their decays to cancellation in 32 bits: exponents (of two) in 64
-            const double av = (double)f16_to_f32(d.a[(uint64_t)row * d.a_stride + head]) +
-                              (double)d.dt_bias[head];
-            const float bv = f16_to_f32(d.b[(uint64_t)row * d.b_stride + head]);
-            const double soft = (av > 0.0 ? av : 0.0) + log1p(exp(-fabs(av)));
-            double x = -exp((double)d.a_log[head]) * soft * 1.4426950408889634;
-            const float beta = 1.0f / (1.0f + expf(-bv));
-            if (av != av || x != x || beta != beta || wrong) {
+            const float av = f16_to_f32(ab) + bias;
+            const float soft = fmaxf(av, 0.0f) + log1pf(expf(-fabsf(av)));
+            float x = av != av ? av : -rate * soft;
+            const float beta = 1.0f / (1.0f + expf(-f16_to_f32(bb)));
+            if (x != x || beta != beta || wrong) {
                 if (r < t.count) atomicMin(valid_at, r);
             }
-            // a decay of 2^-1500 is 0, and sums of 64 stay exact to 2^-35
-            if (x < -1500.0) x = -1500.0;
-            gs[r] = x;
+            gs[r] = x < -1500.0f ? -1500.0f : x;  // a decay of 2^-1500 is 0
             bs[r] = beta;
             rk[r] = 1.0f / sqrtf(kk + d.eps);
             rq[r] = 1.0f / sqrtf(qq + d.eps);
@@ -181,12 +202,8 @@ __global__ __launch_bounds__(256) void prepare_kernel(ChunkArgs p) {
             *reinterpret_cast<uint4*>(keys + r * KS + 8u * (part + 4u * n)) = make_uint4(0, 0, 0, 0);
     if (wave == 0u) {
         const bool in = lane < valid;
-        double sum = in ? gs[lane] : 0.0;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double up = __shfl_up(sum, (unsigned)o, 64);
-            if ((int)lane >= o) sum += up;
-        }
+        // in 64 bits: their differences are what counts
+        const double sum = wave_scan(in ? (double)gs[lane] : 0.0);
         const double end = __shfl(sum, 63, 64);
         g_hi[lane] = (float)sum;
         g_lo[lane] = (float)(sum - (double)(float)sum);
@@ -231,6 +248,18 @@ __global__ __launch_bounds__(256) void prepare_kernel(ChunkArgs p) {
                 qk[n] = mfma(qa, kb, qk[n]);
             }
         }
+        const uint32_t r0 = 16u * wave + 4u * g;
+        const f4_t hi = *reinterpret_cast<const f4_t*>(g_hi + r0);
+        const f4_t lo = *reinterpret_cast<const f4_t*>(g_lo + r0);
+        const f4_t bi = *reinterpret_cast<const f4_t*>(bs + r0) * *reinterpret_cast<const f4_t*>(rk + r0);
+        const f4_t qi = *reinterpret_cast<const f4_t*>(rq + r0) * kUnit;
+        float hj[4], lj[4], kj[4];
+#pragma unroll
+        for (uint32_t n = 0; n < 4u; ++n) {
+            hj[n] = g_hi[16u * n + i16];
+            lj[n] = g_lo[16u * n + i16];
+            kj[n] = rk[16u * n + i16];
+        }
 #pragma unroll
         for (uint32_t n = 0; n < 4u; ++n) {
             const uint32_t j = 16u * n + i16;
@@ -240,15 +269,13 @@ __global__ __launch_bounds__(256) void prepare_kernel(ChunkArgs p) {
                 for (uint32_t e = 0; e < 4u; ++e) pm[(16u * wave + 4u * g + e) * 72u + j] = 0;
                 continue;
             }
-            const float hj = g_hi[j], lj = g_lo[j], kj = rk[j];
 #pragma unroll
             for (uint32_t e = 0; e < 4u; ++e) {
-                const uint32_t i = 16u * wave + 4u * g + e;
-                const float apart = (g_hi[i] - hj) + (g_lo[i] - lj);
-                const float w = exp2f(i >= j ? apart : 0.0f) * kj;
-                am[i * kLd + j] = i > j ? bs[i] * rk[i] * w * kk[n][e] : 0.0f;
-                const float x = i >= j && i < valid ? rq[i] * w * kUnit * qk[n][e] : 0.0f;
-                pm[i * 72u + j] = f32_to_f16(x);
+                const uint32_t i = r0 + e;
+                const float w =
+                    __builtin_amdgcn_exp2f(i >= j ? (hi[e] - hj[n]) + (lo[e] - lj[n]) : 0.0f) * kj[n];
+                am[i * kLd + j] = i > j ? bi[e] * w * kk[n][e] : 0.0f;
+                pm[i * 72u + j] = f32_to_f16(i >= j ? qi[e] * w * qk[n][e] : 0.0f);
             }
         }
     }
