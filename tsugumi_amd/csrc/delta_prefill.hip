@@ -20,11 +20,15 @@
 // is off by that, where row by row it would keep its 24 bits.
 #include "delta_internal.hpp"
 
+#include <type_traits>
+
 namespace tsg {
 namespace {
 
 constexpr uint32_t kChunk = 64;
-constexpr float kUnit = 1024.0f;  // T and the weights are kept times this: far from fp16's least
+// T and the weights are kept times these, away from fp16's least; R is scaled to less than U by
+// T's, so that their product comes out in U's scale.
+constexpr float kTriangle = 32.0f, kWeight = 1024.0f;
 
 // A chunk and value head's record: T's operand pieces (two planes) and the weights', 64
 // lanes x 16 bytes each; the rows' factors; e^G_end and how many rows count.
@@ -73,7 +77,7 @@ __device__ __forceinline__ void split4(f4_t x, h4_t& hi, h4_t& lo) {
         float y = x[e];
         asm("" : "+v"(y));
         hi[e] = (_Float16)y;
-        lo[e] = (_Float16)(y - (float)hi[e]);
+        lo[e] = (_Float16)__builtin_fmaf((float)hi[e], -1.0f, y);  // one instruction, exact
     }
 }
 
@@ -252,7 +256,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(ChunkArgs p) {
         const f4_t hi = *reinterpret_cast<const f4_t*>(g_hi + r0);
         const f4_t lo = *reinterpret_cast<const f4_t*>(g_lo + r0);
         const f4_t bi = *reinterpret_cast<const f4_t*>(bs + r0) * *reinterpret_cast<const f4_t*>(rk + r0);
-        const f4_t qi = *reinterpret_cast<const f4_t*>(rq + r0) * kUnit;
+        const f4_t qi = *reinterpret_cast<const f4_t*>(rq + r0) * kWeight;
         float hj[4], lj[4], kj[4];
 #pragma unroll
         for (uint32_t n = 0; n < 4u; ++n) {
@@ -392,7 +396,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(ChunkArgs p) {
         h4_t hi[2], lo[2];
 #pragma unroll
         for (uint32_t e = 0; e < 2u; ++e)
-            split4(*reinterpret_cast<const f4_t*>(src + 16u * e) * kUnit, hi[e], lo[e]);
+            split4(*reinterpret_cast<const f4_t*>(src + 16u * e) * kTriangle, hi[e], lo[e]);
         h4_t* to = reinterpret_cast<h4_t*>(record + n * kPieceBytes + lane * 16u);
         to[0] = hi[0];
         to[1] = hi[1];
@@ -404,29 +408,38 @@ __global__ __launch_bounds__(256) void prepare_kernel(ChunkArgs p) {
 
 // ------------------------------------------------------- from chunk to chunk
 //
-// A workgroup takes 16 value elements of a sequence and head, its four waves 16 of a
-// chunk's rows and a quarter of the state's key rows each: the state stays in their
-// registers, and what one wave's products need of the others' goes through LDS as
-// operands of the matrix unit, three exchanges a chunk: S, then R = beta (V - e^G K^ S),
-// then U. Operands of the next chunk are loaded as soon as this one's are used.
+// A workgroup takes 16 value elements of a sequence and head. Each of its eight waves
+// holds an eighth of the state's key rows in registers and multiplies 16 rows of K (waves 0
+// to 3) or of Q with the state; the first four go on to U, the others to the outputs. What
+// one wave's products need of the others' goes through LDS as operands of the matrix unit,
+// three exchanges a chunk: S, then R = beta (V - e^G K^ S), then U. Operands of the next
+// chunk are loaded as soon as this one's are used. Bound by the chain of a chunk's steps,
+// which leave the units mostly idle (eight waves of 16 columns: 8192 rows 260 us with
+// four).
+
+constexpr uint32_t kScanThreads = 512;
 
 template <uint32_t DKP>
-__global__ __launch_bounds__(256) void scan_kernel(ChunkArgs p) {
-    constexpr uint32_t NK = DKP / 32u, TW = DKP / 64u;  // key steps, state tiles of a wave
-    constexpr uint32_t SHARE = 2u * kPieceBytes;        // two planes of a piece
+__global__ __launch_bounds__(kScanThreads) void scan_kernel(ChunkArgs p) {
+    constexpr uint32_t NK = DKP / 32u;                 // key steps
+    constexpr uint32_t TW = DKP <= 128u ? 1u : 2u;     // state tiles (16 key rows) of a wave
+    constexpr uint32_t SHARE = 2u * kPieceBytes;       // two planes of a piece
     __shared__ __align__(16) uint8_t s_at[NK * SHARE];
     __shared__ __align__(16) uint8_t r_at[2u * SHARE];
-    __shared__ __align__(16) uint8_t u_at[2u * SHARE];   // U, for the outputs
-    __shared__ __align__(16) uint8_t w_at[2u * SHARE];   // U times the rows' factors, for the state
-    __shared__ __align__(16) float most[16][8];          // [column][wave]: |S|; |v|
+    __shared__ __align__(16) uint8_t u_at[2u * SHARE];  // U, for the outputs
+    __shared__ __align__(16) uint8_t w_at[2u * SHARE];  // U times the rows' factors, for the state
+    __shared__ __align__(16) float most[16][12];        // [column]: |S| of the waves; |v|
     __shared__ float rare[16][8];
+    __shared__ __align__(16) float factors[4][kChunk];  // of V, K S, Q S and U, a chunk's
     // The wave's 16 rows and columns of V or O, between the lane's place in memory (four
     // elements of row lane / 4) and in the matrix unit: one access of 8 bytes a lane for four of 2.
-    __shared__ __align__(16) uint16_t turned_[4][16][20];
+    __shared__ __align__(16) uint16_t turned_[8][16][20];
 
     const DeltaArgs& d = p.d;
     const uint32_t lane = threadIdx.x & 63u, i16 = lane & 15u, g = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t rt = wave & 3u;                 // the wave's tile of 16 rows
+    const bool holds = DKP >= 128u || wave < 4u;   // a part of the state
     // Workgroups go to the XCDs in turn: those of one key head share its rows there.
     const uint32_t inner = d.group * p.slices;
     uint32_t unit = blockIdx.x / inner, at = blockIdx.x % inner;
@@ -441,16 +454,17 @@ __global__ __launch_bounds__(256) void scan_kernel(ChunkArgs p) {
     if (starts_wrong(d.seqs)) return;  // reported, and the rows made NaN, by the first kernel
     const DeltaSeq sq = delta_seq(d.seqs, s);
     const bool bad = out_slots_clash(d.seqs, s) || sq.bad;
-    const uint32_t col = head * d.value_dim + c0 + i16;
     const uint32_t col4 = head * d.value_dim + c0 + 4u * (lane & 3u);
     if (bad) {
         if (at == 0u && kh == 0u && threadIdx.x == 0u) report(d.seqs.error, kErrDeltaSlot);
-        for (uint32_t r = threadIdx.x >> 4; r < sq.count; r += 16u)
-            d.out[(uint64_t)(sq.first + r) * d.out_stride + col] = (uint16_t)kDeltaNan2;
+        for (uint32_t r = threadIdx.x >> 2; r < sq.count; r += kScanThreads / 4u)
+            *reinterpret_cast<uint2*>(d.out + (uint64_t)(sq.first + r) * d.out_stride + col4) =
+                make_uint2(kDeltaNan2, kDeltaNan2);
         return;
     }
 
-    // the state: tile t of the wave's, register e is key row 16 (TW wave + t) + 4 g + e
+    // the state: register e of tile t of the wave's is key row 16 (TW wave + t) + 4 g + e, times
+    // 2^(14 - exponent), the exponent of the column's last bound
     const uint64_t place = (uint64_t)head * d.key_dim * d.value_dim + c0 + i16;
     f4_t st[TW];
     const auto column_most = [&] {
@@ -464,81 +478,33 @@ __global__ __launch_bounds__(256) void scan_kernel(ChunkArgs p) {
 
     const uint32_t chunks = (sq.count + kChunk - 1u) / kChunk;
     const uint32_t chunk0 = delta_tile_base<kChunk>(d.seqs, sq, s);
+    uint16_t(*turned)[20] = turned_[wave];
+    const bool two = rt >= 2u;  // the wave's rows see both halves of the chunk's
+
+    // Loads: a place that is the same for the wave, and the lane's within it.
+    const uint32_t lane16 = lane * 16u;
+    const auto piece = [](const uint8_t* base, uint32_t off) {
+        return *reinterpret_cast<const h8_t*>(base + off);
+    };
     const auto record = [&](uint32_t c) {
         return p.records + ((uint64_t)(chunk0 + c) * d.value_heads + head) * kRecord;
     };
-    uint16_t(*turned)[20] = turned_[wave];
-    const bool two = wave >= 2u;  // the wave's rows see both halves of the chunk's
-
-    h8_t kf[NK], qf[NK], th[2], tl[2], pf[2], kt[TW][2];
-    f4_t f_v, f_s, f_q, f_u;  // the rows' factors: of v, of K S, of Q S, of U
-    uint2 v_row;
-    uint32_t vb[4];
-    float end_decay = 0.0f;
-    uint32_t valid = 0;
-    const auto load_rows = [&](uint32_t c) {
-        const uint8_t* k = p.keys + ((uint64_t)(chunk0 + c) * p.key_heads + kh) * kKeyRecord<DKP> +
-                           kRowsAt<DKP> + wave * NK * kPieceBytes + lane * 16u;
-#pragma unroll
-        for (uint32_t n = 0; n < NK; ++n) {
-            kf[n] = *reinterpret_cast<const h8_t*>(k + n * kPieceBytes);
-            qf[n] = *reinterpret_cast<const h8_t*>(k + (4u * NK + n) * kPieceBytes);
-        }
-    };
-    const auto load_t = [&](uint32_t c) {
-        const uint8_t* r = record(c) + lane * 16u;
-#pragma unroll
-        for (uint32_t h = 0; h < 2u; ++h) {
-            const uint8_t* x = r + piece_of(wave, two ? h : 0u) * kPieceBytes;
-            th[h] = *reinterpret_cast<const h8_t*>(x);
-            tl[h] = *reinterpret_cast<const h8_t*>(x + kPieces * kPieceBytes);
-        }
-    };
-    const auto load_p = [&](uint32_t c) {
-        const uint8_t* r = record(c) + kWeightsAt + lane * 16u;
-#pragma unroll
-        for (uint32_t h = 0; h < 2u; ++h)
-            pf[h] = *reinterpret_cast<const h8_t*>(r + piece_of(wave, two ? h : 0u) * kPieceBytes);
-        const uint8_t* k = p.keys + ((uint64_t)(chunk0 + c) * p.key_heads + kh) * kKeyRecord<DKP> +
-                           lane * 16u;
-#pragma unroll
-        for (uint32_t t = 0; t < TW; ++t)
-#pragma unroll
-            for (uint32_t h = 0; h < 2u; ++h)
-                kt[t][h] = *reinterpret_cast<const h8_t*>(
-                    k + ((TW * wave + t) * 2u + h) * kPieceBytes);
-        const float* f = reinterpret_cast<const float*>(record(c) + kFactorsAt) + 16u * wave + 4u * g;
-        f_q = *reinterpret_cast<const f4_t*>(f + 128);
-        f_u = *reinterpret_cast<const f4_t*>(f + 192);
-    };
-    const auto load_v = [&](uint32_t c) {
-        const uint32_t r = kChunk * c + 16u * wave + (lane >> 2);
-        const uint32_t row = sq.first + (r < sq.count ? r : sq.count - 1u);
-        v_row = *reinterpret_cast<const uint2*>(d.v + (uint64_t)row * d.v_stride + col4);
-        const float* f = reinterpret_cast<const float*>(record(c) + kFactorsAt) + 16u * wave + 4u * g;
-        f_v = *reinterpret_cast<const f4_t*>(f);
-        f_s = *reinterpret_cast<const f4_t*>(f + 64);
+    const auto key_record = [&](uint32_t c) {
+        return p.keys + ((uint64_t)(chunk0 + c) * p.key_heads + kh) * kKeyRecord<DKP>;
     };
     // a split value's planes as the second operand: the wave's tile of 16 rows
     const auto share = [&](uint8_t* to, uint32_t tile, f4_t x) {
         h4_t hi, lo;
         split4(x, hi, lo);
-        uint8_t* o = to + tile / 2u * SHARE + lane * 16u + tile % 2u * 8u;
+        uint8_t* o = to + tile / 2u * SHARE + tile % 2u * 8u + lane16;
         *reinterpret_cast<h4_t*>(o) = hi;
         *reinterpret_cast<h4_t*>(o + kPieceBytes) = lo;
     };
     const auto shared_piece = [&](const uint8_t* from, uint32_t step, uint32_t plane) {
-        return *reinterpret_cast<const h8_t*>(from + step * SHARE + plane * kPieceBytes + lane * 16u);
+        return *reinterpret_cast<const h8_t*>(from + step * SHARE + plane * kPieceBytes + lane16);
     };
 
-    // a column's scale: a power of two that takes its bound to 2^14 at most
     const float reach = sqrtf((float)d.key_dim) * 1.01f;
-    if (chunks) {
-        load_rows(0u);
-        load_v(0u);
-        load_t(0u);
-        load_p(0u);
-    }
 #pragma unroll
     for (uint32_t t = 0; t < TW; ++t)
 #pragma unroll
@@ -548,172 +514,262 @@ __global__ __launch_bounds__(256) void scan_kernel(ChunkArgs p) {
                            ? d.s[(uint64_t)sq.in * d.slot_stride + place + kr * d.value_dim]
                            : 0.0f;
         }
+    const auto most_of_waves = [&] {
+        const f4_t a = *reinterpret_cast<const f4_t*>(&most[i16][0]);
+        const f4_t b = *reinterpret_cast<const f4_t*>(&most[i16][4]);
+        return fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])),
+                     fmaxf(fmaxf(b[0], b[1]), fmaxf(b[2], b[3])));
+    };
     const float m_first = column_most();
     if (g == 0u) most[i16][wave] = m_first;
     lds_barrier();
-    const f4_t m4 = *reinterpret_cast<const f4_t*>(&most[i16][0]);
-    int exponent = __builtin_amdgcn_frexp_expf(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+    int exponent = __builtin_amdgcn_frexp_expf(most_of_waves());
     exponent = exponent > -100 ? exponent : -100;
     lds_barrier();
-    // all loads are there: a wait in the loop counts the loop's own
-    __builtin_amdgcn_s_waitcnt(0x0F70);
-#pragma unroll 1
-    for (uint32_t c = 0; c < chunks; ++c) {
-        const uint32_t next = c + 1u < chunks ? c + 1u : c;
-        {
-            const float* last = reinterpret_cast<const float*>(record(c) + kEndAt);
-            end_decay = last[0];
-            valid = __float_as_uint(last[1]);
-        }
-        const uint32_t r0 = 16u * wave + 4u * g;  // the lane's rows of the chunk: r0 .. r0 + 3
-        const uint32_t rows = sq.count - kChunk * c;
-        *reinterpret_cast<uint2*>(&turned[lane >> 2][4u * (lane & 3u)]) = v_row;
-        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (uint32_t e = 0; e < 4u; ++e) vb[e] = turned[4u * g + e][i16];
+    for (uint32_t t = 0; t < TW; ++t) st[t] *= __builtin_amdgcn_ldexpf(1.0f, 14 - exponent);
 
-        // S, and the sizes of its columns and of the values
-        const float to_s = __builtin_amdgcn_ldexpf(1.0f, 14 - exponent);
-        const float from_s = __builtin_amdgcn_ldexpf(1.0f, exponent - 14);
+    // The loop, of the waves of keys and of queries: each its own code, so that a wait counts
+    // the loads of its own only, with the same barriers.
+    const auto run = [&](auto role) {
+        constexpr bool keys = decltype(role)::value;
+        const bool two = rt >= 2u;  // the wave's rows see both halves of the chunk's
+        h8_t rf[NK], th[2], tl[2], kt[TW][2];  // rows of K or Q; T or the weights; K^T
+        uint2 v_row = make_uint2(0, 0);
+        float f_row = 0.0f;
+        const uint32_t rows_at = kRowsAt<DKP> + wave * NK * kPieceBytes;
+        const auto load_rows = [&](uint32_t c) {
+            const uint8_t* k = key_record(c) + rows_at;
 #pragma unroll
-        for (uint32_t t = 0; t < TW; ++t) share(s_at, TW * wave + t, st[t] * to_s);
-        {
-            uint32_t bits = 0;
-#pragma unroll
-            for (uint32_t e = 0; e < 4u; ++e) {
-                const uint32_t b = r0 + e < rows ? vb[e] & 0x7FFFu : 0u;
-                bits = bits > b ? bits : b;
+            for (uint32_t n = 0; n < NK; ++n) rf[n] = piece(k + n * kPieceBytes, lane16);
+        };
+        const auto load_v = [&](uint32_t c) {  // or a row of factors
+            if constexpr (keys) {
+                const uint32_t base = kChunk * c + 16u * rt;
+                const uint32_t left = sq.count > base ? sq.count - base : 0u;
+                const uint32_t first = left ? base : sq.count - 1u;  // the last row in the place of none
+                uint32_t r = lane >> 2;
+                r = r < left ? r : left ? left - 1u : 0u;
+                v_row = *reinterpret_cast<const uint2*>(
+                    reinterpret_cast<const uint8_t*>(d.v + (uint64_t)(sq.first + first) * d.v_stride) +
+                    2u * (r * d.v_stride + col4));
+            } else {
+                f_row = *reinterpret_cast<const float*>(record(c) + kFactorsAt + 256u * rt + 4u * lane);
             }
-            // infinities and NaN count as infinity
-            const float mv = max_across32(max_across16(
-                bits < 0x7C00u ? f16_to_f32((uint16_t)bits) : __builtin_inff()));
-            const float ms = column_most();
-            if (g == 0u) {
-                most[i16][wave] = ms;
-                most[i16][4u + wave] = mv;
-            }
-        }
-        lds_barrier();
-        f4_t ks = {0, 0, 0, 0}, qs = {0, 0, 0, 0};
-        const f4_t ma = *reinterpret_cast<const f4_t*>(&most[i16][0]);
-        const f4_t mb = *reinterpret_cast<const f4_t*>(&most[i16][4]);
+        };
+        const uint32_t t_0 = piece_of(rt, 0u) * kPieceBytes, t_1 = piece_of(rt, two ? 1u : 0u) * kPieceBytes;
+        const auto load_t = [&](uint32_t c) {
+            const uint8_t* r = record(c) + (keys ? 0u : kWeightsAt);
+            th[0] = piece(r + t_0, lane16);
+            if constexpr (keys) tl[0] = piece(r + t_0 + kPieces * kPieceBytes, lane16);
+            th[1] = piece(r + t_1, lane16);
+            if constexpr (keys) tl[1] = piece(r + t_1 + kPieces * kPieceBytes, lane16);
+        };
+        const auto load_k = [&](uint32_t c) {
+            const uint8_t* k = key_record(c) + (holds ? TW * wave * SHARE : 0u);
 #pragma unroll
-        for (uint32_t n = 0; n < NK; ++n) {
-            const h8_t hi = shared_piece(s_at, n, 0u), lo = shared_piece(s_at, n, 1u);
-            ks = mfma(kf[n], hi, ks);
-            qs = mfma(qf[n], hi, qs);
-            ks = mfma(kf[n], lo, ks);
-            qs = mfma(qf[n], lo, qs);
-        }
-        load_rows(next);
-        float v_most = fmaxf(fmaxf(mb[0], mb[1]), fmaxf(mb[2], mb[3]));
-        uint32_t first_bad = kChunk;  // row of the column's first infinity or NaN
-        if (__ballot(v_most == __builtin_inff())) {  // the same in all waves
-            uint32_t from = kChunk;
-            float fine = 0.0f;
+            for (uint32_t t = 0; t < TW; ++t)
 #pragma unroll
-            for (uint32_t e = 0; e < 4u; ++e) {
-                if (r0 + e >= rows) continue;
-                const uint32_t b = vb[e] & 0x7FFFu;
-                if (b >= 0x7C00u) from = from < r0 + e ? from : r0 + e;
-                else fine = fmaxf(fine, f16_to_f32((uint16_t)b));
-            }
-            fine = max_across32(max_across16(fine));
-            const float first = -max_across32(max_across16(-(float)from));
-            if (g == 0u) {
-                rare[i16][wave] = first;
-                rare[i16][4u + wave] = fine;
-            }
-            lds_barrier();
-            v_most = 0.0f;
-#pragma unroll
-            for (uint32_t w = 0; w < 4u; ++w) {
-                const uint32_t b = (uint32_t)rare[i16][w];
-                first_bad = first_bad < b ? first_bad : b;
-                v_most = fmaxf(v_most, rare[i16][4u + w]);
-            }
-            lds_barrier();
-        }
-        const uint32_t good = valid < first_bad ? valid : first_bad;
-        const float bound = fmaxf(fmaxf(ma[0], ma[1]), fmaxf(ma[2], ma[3])) * reach + 65.0f * v_most;
-        exponent = __builtin_amdgcn_frexp_expf(bound);
-        exponent = exponent > -100 ? exponent : -100;
-        const float to_u = __builtin_amdgcn_ldexpf(1.0f, 14 - exponent);
-        const float from_u = __builtin_amdgcn_ldexpf(1.0f, exponent - 14);
-
-        f4_t x;
-#pragma unroll
-        for (uint32_t e = 0; e < 4u; ++e)
-            x[e] = r0 + e < good ? (f_v[e] * f16_to_f32((uint16_t)vb[e]) - f_s[e] * (ks[e] * from_s)) * to_u
-                                 : 0.0f;
-        share(r_at, wave, x);
-        load_v(next);
-        lds_barrier();
-        f4_t u = {0, 0, 0, 0}, u2 = {0, 0, 0, 0};
-#pragma unroll
-        for (uint32_t h = 0; h < 2u; ++h) {
-            if (h && !two) continue;
-            const h8_t hi = shared_piece(r_at, h, 0u), lo = shared_piece(r_at, h, 1u);
-            u = mfma(th[h], hi, u);
-            u2 = mfma(tl[h], hi, u2);
-            u2 = mfma(th[h], lo, u2);
-        }
-        load_t(next);
-        u = (u + u2) * (1.0f / kUnit);
-        share(u_at, wave, u);
-        share(w_at, wave, u * f_u);
-        lds_barrier();
+                for (uint32_t h = 0; h < 2u; ++h) kt[t][h] = piece(k + (2u * t + h) * kPieceBytes, lane16);
+        };
+        // A chunk's outputs: Q S, and the weights times U, one chunk later while the waves of
+        // keys form R.
         f4_t o = {0, 0, 0, 0};
-#pragma unroll
-        for (uint32_t h = 0; h < 2u; ++h) {
-            if (h && !two) continue;
-            o = mfma(pf[h], shared_piece(u_at, h, 0u), o);
-            o = mfma(pf[h], shared_piece(u_at, h, 1u), o);
-        }
-        f4_t more[TW];
-#pragma unroll
-        for (uint32_t t = 0; t < TW; ++t) more[t] = f4_t{0, 0, 0, 0};
-#pragma unroll
-        for (uint32_t h = 0; h < 2u; ++h) {
-            const h8_t hi = shared_piece(w_at, h, 0u), lo = shared_piece(w_at, h, 1u);
-#pragma unroll
-            for (uint32_t t = 0; t < TW; ++t) {
-                more[t] = mfma(kt[t][h], hi, more[t]);
-                more[t] = mfma(kt[t][h], lo, more[t]);
+        float o_unit = 0.0f;
+        uint32_t o_good = 0;
+        const auto finish = [&](uint32_t c) {
+            f4_t y = {0, 0, 0, 0}, y2 = {0, 0, 0, 0};
+            y = mfma(th[0], shared_piece(u_at, 0u, 0u), y);
+            y2 = mfma(th[0], shared_piece(u_at, 0u, 1u), y2);
+            if (two) {
+                y = mfma(th[1], shared_piece(u_at, 1u, 0u), y);
+                y2 = mfma(th[1], shared_piece(u_at, 1u, 1u), y2);
             }
-        }
-        const float o_u = d.scale * (1.0f / kUnit) * from_u;
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (uint32_t e = 0; e < 4u; ++e)
-            turned[4u * g + e][i16] = r0 + e < good ? f32_to_f16(f_q[e] * (qs[e] * from_s) + o[e] * o_u)
-                                                    : (uint16_t)kDeltaNan2;
-        __builtin_amdgcn_wave_barrier();
-        const uint32_t mine = 16u * wave + (lane >> 2);
-        if (mine < rows)
-            *reinterpret_cast<uint2*>(d.out + (uint64_t)(sq.first + kChunk * c + mine) * d.out_stride +
-                                      col4) =
-                *reinterpret_cast<const uint2*>(&turned[lane >> 2][4u * (lane & 3u)]);
-        __builtin_amdgcn_wave_barrier();
-        const bool lost = first_bad < kChunk || valid < (rows < kChunk ? rows : kChunk);
-#pragma unroll
-        for (uint32_t t = 0; t < TW; ++t)
+            const uint32_t base = kChunk * c + 16u * rt;
 #pragma unroll
             for (uint32_t e = 0; e < 4u; ++e) {
-                st[t][e] = end_decay * st[t][e] + more[t][e] * from_u;
-                if (lost) st[t][e] = __builtin_nanf("");
+                o[e] = __builtin_fmaf(y[e] + y2[e], o_unit, o[e]);
+                if (16u * rt + 4u * g + e >= o_good) o[e] = __builtin_nanf("");
+                turned[4u * g + e][i16] = f32_to_f16(o[e]);
             }
-        load_p(next);
+            __builtin_amdgcn_wave_barrier();
+            if (base + (lane >> 2) < sq.count)
+                *reinterpret_cast<uint2*>(
+                    reinterpret_cast<uint8_t*>(d.out + (uint64_t)(sq.first + base) * d.out_stride) +
+                    2u * ((lane >> 2) * d.out_stride + col4)) =
+                    *reinterpret_cast<const uint2*>(&turned[lane >> 2][4u * (lane & 3u)]);
+            __builtin_amdgcn_wave_barrier();
+        };
+        load_rows(0u);
+        load_v(0u);
+        load_t(0u);
+        load_k(0u);
+#pragma unroll 1
+        for (uint32_t c = 0; c < chunks; ++c) {
+            const uint32_t next = c + 1u < chunks ? c + 1u : c;
+            const uint32_t* last = reinterpret_cast<const uint32_t*>(record(c) + kEndAt);
+            const float end_decay = __uint_as_float(scalar_load(last));
+            const uint32_t valid = scalar_load(last + 1);
+            const uint32_t r0 = 16u * rt + 4u * g;  // the lane's rows of the chunk: r0 .. r0 + 3
+
+            // S, and the sizes of its columns and of the values
+            if (holds) {
+#pragma unroll
+                for (uint32_t t = 0; t < TW; ++t) share(s_at, TW * wave + t, st[t]);
+            }
+            uint32_t vb[4];
+            {
+                const float ms = column_most();
+                if (g == 0u) most[i16][wave] = ms;
+            }
+            if constexpr (keys) {
+                *reinterpret_cast<uint2*>(&turned[lane >> 2][4u * (lane & 3u)]) = v_row;
+                __builtin_amdgcn_wave_barrier();
+                uint32_t bits = 0;
+#pragma unroll
+                for (uint32_t e = 0; e < 4u; ++e) {
+                    vb[e] = turned[4u * g + e][i16];
+                    const uint32_t b = vb[e] & 0x7FFFu;  // behind the last row: its values again
+                    bits = bits > b ? bits : b;
+                }
+                // infinities and NaN count as infinity
+                const float mv = max_across32(max_across16(
+                    bits < 0x7C00u ? f16_to_f32((uint16_t)bits) : __builtin_inff()));
+                if (g == 0u) most[i16][8u + rt] = mv;
+            } else {
+                factors[rt][lane] = f_row;
+            }
+            lds_barrier();
+            // the rows' products with S: of K or of Q
+            f4_t ps = {0, 0, 0, 0}, ps2 = {0, 0, 0, 0};
+#pragma unroll
+            for (uint32_t n = 0; n < NK; ++n) {
+                ps = mfma(rf[n], shared_piece(s_at, n, 0u), ps);
+                ps2 = mfma(rf[n], shared_piece(s_at, n, 1u), ps2);
+            }
+            load_rows(next);
+            const f4_t mb = *reinterpret_cast<const f4_t*>(&most[i16][8]);
+            float v_most = fmaxf(fmaxf(mb[0], mb[1]), fmaxf(mb[2], mb[3]));
+            uint32_t first_bad = kChunk;  // row of the column's first infinity or NaN
+            if (__ballot(v_most == __builtin_inff())) {  // the same in all waves
+                if constexpr (keys) {
+                    uint32_t from = kChunk;
+                    float fine = 0.0f;
+#pragma unroll
+                    for (uint32_t e = 0; e < 4u; ++e) {
+                        const uint32_t b = vb[e] & 0x7FFFu;
+                        if (b >= 0x7C00u) from = from < r0 + e ? from : r0 + e;
+                        else fine = fmaxf(fine, f16_to_f32((uint16_t)b));
+                    }
+                    fine = max_across32(max_across16(fine));
+                    const float first = -max_across32(max_across16(-(float)from));
+                    if (g == 0u) {
+                        rare[i16][rt] = first;
+                        rare[i16][4u + rt] = fine;
+                    }
+                }
+                lds_barrier();
+                v_most = 0.0f;
+#pragma unroll
+                for (uint32_t w = 0; w < 4u; ++w) {
+                    const uint32_t b = (uint32_t)rare[i16][w];
+                    first_bad = first_bad < b ? first_bad : b;
+                    v_most = fmaxf(v_most, rare[i16][4u + w]);
+                }
+                lds_barrier();
+                if constexpr (keys) {
+#pragma unroll
+                    for (uint32_t e = 0; e < 4u; ++e) vb[e] = r0 + e < first_bad ? vb[e] : 0u;
+                }
+            }
+            const uint32_t good = valid < first_bad ? valid : first_bad;
+            // the bound on U and on the next S; no further below the last than fp32 has room for
+            const float from_s = __builtin_amdgcn_ldexpf(1.0f, exponent - 14);
+            int now = __builtin_amdgcn_frexp_expf(most_of_waves() * (reach * from_s) + 65.0f * v_most);
+            now = now > -100 ? now : -100;
+            now = now > exponent - 60 ? now : exponent - 60;
+            const float ratio = __builtin_amdgcn_ldexpf(1.0f, exponent - now);
+            exponent = now;
+            if constexpr (keys) {
+                const float to_r = __builtin_amdgcn_ldexpf(1.0f / kTriangle, 14 - now);
+                const float s_r = ratio * (1.0f / kTriangle);
+                const f4_t f_v = *reinterpret_cast<const f4_t*>(&factors[0][r0]) * to_r;
+                const f4_t f_s = *reinterpret_cast<const f4_t*>(&factors[1][r0]) * s_r;
+                f4_t x;
+#pragma unroll
+                for (uint32_t e = 0; e < 4u; ++e)  // 0 for rows that do not count: their factors are
+                    x[e] = __builtin_fmaf(f16_to_f32((uint16_t)vb[e]), f_v[e],
+                                          -(ps[e] + ps2[e]) * f_s[e]);
+                share(r_at, rt, x);
+            } else {
+                if (c) finish(c - 1u);
+                o = (ps + ps2) * (*reinterpret_cast<const f4_t*>(&factors[2][r0]) * from_s);
+                o_unit = d.scale * __builtin_amdgcn_ldexpf(1.0f / kWeight, now - 14);
+                o_good = good;
+            }
+            load_v(next);
+            lds_barrier();
+            if constexpr (keys) {
+                f4_t u = {0, 0, 0, 0}, u2 = {0, 0, 0, 0};
+#pragma unroll
+                for (uint32_t h = 0; h < 2u; ++h) {
+                    if (h && !two) continue;
+                    const h8_t hi = shared_piece(r_at, h, 0u), lo = shared_piece(r_at, h, 1u);
+                    u = mfma(th[h], hi, u);
+                    u2 = mfma(tl[h], hi, u2);
+                    u2 = mfma(th[h], lo, u2);
+                }
+                u = u + u2;
+                share(w_at, rt, u * *reinterpret_cast<const f4_t*>(&factors[3][r0]));
+                share(u_at, rt, u);
+            }
+            load_t(keys ? next : c);
+            lds_barrier();
+            f4_t more[TW];
+#pragma unroll
+            for (uint32_t t = 0; t < TW; ++t) more[t] = st[t] * (end_decay * ratio);
+            if (holds) {
+#pragma unroll
+                for (uint32_t h = 0; h < 2u; ++h) {
+                    const h8_t hi = shared_piece(w_at, h, 0u), lo = shared_piece(w_at, h, 1u);
+#pragma unroll
+                    for (uint32_t t = 0; t < TW; ++t) {
+                        more[t] = mfma(kt[t][h], lo, more[t]);
+                        more[t] = mfma(kt[t][h], hi, more[t]);
+                    }
+                }
+            }
+            load_k(next);
+            // rows that do not count for what they hold
+            const uint32_t rows = sq.count - kChunk * c;
+            const bool lost = good < (rows < kChunk ? rows : kChunk);
+#pragma unroll
+            for (uint32_t t = 0; t < TW; ++t) st[t] = more[t];
+            if (__ballot(lost)) {
+#pragma unroll
+                for (uint32_t t = 0; t < TW; ++t)
+#pragma unroll
+                    for (uint32_t e = 0; e < 4u; ++e)
+                        if (lost) st[t][e] = __builtin_nanf("");
+            }
+        }
+        if constexpr (!keys) finish(chunks - 1u);
+    };
+    if (chunks) {
+        __builtin_amdgcn_s_waitcnt(0x0F70);
+        if (wave < 4u) run(std::true_type());
+        else run(std::false_type());
     }
     const uint32_t slot = scalar_load(d.seqs.out_slots + s);
     if (slot == TSG_NO_SLOT) return;
+    const float from_s = __builtin_amdgcn_ldexpf(1.0f, exponent - 14);
 #pragma unroll
     for (uint32_t t = 0; t < TW; ++t)
 #pragma unroll
         for (uint32_t e = 0; e < 4u; ++e) {
             const uint32_t kr = 16u * (TW * wave + t) + 4u * g + e;
             if (kr < d.key_dim)
-                d.s[(uint64_t)slot * d.slot_stride + place + kr * d.value_dim] = st[t][e];
+                d.s[(uint64_t)slot * d.slot_stride + place + kr * d.value_dim] = st[t][e] * from_s;
         }
 }
 
@@ -732,9 +788,9 @@ tsg_status launch(const tsg_delta* delta, ChunkArgs p, uint32_t chunks, tsg_stre
     const uint64_t inner = (uint64_t)p.d.group * p.slices;
     p.spread = units % 8u && units < 64u ? 1u : 0u;
     const uint64_t blocks = p.spread ? units * inner : (units + 7u) / 8u * 8u * inner;
-    TSG_REQUIRE(blocks <= kMaxBlocks, TSG_ERR_UNSUPPORTED,
+    TSG_REQUIRE(2u * blocks <= kMaxBlocks, TSG_ERR_UNSUPPORTED,
                 "too many sequences and heads for one launch");
-    hipLaunchKernelGGL(scan_kernel<DKP>, dim3((uint32_t)blocks), dim3(256), 0, as_stream(stream), p);
+    hipLaunchKernelGGL(scan_kernel<DKP>, dim3((uint32_t)blocks), dim3(kScanThreads), 0, as_stream(stream), p);
     return check_launch("delta_scan");
 }
 
