@@ -139,6 +139,27 @@ def test_infinities_reach_no_row_before(tsg, ctx, op, where, value):  # noqa: F8
     assert_near(states[untouched], pool[untouched], pool_tol[untouched])
 
 
+@pytest.mark.parametrize("where", ["a", "b"])
+def test_a_gates_nan_stays_in_its_value_head(tsg, ctx, where):  # noqa: F811
+    """Three value heads share a key head; the first's gate is NaN at a row, the others are right."""
+    c = Case([90], 1, 3, 64, 32, seed=68)
+    d = c.to_device()
+    d["ab"][41, 0 if where == "a" else 3] = float("nan")
+    c.launch(tsg, ctx, "prefill", d=d)
+    ctx.synchronize()
+    out, tol, pool, pool_tol = c.rule(True)
+    assert bool(torch.isnan(d["out"][41:90, 0]).all())
+    assert_near(d["out"][:41], out[:41], tol[:41])
+    assert_near(d["out"][:90, 1:], out[:, 1:], tol[:, 1:])
+    assert_near(d["s"][:, 1:], pool[:, 1:], pool_tol[:, 1:])
+
+
+@pytest.mark.parametrize("seqs", [8, 300])
+def test_prefill_of_many_chunks(tsg, ctx, seqs):  # noqa: F811
+    check(tsg, ctx, Case([64 + 64 * (i % 2) + i % 5 for i in range(seqs)] if seqs < 100 else
+                         [2 * (i % 5) for i in range(seqs)], 2, 6, 32, 16, seed=69), "prefill")
+
+
 def refused(tsg, call, *args, status=1, text=""):  # noqa: F811
     with pytest.raises(tsg.TsgError) as e:
         call(*args)

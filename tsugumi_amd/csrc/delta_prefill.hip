@@ -55,6 +55,7 @@ struct ChunkArgs {
     uint8_t* records;  // [chunk][value head]
     uint8_t* keys;     // [chunk][key head]
     uint32_t key_heads;
+    uint32_t chunks;
     uint32_t slices;   // of the value elements, a head
     uint32_t spread;   // heads' workgroups in order, not an XCD each
 };
@@ -85,12 +86,12 @@ __device__ __forceinline__ void split4(f4_t x, h4_t& hi, h4_t& lo) {
 
 constexpr uint32_t kLd = 68;  // floats of a row of A and T in LDS
 
-// Keys, and in their place T once nobody reads them; A; the weights; what is one a row.
+// Keys, and in their place the weights, then T; A; what is one a row: four workgroups a CU.
 template <uint32_t DKP>
 constexpr uint32_t kKeysBytes = std::max(kChunk * (DKP + 8u) * 2u, kChunk * kLd * 4u);
 template <uint32_t DKP>
 constexpr uint32_t prepare_lds_bytes() {
-    return kKeysBytes<DKP> + kChunk * kLd * 4u + kChunk * 72u * 2u + 6u * kChunk * 4u + 16u;
+    return kKeysBytes<DKP> + kChunk * kLd * 4u + 8u * kChunk * 4u + 16u;
 }
 
 // x and that of the lane that the DPP control names (0 where there is none).
@@ -113,28 +114,36 @@ __device__ __forceinline__ double wave_scan(double x) {
     return add_dpp<0x143, 0xC>(x);
 }
 
+// A workgroup takes a chunk of a value head; those of one key head, which read the same rows,
+// come one after another on one XCD. Bound by the chain of its steps, with four workgroups a
+// CU (a key head's value heads in one workgroup, the rows' products once: 220 registers, 130 us
+// for 91 over 8192 rows and two value heads).
 template <uint32_t DKP>
-__global__ __launch_bounds__(256) void prepare_kernel(ChunkArgs p) {
+__global__ __launch_bounds__(256, 4) void prepare_kernel(ChunkArgs p) {
     constexpr uint32_t KS = DKP + 8u;  // halves of a key row in LDS
     constexpr uint32_t NK = DKP / 32u;
     extern __shared__ __align__(16) uint8_t smem[];
     uint16_t* keys = reinterpret_cast<uint16_t*>(smem);
     float* tm = reinterpret_cast<float*>(smem);
     float* am = reinterpret_cast<float*>(smem + kKeysBytes<DKP>);
-    uint16_t* pm = reinterpret_cast<uint16_t*>(am + kChunk * kLd);
-    float* gs = reinterpret_cast<float*>(pm + kChunk * 72u);
-    float *g_hi = gs + kChunk, *g_lo = g_hi + kChunk, *rk = g_lo + kChunk, *rq = rk + kChunk,
-          *bs = rq + kChunk;
-    uint32_t* valid_at = reinterpret_cast<uint32_t*>(bs + kChunk);
+    uint16_t* pm = keys;  // the weights, 72 halves a row
+    float* k_inv = am + kChunk * kLd;  // 1 / |k|, 1 / |q|
+    float *q_inv = k_inv + kChunk, *gs = q_inv + kChunk, *bs = gs + kChunk;
+    // of the rows that count for the head (0 for others): no NaN goes into the triangles
+    float *g_hi = bs + kChunk, *g_lo = g_hi + kChunk, *rk = g_lo + kChunk, *rq = rk + kChunk;
+    uint32_t* valid_at = reinterpret_cast<uint32_t*>(rq + kChunk);  // the head's, the keys'
 
     const DeltaArgs& d = p.d;
-    const uint32_t head = blockIdx.y, kh = head / d.group;
-    const DeltaTile t = delta_tile<kChunk>(d.seqs, blockIdx.x);
+    const uint32_t j8 = blockIdx.x >> 3, unit = j8 / d.group * 8u + (blockIdx.x & 7u);
+    const uint32_t chunk = unit / p.key_heads, kh = unit % p.key_heads;
+    const uint32_t head = kh * d.group + j8 % d.group;
+    if (chunk >= p.chunks) return;
+    const DeltaTile t = delta_tile<kChunk>(d.seqs, chunk);
     const uint32_t tid = threadIdx.x, lane = tid & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t i16 = lane & 15u, g = lane >> 4;
     if (t.kind == 2u) {
-        if (blockIdx.x == 0u && head == 0u && tid == 0u) report(d.seqs.error, kErrDeltaRows);
+        if (chunk == 0u && head == 0u && tid == 0u) report(d.seqs.error, kErrDeltaRows);
         const uint32_t pieces = d.value_dim / 8u;
         for (uint32_t n = tid; n < t.count * pieces; n += 256u)
             *reinterpret_cast<uint4*>(d.out + (uint64_t)(t.first + n / pieces) * d.out_stride +
@@ -143,19 +152,18 @@ __global__ __launch_bounds__(256) void prepare_kernel(ChunkArgs p) {
         return;
     }
     if (t.count == 0u) return;
-    uint8_t* record = p.records + ((uint64_t)blockIdx.x * d.value_heads + head) * kRecord;
+    uint8_t* record = p.records + ((uint64_t)chunk * d.value_heads + head) * kRecord;
 
     // rows: four threads each; norms, gates, keys to LDS
-    if (tid == 0u) *valid_at = t.count;
-    __syncthreads();
     const uint32_t r = tid >> 2, part = tid & 3u;
     const uint32_t row = t.first + (r < t.count ? r : t.count - 1u);
+    if (tid == 0u) valid_at[0] = valid_at[1] = t.count;
+    __syncthreads();
     {
         const uint16_t* k = d.k + (uint64_t)row * d.k_stride + kh * d.key_dim;
         const uint16_t* q = d.q + (uint64_t)row * d.q_stride + kh * d.key_dim;
-        const uint16_t ab = d.a[(uint64_t)row * d.a_stride + head];
-        const uint16_t bb = d.b[(uint64_t)row * d.b_stride + head];
-        const float bias = d.dt_bias[head], rate = expf(d.a_log[head]) * 1.44269504f;
+        const uint16_t a_bits = d.a[(uint64_t)row * d.a_stride + head];
+        const uint16_t b_bits = d.b[(uint64_t)row * d.b_stride + head];
         float kk = 0.0f, qq = 0.0f;
         uint32_t wrong = 0;
 #pragma unroll
@@ -172,11 +180,11 @@ __global__ __launch_bounds__(256) void prepare_kernel(ChunkArgs p) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 wrong |= not_finite<false>(us[e]);
-                const h2_t a = __builtin_bit_cast(h2_t, us[e]), b = __builtin_bit_cast(h2_t, ws[e]);
-                kk = __builtin_fmaf((float)a[0], (float)a[0], kk);
-                kk = __builtin_fmaf((float)a[1], (float)a[1], kk);
-                qq = __builtin_fmaf((float)b[0], (float)b[0], qq);
-                qq = __builtin_fmaf((float)b[1], (float)b[1], qq);
+                const h2_t x = __builtin_bit_cast(h2_t, us[e]), y = __builtin_bit_cast(h2_t, ws[e]);
+                kk = __builtin_fmaf((float)x[0], (float)x[0], kk);
+                kk = __builtin_fmaf((float)x[1], (float)x[1], kk);
+                qq = __builtin_fmaf((float)y[0], (float)y[0], qq);
+                qq = __builtin_fmaf((float)y[1], (float)y[1], qq);
             }
         }
 #pragma unroll
@@ -186,24 +194,29 @@ __global__ __launch_bounds__(256) void prepare_kernel(ChunkArgs p) {
             wrong |= (uint32_t)__shfl_xor((int)wrong, o, 64);
         }
         if (part == 0u) {
-            const float av = f16_to_f32(ab) + bias;
+            const float av = f16_to_f32(a_bits) + d.dt_bias[head];
             const float soft = fmaxf(av, 0.0f) + log1pf(expf(-fabsf(av)));
-            float x = av != av ? av : -rate * soft;
-            const float beta = 1.0f / (1.0f + expf(-f16_to_f32(bb)));
-            if (x != x || beta != beta || wrong) {
-                if (r < t.count) atomicMin(valid_at, r);
-            }
+            const float x = av != av ? av : -expf(d.a_log[head]) * 1.44269504f * soft;
+            const float beta = 1.0f / (1.0f + expf(-f16_to_f32(b_bits)));
+            if ((x != x || beta != beta) && r < t.count) atomicMin(valid_at, r);
+            if (wrong) atomicMin(valid_at + 1, r);
             gs[r] = x < -1500.0f ? -1500.0f : x;  // a decay of 2^-1500 is 0
             bs[r] = beta;
-            rk[r] = 1.0f / sqrtf(kk + d.eps);
-            rq[r] = 1.0f / sqrtf(qq + d.eps);
+            k_inv[r] = 1.0f / sqrtf(kk + d.eps);
+            q_inv[r] = 1.0f / sqrtf(qq + d.eps);
         }
     }
     __syncthreads();
-    const uint32_t valid = *valid_at;
-    if (r >= valid)
-        for (uint32_t n = 0; n < DKP / 32u; ++n)
-            *reinterpret_cast<uint4*>(keys + r * KS + 8u * (part + 4u * n)) = make_uint4(0, 0, 0, 0);
+    // The head's rows count up to its first wrong gate or key; those behind a wrong key for
+    // none of the key head's, so the keys become zeros there.
+    const uint32_t key_valid = valid_at[1], valid = key_valid < valid_at[0] ? key_valid : valid_at[0];
+    if (key_valid < t.count) {
+        if (r >= key_valid)
+            for (uint32_t n = 0; n < DKP / 32u; ++n)
+                *reinterpret_cast<uint4*>(keys + r * KS + 8u * (part + 4u * n)) = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+    }
+
     if (wave == 0u) {
         const bool in = lane < valid;
         // in 64 bits: their differences are what counts
@@ -213,31 +226,32 @@ __global__ __launch_bounds__(256) void prepare_kernel(ChunkArgs p) {
         g_lo[lane] = (float)(sum - (double)(float)sum);
         float* f = reinterpret_cast<float*>(record + kFactorsAt) + lane;
         const float since = exp2f((float)sum), until = exp2f((float)(end - sum));
-        const float beta = bs[lane], k1 = rk[lane];
+        const float beta = bs[lane], k1 = k_inv[lane];
         // K^T is kept with norms of 2 ... 4, so that U times this stays in fp16's range, and
         // neither's elements near its least
         const int e = __builtin_amdgcn_frexp_expf(1.0f / k1);
         f[0] = in ? beta : 0.0f;
         f[64] = in ? beta * since * k1 : 0.0f;
-        f[128] = in ? since * rq[lane] * d.scale : 0.0f;
+        f[128] = in ? since * q_inv[lane] * d.scale : 0.0f;
         f[192] = in ? until * __builtin_amdgcn_ldexpf(k1, e - 2) : 0.0f;
-        if (!in) bs[lane] = rk[lane] = rq[lane] = 0.0f;  // no NaN into the triangles
+        rk[lane] = in ? k1 : 0.0f;
+        rq[lane] = in ? q_inv[lane] * kWeight : 0.0f;
+        bs[lane] = in ? beta * k1 : 0.0f;
         if (lane == 0u) {
             float* last = reinterpret_cast<float*>(record + kEndAt);
             last[0] = exp2f((float)end);
             last[1] = __uint_as_float(valid);
         }
     }
-    __syncthreads();
 
     // products of the rows' 16-row tiles: K K^T and Q K^T on and below the diagonal
+    f4_t kk[4], qk[4];
+    const uint32_t mine = 16u * wave + i16, r0 = 16u * wave + 4u * g;
+    const uint16_t* q = d.q + (uint64_t)(t.first + (mine < t.count ? mine : t.count - 1u)) * d.q_stride +
+                        kh * d.key_dim;
     {
-        f4_t kk[4], qk[4];
 #pragma unroll
         for (uint32_t n = 0; n < 4u; ++n) kk[n] = qk[n] = f4_t{0, 0, 0, 0};
-        const uint32_t mine = 16u * wave + i16;
-        const uint32_t q_row = t.first + (mine < t.count ? mine : t.count - 1u);
-        const uint16_t* q = d.q + (uint64_t)q_row * d.q_stride + kh * d.key_dim;
 #pragma unroll
         for (uint32_t st = 0; st < NK; ++st) {
             const uint32_t c = 32u * st + 8u * g;
@@ -252,63 +266,21 @@ __global__ __launch_bounds__(256) void prepare_kernel(ChunkArgs p) {
                 qk[n] = mfma(qa, kb, qk[n]);
             }
         }
-        const uint32_t r0 = 16u * wave + 4u * g;
-        const f4_t hi = *reinterpret_cast<const f4_t*>(g_hi + r0);
-        const f4_t lo = *reinterpret_cast<const f4_t*>(g_lo + r0);
-        const f4_t bi = *reinterpret_cast<const f4_t*>(bs + r0) * *reinterpret_cast<const f4_t*>(rk + r0);
-        const f4_t qi = *reinterpret_cast<const f4_t*>(rq + r0) * kWeight;
-        float hj[4], lj[4], kj[4];
-#pragma unroll
-        for (uint32_t n = 0; n < 4u; ++n) {
-            hj[n] = g_hi[16u * n + i16];
-            lj[n] = g_lo[16u * n + i16];
-            kj[n] = rk[16u * n + i16];
-        }
-#pragma unroll
-        for (uint32_t n = 0; n < 4u; ++n) {
-            const uint32_t j = 16u * n + i16;
-            if (n > wave) {
-                if ((n ^ 1u) != wave) continue;  // the other half of a piece
-#pragma unroll
-                for (uint32_t e = 0; e < 4u; ++e) pm[(16u * wave + 4u * g + e) * 72u + j] = 0;
-                continue;
-            }
-#pragma unroll
-            for (uint32_t e = 0; e < 4u; ++e) {
-                const uint32_t i = r0 + e;
-                const float w =
-                    __builtin_amdgcn_exp2f(i >= j ? (hi[e] - hj[n]) + (lo[e] - lj[n]) : 0.0f) * kj[n];
-                am[i * kLd + j] = i > j ? bi[e] * w * kk[n][e] : 0.0f;
-                pm[i * 72u + j] = f32_to_f16(i >= j ? qi[e] * w * qk[n][e] : 0.0f);
-            }
-        }
-    }
-    __syncthreads();
-    for (uint32_t n = wave; n < kPieces; n += 4u) {
-        const uint32_t mt = n < 2u ? n : 2u + (n - 2u) / 2u, half = n < 2u ? 0u : n % 2u;
-        const uint16_t* src = pm + (16u * mt + i16) * 72u + 32u * half + 4u * g;
-        const uint2 lo = *reinterpret_cast<const uint2*>(src), hi = *reinterpret_cast<const uint2*>(src + 16);
-        *reinterpret_cast<uint4*>(record + kWeightsAt + n * kPieceBytes + lane * 16u) =
-            make_uint4(lo.x, lo.y, hi.x, hi.y);
     }
     if (head % d.group == 0u) {
-        uint8_t* to = p.keys + ((uint64_t)blockIdx.x * p.key_heads + kh) * kKeyRecord<DKP>;
+        uint8_t* to = p.keys + ((uint64_t)chunk * p.key_heads + kh) * kKeyRecord<DKP> + lane * 16u;
         for (uint32_t n = wave; n < DKP / 8u; n += 4u) {
             const uint32_t c = 16u * (n / 2u) + i16;
             h8_t x;
 #pragma unroll
             for (uint32_t e = 0; e < 8u; ++e) {
                 const uint32_t at = 32u * (n % 2u) + 16u * (e / 4u) + 4u * g + e % 4u;
-                const int ex = __builtin_amdgcn_frexp_expf(1.0f / rk[at]);
-                x[e] = (_Float16)__builtin_amdgcn_ldexpf(
-                    f16_to_f32(keys[at * KS + c]), 2 - ex);
+                const int ex = __builtin_amdgcn_frexp_expf(1.0f / k_inv[at]);
+                x[e] = (_Float16)__builtin_amdgcn_ldexpf(f16_to_f32(keys[at * KS + c]), 2 - ex);
             }
-            *reinterpret_cast<h8_t*>(to + n * kPieceBytes + lane * 16u) = x;
+            *reinterpret_cast<h8_t*>(to + n * kPieceBytes) = x;
         }
-        to += kRowsAt<DKP> + lane * 16u;
-        const uint32_t mine = 16u * wave + i16;
-        const uint32_t q_row = t.first + (mine < t.count ? mine : t.count - 1u);
-        const uint16_t* q = d.q + (uint64_t)q_row * d.q_stride + kh * d.key_dim;
+        to += kRowsAt<DKP>;
 #pragma unroll
         for (uint32_t st = 0; st < NK; ++st) {
             uint2 a[4];
@@ -325,7 +297,48 @@ __global__ __launch_bounds__(256) void prepare_kernel(ChunkArgs p) {
                 make_uint4(a[2].x, a[2].y, a[3].x, a[3].y);
         }
     }
+
     __syncthreads();
+    {
+        const f4_t hi = *reinterpret_cast<const f4_t*>(g_hi + r0);
+        const f4_t lo = *reinterpret_cast<const f4_t*>(g_lo + r0);
+        const f4_t bi = *reinterpret_cast<const f4_t*>(bs + r0);
+        const f4_t qi = *reinterpret_cast<const f4_t*>(rq + r0);
+        float hj[4], lj[4], kj[4];
+#pragma unroll
+        for (uint32_t n = 0; n < 4u; ++n) {
+            hj[n] = g_hi[16u * n + i16];
+            lj[n] = g_lo[16u * n + i16];
+            kj[n] = rk[16u * n + i16];
+        }
+#pragma unroll
+        for (uint32_t n = 0; n < 4u; ++n) {
+            const uint32_t j = 16u * n + i16;
+            if (n > wave) {
+                if ((n ^ 1u) != wave) continue;  // the other half of a piece
+#pragma unroll
+                for (uint32_t e = 0; e < 4u; ++e) pm[(r0 + e) * 72u + j] = 0;
+                continue;
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < 4u; ++e) {
+                const uint32_t i = r0 + e;
+                const float w =
+                    __builtin_amdgcn_exp2f(i >= j ? (hi[e] - hj[n]) + (lo[e] - lj[n]) : 0.0f) * kj[n];
+                am[i * kLd + j] = i > j ? bi[e] * w * kk[n][e] : 0.0f;
+                // a query's infinity or NaN stays in its row's weights
+                pm[i * 72u + j] = f32_to_f16(i >= j ? qi[e] * w * qk[n][e] : 0.0f);
+            }
+        }
+    }
+    __syncthreads();
+    for (uint32_t n = wave; n < kPieces; n += 4u) {
+        const uint32_t mt = n < 2u ? n : 2u + (n - 2u) / 2u, half = n < 2u ? 0u : n % 2u;
+        const uint16_t* src = pm + (16u * mt + i16) * 72u + 32u * half + 4u * g;
+        const uint2 lo = *reinterpret_cast<const uint2*>(src), hi = *reinterpret_cast<const uint2*>(src + 16);
+        *reinterpret_cast<uint4*>(record + kWeightsAt + n * kPieceBytes + lane * 16u) =
+            make_uint4(lo.x, lo.y, hi.x, hi.y);
+    }
 
     // T: the diagonal tiles by substitution, a column a lane, ...
     {
@@ -420,20 +433,22 @@ __global__ __launch_bounds__(256) void prepare_kernel(ChunkArgs p) {
 constexpr uint32_t kScanThreads = 512;
 
 template <uint32_t DKP>
-__global__ __launch_bounds__(kScanThreads) void scan_kernel(ChunkArgs p) {
+__global__ __launch_bounds__(kScanThreads, (DKP <= 128u ? 4 : 2)) void scan_kernel(ChunkArgs p) {
     constexpr uint32_t NK = DKP / 32u;                 // key steps
     constexpr uint32_t TW = DKP <= 128u ? 1u : 2u;     // state tiles (16 key rows) of a wave
     constexpr uint32_t SHARE = 2u * kPieceBytes;       // two planes of a piece
     __shared__ __align__(16) uint8_t s_at[NK * SHARE];
     __shared__ __align__(16) uint8_t r_at[2u * SHARE];
-    __shared__ __align__(16) uint8_t u_at[2u * SHARE];  // U, for the outputs
+    __shared__ __align__(16) uint8_t u_at[2][2u * SHARE];  // U, for the outputs, of two chunks
     __shared__ __align__(16) uint8_t w_at[2u * SHARE];  // U times the rows' factors, for the state
-    __shared__ __align__(16) float most[16][12];        // [column]: |S| of the waves; |v|
+    __shared__ __align__(16) float most[16][8];         // [column]: |S| of the waves
+    __shared__ __align__(16) float v_most_at[2][16][4];  // |v| of the row tiles, of two chunks
     __shared__ float rare[16][8];
     __shared__ __align__(16) float factors[4][kChunk];  // of V, K S, Q S and U, a chunk's
-    // The wave's 16 rows and columns of V or O, between the lane's place in memory (four
-    // elements of row lane / 4) and in the matrix unit: one access of 8 bytes a lane for four of 2.
-    __shared__ __align__(16) uint16_t turned_[8][16][20];
+    // 16 rows and columns of V and O, between a lane's place in memory (four elements of
+    // row lane / 4) and in the matrix unit: one access of 8 bytes a lane for four of 2.
+    __shared__ __align__(16) uint16_t v_at[2][4][16][20];  // [column][row], of two chunks
+    __shared__ __align__(16) uint16_t o_at[4][16][20];  // [row][column]
 
     const DeltaArgs& d = p.d;
     const uint32_t lane = threadIdx.x & 63u, i16 = lane & 15u, g = lane >> 4;
@@ -478,9 +493,6 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(ChunkArgs p) {
 
     const uint32_t chunks = (sq.count + kChunk - 1u) / kChunk;
     const uint32_t chunk0 = delta_tile_base<kChunk>(d.seqs, sq, s);
-    uint16_t(*turned)[20] = turned_[wave];
-    const bool two = rt >= 2u;  // the wave's rows see both halves of the chunk's
-
     // Loads: a place that is the same for the wave, and the lane's within it.
     const uint32_t lane16 = lane * 16u;
     const auto piece = [](const uint8_t* base, uint32_t off) {
@@ -543,8 +555,9 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(ChunkArgs p) {
 #pragma unroll
             for (uint32_t n = 0; n < NK; ++n) rf[n] = piece(k + n * kPieceBytes, lane16);
         };
-        const auto load_v = [&](uint32_t c) {  // or a row of factors
-            if constexpr (keys) {
+        // the waves of queries also bring the values and the rows' factors
+        const auto load_v = [&](uint32_t c) {
+            if constexpr (!keys) {
                 const uint32_t base = kChunk * c + 16u * rt;
                 const uint32_t left = sq.count > base ? sq.count - base : 0u;
                 const uint32_t first = left ? base : sq.count - 1u;  // the last row in the place of none
@@ -553,9 +566,30 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(ChunkArgs p) {
                 v_row = *reinterpret_cast<const uint2*>(
                     reinterpret_cast<const uint8_t*>(d.v + (uint64_t)(sq.first + first) * d.v_stride) +
                     2u * (r * d.v_stride + col4));
-            } else {
-                f_row = *reinterpret_cast<const float*>(record(c) + kFactorsAt + 256u * rt + 4u * lane);
             }
+        };
+        const auto load_factors = [&](uint32_t c) {
+            if constexpr (!keys)
+                f_row = *reinterpret_cast<const float*>(record(c) + kFactorsAt + 256u * rt + 4u * lane);
+        };
+        // the loaded values' columns, and the largest of each
+        const auto turn_v = [&](uint32_t c) {
+            uint16_t(*v)[20] = v_at[c & 1u][rt];
+            const uint32_t r = lane >> 2, c4 = 4u * (lane & 3u);
+            v[c4][r] = (uint16_t)v_row.x;
+            v[c4 + 1u][r] = (uint16_t)(v_row.x >> 16);
+            v[c4 + 2u][r] = (uint16_t)v_row.y;
+            v[c4 + 3u][r] = (uint16_t)(v_row.y >> 16);
+            __builtin_amdgcn_wave_barrier();
+            const uint2 u = *reinterpret_cast<const uint2*>(&v[i16][4u * g]);
+            const uint32_t b[4] = {u.x & 0x7FFFu, u.x >> 16 & 0x7FFFu, u.y & 0x7FFFu, u.y >> 16 & 0x7FFFu};
+            uint32_t bits = 0;
+#pragma unroll
+            for (uint32_t e = 0; e < 4u; ++e) bits = bits > b[e] ? bits : b[e];
+            // infinities and NaN count as infinity
+            const float mv = max_across32(max_across16(
+                bits < 0x7C00u ? f16_to_f32((uint16_t)bits) : __builtin_inff()));
+            if (g == 0u) v_most_at[c & 1u][i16][rt] = mv;
         };
         const uint32_t t_0 = piece_of(rt, 0u) * kPieceBytes, t_1 = piece_of(rt, two ? 1u : 0u) * kPieceBytes;
         const auto load_t = [&](uint32_t c) {
@@ -573,35 +607,38 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(ChunkArgs p) {
                 for (uint32_t h = 0; h < 2u; ++h) kt[t][h] = piece(k + (2u * t + h) * kPieceBytes, lane16);
         };
         // A chunk's outputs: Q S, and the weights times U, one chunk later while the waves of
-        // keys form R.
-        f4_t o = {0, 0, 0, 0};
+        // keys form U.
+        f4_t o = {0, 0, 0, 0}, o_next = {0, 0, 0, 0};
         float o_unit = 0.0f;
         uint32_t o_good = 0;
         const auto finish = [&](uint32_t c) {
             f4_t y = {0, 0, 0, 0}, y2 = {0, 0, 0, 0};
-            y = mfma(th[0], shared_piece(u_at, 0u, 0u), y);
-            y2 = mfma(th[0], shared_piece(u_at, 0u, 1u), y2);
+            y = mfma(th[0], shared_piece(u_at[c & 1u], 0u, 0u), y);
+            y2 = mfma(th[0], shared_piece(u_at[c & 1u], 0u, 1u), y2);
             if (two) {
-                y = mfma(th[1], shared_piece(u_at, 1u, 0u), y);
-                y2 = mfma(th[1], shared_piece(u_at, 1u, 1u), y2);
+                y = mfma(th[1], shared_piece(u_at[c & 1u], 1u, 0u), y);
+                y2 = mfma(th[1], shared_piece(u_at[c & 1u], 1u, 1u), y2);
             }
             const uint32_t base = kChunk * c + 16u * rt;
 #pragma unroll
             for (uint32_t e = 0; e < 4u; ++e) {
                 o[e] = __builtin_fmaf(y[e] + y2[e], o_unit, o[e]);
                 if (16u * rt + 4u * g + e >= o_good) o[e] = __builtin_nanf("");
-                turned[4u * g + e][i16] = f32_to_f16(o[e]);
+                o_at[rt][4u * g + e][i16] = f32_to_f16(o[e]);
             }
             __builtin_amdgcn_wave_barrier();
             if (base + (lane >> 2) < sq.count)
                 *reinterpret_cast<uint2*>(
                     reinterpret_cast<uint8_t*>(d.out + (uint64_t)(sq.first + base) * d.out_stride) +
                     2u * ((lane >> 2) * d.out_stride + col4)) =
-                    *reinterpret_cast<const uint2*>(&turned[lane >> 2][4u * (lane & 3u)]);
+                    *reinterpret_cast<const uint2*>(&o_at[rt][lane >> 2][4u * (lane & 3u)]);
             __builtin_amdgcn_wave_barrier();
         };
-        load_rows(0u);
         load_v(0u);
+        if constexpr (!keys) turn_v(0u);
+        load_rows(0u);
+        load_factors(0u);
+        load_v(chunks > 1u ? 1u : 0u);
         load_t(0u);
         load_k(0u);
 #pragma unroll 1
@@ -617,28 +654,11 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(ChunkArgs p) {
 #pragma unroll
                 for (uint32_t t = 0; t < TW; ++t) share(s_at, TW * wave + t, st[t]);
             }
-            uint32_t vb[4];
             {
                 const float ms = column_most();
                 if (g == 0u) most[i16][wave] = ms;
             }
-            if constexpr (keys) {
-                *reinterpret_cast<uint2*>(&turned[lane >> 2][4u * (lane & 3u)]) = v_row;
-                __builtin_amdgcn_wave_barrier();
-                uint32_t bits = 0;
-#pragma unroll
-                for (uint32_t e = 0; e < 4u; ++e) {
-                    vb[e] = turned[4u * g + e][i16];
-                    const uint32_t b = vb[e] & 0x7FFFu;  // behind the last row: its values again
-                    bits = bits > b ? bits : b;
-                }
-                // infinities and NaN count as infinity
-                const float mv = max_across32(max_across16(
-                    bits < 0x7C00u ? f16_to_f32((uint16_t)bits) : __builtin_inff()));
-                if (g == 0u) most[i16][8u + rt] = mv;
-            } else {
-                factors[rt][lane] = f_row;
-            }
+            if constexpr (!keys) factors[rt][lane] = f_row;
             lds_barrier();
             // the rows' products with S: of K or of Q
             f4_t ps = {0, 0, 0, 0}, ps2 = {0, 0, 0, 0};
@@ -648,7 +668,10 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(ChunkArgs p) {
                 ps2 = mfma(rf[n], shared_piece(s_at, n, 1u), ps2);
             }
             load_rows(next);
-            const f4_t mb = *reinterpret_cast<const f4_t*>(&most[i16][8]);
+            uint2 vs = make_uint2(0, 0);  // the lane's values
+            if constexpr (keys) vs = *reinterpret_cast<const uint2*>(&v_at[c & 1u][rt][i16][4u * g]);
+            uint32_t vb[4] = {vs.x & 0xFFFFu, vs.x >> 16, vs.y & 0xFFFFu, vs.y >> 16};
+            const f4_t mb = *reinterpret_cast<const f4_t*>(&v_most_at[c & 1u][i16][0]);
             float v_most = fmaxf(fmaxf(mb[0], mb[1]), fmaxf(mb[2], mb[3]));
             uint32_t first_bad = kChunk;  // row of the column's first infinity or NaN
             if (__ballot(v_most == __builtin_inff())) {  // the same in all waves
@@ -702,12 +725,11 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(ChunkArgs p) {
                                           -(ps[e] + ps2[e]) * f_s[e]);
                 share(r_at, rt, x);
             } else {
-                if (c) finish(c - 1u);
-                o = (ps + ps2) * (*reinterpret_cast<const f4_t*>(&factors[2][r0]) * from_s);
-                o_unit = d.scale * __builtin_amdgcn_ldexpf(1.0f / kWeight, now - 14);
-                o_good = good;
+                o_next = (ps + ps2) * (*reinterpret_cast<const f4_t*>(&factors[2][r0]) * from_s);
+                turn_v(c + 1u);  // the next chunk's
             }
-            load_v(next);
+            load_factors(next);
+            load_v(c + 2u < chunks ? c + 2u : next);
             lds_barrier();
             if constexpr (keys) {
                 f4_t u = {0, 0, 0, 0}, u2 = {0, 0, 0, 0};
@@ -721,7 +743,12 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(ChunkArgs p) {
                 }
                 u = u + u2;
                 share(w_at, rt, u * *reinterpret_cast<const f4_t*>(&factors[3][r0]));
-                share(u_at, rt, u);
+                share(u_at[c & 1u], rt, u);
+            } else {
+                if (c) finish(c - 1u);
+                o = o_next;
+                o_unit = d.scale * __builtin_amdgcn_ldexpf(1.0f / kWeight, now - 14);
+                o_good = good;
             }
             load_t(keys ? next : c);
             lds_barrier();
@@ -781,7 +808,10 @@ constexpr uint64_t chunk_bytes(uint64_t value_heads, uint64_t key_heads) {
 template <uint32_t DKP>
 tsg_status launch(const tsg_delta* delta, ChunkArgs p, uint32_t chunks, tsg_stream stream) {
     p.keys = p.records + (uint64_t)chunks * p.d.value_heads * kRecord;
-    hipLaunchKernelGGL(prepare_kernel<DKP>, dim3(chunks, p.d.value_heads), dim3(256),
+    const uint64_t prepared = ((uint64_t)chunks * p.key_heads + 7u) / 8u * 8u * p.d.group;
+    TSG_REQUIRE(prepared <= kMaxBlocks, TSG_ERR_UNSUPPORTED, "too many rows and heads for one launch");
+    p.chunks = chunks;
+    hipLaunchKernelGGL(prepare_kernel<DKP>, dim3((uint32_t)prepared), dim3(256),
                        prepare_lds_bytes<DKP>(), as_stream(stream), p);
     if (tsg_status s = check_launch("delta_prepare")) return s;
     const uint64_t units = (uint64_t)p.d.seqs.num_seqs * p.key_heads;
@@ -825,8 +855,6 @@ tsg_status launch_chunked(const tsg_delta* delta, const DeltaArgs& a, void* scra
     p.slices = a.value_dim / 16u;
     const uint32_t chunks = delta_tiles<kChunk>(a.seqs.rows, a.seqs.num_seqs, a.seqs.seq_rows,
                                                 a.seqs.row_starts != nullptr);
-    TSG_REQUIRE((uint64_t)chunks * a.value_heads <= kMaxBlocks, TSG_ERR_UNSUPPORTED,
-                "too many rows and heads for one launch");
     switch (delta->padded_key) {
         case 64: return launch<64>(delta, p, chunks, stream);
         case 128: return launch<128>(delta, p, chunks, stream);
