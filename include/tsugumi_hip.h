@@ -813,6 +813,34 @@ tsg_status tsg_attn_prefill(tsg_attn* attn, tsg_stream stream, const tsg_kv_page
                             const tsg_attn_batch* batch, const uint16_t* q, uint32_t q_stride,
                             uint16_t* out, uint32_t out_stride);
 
+/* Sequences of a batch that begin alike: group g is sequences group_starts[g] ..
+ * group_starts[g + 1] - 1 [num_groups + 1], whose first shared[g] tokens [num_groups]
+ * lie in the same pages. Their page tables all name these, but only the first
+ * sequence's is read there, as far as its length goes; sequences may be shorter
+ * than what they share, or in no group. Read on the device, as the batch is. Group
+ * starts that fall or pass the sequences make all rows NaN, and
+ * tsg_ctx_synchronize reports TSG_ERR_INVALID_ARGUMENT. */
+typedef struct tsg_attn_prefixes {
+    const uint32_t* group_starts;
+    const uint32_t* shared;
+    uint32_t num_groups;
+} tsg_attn_prefixes;
+
+/* The checks tsg_attn_decode_shared makes of these arguments, without a device
+ * (batch may be NULL: not checked). */
+tsg_status tsg_attn_prefixes_check(const tsg_attn_config* config, const tsg_attn_batch* batch,
+                                   const tsg_attn_prefixes* prefixes);
+/* tsg_attn_decode, the keys that a group shares read once for all of its rows: two
+ * launches, for groups of several sequences and long prefixes. The same results up to
+ * the order of sums; the first sequence's bad page reaches all of its group.
+ * Returns TSG_ERR_DECLINED for a window, more than 8 rows a sequence, more than 2048
+ * sequences, or more than 255 tiles of 128 rows: (rows * query heads a key head / 128
+ * + num_groups) * kv_heads. q, out and the plan's scratch as for tsg_attn_decode. */
+tsg_status tsg_attn_decode_shared(tsg_attn* attn, tsg_stream stream, const tsg_kv_pages* pages,
+                                  const tsg_attn_batch* batch, const tsg_attn_prefixes* prefixes,
+                                  const uint16_t* q, uint32_t q_stride, uint16_t* out,
+                                  uint32_t out_stride);
+
 /* ----------------------------------------------------- gated delta rule ---
  * The token mixer of a layer that keeps a state instead of a key/value cache,
  * between the layer's projections: a short causal convolution with SiLU, whose

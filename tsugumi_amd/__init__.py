@@ -16,7 +16,7 @@ include/tsugumi_hip.h (libtsugumi_hip.so). Names follow the reference:
     SharedExpertInt4        -> SharedExpertInt4 (Gemma's dense int4 MLP)
 
 The attention half of the layer (Attention, PagedKVCache, AttentionBatch,
-HeadNormRope) and the gated delta rule of the layers that keep a state
+SharedPrefixes, HeadNormRope) and the gated delta rule of the layers that keep a state
 instead of a cache (GatedDelta, DeltaStates, DeltaBatch, DeltaGates) are this
 library's own.
 
@@ -40,7 +40,7 @@ __all__ = [
     "PrefillRouter", "PrefillMoEGrouping",
     "PrefillRoutedGEMMPlanner", "PrefillGroupedRoutedMoE", "PrefillMoE", "ResidentLayer",
     "MoEPack", "SharedExpertInt4", "PrefillLayerTail", "FusedLayerTail", "PrefillInt4QMM",
-    "Attention", "PagedKVCache", "AttentionBatch", "HeadNormRope",
+    "Attention", "PagedKVCache", "AttentionBatch", "SharedPrefixes", "HeadNormRope",
     "GatedDelta", "DeltaStates", "DeltaBatch", "DeltaGates",
     "ExpertOffsets", "TsgError", "PAIR_DTYPE", "BLOCK_DTYPE", "GROUP_DTYPE", "TILE_DTYPE",
     "generators", "load",
@@ -936,6 +936,28 @@ class AttentionBatch:
         self.kind = attn.batch_kind
 
 
+class SharedPrefixes:
+    """Groups of a batch's sequences that begin alike (tsg_attn_prefixes): group_starts
+    [groups + 1] and the tokens that each shares, [groups], of 32-bit integers. For calls of any
+    Attention without a window on this device."""
+
+    def __init__(self, attn: "Attention", group_starts, shared):
+        for t in (group_starts, shared):
+            if not t.is_cuda or t.device.index != attn.ctx.device:
+                _refuse("prefix tensors must be on the context's device")
+            if t.dtype not in _types("int32", "uint32") or not t.is_contiguous() or t.dim() != 1:
+                _refuse("prefix tensors must be contiguous vectors of 32-bit integers")
+        groups = int(shared.shape[0])
+        if group_starts.shape[0] != groups + 1:
+            _refuse("group_starts must be [groups + 1] and shared [groups]")
+        _words(num_groups=groups)
+        self._keep = (group_starts, shared)
+        self.device = attn.ctx.device
+        self.prefixes = _abi.AttnPrefixes(_ptr(group_starts), _ptr(shared), groups)
+        self._ref = C.addressof(self.prefixes)
+        check(attn.lib.tsg_attn_prefixes_check(C.addressof(attn.config), None, self._ref))
+
+
 class HeadNormRope:
     """Head norms (bf16 weights [head_dim] or None) and position rotation
     (inv_freq: fp32 [rotary_dim / 2] or None) of tsg_attn_append."""
@@ -1003,6 +1025,9 @@ class Attention:
 
     def batch(self, page_table, lengths, rows, row_starts=None) -> AttentionBatch:
         return AttentionBatch(self, page_table, lengths, rows, row_starts)
+
+    def prefixes(self, group_starts, shared) -> SharedPrefixes:
+        return SharedPrefixes(self, group_starts, shared)
 
     def _rows(self, t, rows: int, heads: int, width: int):
         """Address and row stride of a row operand."""
@@ -1085,6 +1110,20 @@ class Attention:
     def encode_decode(self, cache, batch, q, out, stream=None):
         """Attention of 1..8 new tokens of every sequence."""
         self._attend(self._decode, cache, batch, q, out, stream)
+
+    def encode_decode_shared(self, cache, batch, prefixes, q, out, stream=None):
+        """encode_decode, with the keys that groups of sequences share read once a group."""
+        n, hq, _, _, width, _ = batch.rows, *self._layout
+        if cache.kind is not self.cache_kind or batch.kind is not self.batch_kind:
+            self._fits(cache, batch)  # made by another plan
+        if prefixes.device != self._device:
+            _refuse("prefixes must be on the context's device")
+        q, qs = self._rows(q, n, hq, width)
+        out, os = self._rows(out, n, hq, width)
+        status = self.lib.tsg_attn_decode_shared(self.handle, self._after_last(stream), cache._ref,
+                                                 batch._ref, prefixes._ref, q, qs, out, os)
+        if status:
+            check(status)
 
     def encode_prefill(self, cache, batch, q, out, stream=None):
         """Attention of a prompt's rows, or of the next chunk of one."""

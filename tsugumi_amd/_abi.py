@@ -109,6 +109,11 @@ class AttnBatch(C.Structure):
                 ("table_stride", C.c_uint32), ("num_seqs", C.c_uint32), ("rows", C.c_uint32)]
 
 
+class AttnPrefixes(C.Structure):
+    """tsg_attn_prefixes: groups of sequences that share their first tokens."""
+    _fields_ = [("group_starts", C.c_void_p), ("shared", C.c_void_p), ("num_groups", C.c_uint32)]
+
+
 class AttnRows(C.Structure):
     """tsg_attn_rows: projected query, key and value rows."""
     _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
@@ -230,6 +235,8 @@ SIGNATURES = {
     "tsg_attn_append": (C.c_int, [P, P, P, P, P, P, P, U32]),
     "tsg_attn_decode": (C.c_int, [P, P, P, P, P, U32, P, U32]),
     "tsg_attn_prefill": (C.c_int, [P, P, P, P, P, U32, P, U32]),
+    "tsg_attn_prefixes_check": (C.c_int, [P, P, P]),
+    "tsg_attn_decode_shared": (C.c_int, [P, P, P, P, P, P, U32, P, U32]),
     "tsg_delta_check": (C.c_int, [P, P, P, P]),
     "tsg_delta_create": (C.c_int, [P, P, C.POINTER(P)]),
     "tsg_delta_destroy": (None, [P]),

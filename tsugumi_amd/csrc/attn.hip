@@ -566,6 +566,56 @@ extern "C" tsg_status tsg_attn_decode(tsg_attn* attn, tsg_stream stream, const t
     return launch_decode(attn, a, stream);
 }
 
+static tsg_status check_prefixes(const tsg_attn_config& c, const tsg_attn_batch* b,
+                                 const tsg_attn_prefixes* x) {
+    TSG_REQUIRE(x, TSG_ERR_INVALID_ARGUMENT, "attention prefixes are NULL");
+    TSG_REQUIRE(x->num_groups > 0 && x->num_groups <= kMaxAttnRows, TSG_ERR_INVALID_ARGUMENT,
+                "num_groups must be in 1...%u", kMaxAttnRows);
+    TSG_REQUIRE(x->group_starts && x->shared, TSG_ERR_INVALID_ARGUMENT,
+                "NULL group starts or shared lengths");
+    TSG_REQUIRE(is4(x->group_starts) && is4(x->shared), TSG_ERR_ALIGNMENT,
+                "group starts and shared lengths must be 4-byte aligned");
+    TSG_REQUIRE(c.window == 0, TSG_ERR_DECLINED,
+                "a window leaves little of a prefix to share: tsg_attn_decode");
+    if (!b) return TSG_OK;
+    TSG_REQUIRE(!b->row_starts, TSG_ERR_INVALID_ARGUMENT,
+                "decode takes the same 1...%u rows of every sequence (no row starts)",
+                kMaxDecodeRows);
+    TSG_REQUIRE(b->rows / b->num_seqs <= kMaxDecodeRows, TSG_ERR_DECLINED,
+                "more than %u rows a sequence: tsg_attn_prefill", kMaxDecodeRows);
+    TSG_REQUIRE(b->num_seqs <= kMaxSharedSeqs, TSG_ERR_DECLINED,
+                "more than %u sequences: tsg_attn_decode", kMaxSharedSeqs);
+    return TSG_OK;
+}
+
+extern "C" tsg_status tsg_attn_prefixes_check(const tsg_attn_config* config,
+                                              const tsg_attn_batch* batch,
+                                              const tsg_attn_prefixes* prefixes) {
+    if (tsg_status s = check_attn_config(config)) return s;
+    if (batch)
+        if (tsg_status s = check_attn_batch(*config, batch)) return s;
+    return check_prefixes(*config, batch, prefixes);
+}
+
+extern "C" tsg_status tsg_attn_decode_shared(tsg_attn* attn, tsg_stream stream,
+                                             const tsg_kv_pages* pages,
+                                             const tsg_attn_batch* batch,
+                                             const tsg_attn_prefixes* prefixes, const uint16_t* q,
+                                             uint32_t q_stride, uint16_t* out,
+                                             uint32_t out_stride) {
+    AttnArgs a{};
+    if (tsg_status s = attn_args(attn, pages, batch, q, q_stride, out, out_stride, &a)) return s;
+    if (tsg_status s = check_prefixes(attn->cfg, batch, prefixes)) return s;
+    PrefixArgs x{};
+    x.group_starts = prefixes->group_starts;
+    x.shared = prefixes->shared;
+    x.num_groups = prefixes->num_groups;
+    DeviceScope scope(attn->device);
+    TSG_HIP_TRY(scope.status);
+    if (tsg_status s = launch_prefixes(attn, a, &x, stream)) return s;
+    return launch_decode(attn, a, stream, &x);
+}
+
 // Few rows of wide heads, and so few tiles of them that most of the card would
 // idle: the decode kernel splits the keys finer. One sequence, heads of 512 (16
 // query, 2 key heads), decode against prefill kernel: 32 rows of the group over 4000

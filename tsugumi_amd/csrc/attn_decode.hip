@@ -36,6 +36,7 @@ struct DecodeArgs {
     uint32_t row_tiles;  // 16-row tiles of a sequence's rows and group
     uint32_t pairs;      // key heads * (most runs there can be)
     float join_cost;     // of a split in the join, against a tile's of its run
+    PrefixArgs x;        // what the sequences share, summed up already
 };
 
 constexpr uint32_t kMinTiles = kWaves;  // key tiles worth a workgroup: one a wave
@@ -58,11 +59,18 @@ struct Run {
     uint32_t slot;    // of the sequence's first partial sum
     uint32_t length;  // the sequence's
 };
-__device__ __forceinline__ uint32_t seq_key_tiles(const AttnArgs& a, uint32_t length) {
+template <bool SHARED>
+__device__ __forceinline__ uint32_t seq_key_tiles(const DecodeArgs& p, uint32_t s, uint32_t length) {
+    const AttnArgs& a = p.a;
     if (length > (a.table_stride << a.page_shift)) return 0u;  // reported; its rows are NaN
+    if constexpr (SHARED) {  // those behind the shared ones
+        const uint32_t first = p.x.info[s].x / kTile, end = (length + kTile - 1u) / kTile;
+        return end > first ? end - first : 0u;
+    }
     const int32_t lo = (int32_t)length - (int32_t)a.seq_rows;
     return tile_span<kTile>(lo < 0 ? 0 : lo, (int32_t)length - 1, a.window, a.sinks).count;
 }
+template <bool SHARED>
 __device__ __forceinline__ bool find_run(const DecodeArgs& p, uint32_t at, Run* r) {
     const AttnArgs& a = p.a;
     if (p.chunks == 0u) {
@@ -86,7 +94,7 @@ __device__ __forceinline__ bool find_run(const DecodeArgs& p, uint32_t at, Run* 
     };
     if (a.num_seqs == 1u) {
         const uint32_t length = scalar_load(a.lengths);
-        const uint32_t tiles = seq_key_tiles(a, length);
+        const uint32_t tiles = seq_key_tiles<SHARED>(p, 0u, length);
         const uint32_t even = (tiles + p.chunks - 1u) / p.chunks;
         const uint32_t per = run_length(tiles, even > kMinTiles ? even : kMinTiles);
         *r = Run{0u, at, runs_of(tiles, per), per, 0u, length};
@@ -97,7 +105,7 @@ __device__ __forceinline__ bool find_run(const DecodeArgs& p, uint32_t at, Run* 
     uint64_t total = 0;  // of 256 sequences of up to 2^26 tiles each
     for (uint32_t base = 0; base < a.num_seqs; base += 64u) {
         const uint32_t length = base + lane < a.num_seqs ? a.lengths[base + lane] : 0u;
-        uint32_t n = base + lane < a.num_seqs ? seq_key_tiles(a, length) : 0u;
+        uint32_t n = base + lane < a.num_seqs ? seq_key_tiles<SHARED>(p, base + lane, length) : 0u;
         if (base == 0u) first = length;
         n -= n >> 26;  // 64 of them stay under 2^32
 #pragma unroll
@@ -113,7 +121,7 @@ __device__ __forceinline__ bool find_run(const DecodeArgs& p, uint32_t at, Run* 
     for (uint32_t base = 0; base < a.num_seqs; base += 64u) {
         const bool live = base + lane < a.num_seqs;
         const uint32_t length = base == 0u ? first : live ? a.lengths[base + lane] : 0u;
-        const uint32_t tiles = live ? seq_key_tiles(a, length) : 0u;
+        const uint32_t tiles = live ? seq_key_tiles<SHARED>(p, base + lane, length) : 0u;
         const uint32_t own = run_length(tiles, per);
         const uint32_t runs = live ? runs_of(tiles, own) : 0u;
         // runs, and above them those of split sequences: both sums stay under 2^16
@@ -180,7 +188,8 @@ template <int DP, bool E4M3, bool FULL>
 constexpr int kSimdWaves = kDirect<E4M3, FULL> ? (DP <= 128 ? 4 : 2)
                                                : (DP <= 128 ? 3 : DP <= 256 ? 2 : 1);
 
-template <int DP, bool E4M3, bool FULL>
+// SHARED: the keys behind those that a group of sequences shares, whose sums are there.
+template <int DP, bool E4M3, bool FULL, bool SHARED = false>
 __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kernel(DecodeArgs p) {
     constexpr uint32_t NS = DP / 32, NB = DP / 16;   // key-product steps, value blocks
     constexpr uint32_t CELL = E4M3 ? 1 : 2;
@@ -201,7 +210,7 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
     }
     const uint32_t kvh = pair % a.kv_heads;
     Run run;
-    if (!find_run(p, pair / a.kv_heads, &run)) return;
+    if (!find_run<SHARED>(p, pair / a.kv_heads, &run)) return;
     const uint32_t s = run.seq;
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -215,7 +224,15 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
     const int32_t base = (int32_t)sr.length - (int32_t)sr.count;
     // positions of all of the sequence's rows: its row tiles take the same runs
     const int32_t p_lo = base, p_hi = (int32_t)sr.length - 1;
-    const TileSpan span = tile_span<kTile>(p_lo < 0 ? 0 : p_lo, p_hi, a.window, a.sinks);
+    TileSpan span = tile_span<kTile>(p_lo < 0 ? 0 : p_lo, p_hi, a.window, a.sinks);
+    uint32_t shared = 0;     // tokens
+    bool bad_groups = false;
+    if constexpr (SHARED) {
+        shared = scalar_load(&p.x.info[s].x);
+        bad_groups = scalar_load(&p.x.info[s].w) != 0u;
+        span.first = shared / kTile;
+        span.count = span.count > span.first ? span.count - span.first : 0u;
+    }
     const uint32_t used = run.used;
     const uint32_t tile_first = run.split * run.per;  // one run: split 0
     const uint32_t tile_end =
@@ -479,6 +496,7 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
         l = __builtin_nanf("");
         if (lane == 0) report(a.error, sr.bad ? sr.bad : kErrAttnPage);
     }
+    if (SHARED && bad_groups) l = __builtin_nanf("");  // reported
 
     // the four waves' sums: lane (row i16, g) holds elements 16 b + 4 g .. + 3
     float* so = reinterpret_cast<float*>(smem);
@@ -518,6 +536,44 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
                    ((uint32_t)f32_to_f16(acc[2 * e + 1] * inv) << 16);
         *reinterpret_cast<uint4*>(out) = make_uint4(h[0], h[1], h[2], h[3]);
     };
+    // The sums of the shared keys, every ways-th split of them, added to a row's piece.
+    const auto add_shared = [&](uint32_t r, uint32_t c, float* acc, float& sum, float& mm,
+                                uint32_t way, uint32_t ways) {
+        const uint32_t splits = prefix_split(p.x, shared / kTileKeys<DP>).used;
+        const uint32_t row_at = scalar_load(&p.x.info[s].z) + r0 + r;
+        const uint32_t tile = scalar_load(&p.x.info[s].y) + row_at / kPrefillRows;
+        const uint64_t first = ((uint64_t)tile * a.kv_heads + kvh) * p.x.splits;
+#pragma unroll 1
+        for (uint32_t w0 = way; w0 < splits; w0 += kJoinLoads * ways) {
+            f4_t lo[kJoinLoads], hi[kJoinLoads];
+            float2 ml[kJoinLoads];
+#pragma unroll
+            for (uint32_t k = 0; k < kJoinLoads; ++k) {
+                const uint32_t w = w0 + k * ways < splits ? w0 + k * ways : w0;
+                const uint64_t at = (first + w) * kPrefillRows + row_at % kPrefillRows;
+                ml[k] = *reinterpret_cast<const float2*>(p.x.part_ml + at * 2u);
+                const f4_t* src = reinterpret_cast<const f4_t*>(p.x.part_o + at * DP + 8u * c);
+                lo[k] = src[0];
+                hi[k] = src[1];
+            }
+            float mn = mm;
+#pragma unroll
+            for (uint32_t k = 0; k < kJoinLoads; ++k) mn = fmaxf(mn, ml[k].x);
+            const float f0 = __builtin_amdgcn_exp2f((mm - mn) * a.scale_log2);
+            mm = mn;
+            sum *= f0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] *= f0;
+#pragma unroll
+            for (uint32_t k = 0; k < kJoinLoads; ++k) {
+                if (w0 + k * ways >= splits) continue;
+                const float f = __builtin_amdgcn_exp2f((ml[k].x - mn) * a.scale_log2);
+                sum += ml[k].y * f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[e] += (e < 4 ? lo[k][e & 3] : hi[k][e & 3]) * f;
+            }
+        }
+    };
 #pragma unroll 1
     for (uint32_t n = 0; n < PIECES; ++n) {
         const uint32_t piece = threadIdx.x + 256u * n, r = piece / C8, c = piece % C8;
@@ -545,6 +601,7 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
             }
         }
         if (used == 1u) {
+            if constexpr (SHARED) add_shared(r, c, acc, sum, mm, 0u, 1u);
             emit(r, c, acc, sum);
         } else {
             const uint64_t slot = slot_of(run.split) * 16u + r;
@@ -624,6 +681,8 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
                 }
             }
         }
+        if constexpr (SHARED)
+            if (in) add_shared(r, c, acc, sum, mm, way, ways);
         for (uint32_t o = 1; o < ways; o <<= 1) {
             const float m2 = __shfl_xor(mm, (int)o, 64), mn = fmaxf(mm, m2);
             const float f0 = __builtin_amdgcn_exp2f((mm - mn) * a.scale_log2);
@@ -640,24 +699,29 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
 
 typedef void (*DecodeKernel)(DecodeArgs);
 
-template <int DP>
+template <int DP, bool SHARED>
 DecodeKernel kernel_of(bool e4m3, bool full) {
-    if (e4m3) return full ? decode_kernel<DP, true, true> : decode_kernel<DP, true, false>;
-    return full ? decode_kernel<DP, false, true> : decode_kernel<DP, false, false>;
+    if (e4m3)
+        return full ? decode_kernel<DP, true, true, SHARED> : decode_kernel<DP, true, false, SHARED>;
+    return full ? decode_kernel<DP, false, true, SHARED> : decode_kernel<DP, false, false, SHARED>;
 }
 
 struct Variant {
-    DecodeKernel kernel;
+    DecodeKernel kernel, shared;
     uint32_t lds;
 };
+template <int DP>
+Variant variant(bool e4m3, bool full) {
+    return {kernel_of<DP, false>(e4m3, full), kernel_of<DP, true>(e4m3, full), decode_lds_bytes<DP>()};
+}
 Variant variant_of(const tsg_attn* attn) {
     const bool e4m3 = attn->cfg.kv_type == TSG_KV_E4M3;
     const bool full = attn->cfg.head_dim == attn->padded_dim;
     switch (attn->padded_dim) {
-        case 64: return {kernel_of<64>(e4m3, full), decode_lds_bytes<64>()};
-        case 128: return {kernel_of<128>(e4m3, full), decode_lds_bytes<128>()};
-        case 256: return {kernel_of<256>(e4m3, full), decode_lds_bytes<256>()};
-        default: return {kernel_of<512>(e4m3, full), decode_lds_bytes<512>()};
+        case 64: return variant<64>(e4m3, full);
+        case 128: return variant<128>(e4m3, full);
+        case 256: return variant<256>(e4m3, full);
+        default: return variant<512>(e4m3, full);
     }
 }
 
@@ -665,14 +729,17 @@ Variant variant_of(const tsg_attn* attn) {
 
 tsg_status prepare_decode(const tsg_attn* attn) {
     const Variant v = variant_of(attn);
-    TSG_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(v.kernel),
-                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)v.lds));
+    for (DecodeKernel kernel : {v.kernel, v.shared})
+        TSG_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)v.lds));
     return TSG_OK;
 }
 
-tsg_status launch_decode(const tsg_attn* attn, const AttnArgs& a, tsg_stream stream) {
+tsg_status launch_decode(const tsg_attn* attn, const AttnArgs& a, tsg_stream stream,
+                         const PrefixArgs* prefix) {
     DecodeArgs p{};
     p.a = a;
+    if (prefix) p.x = *prefix;
     p.row_tiles = (a.seq_rows * a.group + kDecodeTileRows - 1u) / kDecodeTileRows;
     // As many runs as workgroups fit the card at once (LDS: four a CU up to
     // heads of 128, then two and one); a batch of so many sequences that its
@@ -699,7 +766,8 @@ tsg_status launch_decode(const tsg_attn* attn, const AttnArgs& a, tsg_stream str
     p.part_ml = attn->partials + (uint64_t)kMaxPartials * 16u * attn->padded_dim;
     p.arrivals = attn->arrivals;
     const Variant v = variant_of(attn);
-    hipLaunchKernelGGL(v.kernel, dim3((uint32_t)blocks), dim3(256), v.lds, as_stream(stream), p);
+    hipLaunchKernelGGL(prefix ? v.shared : v.kernel, dim3((uint32_t)blocks), dim3(256), v.lds,
+                       as_stream(stream), p);
     return check_launch("attn_decode");
 }
 

@@ -27,6 +27,7 @@ namespace tsg {
 constexpr uint32_t kErrAttnPage = 256u;
 constexpr uint32_t kErrAttnLength = 512u;
 constexpr uint32_t kErrAttnRows = 1024u;
+constexpr uint32_t kErrAttnGroups = 8192u;  // group starts that fall or pass the sequences
 // The delta rule's: a slot past the pool or an out slot that is another
 // sequence's; wrong row starts.
 constexpr uint32_t kErrDeltaSlot = 2048u;
@@ -61,6 +62,30 @@ struct AttnArgs {
 typedef __attribute__((address_space(4))) const uint32_t const_u32_t;
 __device__ __forceinline__ uint32_t scalar_load(const uint32_t* p) {
     return *(const_u32_t*)(uintptr_t)p;
+}
+
+// Sequences that share their first tokens. What all of a group's rows see of them, the first
+// kernel sums up (attn_prefill.hip) and the second takes in when it joins a row's own keys'
+// sums (attn_decode.hip). Rows (sequence, token, head of the key head's group) of a group are
+// counted from its first, in tiles of 128; group g's begin at tile row0 / 128 + g.
+constexpr uint32_t kShareTokens = 64;  // shared tokens are taken in whole key tiles
+struct PrefixArgs {
+    const uint32_t* group_starts;
+    const uint32_t* shared;
+    uint4* info;     // [seqs]: shared tokens, the group's first tile, the sequence's first row in
+                     // the group, whether the group starts are wrong
+    float* part_o;   // [tile][key head][split][128][DP]
+    float* part_ml;  // [tile][key head][split][128][2]
+    uint32_t num_groups, tiles, splits, min_tiles;
+};
+// Splits of so many key tiles, and the tiles of one.
+struct PrefixSplit {
+    uint32_t used, per;
+};
+__device__ __forceinline__ PrefixSplit prefix_split(const PrefixArgs& x, uint32_t key_tiles) {
+    const uint32_t even = (key_tiles + x.splits - 1u) / x.splits;
+    const uint32_t per = even > x.min_tiles ? even : x.min_tiles;
+    return PrefixSplit{(key_tiles + per - 1u) / per, per};
 }
 
 struct SeqRows {
@@ -313,6 +338,9 @@ tsg_status attn_args(const tsg_attn* attn, const tsg_kv_pages* pages, const tsg_
                      const uint16_t* q, uint32_t q_stride, uint16_t* out, uint32_t out_stride,
                      AttnArgs* a);
 
+template <int DP>
+constexpr uint32_t kTileKeys = DP <= 128 ? 64 : 32;  // of the prefill kernel
+
 // attn_decode.hip
 constexpr uint32_t kDecodeTileRows = 16;
 constexpr uint32_t kMaxPartials = 2048;  // partial sums (of a 16-row tile) of one call
@@ -322,9 +350,18 @@ constexpr uint32_t kPrefillRows = 128;
 constexpr uint32_t kPartialRows = std::max(kMaxPartials * kDecodeTileRows,
                                            kMaxPrefillPartials * kPrefillRows);
 tsg_status prepare_decode(const tsg_attn* attn);  // once a plan, its device current
-tsg_status launch_decode(const tsg_attn* attn, const AttnArgs& a, tsg_stream stream);
+// `prefix`: NULL, or what launch_prefixes has made ready
+tsg_status launch_decode(const tsg_attn* attn, const AttnArgs& a, tsg_stream stream,
+                         const PrefixArgs* prefix = nullptr);
 // attn_prefill.hip
 tsg_status prepare_prefill(const tsg_attn* attn);
 tsg_status launch_prefill(const tsg_attn* attn, const AttnArgs& a, tsg_stream stream);
+// A decode call's shared keys: the scratch behind what launch_decode uses holds
+// their partial sums, kMaxPrefixBlocks of 128 rows, and `info` of kMaxSharedSeqs.
+constexpr uint32_t kMaxPrefixBlocks = kPartialRows / kPrefillRows - kMaxPartials * kDecodeTileRows / kPrefillRows - 1u;
+constexpr uint32_t kMaxSharedSeqs = 2048;
+static_assert(kMaxSharedSeqs * 16u <= kPrefillRows * (64u + 2u) * 4u, "info fits a block");
+tsg_status launch_prefixes(const tsg_attn* attn, const AttnArgs& a, PrefixArgs* x,
+                           tsg_stream stream);
 
 }  // namespace tsg

@@ -33,10 +33,9 @@ struct PrefillArgs {
     float* part_ml;  // [tile block][split][128][2]
     uint32_t splits, min_tiles;
     uint32_t seq_tiles;  // row tiles of a sequence when its rows are uniform
+    PrefixArgs x;        // for the keys that groups of sequences share
 };
 
-template <int DP>
-constexpr uint32_t kTileKeys = DP <= 128 ? 64 : 32;
 // Head elements a wave takes. At 512 a wave's sums and queries would fill all
 // registers of a SIMD: two waves share the rows instead, each with one half of
 // the elements, and add up their halves of the key products through LDS.
@@ -152,7 +151,77 @@ __device__ __forceinline__ TilePlan<DP> tile_plan(const PrefillArgs& p, const Se
     return t;
 }
 
-template <int DP, bool E4M3, bool FULL>
+// Shared keys: group and tile `at` of its rows; kind 0: none, or wrong group starts.
+struct GroupTile {
+    uint32_t kind, first_seq, seqs, tile, tokens;
+};
+__device__ __forceinline__ uint32_t shared_tokens(const AttnArgs& a, const PrefixArgs& x,
+                                                  uint32_t g, uint32_t first_seq, uint32_t seqs) {
+    // of the first sequence's pages, in whole key tiles; one sequence shares with none
+    const uint32_t capacity = a.table_stride << a.page_shift;
+    uint32_t n = x.shared[g];
+    const uint32_t length = a.lengths[first_seq];
+    n = n < length ? n : length;
+    n = n < capacity ? n : capacity;
+    return seqs > 1u ? n / kShareTokens * kShareTokens : 0u;
+}
+__device__ __forceinline__ uint32_t group_tile0(const AttnArgs& a, uint32_t g, uint32_t first_seq) {
+    return first_seq * (a.seq_rows * a.group) / kRows + g;
+}
+__device__ __forceinline__ GroupTile find_group_tile(const AttnArgs& a, const PrefixArgs& x,
+                                                     uint32_t at) {
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t before = 0;  // groups whose tiles begin at or before `at`
+    bool wrong = false;
+    for (uint32_t base = 0; base < x.num_groups; base += 64u) {
+        const uint32_t g = base + lane;
+        const bool live = g < x.num_groups;
+        const uint32_t lo = live ? x.group_starts[g] : 0u, hi = live ? x.group_starts[g + 1u] : 0u;
+        wrong = wrong || lo > hi || hi > a.num_seqs;
+        before += (uint32_t)__builtin_popcountll(
+            __ballot(live && lo <= a.num_seqs && group_tile0(a, g, lo) <= at));
+    }
+    if (__ballot(wrong) || before == 0u) return GroupTile{0u, 0u, 0u, 0u, 0u};
+    const uint32_t g = before - 1u;
+    const uint32_t lo = scalar_load(x.group_starts + g), hi = scalar_load(x.group_starts + g + 1u);
+    const uint32_t tile = at - group_tile0(a, g, lo);
+    if (hi == lo || tile * kRows >= (hi - lo) * a.seq_rows * a.group) return GroupTile{0u, 0u, 0u, 0u, 0u};
+    const uint32_t tokens = __builtin_amdgcn_readfirstlane(shared_tokens(a, x, g, lo, hi - lo));
+    return GroupTile{tokens ? 1u : 0u, lo, hi - lo, tile, tokens};
+}
+// What the joining kernel needs to know of every sequence.
+__device__ __forceinline__ void write_info(const AttnArgs& a, const PrefixArgs& x) {
+    uint32_t wrong = 0;
+    for (uint32_t g = threadIdx.x; g < x.num_groups; g += blockDim.x) {
+        const uint32_t lo = x.group_starts[g], hi = x.group_starts[g + 1u];
+        wrong |= lo > hi || hi > a.num_seqs ? 1u : 0u;
+    }
+    wrong = __syncthreads_or((int)wrong) ? 1u : 0u;
+    if (wrong && threadIdx.x == 0) report(a.error, kErrAttnGroups);
+    for (uint32_t s = threadIdx.x; s < a.num_seqs; s += blockDim.x) {
+        uint4 info = make_uint4(0u, 0u, 0u, wrong);
+        if (!wrong && x.num_groups) {
+            uint32_t lo = 0, hi = x.num_groups;  // the last group that starts at or before s
+            while (lo < hi) {
+                const uint32_t mid = (lo + hi) / 2u;
+                if (x.group_starts[mid] <= s) lo = mid + 1u;
+                else hi = mid;
+            }
+            if (lo) {
+                const uint32_t g = lo - 1u, first = x.group_starts[g], end = x.group_starts[g + 1u];
+                if (s < end)
+                    info = make_uint4(shared_tokens(a, x, g, first, end - first),
+                                      group_tile0(a, g, first), (s - first) * a.seq_rows * a.group,
+                                      0u);
+            }
+        }
+        x.info[s] = info;
+    }
+}
+
+// SHARED: the rows of a group of sequences over the keys that it shares, which leave
+// partial sums.
+template <int DP, bool E4M3, bool FULL, bool SHARED = false>
 __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p) {
     constexpr uint32_t TK = kTileKeys<DP>;
     constexpr uint32_t DW = kWaveDim<DP>, THREADS = kThreads<DP>, SHARE = DP / DW;
@@ -168,19 +237,54 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
     const uint32_t split = blockIdx.y;
     const uint32_t kvh = blockIdx.x % a.kv_heads;
     const uint32_t at = blockIdx.x / a.kv_heads;
-    const RowTile rt = find_tile(p, at, gridDim.x / a.kv_heads, at == 0u && split == 0u);
-    if (rt.kind != 1u) {
-        if (rt.kind == 2u && split == 0u) poison_rows(a, kvh, rt.tile, rt.count, rt.seq);
-        return;
+    uint32_t s = 0;
+    SeqRows sr{};
+    TilePlan<DP> t{};
+    uint32_t tile_first = 0, tile_end = 0, shared = 0;
+    if constexpr (SHARED) {
+        if (at >= p.x.tiles) {
+            if (kvh == 0u && split == 0u) write_info(a, p.x);
+            return;
+        }
+        const GroupTile gt = find_group_tile(a, p.x, at);
+        if (gt.kind == 0u) return;
+        s = gt.first_seq;  // its page table
+        shared = gt.tokens;
+        const PrefixSplit ps = prefix_split(p.x, shared / TK);
+        if (split >= ps.used) return;
+        t.rows = gt.seqs * a.seq_rows * a.group;
+        t.r0 = gt.tile * kRows;
+        t.live = t.rows - t.r0 < kRows ? t.rows - t.r0 : kRows;
+        t.used = 2u;  // partial sums
+        tile_first = split * ps.per;
+        tile_end = tile_first + ps.per;
+    } else {
+        const RowTile rt = find_tile(p, at, gridDim.x / a.kv_heads, at == 0u && split == 0u);
+        if (rt.kind != 1u) {
+            if (rt.kind == 2u && split == 0u) poison_rows(a, kvh, rt.tile, rt.count, rt.seq);
+            return;
+        }
+        s = rt.seq;
+        const uint32_t capacity = a.table_stride << a.page_shift;
+        sr = seq_rows(a.row_starts, a.lengths, s, a.seq_rows, a.rows, capacity);
+        t = tile_plan<DP>(p, sr, rt.tile);
+        if (split >= t.used) return;
+        tile_first = split * t.per;
+        tile_end = tile_first + t.per < t.span.count ? tile_first + t.per : t.span.count;
+        if (sr.bad) tile_end = tile_first;
     }
-    const uint32_t s = rt.seq;
-    const uint32_t capacity = a.table_stride << a.page_shift;
-    const SeqRows sr = seq_rows(a.row_starts, a.lengths, s, a.seq_rows, a.rows, capacity);
-    const TilePlan<DP> t = tile_plan<DP>(p, sr, rt.tile);
-    if (split >= t.used) return;
-    const uint32_t tile_first = split * t.per;
-    uint32_t tile_end = tile_first + t.per < t.span.count ? tile_first + t.per : t.span.count;
-    if (sr.bad) tile_end = tile_first;
+    // position of row r of the workgroup's: of its own keys the last, of shared ones at most
+    const auto row_pos = [&](uint32_t r) -> int32_t {
+        if constexpr (SHARED) {
+            const uint32_t token = (t.r0 + r) / a.group, seq = s + token / a.seq_rows;
+            const uint32_t capacity = a.table_stride << a.page_shift, length = a.lengths[seq];
+            const int32_t pos = (int32_t)(length < capacity ? length : capacity) -
+                                (int32_t)a.seq_rows + (int32_t)(token % a.seq_rows);
+            return pos < (int32_t)shared ? pos : (int32_t)shared - 1;
+        } else {
+            return t.base + (int32_t)((t.r0 + r) / a.group);
+        }
+    };
 
     const uint32_t lane = threadIdx.x & 63u, i32 = lane & 31u, h = lane >> 5;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -190,11 +294,33 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
     const uint32_t d0 = (wave >> 2) * DW;         // its first head element
     const bool wave_live = w0 < t.live;
     const uint32_t w_last = w0 + 31u < t.live ? w0 + 31u : t.live - 1u;
-    const int32_t p_lo = t.base + (int32_t)((t.r0 + (wave_live ? w0 : 0u)) / a.group);
-    const int32_t p_hi = t.base + (int32_t)((t.r0 + w_last) / a.group);
     const uint32_t row = t.r0 + (w0 + i32 < t.live ? w0 + i32 : t.live - 1u);
     const uint32_t tok = row / a.group;
-    const int32_t pos = t.base + (int32_t)tok;
+    const int32_t pos = row_pos(row - t.r0);
+    int32_t p_lo, p_hi;
+    if constexpr (SHARED) {  // of the workgroup's rows, of sequences of any lengths
+        const uint32_t r1 = lane < t.live ? lane : t.live - 1u;
+        const uint32_t r2 = lane + 64u < t.live ? lane + 64u : t.live - 1u;
+        const int32_t p1 = row_pos(r1), p2 = row_pos(r2);
+        p_lo = p1 < p2 ? p1 : p2;
+        p_hi = p1 < p2 ? p2 : p1;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const int32_t lo = __shfl_xor(p_lo, o, 64), hi = __shfl_xor(p_hi, o, 64);
+            p_lo = p_lo < lo ? p_lo : lo;
+            p_hi = p_hi > hi ? p_hi : hi;
+        }
+        p_lo = __builtin_amdgcn_readfirstlane(p_lo);
+        p_hi = __builtin_amdgcn_readfirstlane(p_hi);
+        t.p_lo = p_lo;
+        t.p_hi = p_hi;
+        t.span = tile_span<TK>(0, p_hi, 0u, 0u);
+        tile_end = tile_end < t.span.count ? tile_end : t.span.count;
+        sr.first = s * a.seq_rows;
+    } else {
+        p_lo = t.base + (int32_t)((t.r0 + (wave_live ? w0 : 0u)) / a.group);
+        p_hi = t.base + (int32_t)((t.r0 + w_last) / a.group);
+    }
     const uint32_t q_head = kvh * a.group + row % a.group;
     const uint16_t* q = a.q + (uint64_t)(sr.first + tok) * a.q_stride + (uint64_t)q_head * a.dim;
     h8_t qf[NS];  // step st takes, from lane half h, elements 16 st + 8 h ..
@@ -446,8 +572,7 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
             const uint32_t mark = (bits & 0x3FFu ? 3u : bits & 0x8000u ? 2u : 1u) << (2u * (dim & 15u));
 #pragma unroll 1
             for (uint32_t r = 0; r < t.live; ++r)
-                if (key_seen((int32_t)(key0 + k), t.base + (int32_t)((t.r0 + r) / a.group), a.window,
-                             a.sinks))
+                if (key_seen((int32_t)(key0 + k), row_pos(r), a.window, a.sinks))
                     atomicOr(marks + r * (DP / 16u) + dim / 16u, mark);
         }
         __syncthreads();
@@ -520,7 +645,7 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
     }
 
     // lane half h holds elements 32 b + 8 k + 4 h .. + 3 of its row
-    if (t.used == 1u) {
+    if (!SHARED && t.used == 1u) {
         const float inv = row_inverse(l, pos, a.v_scale);
         uint16_t* out = a.out + (uint64_t)(sr.first + tok) * a.out_stride + (uint64_t)q_head * a.dim;
 #pragma unroll
@@ -537,15 +662,17 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
                 *reinterpret_cast<uint2*>(out + e) = u;
             }
     } else {
-        const uint64_t slot = ((uint64_t)blockIdx.x * p.splits + split) * kRows + w0 + i32;
-        float* dst = p.part_o + slot * DP;
+        const uint64_t slot =
+            ((uint64_t)blockIdx.x * (SHARED ? p.x.splits : p.splits) + split) * kRows + w0 + i32;
+        float* part_ml = SHARED ? p.x.part_ml : p.part_ml;
+        float* dst = (SHARED ? p.x.part_o : p.part_o) + slot * DP;
 #pragma unroll
         for (uint32_t b = 0; b < NB; ++b)
 #pragma unroll
             for (uint32_t k = 0; k < 4u; ++k)
                 *reinterpret_cast<float4*>(dst + d0 + 32u * b + 8u * k + 4u * h) = make_float4(
                     o[b][4 * k], o[b][4 * k + 1], o[b][4 * k + 2], o[b][4 * k + 3]);
-        if (h == 0 && d0 == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2u) = make_float2(m, l);
+        if (h == 0 && d0 == 0) *reinterpret_cast<float2*>(part_ml + slot * 2u) = make_float2(m, l);
     }
 }
 
@@ -611,20 +738,21 @@ __global__ __launch_bounds__(256) void prefill_join_kernel(PrefillArgs p) {
 
 typedef void (*PrefillKernel)(PrefillArgs);
 
-template <int DP>
+template <int DP, bool SHARED>
 PrefillKernel kernel_of(bool e4m3, bool full) {
-    if (e4m3) return full ? prefill_kernel<DP, true, true> : prefill_kernel<DP, true, false>;
-    return full ? prefill_kernel<DP, false, true> : prefill_kernel<DP, false, false>;
+    if (e4m3)
+        return full ? prefill_kernel<DP, true, true, SHARED> : prefill_kernel<DP, true, false, SHARED>;
+    return full ? prefill_kernel<DP, false, true, SHARED> : prefill_kernel<DP, false, false, SHARED>;
 }
 
 struct Variant {
-    PrefillKernel kernel, join;
+    PrefillKernel kernel, join, shared;
     uint32_t threads, lds, tile_keys;
 };
 template <int DP>
 Variant variant(bool e4m3, bool full) {
-    return {kernel_of<DP>(e4m3, full), prefill_join_kernel<DP>, kThreads<DP>,
-            prefill_lds_bytes<DP>(), kTileKeys<DP>};
+    return {kernel_of<DP, false>(e4m3, full), prefill_join_kernel<DP>, kernel_of<DP, true>(e4m3, full),
+            kThreads<DP>, prefill_lds_bytes<DP>(), kTileKeys<DP>};
 }
 Variant variant_of(const tsg_attn* attn) {
     const bool e4m3 = attn->cfg.kv_type == TSG_KV_E4M3;
@@ -641,9 +769,40 @@ Variant variant_of(const tsg_attn* attn) {
 
 tsg_status prepare_prefill(const tsg_attn* attn) {
     const Variant v = variant_of(attn);
-    TSG_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(v.kernel),
-                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)v.lds));
+    for (PrefillKernel kernel : {v.kernel, v.shared})
+        TSG_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)v.lds));
     return TSG_OK;
+}
+
+tsg_status launch_prefixes(const tsg_attn* attn, const AttnArgs& a, PrefixArgs* x,
+                           tsg_stream stream) {
+    const Variant v = variant_of(attn);
+    // each group may end inside a tile
+    const uint64_t tiles = (uint64_t)a.rows * a.group / kRows + std::min(x->num_groups, a.num_seqs);
+    const uint64_t blocks = tiles * a.kv_heads;
+    TSG_REQUIRE(blocks <= kMaxPrefixBlocks, TSG_ERR_DECLINED,
+                "too many rows, heads and groups for the plan's scratch: tsg_attn_decode");
+    // up to twice as many workgroups as the card holds, of at least four key tiles
+    const uint64_t capacity_tiles =
+        (((uint64_t)a.table_stride << a.page_shift) + v.tile_keys - 1u) / v.tile_keys;
+    x->min_tiles = 4u;
+    const uint64_t resident = 2u * (uint64_t)attn->ctx->num_cus * 256u / v.threads;
+    uint64_t splits = 2u * resident / std::max<uint64_t>(blocks, 1u);
+    splits = std::min(splits, (capacity_tiles + x->min_tiles - 1u) / x->min_tiles);
+    splits = std::min<uint64_t>(splits, kMaxPrefixBlocks / std::max<uint64_t>(blocks, 1u));
+    x->splits = (uint32_t)std::max<uint64_t>(splits, 1u);
+    x->tiles = (uint32_t)tiles;
+    const uint64_t row0 = kMaxPartials * (uint64_t)kDecodeTileRows, dp = attn->padded_dim;
+    x->part_o = attn->partials + row0 * (dp + 2u);
+    x->part_ml = x->part_o + (uint64_t)kMaxPrefixBlocks * kRows * dp;
+    x->info = reinterpret_cast<uint4*>(x->part_ml + (uint64_t)kMaxPrefixBlocks * kRows * 2u);
+    PrefillArgs p{};
+    p.a = a;
+    p.x = *x;
+    hipLaunchKernelGGL(v.shared, dim3((uint32_t)blocks + a.kv_heads, x->splits), dim3(v.threads), v.lds,
+                       as_stream(stream), p);
+    return check_launch("attn_prefixes");
 }
 
 tsg_status launch_prefill(const tsg_attn* attn, const AttnArgs& a, tsg_stream stream) {

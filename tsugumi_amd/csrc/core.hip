@@ -181,6 +181,8 @@ constexpr DeviceError kDeviceErrors[] = {
     {kErrAttnRows, TSG_ERR_INVALID_ARGUMENT,
      "attention: row starts that fall or pass the batch's rows; the rows before the sequences "
      "behind the last such one are NaN and not appended"},
+    {kErrAttnGroups, TSG_ERR_INVALID_ARGUMENT,
+     "attention: group starts that fall or pass the batch's sequences; all rows are NaN"},
     {kErrDeltaSlot, TSG_ERR_INVALID_ARGUMENT,
      "delta rule: a slot past the pool, or a sequence's out slot that is another's in or out slot; "
      "its rows are NaN and its state was not written"},
