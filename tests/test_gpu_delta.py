@@ -217,6 +217,12 @@ def test_prefill_many_sequences(tsg, ctx):
     check(tsg, ctx, Case(rows, 1, 1, 32, 32, seed=49), "prefill")
 
 
+@pytest.mark.parametrize("rows,heads,dk", [([64] * 32, (16, 64), 16), ([130] * 12, (32, 64), 64)])
+def test_prefill_with_a_full_card(tsg, ctx, rows, heads, dk):
+    """More workgroups than the card holds at once: their waves drift apart."""
+    check(tsg, ctx, Case(rows, *heads, dk, 16, seed=52), "prefill")
+
+
 def test_prefill_columns_of_different_sizes(tsg, ctx):
     """Value elements and states from 1e-6 to 1e4 side by side: each column is held to its own
     size."""

@@ -340,6 +340,7 @@ __global__ __launch_bounds__(256, 4) void prepare_kernel(ChunkArgs p) {
             make_uint4(lo.x, lo.y, hi.x, hi.y);
     }
 
+    __syncthreads();  // T takes the weights' place
     // T: the diagonal tiles by substitution, a column a lane, ...
     {
         float x[16];
