@@ -773,8 +773,8 @@ typedef struct tsg_attn tsg_attn; /* one kind of attention layer and its scratch
  * (pages and batch may be NULL: not checked). */
 tsg_status tsg_attn_check(const tsg_attn_config* config, const tsg_kv_pages* pages,
                           const tsg_attn_batch* batch);
-/* Calls on one tsg_attn run in stream order (they share its scratch: 17, 34, 68 or
- * 135 MB for head sizes up to 64, 128, 256, 512; two that overlap leave it unfit
+/* Calls on one tsg_attn run in stream order (they share its scratch: 26, 52, 102 or
+ * 203 MB for head sizes up to 64, 128, 256, 512; two that overlap leave it unfit
  * for later ones); two tsg_attn may run beside each other. Graphs captured with one
  * are replayed one after the other, beside no other call of it, and before its
  * end. Not while a stream is captured (it allocates). The context outlives the
@@ -819,7 +819,8 @@ tsg_status tsg_attn_prefill(tsg_attn* attn, tsg_stream stream, const tsg_kv_page
  * sequence's is read there, as far as its length goes; sequences may be shorter
  * than what they share, or in no group. Read on the device, as the batch is. Group
  * starts that fall or pass the sequences make all rows NaN, and
- * tsg_ctx_synchronize reports TSG_ERR_INVALID_ARGUMENT. */
+ * tsg_ctx_synchronize reports TSG_ERR_INVALID_ARGUMENT (unless the call is
+ * tsg_attn_decode's, see there). */
 typedef struct tsg_attn_prefixes {
     const uint32_t* group_starts;
     const uint32_t* shared;
@@ -831,11 +832,13 @@ typedef struct tsg_attn_prefixes {
 tsg_status tsg_attn_prefixes_check(const tsg_attn_config* config, const tsg_attn_batch* batch,
                                    const tsg_attn_prefixes* prefixes);
 /* tsg_attn_decode, the keys that a group shares read once for all of its rows: two
- * launches, for groups of several sequences and long prefixes. The same results up to
- * the order of sums; the first sequence's bad page reaches all of its group.
- * Returns TSG_ERR_DECLINED for a window, more than 8 rows a sequence, more than 2048
- * sequences, or more than 255 tiles of 128 rows: (rows * query heads a key head / 128
- * + num_groups) * kv_heads. q, out and the plan's scratch as for tsg_attn_decode. */
+ * launches, for groups of several sequences and prefixes of a few thousand tokens
+ * on. The same results up to the order of sums; the first sequence's bad page
+ * reaches all of its group. Few rows a group of heads over 128 (under 32 rows x query
+ * heads a key head, on the average) take tsg_attn_decode's kernel, which asks for no
+ * groups. Returns TSG_ERR_DECLINED for a window, more than 8 rows a sequence, more than
+ * 2048 sequences, or rows * q_heads over 65,472. q, out and the plan's scratch as for
+ * tsg_attn_decode. */
 tsg_status tsg_attn_decode_shared(tsg_attn* attn, tsg_stream stream, const tsg_kv_pages* pages,
                                   const tsg_attn_batch* batch, const tsg_attn_prefixes* prefixes,
                                   const uint16_t* q, uint32_t q_stride, uint16_t* out,

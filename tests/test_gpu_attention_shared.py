@@ -67,6 +67,19 @@ def test_head_layouts(tsg, ctx, q_heads, kv_heads, dim, kv):  # noqa: F811
     check(tsg, ctx, share(c, [0, 3, 5], [192, 128]))
 
 
+@pytest.mark.parametrize("kv", ["f16", "e4m3"])
+@pytest.mark.parametrize("q_heads,kv_heads,dim", [(4, 2, 256), (8, 1, 272), (16, 2, 144), (4, 1, 512)])
+@pytest.mark.parametrize("prefix", [64, 1600])
+def test_wide_heads_of_many_rows(tsg, ctx, q_heads, kv_heads, dim, kv, prefix):  # noqa: F811
+    """On the side of the rule where heads over 128 share: also rows inside the prefix, and over
+    several splits."""
+    seqs = -(-64 * kv_heads // (2 * q_heads)) + 2
+    lengths = [prefix + 40 + 9 * s for s in range(seqs)]
+    lengths[1] = prefix - 20
+    c = Case([2] * seqs, lengths, q_heads, kv_heads, dim, kv=kv, seed=dim)
+    check(tsg, ctx, share(c, [0, seqs // 2, seqs], [prefix, prefix]))
+
+
 @pytest.mark.parametrize("rows", [1, 2, 3, 5, 8])
 @pytest.mark.parametrize("heads", [(1, 1), (7, 1), (16, 2), (40, 1)])
 def test_blocks_of_rows(tsg, ctx, rows, heads):  # noqa: F811
@@ -280,10 +293,10 @@ def test_call_refusals(tsg, ctx):  # noqa: F811
     table = torch.zeros(2049, 1, dtype=torch.int32, device="cuda")
     many = torch.zeros(2049, 4, 64, dtype=torch.float16, device="cuda")
     refused(4, shared, cache, attn.batch(table, lengths, 2049), good, many, many)
-    groups = attn.prefixes(torch.arange(129, dtype=torch.int32, device="cuda"), torch.zeros(
-        128, dtype=torch.int32, device="cuda"))
-    refused(4, shared, cache, attn.batch(table[:2048], lengths[:2048], 2048), groups, many[:2048],
-            many[:2048])
+    big = tsg.Attention(ctx, 32, 1, 64, 16)
+    many = torch.zeros(2047, 32, 64, dtype=torch.float16, device="cuda")
+    refused(4, big.encode_decode_shared, big.cache(d["k"][:, :1], d["v"][:, :1]),
+            big.batch(table[:2047], lengths[:2047], 2047), good, many, many)
     torch.cuda.synchronize()
     assert bool((out == -77).all())
     ctx.synchronize()

@@ -229,7 +229,7 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
     bool bad_groups = false;
     if constexpr (SHARED) {
         shared = scalar_load(&p.x.info[s].x);
-        bad_groups = scalar_load(&p.x.info[s].w) != 0u;
+        bad_groups = scalar_load(&p.x.info[s].y) != 0u;
         span.first = shared / kTile;
         span.count = span.count > span.first ? span.count - span.first : 0u;
     }
@@ -540,9 +540,7 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
     const auto add_shared = [&](uint32_t r, uint32_t c, float* acc, float& sum, float& mm,
                                 uint32_t way, uint32_t ways) {
         const uint32_t splits = prefix_split(p.x, shared / kTileKeys<DP>).used;
-        const uint32_t row_at = scalar_load(&p.x.info[s].z) + r0 + r;
-        const uint32_t tile = scalar_load(&p.x.info[s].y) + row_at / kPrefillRows;
-        const uint64_t first = ((uint64_t)tile * a.kv_heads + kvh) * p.x.splits;
+        const uint64_t first = (uint64_t)kvh * p.x.splits * p.x.rows + s * rows + r0 + r;
 #pragma unroll 1
         for (uint32_t w0 = way; w0 < splits; w0 += kJoinLoads * ways) {
             f4_t lo[kJoinLoads], hi[kJoinLoads];
@@ -550,7 +548,7 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
 #pragma unroll
             for (uint32_t k = 0; k < kJoinLoads; ++k) {
                 const uint32_t w = w0 + k * ways < splits ? w0 + k * ways : w0;
-                const uint64_t at = (first + w) * kPrefillRows + row_at % kPrefillRows;
+                const uint64_t at = first + (uint64_t)w * p.x.rows;
                 ml[k] = *reinterpret_cast<const float2*>(p.x.part_ml + at * 2u);
                 const f4_t* src = reinterpret_cast<const f4_t*>(p.x.part_o + at * DP + 8u * c);
                 lo[k] = src[0];
@@ -574,9 +572,16 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
             }
         }
     };
+    // neighbouring lanes that share a piece, where the row's keys are this workgroup's and
+    // shared ones: the first has the former, each some splits of the latter
+    uint32_t share_log2 = 0;
+    if constexpr (SHARED)
+        if (used == 1u && shared)
+            while ((live * C8 << (share_log2 + 1u)) <= 256u && share_log2 < 5u) ++share_log2;
+    const uint32_t share_way = threadIdx.x & ((1u << share_log2) - 1u);
 #pragma unroll 1
     for (uint32_t n = 0; n < PIECES; ++n) {
-        const uint32_t piece = threadIdx.x + 256u * n, r = piece / C8, c = piece % C8;
+        const uint32_t piece = (threadIdx.x >> share_log2) + 256u * n, r = piece / C8, c = piece % C8;
         if (r >= live || 8u * c >= a.dim) continue;
         float mm = sm[r];
 #pragma unroll
@@ -584,6 +589,7 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
         float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0.0f;
 #pragma unroll
         for (uint32_t w = 0; w < kWaves; ++w) {
+            if (SHARED && share_way) break;
             const float f = __builtin_amdgcn_exp2f((sm[w * 16u + r] - mm) * a.scale_log2);
             sum += sl[w * 16u + r] * f;
             const float* src = so + (w * 16u + r) * (DP + 4u) + 8u * c;
@@ -591,7 +597,7 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
             for (int e = 0; e < 8; ++e) acc[e] += src[e] * f;
         }
         for (uint32_t w = 0; w < kWaves; ++w) {
-            if (!sx[w]) continue;
+            if (!sx[w] || (SHARED && share_way)) continue;
             const uint32_t mark = reinterpret_cast<const uint16_t*>(
                 smem + decode_lds_bytes<DP>() - kMarkBytes<DP>)[(w * 16u + r) * (DP / 8u) + c];
 #pragma unroll
@@ -601,7 +607,21 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
             }
         }
         if (used == 1u) {
-            if constexpr (SHARED) add_shared(r, c, acc, sum, mm, 0u, 1u);
+            if constexpr (SHARED) {
+                add_shared(r, c, acc, sum, mm, share_way, 1u << share_log2);
+                // the lanes of a piece are all here
+                for (uint32_t o = 1; o < 1u << share_log2; o <<= 1) {
+                    const float m2 = __shfl_xor(mm, (int)o, 64), mn = fmaxf(mm, m2);
+                    const float f0 = __builtin_amdgcn_exp2f((mm - mn) * a.scale_log2);
+                    const float f1 = __builtin_amdgcn_exp2f((m2 - mn) * a.scale_log2);
+                    mm = mn;
+                    sum = sum * f0 + __shfl_xor(sum, (int)o, 64) * f1;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        acc[e] = acc[e] * f0 + __shfl_xor(acc[e], (int)o, 64) * f1;
+                }
+                if (share_way) continue;
+            }
             emit(r, c, acc, sum);
         } else {
             const uint64_t slot = slot_of(run.split) * 16u + r;

@@ -66,17 +66,17 @@ __device__ __forceinline__ uint32_t scalar_load(const uint32_t* p) {
 
 // Sequences that share their first tokens. What all of a group's rows see of them, the first
 // kernel sums up (attn_prefill.hip) and the second takes in when it joins a row's own keys'
-// sums (attn_decode.hip). Rows (sequence, token, head of the key head's group) of a group are
-// counted from its first, in tiles of 128; group g's begin at tile row0 / 128 + g.
+// sums (attn_decode.hip). Rows (sequence, token, head of the key head's group) are taken in
+// tiles of 128 from a group's first; group g's begin at tile (its first row) / 128 + g.
 constexpr uint32_t kShareTokens = 64;  // shared tokens are taken in whole key tiles
 struct PrefixArgs {
     const uint32_t* group_starts;
     const uint32_t* shared;
-    uint4* info;     // [seqs]: shared tokens, the group's first tile, the sequence's first row in
-                     // the group, whether the group starts are wrong
-    float* part_o;   // [tile][key head][split][128][DP]
-    float* part_ml;  // [tile][key head][split][128][2]
+    uint2* info;     // [seqs]: shared tokens, whether the group starts are wrong
+    float* part_o;   // [key head][split][row][DP]
+    float* part_ml;  // [key head][split][row][2]
     uint32_t num_groups, tiles, splits, min_tiles;
+    uint32_t rows;   // of all sequences
 };
 // Splits of so many key tiles, and the tiles of one.
 struct PrefixSplit {
@@ -346,7 +346,7 @@ constexpr uint32_t kDecodeTileRows = 16;
 constexpr uint32_t kMaxPartials = 2048;  // partial sums (of a 16-row tile) of one call
 constexpr uint32_t kMaxPrefillPartials = 512;  // (row tile, key head, split) of one call
 constexpr uint32_t kPrefillRows = 128;
-// rows of partial results the plan's scratch holds, padded_dim + 2 floats each
+// rows of partial results of a decode or prefill call, padded_dim + 2 floats each
 constexpr uint32_t kPartialRows = std::max(kMaxPartials * kDecodeTileRows,
                                            kMaxPrefillPartials * kPrefillRows);
 tsg_status prepare_decode(const tsg_attn* attn);  // once a plan, its device current
@@ -357,10 +357,13 @@ tsg_status launch_decode(const tsg_attn* attn, const AttnArgs& a, tsg_stream str
 tsg_status prepare_prefill(const tsg_attn* attn);
 tsg_status launch_prefill(const tsg_attn* attn, const AttnArgs& a, tsg_stream stream);
 // A decode call's shared keys: the scratch behind what launch_decode uses holds
-// their partial sums, kMaxPrefixBlocks of 128 rows, and `info` of kMaxSharedSeqs.
-constexpr uint32_t kMaxPrefixBlocks = kPartialRows / kPrefillRows - kMaxPartials * kDecodeTileRows / kPrefillRows - 1u;
+// their partial sums, of kMaxPrefixRows rows, and `info` of kMaxSharedSeqs.
+constexpr uint32_t kMaxPrefixRows = 65472;
 constexpr uint32_t kMaxSharedSeqs = 2048;
-static_assert(kMaxSharedSeqs * 16u <= kPrefillRows * (64u + 2u) * 4u, "info fits a block");
+constexpr uint32_t kInfoRows = 64;
+static_assert(kMaxSharedSeqs * 8u <= kInfoRows * (64u + 2u) * 4u, "info fits its rows");
+constexpr uint32_t kScratchRows = kMaxPartials * kDecodeTileRows + kMaxPrefixRows + kInfoRows;
+static_assert(kScratchRows >= kPartialRows, "the scratch holds a prefill call's partial results");
 tsg_status launch_prefixes(const tsg_attn* attn, const AttnArgs& a, PrefixArgs* x,
                            tsg_stream stream);
 

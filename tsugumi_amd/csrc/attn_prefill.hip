@@ -199,7 +199,7 @@ __device__ __forceinline__ void write_info(const AttnArgs& a, const PrefixArgs& 
     wrong = __syncthreads_or((int)wrong) ? 1u : 0u;
     if (wrong && threadIdx.x == 0) report(a.error, kErrAttnGroups);
     for (uint32_t s = threadIdx.x; s < a.num_seqs; s += blockDim.x) {
-        uint4 info = make_uint4(0u, 0u, 0u, wrong);
+        uint2 info = make_uint2(0u, wrong);
         if (!wrong && x.num_groups) {
             uint32_t lo = 0, hi = x.num_groups;  // the last group that starts at or before s
             while (lo < hi) {
@@ -209,10 +209,7 @@ __device__ __forceinline__ void write_info(const AttnArgs& a, const PrefixArgs& 
             }
             if (lo) {
                 const uint32_t g = lo - 1u, first = x.group_starts[g], end = x.group_starts[g + 1u];
-                if (s < end)
-                    info = make_uint4(shared_tokens(a, x, g, first, end - first),
-                                      group_tile0(a, g, first), (s - first) * a.seq_rows * a.group,
-                                      0u);
+                if (s < end) info.x = shared_tokens(a, x, g, first, end - first);
             }
         }
         x.info[s] = info;
@@ -234,9 +231,11 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
     extern __shared__ __align__(16) uint8_t smem[];
     const AttnArgs& a = p.a;
 
-    const uint32_t split = blockIdx.y;
+    // A group's tiles that have no rows come behind all others: between them, in turn with
+    // live ones, they would leave whole shader engines without work.
+    const uint32_t split = SHARED ? blockIdx.x / a.kv_heads : blockIdx.y;
     const uint32_t kvh = blockIdx.x % a.kv_heads;
-    const uint32_t at = blockIdx.x / a.kv_heads;
+    const uint32_t at = SHARED ? blockIdx.y : blockIdx.x / a.kv_heads;
     uint32_t s = 0;
     SeqRows sr{};
     TilePlan<DP> t{};
@@ -663,7 +662,9 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
             }
     } else {
         const uint64_t slot =
-            ((uint64_t)blockIdx.x * (SHARED ? p.x.splits : p.splits) + split) * kRows + w0 + i32;
+            SHARED ? (uint64_t)(kvh * p.x.splits + split) * p.x.rows +
+                         s * a.seq_rows * a.group + t.r0 + w0 + i32
+                   : ((uint64_t)blockIdx.x * p.splits + split) * kRows + w0 + i32;
         float* part_ml = SHARED ? p.x.part_ml : p.part_ml;
         float* dst = (SHARED ? p.x.part_o : p.part_o) + slot * DP;
 #pragma unroll
@@ -778,30 +779,32 @@ tsg_status prepare_prefill(const tsg_attn* attn) {
 tsg_status launch_prefixes(const tsg_attn* attn, const AttnArgs& a, PrefixArgs* x,
                            tsg_stream stream) {
     const Variant v = variant_of(attn);
-    // each group may end inside a tile
-    const uint64_t tiles = (uint64_t)a.rows * a.group / kRows + std::min(x->num_groups, a.num_seqs);
-    const uint64_t blocks = tiles * a.kv_heads;
-    TSG_REQUIRE(blocks <= kMaxPrefixBlocks, TSG_ERR_DECLINED,
-                "too many rows, heads and groups for the plan's scratch: tsg_attn_decode");
-    // up to twice as many workgroups as the card holds, of at least four key tiles
+    const uint64_t rows = (uint64_t)a.rows * a.group, groups = std::min(x->num_groups, a.num_seqs);
+    TSG_REQUIRE(rows * a.kv_heads <= kMaxPrefixRows, TSG_ERR_DECLINED,
+                "too many rows and query heads for the plan's scratch: tsg_attn_decode");
+    // each group may end inside a tile, and has one at least
+    const uint64_t tiles = rows / kRows + groups;
+    const uint64_t live = std::max((rows + kRows - 1u) / kRows, groups) * a.kv_heads;
+    // (a launch of few enough blocks: tiles and key heads are bounded by the rows)
+    // as many workgroups as the card holds, of at least four key tiles
     const uint64_t capacity_tiles =
         (((uint64_t)a.table_stride << a.page_shift) + v.tile_keys - 1u) / v.tile_keys;
     x->min_tiles = 4u;
-    const uint64_t resident = 2u * (uint64_t)attn->ctx->num_cus * 256u / v.threads;
-    uint64_t splits = 2u * resident / std::max<uint64_t>(blocks, 1u);
+    uint64_t splits = 2u * (uint64_t)attn->ctx->num_cus * 256u / v.threads / live;
     splits = std::min(splits, (capacity_tiles + x->min_tiles - 1u) / x->min_tiles);
-    splits = std::min<uint64_t>(splits, kMaxPrefixBlocks / std::max<uint64_t>(blocks, 1u));
+    splits = std::min<uint64_t>(splits, kMaxPrefixRows / (rows * a.kv_heads));
     x->splits = (uint32_t)std::max<uint64_t>(splits, 1u);
     x->tiles = (uint32_t)tiles;
+    x->rows = (uint32_t)rows;
     const uint64_t row0 = kMaxPartials * (uint64_t)kDecodeTileRows, dp = attn->padded_dim;
     x->part_o = attn->partials + row0 * (dp + 2u);
-    x->part_ml = x->part_o + (uint64_t)kMaxPrefixBlocks * kRows * dp;
-    x->info = reinterpret_cast<uint4*>(x->part_ml + (uint64_t)kMaxPrefixBlocks * kRows * 2u);
+    x->part_ml = x->part_o + kMaxPrefixRows * dp;
+    x->info = reinterpret_cast<uint2*>(x->part_ml + kMaxPrefixRows * 2u);
     PrefillArgs p{};
     p.a = a;
     p.x = *x;
-    hipLaunchKernelGGL(v.shared, dim3((uint32_t)blocks + a.kv_heads, x->splits), dim3(v.threads), v.lds,
-                       as_stream(stream), p);
+    hipLaunchKernelGGL(v.shared, dim3(a.kv_heads * x->splits, (uint32_t)tiles + 1u),
+                       dim3(v.threads), v.lds, as_stream(stream), p);
     return check_launch("attn_prefixes");
 }
 
