@@ -784,13 +784,15 @@ tsg_status launch_prefixes(const tsg_attn* attn, const AttnArgs& a, PrefixArgs* 
                 "too many rows and query heads for the plan's scratch: tsg_attn_decode");
     // each group may end inside a tile, and has one at least
     const uint64_t tiles = rows / kRows + groups;
-    const uint64_t live = std::max((rows + kRows - 1u) / kRows, groups) * a.kv_heads;
+    const uint64_t live = std::max(rows / kRows + (groups + 1u) / 2u, groups) * a.kv_heads;  // about
     // (a launch of few enough blocks: tiles and key heads are bounded by the rows)
-    // as many workgroups as the card holds, of at least four key tiles
+    // One workgroup a CU, of at least four key tiles: with two, the partial sums' way through
+    // memory costs what the shorter runs gain (64 sequences behind 16,000 tokens 57 us with one
+    // and with two, 32 sequences 50 and 62, 8 30 and 33; 8 groups of 8 behind 4000 49 and 47).
     const uint64_t capacity_tiles =
         (((uint64_t)a.table_stride << a.page_shift) + v.tile_keys - 1u) / v.tile_keys;
     x->min_tiles = 4u;
-    uint64_t splits = 2u * (uint64_t)attn->ctx->num_cus * 256u / v.threads / live;
+    uint64_t splits = (uint64_t)attn->ctx->num_cus * 256u / v.threads / live;
     splits = std::min(splits, (capacity_tiles + x->min_tiles - 1u) / x->min_tiles);
     splits = std::min<uint64_t>(splits, kMaxPrefixRows / (rows * a.kv_heads));
     x->splits = (uint32_t)std::max<uint64_t>(splits, 1u);

@@ -433,6 +433,19 @@ __global__ __launch_bounds__(256, 4) void prepare_kernel(ChunkArgs p) {
 
 constexpr uint32_t kScanThreads = 512;
 
+// The sequence of the n-th most rows, of up to 64: the longest chains are begun first.
+__device__ __forceinline__ uint32_t longest_first(const DeltaSeqs& d, uint32_t n) {
+    const uint32_t lane = threadIdx.x & 63u;
+    const bool live = lane < d.num_seqs;
+    const uint32_t count = live ? d.row_starts[lane + 1u] - d.row_starts[lane] : 0u;
+    uint32_t rank = 0;
+    for (uint32_t j = 0; j < d.num_seqs; ++j) {
+        const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)count, (int)j);
+        rank += other > count || (other == count && j < lane) ? 1u : 0u;
+    }
+    return (uint32_t)__builtin_ctzll(__ballot(live && rank == n));
+}
+
 template <uint32_t DKP>
 __global__ __launch_bounds__(kScanThreads, (DKP <= 128u ? 4 : 2)) void scan_kernel(ChunkArgs p) {
     constexpr uint32_t NK = DKP / 32u;                 // key steps
@@ -464,10 +477,12 @@ __global__ __launch_bounds__(kScanThreads, (DKP <= 128u ? 4 : 2)) void scan_kern
         unit = j / inner * 8u + (blockIdx.x & 7u);
         at = j % inner;
     }
-    const uint32_t s = unit / p.key_heads, kh = unit % p.key_heads;
+    uint32_t s = unit / p.key_heads;
+    const uint32_t kh = unit % p.key_heads;
     if (s >= d.seqs.num_seqs) return;
     const uint32_t head = kh * d.group + at / p.slices, c0 = at % p.slices * 16u;
     if (starts_wrong(d.seqs)) return;  // reported, and the rows made NaN, by the first kernel
+    if (d.seqs.row_starts && d.seqs.num_seqs <= 64u) s = longest_first(d.seqs, s);
     const DeltaSeq sq = delta_seq(d.seqs, s);
     const bool bad = out_slots_clash(d.seqs, s) || sq.bad;
     const uint32_t col4 = head * d.value_dim + c0 + 4u * (lane & 3u);
