@@ -907,8 +907,9 @@ typedef struct tsg_delta_batch {
 } tsg_delta_batch;
 
 /* Rows, fp16: row r of q at q + r * q_stride (elements), heads key_dim (v:
- * value_dim) apart; a and b have value_heads elements a row. q, k, v may lie in the
- * convolution's output, a and b in one buffer. */
+ * value_dim) apart, up to 2^27 elements from row to row (out as well); a and b have
+ * value_heads elements a row. q, k, v may lie in the convolution's output, a and b
+ * in one buffer. */
 typedef struct tsg_delta_rows {
     const uint16_t* q;
     const uint16_t* k;

@@ -104,6 +104,7 @@ def test_batch_refusals(abi, over, want):
     *[({n: 8 + (1 << 16)}, ALIGNMENT) for n in "qkv"], *[({n: 1 + (1 << 16)}, ALIGNMENT) for n in "ab"],
     *[({n + "_stride": 120}, INVALID) for n in "qkv"], *[({n + "_stride": 132}, ALIGNMENT) for n in "qkv"],
     (dict(a_stride=3), INVALID), (dict(b_stride=0), INVALID),
+    *[({n + "_stride": (1 << 27) + 8}, UNSUPPORTED) for n in "qkv"],
 ])
 def test_row_refusals(abi, over, want):
     assert status(abi, config(abi), None, None, rows(abi, **over)) == want

@@ -12,6 +12,7 @@ constexpr uint32_t kMaxValueHeads = 256, kMaxKeyDim = 256, kMaxValueDim = 512;
 constexpr uint32_t kMinConv = 2, kMaxConv = 8;
 constexpr uint32_t kMaxDeltaSeqs = 1u << 16;
 constexpr uint32_t kMaxDeltaRows = 1u << 22;
+constexpr uint32_t kMaxStride = 1u << 27;
 
 bool is16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 bool is4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
@@ -87,6 +88,9 @@ tsg_status check_rows(const tsg_delta_config& c, const tsg_delta_rows* r) {
                 TSG_ERR_INVALID_ARGUMENT, "q, k or v stride is too small");
     TSG_REQUIRE(r->a_stride >= c.value_heads && r->b_stride >= c.value_heads,
                 TSG_ERR_INVALID_ARGUMENT, "a or b stride is too small");
+    // 16 rows are addressed by 32-bit byte offsets
+    TSG_REQUIRE(r->q_stride <= kMaxStride && r->k_stride <= kMaxStride && r->v_stride <= kMaxStride,
+                TSG_ERR_UNSUPPORTED, "row strides must be at most %u elements", kMaxStride);
     TSG_REQUIRE(is16(r->q) && is16(r->k) && is16(r->v) && r->q_stride % 8u == 0 &&
                     r->k_stride % 8u == 0 && r->v_stride % 8u == 0,
                 TSG_ERR_ALIGNMENT, "q, k and v rows must be 16-byte aligned");
@@ -407,6 +411,8 @@ tsg_status delta_args(const tsg_delta* delta, const tsg_delta_states* states,
                 "a_log and dt_bias must be 4-byte aligned");
     const uint32_t kw = c.key_heads * c.key_dim, vw = c.value_heads * c.value_dim;
     TSG_REQUIRE(out_stride >= vw, TSG_ERR_INVALID_ARGUMENT, "out stride is too small");
+    TSG_REQUIRE(out_stride <= kMaxStride, TSG_ERR_UNSUPPORTED,
+                "row strides must be at most %u elements", kMaxStride);
     TSG_REQUIRE(is16(out) && out_stride % 8u == 0, TSG_ERR_ALIGNMENT,
                 "out rows must be 16-byte aligned");
     const struct {
