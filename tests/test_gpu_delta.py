@@ -79,6 +79,26 @@ def test_convolution_large_prompt(tsg, ctx):
     check(tsg, ctx, Case([700, 301], 4, 8, 64, 64, seed=24), "conv")
 
 
+def test_convolution_of_more_than_a_million_rows(tsg, ctx):
+    """More row tiles than 65536: the reference at the sequences' ends and past that tile."""
+    n = 16 * 65536 + 300
+    c = Case([n - 37, 37], 1, 1, 16, 16, seed=26)
+    d = c.launch(tsg, ctx, "conv")
+    ctx.synchronize()
+    w, x = c.weight.double().T, c.x.double()
+    for s, first, last in ((0, 0, n - 38), (1, n - 37, n - 1)):
+        assert torch.equal(d["conv"][c.outs[s]].cpu(), c.x[last - 2:last + 1])
+        old = c.conv[c.ins[s]].double()
+        for row in (first, first + 1, first + 36, last, max(first, 16 * 65536 + 5)):
+            rows = torch.stack([x[row - j] if row - j >= first else old[row - j - first + 3]
+                                for j in (3, 2, 1, 0)])
+            y, size = (rows * w).sum(0), (rows * w).abs().sum(0)
+            want = y * torch.sigmoid(y)
+            tol = 5.5 * 2.0 ** -24 * size + want.abs() * (2.0 ** -11 + 2.0 ** -21
+                                                          + y.abs() * 2.0 ** -22) + 2.0 ** -25
+            assert_near(d["conv_out"][row], want, tol)
+
+
 def test_convolution_extremes(tsg, ctx):
     """Sums far on either side of zero, and an infinity that only the rows that it reaches take."""
     c = Case([40], 1, 1, 16, 16, seed=25, size=300.0)

@@ -145,6 +145,7 @@ struct ConvArgs {
     uint16_t* states;
     uint64_t slot_stride;
     uint32_t x_stride, out_stride, channels;
+    uint32_t pieces;  // workgroups across the channels
 };
 
 __device__ __forceinline__ void unpack8(uint4 u, float (&f)[8]) {
@@ -159,21 +160,21 @@ __device__ __forceinline__ void unpack8(uint4 u, float (&f)[8]) {
 template <uint32_t W>
 __global__ __launch_bounds__(256) void conv_kernel(ConvArgs p) {
     const DeltaSeqs& d = p.seqs;
-    const DeltaTile t = delta_tile<kConvRows>(d, blockIdx.y);
+    const DeltaTile t = delta_tile<kConvRows>(d, blockIdx.x / p.pieces);
     if (t.kind == 0u) return;
-    const uint32_t c0 = (blockIdx.x * blockDim.x + threadIdx.x) * 8u;
+    const uint32_t piece = blockIdx.x % p.pieces, c0 = (piece * blockDim.x + threadIdx.x) * 8u;
     const bool live = c0 < p.channels;
     const uint4 nan8 = make_uint4(kDeltaNan2, kDeltaNan2, kDeltaNan2, kDeltaNan2);
     if (t.kind == 2u) {
         if (live)
             for (uint32_t r = t.first; r < t.first + t.count; ++r)
                 *reinterpret_cast<uint4*>(p.out + (uint64_t)r * p.out_stride + c0) = nan8;
-        if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) report(d.error, kErrDeltaRows);
+        if (blockIdx.x == 0 && threadIdx.x == 0) report(d.error, kErrDeltaRows);
         return;
     }
     const DeltaSeq q = delta_seq(d, t.seq);
     const bool bad = out_slots_clash(d, t.seq) || q.bad;
-    if (bad && t.tile == 0u && blockIdx.x == 0 && threadIdx.x == 0) report(d.error, kErrDeltaSlot);
+    if (bad && t.tile == 0u && piece == 0u && threadIdx.x == 0) report(d.error, kErrDeltaSlot);
     if (!live) return;
     const uint16_t* x = p.x + c0;
     uint16_t* out = p.out + c0;
@@ -223,6 +224,8 @@ __global__ __launch_bounds__(256) void conv_kernel(ConvArgs p) {
 #pragma unroll
                 for (uint32_t i = 0; i < W - 1u; ++i)
                     if (i == at) u[j] = in[i];
+                // else the compiler loads one of two addresses here, and `in` goes to memory
+                asm("" : "+v"(u[j].x), "+v"(u[j].y), "+v"(u[j].z), "+v"(u[j].w));
             } else {
                 u[j] = *reinterpret_cast<const uint4*>(
                     x + (uint64_t)(q.first + at - (W - 1u)) * p.x_stride);
@@ -542,18 +545,18 @@ extern "C" tsg_status tsg_delta_conv(tsg_delta* delta, tsg_stream stream,
     a.channels = delta->channels;
     const uint32_t tiles =
         delta_tiles<kConvRows>(batch->rows, batch->num_seqs, a.seqs.seq_rows, batch->row_starts);
-    const uint32_t pieces = delta->channels / 8u;
+    const uint32_t lanes = delta->channels / 8u;
     // few rows: one wave a workgroup, so that they spread over the CUs
-    const uint32_t threads = (uint64_t)tiles * pieces <= 256u * (uint64_t)delta->ctx->num_cus ? 64u : 256u;
-    const dim3 grid((pieces + threads - 1u) / threads, tiles);
-    TSG_REQUIRE((uint64_t)grid.x * tiles <= kMaxBlocks, TSG_ERR_UNSUPPORTED,
+    const uint32_t threads = (uint64_t)tiles * lanes <= 256u * (uint64_t)delta->ctx->num_cus ? 64u : 256u;
+    a.pieces = (lanes + threads - 1u) / threads;
+    TSG_REQUIRE((uint64_t)a.pieces * tiles <= kMaxBlocks, TSG_ERR_UNSUPPORTED,
                 "too many rows and channels for one launch");
     DeviceScope scope(delta->device);
     TSG_HIP_TRY(scope.status);
     static constexpr void (*kKernels[])(ConvArgs) = {conv_kernel<2>, conv_kernel<3>, conv_kernel<4>,
                                                      conv_kernel<5>, conv_kernel<6>, conv_kernel<7>,
                                                      conv_kernel<8>};
-    hipLaunchKernelGGL(kKernels[delta->cfg.conv_width - kMinConv], grid, dim3(threads), 0,
+    hipLaunchKernelGGL(kKernels[delta->cfg.conv_width - kMinConv], dim3(a.pieces * tiles), dim3(threads), 0,
                        as_stream(stream), a);
     return check_launch("delta_conv");
 }
