@@ -233,6 +233,37 @@ def test_refusals(tsg, ctx):  # noqa: F811
     ctx.synchronize()
 
 
+def test_too_large_for_one_launch(tsg, ctx):  # noqa: F811
+    """Refused before anything is launched."""
+    seqs, hv, dk, dv = 1040, 256, 16, 512
+    delta = tsg.GatedDelta(ctx, 1, hv, dk, dv)
+    half = lambda *shape: torch.zeros(*shape, dtype=torch.float16, device="cuda")  # noqa: E731
+    none = torch.full((seqs,), NONE, dtype=torch.int32, device="cuda")
+    gates = tsg.DeltaGates(torch.zeros(hv, device="cuda"), torch.zeros(hv, device="cuda"))
+    out = torch.full((seqs, hv, dv), -77.0, dtype=torch.float16, device="cuda")
+    scratch = torch.zeros(delta.scratch_bytes(seqs, seqs), dtype=torch.uint8, device="cuda")
+    refused(tsg, delta.encode_prefill, delta.states(torch.zeros(1, hv, dk, dv, device="cuda")),
+            delta.batch(none, none, seqs), half(seqs, dk), half(seqs, dk), half(seqs, hv * dv),
+            half(seqs, hv), half(seqs, hv), gates, out, scratch, status=3, text="launch")
+    torch.cuda.synchronize()
+    assert bool((out == -77).all()) and not bool(scratch.any())
+    ctx.synchronize()
+
+
+def test_a_sequence_without_rows_hands_its_state_on(tsg, ctx):  # noqa: F811
+    """Bit for bit, whatever the sizes beside each other in a column."""
+    c = Case([0, 70, 0], 1, 2, 64, 32, seed=71)
+    e = torch.randint(-140, 127, c.s[0].shape, generator=torch.Generator().manual_seed(72))
+    c.s[c.ins[0]] = torch.ldexp(c.s[c.ins[0]] + 1, e)
+    c.s[c.ins[2], :, ::5] = float("inf")
+    c.s[c.ins[2], :, 1::5] = 3e38
+    d = c.to_device()
+    c.launch(tsg, ctx, "prefill", d=d)
+    ctx.synchronize()
+    for s in (0, 2):
+        assert torch.equal(d["s"][c.outs[s]].cpu(), c.s[c.ins[s]])
+
+
 def test_closed_context_and_plan(tsg):  # noqa: F811
     c = Case([2], 1, 1, 64, 32, seed=64)
     d = c.to_device()

@@ -428,8 +428,10 @@ __global__ __launch_bounds__(256, 4) void prepare_kernel(ChunkArgs p) {
 // one wave's products need of the others' goes through LDS as operands of the matrix unit,
 // three exchanges a chunk: S, then R = beta (V - e^G K^ S), then U. Operands of the next
 // chunk are loaded as soon as this one's are used. Bound by the chain of a chunk's steps,
-// which leave the units mostly idle (eight waves of 16 columns: 8192 rows 260 us with
-// four).
+// which leave the units mostly idle: 1.6 us each with one workgroup a CU (8192 rows x 32 heads
+// of 128 x 128: 202 us; waves 0 to 3 alone, with the outputs' products after theirs, 260), a
+// seventh more with two, which share its LDS. 32 columns a workgroup halve the loads, but one
+// workgroup fits a CU then (11207 rows of 17 prompts: 292 us for 268).
 
 constexpr uint32_t kScanThreads = 512;
 
@@ -497,6 +499,16 @@ __global__ __launch_bounds__(kScanThreads, (DKP <= 128u ? 4 : 2)) void scan_kern
     // the state: register e of tile t of the wave's is key row 16 (TW wave + t) + 4 g + e, times
     // 2^(14 - exponent), the exponent of the column's last bound
     const uint64_t place = (uint64_t)head * d.key_dim * d.value_dim + c0 + i16;
+    if (sq.count == 0u) {  // handed on as it is
+        const uint32_t slot = scalar_load(d.seqs.out_slots + s);
+        if (slot == TSG_NO_SLOT) return;
+        for (uint32_t kr = threadIdx.x >> 4; kr < d.key_dim; kr += kScanThreads / 16u) {
+            const uint64_t at_kr = place + kr * d.value_dim;
+            d.s[(uint64_t)slot * d.slot_stride + at_kr] =
+                sq.fresh ? 0.0f : d.s[(uint64_t)sq.in * d.slot_stride + at_kr];
+        }
+        return;
+    }
     f4_t st[TW];
     const auto column_most = [&] {
         float m = 0.0f;
@@ -798,11 +810,9 @@ __global__ __launch_bounds__(kScanThreads, (DKP <= 128u ? 4 : 2)) void scan_kern
         }
         if constexpr (!keys) finish(chunks - 1u);
     };
-    if (chunks) {
-        __builtin_amdgcn_s_waitcnt(0x0F70);
-        if (wave < 4u) run(std::true_type());
-        else run(std::false_type());
-    }
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    if (wave < 4u) run(std::true_type());
+    else run(std::false_type());
     const uint32_t slot = scalar_load(d.seqs.out_slots + s);
     if (slot == TSG_NO_SLOT) return;
     const float from_s = __builtin_amdgcn_ldexpf(1.0f, exponent - 14);
@@ -826,16 +836,16 @@ tsg_status launch(const tsg_delta* delta, ChunkArgs p, uint32_t chunks, tsg_stre
     p.keys = p.records + (uint64_t)chunks * p.d.value_heads * kRecord;
     const uint64_t prepared = ((uint64_t)chunks * p.key_heads + 7u) / 8u * 8u * p.d.group;
     TSG_REQUIRE(prepared <= kMaxBlocks, TSG_ERR_UNSUPPORTED, "too many rows and heads for one launch");
-    p.chunks = chunks;
-    hipLaunchKernelGGL(prepare_kernel<DKP>, dim3((uint32_t)prepared), dim3(256),
-                       prepare_lds_bytes<DKP>(), as_stream(stream), p);
-    if (tsg_status s = check_launch("delta_prepare")) return s;
     const uint64_t units = (uint64_t)p.d.seqs.num_seqs * p.key_heads;
     const uint64_t inner = (uint64_t)p.d.group * p.slices;
     p.spread = units % 8u && units < 64u ? 1u : 0u;
     const uint64_t blocks = p.spread ? units * inner : (units + 7u) / 8u * 8u * inner;
     TSG_REQUIRE(2u * blocks <= kMaxBlocks, TSG_ERR_UNSUPPORTED,
                 "too many sequences and heads for one launch");
+    p.chunks = chunks;
+    hipLaunchKernelGGL(prepare_kernel<DKP>, dim3((uint32_t)prepared), dim3(256),
+                       prepare_lds_bytes<DKP>(), as_stream(stream), p);
+    if (tsg_status s = check_launch("delta_prepare")) return s;
     hipLaunchKernelGGL(scan_kernel<DKP>, dim3((uint32_t)blocks), dim3(kScanThreads), 0, as_stream(stream), p);
     return check_launch("delta_scan");
 }
