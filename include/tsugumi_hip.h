@@ -817,8 +817,8 @@ tsg_status tsg_attn_prefill(tsg_attn* attn, tsg_stream stream, const tsg_kv_page
  * group_starts[g + 1] - 1 [num_groups + 1], whose first shared[g] tokens [num_groups]
  * lie in the same pages. Their page tables all name these, but only the first
  * sequence's is read there, as far as its length goes; sequences may be shorter
- * than what they share, or in no group. Read on the device, as the batch is. Group
- * starts that fall or pass the sequences make all rows NaN, and
+ * than what they share, or in no group, and groups (1...2048) of no sequence. Read on
+ * the device, as the batch is. Group starts that fall or pass the sequences make all rows NaN, and
  * tsg_ctx_synchronize reports TSG_ERR_INVALID_ARGUMENT (unless the call is
  * tsg_attn_decode's, see there). */
 typedef struct tsg_attn_prefixes {

@@ -107,9 +107,11 @@ def test_page_sizes(tsg, ctx, page):  # noqa: F811
 @pytest.mark.parametrize("starts,shared", [
     ([0, 8], [128]), ([2, 5], [128]), ([0, 1, 8], [128, 64]), ([0, 4, 4, 8], [128, 64, 192]),
     ([0, 2, 4, 6, 8], [64, 128, 192, 70]), ([3, 3], [64]), ([8, 8, 8], [64, 64]),
-    ([1, 2, 3, 4, 5, 6, 7, 8], [64] * 7)])
+    ([1, 2, 3, 4, 5, 6, 7, 8], [64] * 7), ([0] * 40 + [8], [64] * 39 + [128]),
+    ([0] * 2047 + [5, 8], [0] * 2046 + [192, 64])])
 def test_groups(tsg, ctx, starts, shared):  # noqa: F811
-    """Sequences before, between and behind groups; groups of one sequence and of none."""
+    """Sequences before, between and behind groups; groups of one sequence and of none, these
+    also more than there are sequences."""
     c = Case([1] * 8, [200, 230, 199, 300, 195, 210, 222, 201], 6, 2, 64, seed=4)
     check(tsg, ctx, share(c, starts, shared))
 

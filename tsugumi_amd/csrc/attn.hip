@@ -569,8 +569,8 @@ extern "C" tsg_status tsg_attn_decode(tsg_attn* attn, tsg_stream stream, const t
 static tsg_status check_prefixes(const tsg_attn_config& c, const tsg_attn_batch* b,
                                  const tsg_attn_prefixes* x) {
     TSG_REQUIRE(x, TSG_ERR_INVALID_ARGUMENT, "attention prefixes are NULL");
-    TSG_REQUIRE(x->num_groups > 0 && x->num_groups <= kMaxAttnRows, TSG_ERR_INVALID_ARGUMENT,
-                "num_groups must be in 1...%u", kMaxAttnRows);
+    TSG_REQUIRE(x->num_groups > 0 && x->num_groups <= kMaxSharedSeqs, TSG_ERR_INVALID_ARGUMENT,
+                "num_groups must be in 1...%u", kMaxSharedSeqs);
     TSG_REQUIRE(x->group_starts && x->shared, TSG_ERR_INVALID_ARGUMENT,
                 "NULL group starts or shared lengths");
     TSG_REQUIRE(is4(x->group_starts) && is4(x->shared), TSG_ERR_ALIGNMENT,

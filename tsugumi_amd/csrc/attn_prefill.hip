@@ -782,10 +782,10 @@ tsg_status launch_prefixes(const tsg_attn* attn, const AttnArgs& a, PrefixArgs* 
     const uint64_t rows = (uint64_t)a.rows * a.group, groups = std::min(x->num_groups, a.num_seqs);
     TSG_REQUIRE(rows * a.kv_heads <= kMaxPrefixRows, TSG_ERR_DECLINED,
                 "too many rows and query heads for the plan's scratch: tsg_attn_decode");
-    // each group may end inside a tile, and has one at least
-    const uint64_t tiles = rows / kRows + groups;
+    // each group may end inside a tile, and has one at least, also one of no sequences
+    const uint64_t tiles = rows / kRows + x->num_groups;
     const uint64_t live = std::max(rows / kRows + (groups + 1u) / 2u, groups) * a.kv_heads;  // about
-    // (a launch of few enough blocks: tiles and key heads are bounded by the rows)
+    // (a launch of few enough blocks: the rows bound tiles and key heads, 2048 the groups)
     // One workgroup a CU, of at least four key tiles: with two, the partial sums' way through
     // memory costs what the shorter runs gain (64 sequences behind 16,000 tokens 57 us with one
     // and with two, 32 sequences 50 and 62, 8 30 and 33; 8 groups of 8 behind 4000 49 and 47).
