@@ -17,6 +17,10 @@
 //
 // Where the rows are few and the keys many, the keys are split over several
 // workgroups, and a second kernel joins their sums in the order of the splits.
+//
+// The keys that a group of decoded sequences shares are taken the same way, the group's rows in
+// tiles of 128 (SHARED); the decode kernel joins these sums with each row's own keys'. 64
+// sequences of 8 key heads of 128 behind 16,000 keys: 44 us, and 24 the decode kernel's.
 #include "attn_internal.hpp"
 
 namespace tsg {

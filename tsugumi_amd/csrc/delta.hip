@@ -133,7 +133,8 @@ void fill_seqs(const tsg_delta* delta, const tsg_delta_states* states, const tsg
 // bounds a prompt: a thread takes 8 channels (16 bytes) of up to 16 rows, all of
 // whose loads go out together, and reads the W - 1 rows before them again (from L2).
 // The thread with a sequence's first rows also moves its state, which it alone
-// reads and writes, so one slot may be both in and out.
+// reads and writes, so one slot may be both in and out. 11207 rows of 8192 channels 76 us
+// (4.85 TB/s); a token 4.3 us.
 
 constexpr uint32_t kConvRows = 16;
 
@@ -273,7 +274,7 @@ __global__ __launch_bounds__(256) void conv_kernel(ConvArgs p) {
 // elements a row, and the state stays in registers: a wave takes 32 of a head's
 // value elements (128-byte pieces of the state's rows), a lane four of them and
 // an eighth of the key elements. Every state is read and written once: HBM bounds
-// a batch, latency one sequence.
+// a batch, latency one sequence (64 states of 32 heads of 128 x 128 58 us, 4.7 TB/s; one 6 us).
 
 template <uint32_t DKP>
 __global__ __launch_bounds__(256) void recurrent_kernel(DeltaArgs p) {
