@@ -293,6 +293,52 @@ def test_pools_of_wider_slots(tsg, ctx):  # noqa: F811
 
 
 @pytest.mark.parametrize("op", OPS)
+def test_far_slots(tsg, ctx, op):  # noqa: F811
+    """Slots whose places pass 2^32 elements of the pool."""
+    c = Case([1 if op == "decode" else 21] * 9, 1, 2, 64, 32, seed=74)
+    d = c.to_device()
+    for name, type in (("s", torch.float32), ("conv", torch.float16)):
+        shape = d[name].shape
+        far = torch.empty_strided(shape, (2 ** 28 - 16, *d[name].stride()[1:]), dtype=type, device="cuda")
+        d[name] = far.copy_(d[name])
+    assert 2 ** 28 * max(c.ins + c.outs) >= 2 ** 32
+    check(tsg, ctx, c, op, d=d)
+
+
+def test_calls_beside_each_other(tsg, ctx):  # noqa: F811
+    """One plan's calls on two streams at once, each with its slots and scratch: as one by one."""
+    cases = [(Case([700, 130], 2, 8, 64, 64, seed=75), "prefill"),
+             (Case([8] * 40, 2, 8, 64, 64, seed=76), "decode"),
+             (Case([500, 333], 2, 8, 64, 64, seed=77), "conv"),
+             (Case([411] * 2, 2, 8, 64, 64, seed=78), "prefill")]
+    wants = [c.launch(tsg, ctx, op) for c, op in cases]
+    ctx.synchronize()
+    runs, delta = [], cases[0][0].plan(tsg, ctx)
+    for c, op in cases:
+        d = c.to_device()
+        runs.append((op, d, delta.states(d["s"], d["conv"]), tsg.DeltaGates(d["a_log"], d["dt_bias"]),
+                     delta.batch(d["ins"], d["outs"], c.total, None if c.uniform else d["starts"]),
+                     [*c.split(d["qkv"]), *d["ab"].split(c.hv, 1)],
+                     torch.empty(delta.scratch_bytes(c.total, len(c.rows)), dtype=torch.uint8, device="cuda")))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for turn in range(6):
+        for i, (op, d, states, gates, batch, rows, scratch) in enumerate(runs):
+            stream = streams[i % 2]
+            if op == "conv":
+                delta.encode_conv(states, batch, d["x"], d["weight"], d["conv_out"], stream=stream)
+            elif op == "decode":
+                delta.encode_decode(states, batch, *rows, gates, d["out"], stream=stream)
+            else:
+                delta.encode_prefill(states, batch, *rows, gates, d["out"], scratch, stream=stream)
+    torch.cuda.synchronize()
+    ctx.synchronize()
+    for (c, op), run, want in zip(cases, runs, wants):
+        for got, ref in zip(outputs(c, op, run[1]), outputs(c, op, want)):
+            assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("op", OPS)
 def test_on_another_stream(tsg, ctx, op):  # noqa: F811
     c = case(op)
     stream = torch.cuda.Stream()
