@@ -224,6 +224,27 @@ def test_tokens_outside_heads(tsg, ctx):  # noqa: F811
     check(tsg, ctx, share(c, [0, 2], [144]))
 
 
+@pytest.mark.parametrize("kv", ["f16", "e4m3"])
+def test_far_pages(tsg, ctx, kv):  # noqa: F811
+    """Shared and own pages whose places pass 2^32 elements of the pool."""
+    c = share(Case([2] * 4, [300, 311, 290, 333], 8, 2, 128, kv=kv, seed=10), [0, 4], [256])
+    d = c.to_device()
+    pages = c.k.shape[0]
+    stride = -(-(2 ** 33) // pages) // 16 * 16
+    shared = c.table[0, :16].long()  # at the pool's end, where their places are the farthest
+    order = torch.cat([torch.tensor([i for i in range(pages) if i not in shared.tolist()]), shared])
+    for name in ("k", "v"):
+        x = d[name].view(torch.uint8 if kv == "e4m3" else torch.int16)
+        far = torch.empty_strided(x.shape, (stride, *x.stride()[1:]), dtype=x.dtype, device="cuda")
+        far.copy_(x[order.cuda()])
+        d[name] = far.view(d[name].dtype)
+    place = torch.empty(pages, dtype=torch.int32)
+    place[order] = torch.arange(pages, dtype=torch.int32)
+    d["table"] = place[c.table.long()].cuda()
+    assert int(d["table"][0, 0]) * stride > 2 ** 32
+    check(tsg, ctx, c, d=d)
+
+
 def reported(tsg, ctx, text):  # noqa: F811
     with pytest.raises(tsg.TsgError) as e:
         ctx.synchronize()
