@@ -12,12 +12,14 @@
 // (their norms are factors of rows), every other operand is split into two halves of
 // fp16 (22 bits; three products where both are split), T is formed in fp32, and all
 // sums are in fp32. Only the weights of O are rounded to fp16 once, half a step of
-// 2^-11 each as O itself. fp16's range is no limit: a state's columns and U are
+// 2^-11 each as O itself. fp16's range is no limit: a state's columns, R and U are
 // scaled by a power of two from bounds on them. |k^| <= 1, beta <= 1 and decays <= 1, so
-// a row does not lengthen a column of the state beyond |v|: columns and U stay
-// within B = sqrt(key_dim) max|S| + 65 max|v|. |T| and the weights are at most 1. What a
-// half's least step leaves out is under 2^-38 B: a state that a chunk all but forgets
-// is off by that, where row by row it would keep its 24 bits.
+// a row does not lengthen a column of the state beyond |v|: columns, R and U stay
+// within B = sqrt(key_dim) max|S| + 65 max|v|, scaled to 2^13 ... 2^14. |T| and the weights
+// are at most 1. Lower halves are kept times 2^11, in the upper ones' range, so that fp16's
+// least step leaves out no more than 2^-49 B of an element: B is a column's and a
+// chunk's, and rows of one may differ by all of fp16's range (unscaled, the halves end at
+// 2^-38 B: one value of 60,000 took all bits from the rows of 1e-3 before it).
 #include "delta_internal.hpp"
 
 #include <type_traits>
@@ -26,9 +28,10 @@ namespace tsg {
 namespace {
 
 constexpr uint32_t kChunk = 64;
-// T and the weights are kept times these, away from fp16's least; R is scaled to less than U by
-// T's, so that their product comes out in U's scale.
+// T and the weights are kept times these, away from fp16's least.
 constexpr float kTriangle = 32.0f, kWeight = 1024.0f;
+// The lower halves of split operands, to the upper ones.
+constexpr float kLower = 1.0f / 2048.0f;
 
 // A chunk and value head's record: T's operand pieces (two planes) and the weights', 64
 // lanes x 16 bytes each; the rows' factors; e^G_end and how many rows count.
@@ -69,16 +72,16 @@ __device__ __forceinline__ f4_t mfma(h8_t a, h8_t b, f4_t c) {
 }
 __device__ __forceinline__ h8_t as_h8(uint4 u) { return __builtin_bit_cast(h8_t, u); }
 
-// x = hi + lo to 22 bits. The empty asm keeps the product that x came from out of the
-// conversion: rounded once from the exact product in one use and twice in the other, the two
-// hi would differ near ties, and lo be what is missing to another hi.
+// x = hi + kLower lo to 22 bits, or 2^-36. The empty asm keeps the product that x came from
+// out of the conversion: rounded once from the exact product in one use and twice in the other,
+// the two hi would differ near ties, and lo be what is missing to another hi.
 __device__ __forceinline__ void split4(f4_t x, h4_t& hi, h4_t& lo) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         float y = x[e];
         asm("" : "+v"(y));
         hi[e] = (_Float16)y;
-        lo[e] = (_Float16)__builtin_fmaf((float)hi[e], -1.0f, y);  // one instruction, exact
+        lo[e] = (_Float16)(__builtin_fmaf((float)hi[e], -1.0f, y) * (1.0f / kLower));  // exact but for the cast
     }
 }
 
@@ -650,7 +653,7 @@ __global__ __launch_bounds__(kScanThreads, (DKP <= 128u ? 4 : 2)) void scan_kern
             const uint32_t base = kChunk * c + 16u * rt;
 #pragma unroll
             for (uint32_t e = 0; e < 4u; ++e) {
-                o[e] = __builtin_fmaf(y[e] + y2[e], o_unit, o[e]);
+                o[e] = __builtin_fmaf(__builtin_fmaf(y2[e], kLower, y[e]), o_unit, o[e]);
                 if (16u * rt + 4u * g + e >= o_good) o[e] = __builtin_nanf("");
                 o_at[rt][4u * g + e][i16] = f32_to_f16(o[e]);
             }
@@ -695,6 +698,7 @@ __global__ __launch_bounds__(kScanThreads, (DKP <= 128u ? 4 : 2)) void scan_kern
                 ps = mfma(rf[n], shared_piece(s_at, n, 0u), ps);
                 ps2 = mfma(rf[n], shared_piece(s_at, n, 1u), ps2);
             }
+            ps += ps2 * kLower;
             load_rows(next);
             uint2 vs = make_uint2(0, 0);  // the lane's values
             if constexpr (keys) vs = *reinterpret_cast<const uint2*>(&v_at[c & 1u][rt][i16][4u * g]);
@@ -742,18 +746,17 @@ __global__ __launch_bounds__(kScanThreads, (DKP <= 128u ? 4 : 2)) void scan_kern
             const float ratio = __builtin_amdgcn_ldexpf(1.0f, exponent - now);
             exponent = now;
             if constexpr (keys) {
-                const float to_r = __builtin_amdgcn_ldexpf(1.0f / kTriangle, 14 - now);
-                const float s_r = ratio * (1.0f / kTriangle);
+                const float to_r = __builtin_amdgcn_ldexpf(1.0f, 14 - now);
                 const f4_t f_v = *reinterpret_cast<const f4_t*>(&factors[0][r0]) * to_r;
-                const f4_t f_s = *reinterpret_cast<const f4_t*>(&factors[1][r0]) * s_r;
+                const f4_t f_s = *reinterpret_cast<const f4_t*>(&factors[1][r0]) * ratio;
                 f4_t x;
 #pragma unroll
                 for (uint32_t e = 0; e < 4u; ++e)  // 0 for rows that do not count: their factors are
                     x[e] = __builtin_fmaf(f16_to_f32((uint16_t)vb[e]), f_v[e],
-                                          -(ps[e] + ps2[e]) * f_s[e]);
+                                          -ps[e] * f_s[e]);
                 share(r_at, rt, x);
             } else {
-                o_next = (ps + ps2) * (*reinterpret_cast<const f4_t*>(&factors[2][r0]) * from_s);
+                o_next = ps * (*reinterpret_cast<const f4_t*>(&factors[2][r0]) * from_s);
                 turn_v(c + 1u);  // the next chunk's
             }
             load_factors(next);
@@ -769,7 +772,7 @@ __global__ __launch_bounds__(kScanThreads, (DKP <= 128u ? 4 : 2)) void scan_kern
                     u2 = mfma(tl[h], hi, u2);
                     u2 = mfma(th[h], lo, u2);
                 }
-                u = u + u2;
+                u = (u + u2 * kLower) * (1.0f / kTriangle);
                 share(w_at, rt, u * *reinterpret_cast<const f4_t*>(&factors[3][r0]));
                 share(u_at[c & 1u], rt, u);
             } else {
@@ -780,16 +783,19 @@ __global__ __launch_bounds__(kScanThreads, (DKP <= 128u ? 4 : 2)) void scan_kern
             }
             load_t(keys ? next : c);
             lds_barrier();
-            f4_t more[TW];
+            f4_t more[TW], more2[TW];
 #pragma unroll
-            for (uint32_t t = 0; t < TW; ++t) more[t] = st[t] * (end_decay * ratio);
+            for (uint32_t t = 0; t < TW; ++t) {
+                more[t] = st[t] * (end_decay * ratio);
+                more2[t] = f4_t{0, 0, 0, 0};
+            }
             if (holds) {
 #pragma unroll
                 for (uint32_t h = 0; h < 2u; ++h) {
                     const h8_t hi = shared_piece(w_at, h, 0u), lo = shared_piece(w_at, h, 1u);
 #pragma unroll
                     for (uint32_t t = 0; t < TW; ++t) {
-                        more[t] = mfma(kt[t][h], lo, more[t]);
+                        more2[t] = mfma(kt[t][h], lo, more2[t]);
                         more[t] = mfma(kt[t][h], hi, more[t]);
                     }
                 }
@@ -799,7 +805,7 @@ __global__ __launch_bounds__(kScanThreads, (DKP <= 128u ? 4 : 2)) void scan_kern
             const uint32_t rows = sq.count - kChunk * c;
             const bool lost = good < (rows < kChunk ? rows : kChunk);
 #pragma unroll
-            for (uint32_t t = 0; t < TW; ++t) st[t] = more[t];
+            for (uint32_t t = 0; t < TW; ++t) st[t] = more[t] + more2[t] * kLower;
             if (__ballot(lost)) {
 #pragma unroll
                 for (uint32_t t = 0; t < TW; ++t)
