@@ -99,3 +99,22 @@ def test_causal_up_to_its_bits(tsg, ctx):  # noqa: F811
     ctx.synchronize()
     _, tol, _, _ = a.rule(True)
     assert_near(got[0], got[1], 2 * tol[:63])
+
+
+class Fine(Split):
+    """Weights split as the rest: rounded by 2^-22 of their size, 2^-22 more for the lower halves'
+    product, which is left out; half a least step, times 2^-11, 2^-46 at 1024 for 1."""
+    weights, weights_least = 2.0 ** -21, 2.0 ** -46
+
+
+@pytest.mark.parametrize("slots", ["fresh", "apart"])
+@pytest.mark.parametrize("dk,dv", [(16, 16), (64, 80), (128, 128), (192, 64), (256, 512)])
+def test_outputs_are_rounded_once(tsg, ctx, dk, dv, slots):  # noqa: F811
+    """A prompt's outputs are as far off as a token's: what their own rounding and fp32's sums
+    leave, also where a row's parts cancel."""
+    check(tsg, ctx, Fine([150, 64, 7], 1, 2, dk, dv, seed=93, slots=slots, gate=2.0), "prefill")
+
+
+@pytest.mark.parametrize("large,small", SIZES)
+def test_outputs_are_rounded_once_at_any_size(tsg, ctx, large, small):  # noqa: F811
+    check(tsg, ctx, of_sizes(Fine, 128, "apart", large, small, 30, rows=(100,)), "prefill")

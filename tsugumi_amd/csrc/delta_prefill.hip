@@ -10,9 +10,8 @@
 //
 // The state and what goes into it keep fp32's precision: q and k are fp16 as they are
 // (their norms are factors of rows), every other operand is split into two halves of
-// fp16 (22 bits; three products where both are split), T is formed in fp32, and all
-// sums are in fp32. Only the weights of O are rounded to fp16 once, half a step of
-// 2^-11 each as O itself. fp16's range is no limit: a state's columns, R and U are
+// fp16 (22 bits; three products where both are split), T and the weights of O are formed in
+// fp32, and all sums are in fp32. fp16's range is no limit: a state's columns, R and U are
 // scaled by a power of two from bounds on them. |k^| <= 1, beta <= 1 and decays <= 1, so
 // a row does not lengthen a column of the state beyond |v|: columns, R and U stay
 // within B = sqrt(key_dim) max|S| + 65 max|v|, scaled to 2^13 ... 2^14. |T| and the weights
@@ -33,13 +32,13 @@ constexpr float kTriangle = 32.0f, kWeight = 1024.0f;
 // The lower halves of split operands, to the upper ones.
 constexpr float kLower = 1.0f / 2048.0f;
 
-// A chunk and value head's record: T's operand pieces (two planes) and the weights', 64
-// lanes x 16 bytes each; the rows' factors; e^G_end and how many rows count.
+// A chunk and value head's record: T's operand pieces and the weights' (two planes each), 64
+// lanes x 16 bytes a piece; the rows' factors; e^G_end and how many rows count.
 // Pieces (16 rows, 32 columns) of the lower triangle: row tiles 0 and 1 need the first
 // column half, 2 and 3 both.
 constexpr uint32_t kPieces = 6, kPieceBytes = 1024;
 constexpr uint32_t kWeightsAt = 2u * kPieces * kPieceBytes;
-constexpr uint32_t kFactorsAt = kWeightsAt + kPieces * kPieceBytes;
+constexpr uint32_t kFactorsAt = kWeightsAt + 2u * kPieces * kPieceBytes;
 constexpr uint32_t kEndAt = kFactorsAt + 4u * kChunk * 4u;
 constexpr uint32_t kRecord = kEndAt + 256u;
 __device__ __forceinline__ uint32_t piece_of(uint32_t mt, uint32_t half) {
@@ -129,7 +128,7 @@ __global__ __launch_bounds__(256, 4) void prepare_kernel(ChunkArgs p) {
     uint16_t* keys = reinterpret_cast<uint16_t*>(smem);
     float* tm = reinterpret_cast<float*>(smem);
     float* am = reinterpret_cast<float*>(smem + kKeysBytes<DKP>);
-    uint16_t* pm = keys;  // the weights, 72 halves a row
+    float* wm = tm;  // the weights
     float* k_inv = am + kChunk * kLd;  // 1 / |k|, 1 / |q|
     float *q_inv = k_inv + kChunk, *gs = q_inv + kChunk, *bs = gs + kChunk;
     // of the rows that count for the head (0 for others): no NaN goes into the triangles
@@ -320,7 +319,7 @@ __global__ __launch_bounds__(256, 4) void prepare_kernel(ChunkArgs p) {
             if (n > wave) {
                 if ((n ^ 1u) != wave) continue;  // the other half of a piece
 #pragma unroll
-                for (uint32_t e = 0; e < 4u; ++e) pm[(r0 + e) * 72u + j] = 0;
+                for (uint32_t e = 0; e < 4u; ++e) wm[(r0 + e) * kLd + j] = 0.0f;
                 continue;
             }
 #pragma unroll
@@ -330,18 +329,29 @@ __global__ __launch_bounds__(256, 4) void prepare_kernel(ChunkArgs p) {
                     __builtin_amdgcn_exp2f(i >= j ? (hi[e] - hj[n]) + (lo[e] - lj[n]) : 0.0f) * kj[n];
                 am[i * kLd + j] = i > j ? bi[e] * w * kk[n][e] : 0.0f;
                 // a query's infinity or NaN stays in its row's weights
-                pm[i * 72u + j] = f32_to_f16(i >= j ? qi[e] * w * qk[n][e] : 0.0f);
+                wm[i * kLd + j] = i >= j ? qi[e] * w * qk[n][e] : 0.0f;
             }
         }
     }
     __syncthreads();
-    for (uint32_t n = wave; n < kPieces; n += 4u) {
-        const uint32_t mt = n < 2u ? n : 2u + (n - 2u) / 2u, half = n < 2u ? 0u : n % 2u;
-        const uint16_t* src = pm + (16u * mt + i16) * 72u + 32u * half + 4u * g;
-        const uint2 lo = *reinterpret_cast<const uint2*>(src), hi = *reinterpret_cast<const uint2*>(src + 16);
-        *reinterpret_cast<uint4*>(record + kWeightsAt + n * kPieceBytes + lane * 16u) =
-            make_uint4(lo.x, lo.y, hi.x, hi.y);
-    }
+    // A triangle's pieces, in two planes.
+    const auto put_pieces = [&](const float* m, float times, uint8_t* to) {
+        for (uint32_t n = wave; n < kPieces; n += 4u) {
+            const uint32_t mt = n < 2u ? n : 2u + (n - 2u) / 2u, half = n < 2u ? 0u : n % 2u;
+            const float* src = m + (16u * mt + i16) * kLd + 32u * half + 4u * g;
+            h4_t hi[2], lo[2];
+#pragma unroll
+            for (uint32_t e = 0; e < 2u; ++e)
+                split4(*reinterpret_cast<const f4_t*>(src + 16u * e) * times, hi[e], lo[e]);
+            h4_t* o = reinterpret_cast<h4_t*>(to + n * kPieceBytes + lane * 16u);
+            o[0] = hi[0];
+            o[1] = hi[1];
+            o += kPieces * kPieceBytes / 8u;
+            o[0] = lo[0];
+            o[1] = lo[1];
+        }
+    };
+    put_pieces(wm, 1.0f, record + kWeightsAt);
 
     __syncthreads();  // T takes the weights' place
     // T: the diagonal tiles by substitution, a column a lane, ...
@@ -407,20 +417,7 @@ __global__ __launch_bounds__(256, 4) void prepare_kernel(ChunkArgs p) {
         put(y, mt, nt);
     }
     __syncthreads();
-    for (uint32_t n = wave; n < kPieces; n += 4u) {
-        const uint32_t mt = n < 2u ? n : 2u + (n - 2u) / 2u, half = n < 2u ? 0u : n % 2u;
-        const float* src = tm + (16u * mt + i16) * kLd + 32u * half + 4u * g;
-        h4_t hi[2], lo[2];
-#pragma unroll
-        for (uint32_t e = 0; e < 2u; ++e)
-            split4(*reinterpret_cast<const f4_t*>(src + 16u * e) * kTriangle, hi[e], lo[e]);
-        h4_t* to = reinterpret_cast<h4_t*>(record + n * kPieceBytes + lane * 16u);
-        to[0] = hi[0];
-        to[1] = hi[1];
-        to += kPieces * kPieceBytes / 8u;
-        to[0] = lo[0];
-        to[1] = lo[1];
-    }
+    put_pieces(tm, kTriangle, record);
 }
 
 // ------------------------------------------------------- from chunk to chunk
@@ -626,9 +623,9 @@ __global__ __launch_bounds__(kScanThreads, (DKP <= 128u ? 4 : 2)) void scan_kern
         const auto load_t = [&](uint32_t c) {
             const uint8_t* r = record(c) + (keys ? 0u : kWeightsAt);
             th[0] = piece(r + t_0, lane16);
-            if constexpr (keys) tl[0] = piece(r + t_0 + kPieces * kPieceBytes, lane16);
+            tl[0] = piece(r + t_0 + kPieces * kPieceBytes, lane16);
             th[1] = piece(r + t_1, lane16);
-            if constexpr (keys) tl[1] = piece(r + t_1 + kPieces * kPieceBytes, lane16);
+            tl[1] = piece(r + t_1 + kPieces * kPieceBytes, lane16);
         };
         const auto load_k = [&](uint32_t c) {
             const uint8_t* k = key_record(c) + (holds ? TW * wave * SHARE : 0u);
@@ -637,6 +634,17 @@ __global__ __launch_bounds__(kScanThreads, (DKP <= 128u ? 4 : 2)) void scan_kern
 #pragma unroll
                 for (uint32_t h = 0; h < 2u; ++h) kt[t][h] = piece(k + (2u * t + h) * kPieceBytes, lane16);
         };
+        // the rows of T or the weights times what is shared: x + kLower x2
+        const auto triangle = [&](const uint8_t* from, f4_t& x, f4_t& x2) {
+#pragma unroll
+            for (uint32_t h = 0; h < 2u; ++h) {
+                if (h && !two) continue;
+                const h8_t hi = shared_piece(from, h, 0u), lo = shared_piece(from, h, 1u);
+                x = mfma(th[h], hi, x);
+                x2 = mfma(tl[h], hi, x2);
+                x2 = mfma(th[h], lo, x2);
+            }
+        };
         // A chunk's outputs: Q S, and the weights times U, one chunk later while the waves of
         // keys form U.
         f4_t o = {0, 0, 0, 0}, o_next = {0, 0, 0, 0};
@@ -644,12 +652,7 @@ __global__ __launch_bounds__(kScanThreads, (DKP <= 128u ? 4 : 2)) void scan_kern
         uint32_t o_good = 0;
         const auto finish = [&](uint32_t c) {
             f4_t y = {0, 0, 0, 0}, y2 = {0, 0, 0, 0};
-            y = mfma(th[0], shared_piece(u_at[c & 1u], 0u, 0u), y);
-            y2 = mfma(th[0], shared_piece(u_at[c & 1u], 0u, 1u), y2);
-            if (two) {
-                y = mfma(th[1], shared_piece(u_at[c & 1u], 1u, 0u), y);
-                y2 = mfma(th[1], shared_piece(u_at[c & 1u], 1u, 1u), y2);
-            }
+            triangle(u_at[c & 1u], y, y2);
             const uint32_t base = kChunk * c + 16u * rt;
 #pragma unroll
             for (uint32_t e = 0; e < 4u; ++e) {
@@ -764,14 +767,7 @@ __global__ __launch_bounds__(kScanThreads, (DKP <= 128u ? 4 : 2)) void scan_kern
             lds_barrier();
             if constexpr (keys) {
                 f4_t u = {0, 0, 0, 0}, u2 = {0, 0, 0, 0};
-#pragma unroll
-                for (uint32_t h = 0; h < 2u; ++h) {
-                    if (h && !two) continue;
-                    const h8_t hi = shared_piece(r_at, h, 0u), lo = shared_piece(r_at, h, 1u);
-                    u = mfma(th[h], hi, u);
-                    u2 = mfma(tl[h], hi, u2);
-                    u2 = mfma(th[h], lo, u2);
-                }
+                triangle(r_at, u, u2);
                 u = (u + u2 * kLower) * (1.0f / kTriangle);
                 share(w_at, rt, u * *reinterpret_cast<const f4_t*>(&factors[3][r0]));
                 share(u_at[c & 1u], rt, u);
@@ -822,13 +818,15 @@ __global__ __launch_bounds__(kScanThreads, (DKP <= 128u ? 4 : 2)) void scan_kern
     const uint32_t slot = scalar_load(d.seqs.out_slots + s);
     if (slot == TSG_NO_SLOT) return;
     const float from_s = __builtin_amdgcn_ldexpf(1.0f, exponent - 14);
+    // the lane anew: kept over the loop, its places take registers that the loop lacks
+    const uint32_t now = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+    float* to = d.s + (uint64_t)slot * d.slot_stride + (uint64_t)head * d.key_dim * d.value_dim + c0;
 #pragma unroll
     for (uint32_t t = 0; t < TW; ++t)
 #pragma unroll
         for (uint32_t e = 0; e < 4u; ++e) {
-            const uint32_t kr = 16u * (TW * wave + t) + 4u * g + e;
-            if (kr < d.key_dim)
-                d.s[(uint64_t)slot * d.slot_stride + place + kr * d.value_dim] = st[t][e] * from_s;
+            const uint32_t kr = 16u * (TW * wave + t) + 4u * (now >> 4) + e;
+            if (kr < d.key_dim) to[(now & 15u) + kr * d.value_dim] = st[t][e] * from_s;
         }
 }
 
