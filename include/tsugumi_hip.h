@@ -833,11 +833,14 @@ tsg_status tsg_attn_prefixes_check(const tsg_attn_config* config, const tsg_attn
                                    const tsg_attn_prefixes* prefixes);
 /* tsg_attn_decode, the keys that a group shares read once for all of its rows: two
  * launches, for groups of several sequences and prefixes of a few thousand tokens
- * on. The same results up to the order of sums; the first sequence's bad page
- * reaches all of its group. Few rows a group of heads over 128 (under 32 rows x query
- * heads a key head, on the average) take tsg_attn_decode's kernel, which asks for no
- * groups. Returns TSG_ERR_DECLINED for a window, more than 8 rows a sequence, more than
- * 2048 sequences, or rows * q_heads over 65,472. q, out and the plan's scratch as for
+ * on. The same results up to the order of sums, which is the same beside groups that
+ * share nothing (of one sequence or none) as without them; the first sequence's bad
+ * page reaches all of its group. With heads over 128, a group of under 32 rows x query
+ * heads a key head reads its prefix a sequence, unless it has 8 sequences and 8192
+ * shared tokens; and where the batch as one group would, with all that its page tables
+ * hold, the call is tsg_attn_decode's, which asks for no groups. Returns
+ * TSG_ERR_DECLINED for a window, more than 8 rows a sequence, more than 2048
+ * sequences, or rows * q_heads over 65,472. q, out and the plan's scratch as for
  * tsg_attn_decode. */
 tsg_status tsg_attn_decode_shared(tsg_attn* attn, tsg_stream stream, const tsg_kv_pages* pages,
                                   const tsg_attn_batch* batch, const tsg_attn_prefixes* prefixes,

@@ -612,12 +612,8 @@ extern "C" tsg_status tsg_attn_decode_shared(tsg_attn* attn, tsg_stream stream,
     x.num_groups = prefixes->num_groups;
     DeviceScope scope(attn->device);
     TSG_HIP_TRY(scope.status);
-    // Few rows of wide heads a group leave most of a tile of 128 empty: every sequence reads the
-    // prefix then, from L2 but for the first (heads of 256 (16 query, 8 key heads), 8 rows a
-    // group over 2048 keys, decode against shared 17 and 24 us, over 32,768 87 and 97; 16 rows 20
-    // and 25, 129 and 104; 32 rows 28 and 32, over 8192 62 and 57, over 32,768 237 and 116. Heads
-    // of 128, 8 rows over 2048 keys 19 and 20, over 8192 26 and 24, 16 rows 24 and 20).
-    if (attn->padded_dim >= 256u && (uint64_t)a.rows * a.group < 32u * (uint64_t)x.num_groups)
+    // no group can share: all of the rows as one, over all that the page tables hold
+    if (!share_pays(attn->padded_dim, a.num_seqs, a.rows * a.group, a.table_stride << a.page_shift))
         return launch_decode(attn, a, stream);
     if (tsg_status s = launch_prefixes(attn, a, &x, stream)) return s;
     return launch_decode(attn, a, stream, &x);

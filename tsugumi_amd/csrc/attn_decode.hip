@@ -225,11 +225,13 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
     // positions of all of the sequence's rows: its row tiles take the same runs
     const int32_t p_lo = base, p_hi = (int32_t)sr.length - 1;
     TileSpan span = tile_span<kTile>(p_lo < 0 ? 0 : p_lo, p_hi, a.window, a.sinks);
-    uint32_t shared = 0;     // tokens
+    uint32_t shared = 0, shared_splits = 1;  // tokens
     bool bad_groups = false;
     if constexpr (SHARED) {
         shared = scalar_load(&p.x.info[s].x);
-        bad_groups = scalar_load(&p.x.info[s].y) != 0u;
+        const uint32_t y = scalar_load(&p.x.info[s].y);
+        bad_groups = (y & 1u) != 0u;
+        shared_splits = y >> 1;
         span.first = shared / kTile;
         span.count = span.count > span.first ? span.count - span.first : 0u;
     }
@@ -539,7 +541,7 @@ __global__ __launch_bounds__(256, (kSimdWaves<DP, E4M3, FULL>)) void decode_kern
     // The sums of the shared keys, every ways-th split of them, added to a row's piece.
     const auto add_shared = [&](uint32_t r, uint32_t c, float* acc, float& sum, float& mm,
                                 uint32_t way, uint32_t ways) {
-        const uint32_t splits = prefix_split(p.x, shared / kTileKeys<DP>).used;
+        const uint32_t splits = prefix_split(p.x, shared_splits, shared / kTileKeys<DP>).used;
         const uint64_t first = (uint64_t)kvh * p.x.splits * p.x.rows + s * rows + r0 + r;
 #pragma unroll 1
         for (uint32_t w0 = way; w0 < splits; w0 += kJoinLoads * ways) {

@@ -67,23 +67,36 @@ __device__ __forceinline__ uint32_t scalar_load(const uint32_t* p) {
 // Sequences that share their first tokens. What all of a group's rows see of them, the first
 // kernel sums up (attn_prefill.hip) and the second takes in when it joins a row's own keys'
 // sums (attn_decode.hip). Rows (sequence, token, head of the key head's group) are taken in
-// tiles of 128 from a group's first; group g's begin at tile (its first row) / 128 + g.
+// tiles of 128 from a group's first.
 constexpr uint32_t kShareTokens = 64;  // shared tokens are taken in whole key tiles
 struct PrefixArgs {
     const uint32_t* group_starts;
     const uint32_t* shared;
-    uint2* info;     // [seqs]: shared tokens, whether the group starts are wrong
+    uint2* info;     // [seqs]: shared tokens; the splits there may be, times 2, and whether the
+                     // group starts are wrong
     float* part_o;   // [key head][split][row][DP]
     float* part_ml;  // [key head][split][row][2]
-    uint32_t num_groups, tiles, splits, min_tiles;
+    uint32_t num_groups, splits, min_tiles;  // splits: that the scratch has room for
+    uint32_t units;  // (tile, split) that a key head's workgroups can take at once
     uint32_t rows;   // of all sequences
 };
-// Splits of so many key tiles, and the tiles of one.
+// Whether a group reads what it shares once: few rows of wide heads leave most of a tile of 128
+// empty, and every sequence reads the prefix then, from L2 but for the first. Decode against
+// shared, us, heads of 256 (16 query, 8 key heads): 4 sequences behind 8192 tokens 27 and 35; 8
+// behind 4096 26 and 30, 8192 37 and 36, 32,768 125 and 73; 16 (32 rows) behind 2048 28 and 32,
+// 4096 39 and 37, 32,768 230 and 79. 4 heads of 512, 8 sequences behind 4096 33 and 36, 8192 52
+// and 45. Heads of 128 (32 and 8): 8 behind 2048 20 and 22, 8192 31 and 27.
+__host__ __device__ __forceinline__ bool share_pays(uint32_t padded_dim, uint32_t seqs,
+                                                    uint32_t rows, uint32_t tokens) {
+    return padded_dim < 256u || rows >= 32u || (seqs >= 8u && tokens >= 8192u);
+}
+// Splits of so many key tiles, where there may be `splits`, and the tiles of one.
 struct PrefixSplit {
     uint32_t used, per;
 };
-__device__ __forceinline__ PrefixSplit prefix_split(const PrefixArgs& x, uint32_t key_tiles) {
-    const uint32_t even = (key_tiles + x.splits - 1u) / x.splits;
+__device__ __forceinline__ PrefixSplit prefix_split(const PrefixArgs& x, uint32_t splits,
+                                                    uint32_t key_tiles) {
+    const uint32_t even = (key_tiles + splits - 1u) / splits;
     const uint32_t per = even > x.min_tiles ? even : x.min_tiles;
     return PrefixSplit{(key_tiles + per - 1u) / per, per};
 }

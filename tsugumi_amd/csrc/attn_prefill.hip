@@ -155,56 +155,93 @@ __device__ __forceinline__ TilePlan<DP> tile_plan(const PrefillArgs& p, const Se
     return t;
 }
 
-// Shared keys: group and tile `at` of its rows; kind 0: none, or wrong group starts.
-struct GroupTile {
-    uint32_t kind, first_seq, seqs, tile, tokens;
-};
+// Shared keys. A group's tokens that its sequences share: of the first one's pages, in whole
+// key tiles; one sequence shares with none.
+template <int DP>
 __device__ __forceinline__ uint32_t shared_tokens(const AttnArgs& a, const PrefixArgs& x,
                                                   uint32_t g, uint32_t first_seq, uint32_t seqs) {
-    // of the first sequence's pages, in whole key tiles; one sequence shares with none
-    const uint32_t capacity = a.table_stride << a.page_shift;
-    uint32_t n = x.shared[g];
+    if (seqs < 2u) return 0u;
+    const uint32_t capacity = a.table_stride << a.page_shift, rows = seqs * a.seq_rows * a.group;
     const uint32_t length = a.lengths[first_seq];
+    uint32_t n = x.shared[g];
     n = n < length ? n : length;
     n = n < capacity ? n : capacity;
-    return seqs > 1u ? n / kShareTokens * kShareTokens : 0u;
+    return share_pays(DP, seqs, rows, n) ? n / kShareTokens * kShareTokens : 0u;
 }
-__device__ __forceinline__ uint32_t group_tile0(const AttnArgs& a, uint32_t g, uint32_t first_seq) {
-    return first_seq * (a.seq_rows * a.group) / kRows + g;
+// A group's row tiles, if it shares anything.
+struct Group {
+    uint32_t first_seq, seqs, tokens, tiles;
+    bool wrong;  // its starts
+};
+template <int DP>
+__device__ __forceinline__ Group group_of(const AttnArgs& a, const PrefixArgs& x, uint32_t g) {
+    if (g >= x.num_groups) return Group{0u, 0u, 0u, 0u, false};
+    const uint32_t lo = x.group_starts[g], hi = x.group_starts[g + 1u];
+    if (lo > hi || hi > a.num_seqs) return Group{0u, 0u, 0u, 0u, true};
+    const uint32_t tokens = lo < hi ? shared_tokens<DP>(a, x, g, lo, hi - lo) : 0u;
+    const uint32_t tiles = tokens ? ((hi - lo) * a.seq_rows * a.group + kRows - 1u) / kRows : 0u;
+    return Group{lo, hi - lo, tokens, tiles, false};
 }
+// All of a call's groups: the row tiles, and the splits that each one's keys may have, one
+// workgroup a CU. Groups that share nothing, of no sequence or of one, count for nothing.
+struct Groups {
+    uint32_t tiles, splits;
+    bool wrong;
+};
+template <int DP>
+__device__ __forceinline__ Groups all_groups(const AttnArgs& a, const PrefixArgs& x) {
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t tiles = 0;
+    bool wrong = false;
+#pragma unroll 4
+    for (uint32_t base = 0; base < x.num_groups; base += 64u) {
+        const Group g = group_of<DP>(a, x, base + lane);
+        wrong = wrong || g.wrong;
+        tiles += g.tiles;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) tiles += (uint32_t)__shfl_xor((int)tiles, o, 64);
+    tiles = __builtin_amdgcn_readfirstlane(tiles);
+    uint32_t splits = tiles ? x.units / tiles : 1u;
+    splits = splits < x.splits ? splits : x.splits;
+    return Groups{tiles, splits ? splits : 1u, __ballot(wrong) != 0};
+}
+// Row tile `at` of all groups'.
+struct GroupTile {
+    uint32_t first_seq, seqs, tile, tokens;
+};
+template <int DP>
 __device__ __forceinline__ GroupTile find_group_tile(const AttnArgs& a, const PrefixArgs& x,
                                                      uint32_t at) {
     const uint32_t lane = threadIdx.x & 63u;
-    uint32_t before = 0;  // groups whose tiles begin at or before `at`
-    bool wrong = false;
+    uint32_t before = 0;
     for (uint32_t base = 0; base < x.num_groups; base += 64u) {
-        const uint32_t g = base + lane;
-        const bool live = g < x.num_groups;
-        const uint32_t lo = live ? x.group_starts[g] : 0u, hi = live ? x.group_starts[g + 1u] : 0u;
-        wrong = wrong || lo > hi || hi > a.num_seqs;
-        before += (uint32_t)__builtin_popcountll(
-            __ballot(live && lo <= a.num_seqs && group_tile0(a, g, lo) <= at));
+        const Group g = group_of<DP>(a, x, base + lane);
+        uint32_t end = g.tiles;
+#pragma unroll
+        for (uint32_t o = 1; o < 64u; o <<= 1) {
+            const uint32_t below = (uint32_t)__shfl_up((int)end, o, 64);
+            end += lane >= o ? below : 0u;
+        }
+        const uint64_t behind = __ballot(before + end > at);
+        if (behind) {
+            const int l = __builtin_ctzll(behind);
+            const auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
+            return GroupTile{of(g.first_seq), of(g.seqs), at - (before + of(end) - of(g.tiles)),
+                             of(g.tokens)};
+        }
+        before += (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
     }
-    if (__ballot(wrong) || before == 0u) return GroupTile{0u, 0u, 0u, 0u, 0u};
-    const uint32_t g = before - 1u;
-    const uint32_t lo = scalar_load(x.group_starts + g), hi = scalar_load(x.group_starts + g + 1u);
-    const uint32_t tile = at - group_tile0(a, g, lo);
-    if (hi == lo || tile * kRows >= (hi - lo) * a.seq_rows * a.group) return GroupTile{0u, 0u, 0u, 0u, 0u};
-    const uint32_t tokens = __builtin_amdgcn_readfirstlane(shared_tokens(a, x, g, lo, hi - lo));
-    return GroupTile{tokens ? 1u : 0u, lo, hi - lo, tile, tokens};
+    return GroupTile{0u, 0u, 0u, 0u};
 }
 // What the joining kernel needs to know of every sequence.
+template <int DP>
 __device__ __forceinline__ void write_info(const AttnArgs& a, const PrefixArgs& x) {
-    uint32_t wrong = 0;
-    for (uint32_t g = threadIdx.x; g < x.num_groups; g += blockDim.x) {
-        const uint32_t lo = x.group_starts[g], hi = x.group_starts[g + 1u];
-        wrong |= lo > hi || hi > a.num_seqs ? 1u : 0u;
-    }
-    wrong = __syncthreads_or((int)wrong) ? 1u : 0u;
-    if (wrong && threadIdx.x == 0) report(a.error, kErrAttnGroups);
+    const Groups all = all_groups<DP>(a, x);
+    if (all.wrong && threadIdx.x == 0) report(a.error, kErrAttnGroups);
     for (uint32_t s = threadIdx.x; s < a.num_seqs; s += blockDim.x) {
-        uint2 info = make_uint2(0u, wrong);
-        if (!wrong && x.num_groups) {
+        uint2 info = make_uint2(0u, all.splits * 2u + (all.wrong ? 1u : 0u));
+        if (!all.wrong) {
             uint32_t lo = 0, hi = x.num_groups;  // the last group that starts at or before s
             while (lo < hi) {
                 const uint32_t mid = (lo + hi) / 2u;
@@ -213,7 +250,7 @@ __device__ __forceinline__ void write_info(const AttnArgs& a, const PrefixArgs& 
             }
             if (lo) {
                 const uint32_t g = lo - 1u, first = x.group_starts[g], end = x.group_starts[g + 1u];
-                if (s < end) info.x = shared_tokens(a, x, g, first, end - first);
+                if (s < end) info.x = shared_tokens<DP>(a, x, g, first, end - first);
             }
         }
         x.info[s] = info;
@@ -235,25 +272,25 @@ __global__ __launch_bounds__(kThreads<DP>, 2) void prefill_kernel(PrefillArgs p)
     extern __shared__ __align__(16) uint8_t smem[];
     const AttnArgs& a = p.a;
 
-    // A group's tiles that have no rows come behind all others: between them, in turn with
-    // live ones, they would leave whole shader engines without work.
-    const uint32_t split = SHARED ? blockIdx.x / a.kv_heads : blockIdx.y;
+    // of shared keys: the tiles of a split beside each other, workgroups without one behind all
+    uint32_t split = SHARED ? 0u : blockIdx.y, at = blockIdx.x / a.kv_heads;
     const uint32_t kvh = blockIdx.x % a.kv_heads;
-    const uint32_t at = SHARED ? blockIdx.y : blockIdx.x / a.kv_heads;
     uint32_t s = 0;
     SeqRows sr{};
     TilePlan<DP> t{};
     uint32_t tile_first = 0, tile_end = 0, shared = 0;
     if constexpr (SHARED) {
-        if (at >= p.x.tiles) {
-            if (kvh == 0u && split == 0u) write_info(a, p.x);
+        if (blockIdx.x == gridDim.x - 1u) {
+            write_info<DP>(a, p.x);
             return;
         }
-        const GroupTile gt = find_group_tile(a, p.x, at);
-        if (gt.kind == 0u) return;
+        const Groups all = all_groups<DP>(a, p.x);
+        if (all.wrong || at >= all.tiles * all.splits) return;
+        split = at / all.tiles;
+        const GroupTile gt = find_group_tile<DP>(a, p.x, at % all.tiles);
         s = gt.first_seq;  // its page table
         shared = gt.tokens;
-        const PrefixSplit ps = prefix_split(p.x, shared / TK);
+        const PrefixSplit ps = prefix_split(p.x, all.splits, shared / TK);
         if (split >= ps.used) return;
         t.rows = gt.seqs * a.seq_rows * a.group;
         t.r0 = gt.tile * kRows;
@@ -783,24 +820,22 @@ tsg_status prepare_prefill(const tsg_attn* attn) {
 tsg_status launch_prefixes(const tsg_attn* attn, const AttnArgs& a, PrefixArgs* x,
                            tsg_stream stream) {
     const Variant v = variant_of(attn);
-    const uint64_t rows = (uint64_t)a.rows * a.group, groups = std::min(x->num_groups, a.num_seqs);
+    const uint64_t rows = (uint64_t)a.rows * a.group;
     TSG_REQUIRE(rows * a.kv_heads <= kMaxPrefixRows, TSG_ERR_DECLINED,
                 "too many rows and query heads for the plan's scratch: tsg_attn_decode");
-    // each group may end inside a tile, and has one at least, also one of no sequences
-    const uint64_t tiles = rows / kRows + x->num_groups;
-    const uint64_t live = std::max(rows / kRows + (groups + 1u) / 2u, groups) * a.kv_heads;  // about
-    // (a launch of few enough blocks: the rows bound tiles and key heads, 2048 the groups)
     // One workgroup a CU, of at least four key tiles: with two, the partial sums' way through
     // memory costs what the shorter runs gain (64 sequences behind 16,000 tokens 57 us with one
     // and with two, 32 sequences 50 and 62, 8 30 and 33; 8 groups of 8 behind 4000 49 and 47).
+    // How many tiles there are, the device sees: a group that shares has two sequences at least,
+    // and may end inside a tile.
+    const uint64_t most = rows / kRows + std::min(x->num_groups, a.num_seqs / 2u);
     const uint64_t capacity_tiles =
         (((uint64_t)a.table_stride << a.page_shift) + v.tile_keys - 1u) / v.tile_keys;
     x->min_tiles = 4u;
-    uint64_t splits = (uint64_t)attn->ctx->num_cus * 256u / v.threads / live;
-    splits = std::min(splits, (capacity_tiles + x->min_tiles - 1u) / x->min_tiles);
+    x->units = std::max<uint32_t>(attn->ctx->num_cus * 256u / v.threads / a.kv_heads, 1u);
+    uint64_t splits = (capacity_tiles + x->min_tiles - 1u) / x->min_tiles;
     splits = std::min<uint64_t>(splits, kMaxPrefixRows / (rows * a.kv_heads));
     x->splits = (uint32_t)std::max<uint64_t>(splits, 1u);
-    x->tiles = (uint32_t)tiles;
     x->rows = (uint32_t)rows;
     const uint64_t row0 = kMaxPartials * (uint64_t)kDecodeTileRows, dp = attn->padded_dim;
     x->part_o = attn->partials + row0 * (dp + 2u);
@@ -809,8 +844,9 @@ tsg_status launch_prefixes(const tsg_attn* attn, const AttnArgs& a, PrefixArgs* 
     PrefillArgs p{};
     p.a = a;
     p.x = *x;
-    hipLaunchKernelGGL(v.shared, dim3(a.kv_heads * x->splits, (uint32_t)tiles + 1u),
-                       dim3(v.threads), v.lds, as_stream(stream), p);
+    const uint64_t units = std::max<uint64_t>(x->units, most);  // few: the rows bound them
+    hipLaunchKernelGGL(v.shared, dim3((uint32_t)(a.kv_heads * units) + 1u), dim3(v.threads), v.lds,
+                       as_stream(stream), p);
     return check_launch("attn_prefixes");
 }
 
