@@ -774,11 +774,11 @@ typedef struct tsg_attn tsg_attn; /* one kind of attention layer and its scratch
 tsg_status tsg_attn_check(const tsg_attn_config* config, const tsg_kv_pages* pages,
                           const tsg_attn_batch* batch);
 /* Calls on one tsg_attn run in stream order (they share its scratch: 26, 52, 102 or
- * 203 MB for head sizes up to 64, 128, 256, 512; two that overlap leave it unfit
- * for later ones); two tsg_attn may run beside each other. Graphs captured with one
- * are replayed one after the other, beside no other call of it, and before its
- * end. Not while a stream is captured (it allocates). The context outlives the
- * calls. */
+ * 203 MB for head sizes up to 64, 128, 256, 512, with a window two thirds of that;
+ * two that overlap leave it unfit for later ones); two tsg_attn may run beside each
+ * other. Graphs captured with one are replayed one after the other, beside no other
+ * call of it, and before its end. Not while a stream is captured (it allocates).
+ * The context outlives the calls. */
 tsg_status tsg_attn_create(tsg_ctx* ctx, const tsg_attn_config* config, tsg_attn** out);
 void tsg_attn_destroy(tsg_attn* attn);
 

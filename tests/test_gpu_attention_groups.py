@@ -2,6 +2,8 @@
 that do: neither their splits nor their sharing."""
 from __future__ import annotations
 
+import gc
+
 import pytest
 import torch
 
@@ -100,3 +102,20 @@ def test_more_tiles_than_the_card_holds(tsg, ctx):  # noqa: F811
     c = Case([1] * seqs, lengths, 4, 1, 32, seed=5)
     share(c, list(range(0, seqs + 1, 2)), [128] * (seqs // 2))
     check(tsg, ctx, c)
+
+
+@pytest.mark.parametrize("dim", [128, 512])
+def test_layers_with_a_window_hold_no_scratch_for_prefixes(tsg, ctx, dim):  # noqa: F811
+    """Their scratch is a prefill call's partial sums: 65,536 rows (whole in 2 MiB, and so allocated)."""
+    def held(window, plans=6):
+        gc.collect()
+        torch.cuda.synchronize()
+        before = torch.cuda.mem_get_info()[0]
+        keep = [tsg.Attention(ctx, 8, 1, dim, 16, window=window) for _ in range(plans)]
+        used = before - torch.cuda.mem_get_info()[0]
+        del keep
+        return used / plans
+
+    rows = 4 * (dim + 2)
+    assert 65536 * rows <= held(1024) <= 65536 * rows + 2 ** 22
+    assert 98304 * rows <= held(0) <= 98304 * rows + 2 ** 22

@@ -426,7 +426,8 @@ extern "C" tsg_status tsg_attn_create(tsg_ctx* ctx, const tsg_attn_config* confi
     while (attn->padded_dim < config->head_dim) attn->padded_dim *= 2u;
     DeviceScope scope(ctx->device);
     hipError_t e = scope.status;
-    const size_t words = (size_t)kScratchRows * (attn->padded_dim + 2u);
+    // a layer with a window takes no call that shares prefixes
+    const size_t words = (size_t)(config->window ? kPartialRows : kScratchRows) * (attn->padded_dim + 2u);
     if (e == hipSuccess) e = hipMalloc(&attn->partials, words * sizeof(float));
     if (e == hipSuccess) e = hipMalloc(&attn->arrivals, kMaxPartials * sizeof(uint32_t));
     if (e == hipSuccess) e = hipMemset(attn->arrivals, 0, kMaxPartials * sizeof(uint32_t));
