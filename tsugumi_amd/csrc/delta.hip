@@ -289,15 +289,8 @@ __global__ __launch_bounds__(256) void recurrent_kernel(DeltaArgs p) {
     const uint32_t c = id % slices * 32u + 4u * (lane & 7u), r0 = (lane >> 3) * R;
     const bool c_in = c < p.value_dim;
     const uint32_t vc = head * p.value_dim + c;
-    if (starts_wrong(d)) {
-        if (id == 0u && lane == 0u) report(d.error, kErrDeltaRows);
-        if (c_in && lane < 8u)
-            for (uint64_t row = s; row < d.rows; row += d.num_seqs)
-                *reinterpret_cast<uint2*>(p.out + row * p.out_stride + vc) =
-                    make_uint2(kDeltaNan2, kDeltaNan2);
-        return;
-    }
-    const DeltaSeq sq = delta_seq(d, s);
+    const DeltaSlot sq = delta_slot(d, s);
+    const uint32_t first = s * d.seq_rows;
     const uint64_t place = (uint64_t)head * p.key_dim * p.value_dim + (uint64_t)r0 * p.value_dim + c;
     // key_dim is a multiple of 16: eight rows are in or out together
     const auto in8 = [&](uint32_t i) { return c_in && r0 + (i & ~7u) < p.key_dim; };
@@ -331,16 +324,16 @@ __global__ __launch_bounds__(256) void recurrent_kernel(DeltaArgs p) {
     uint2 vn = make_uint2(0, 0);
     uint32_t an = 0, bn = 0;
     const auto fetch = [&](uint32_t i) {
-        const uint64_t row = sq.first + i;
+        const uint64_t row = first + i;
         load_key(p.q + row * p.q_stride, qn);
         load_key(p.k + row * p.k_stride, kn);
         if (c_in) vn = *reinterpret_cast<const uint2*>(p.v + row * p.v_stride + vc);
         an = p.a[row * p.a_stride + head];
         bn = p.b[row * p.b_stride + head];
     };
-    if (sq.count) fetch(0u);
+    fetch(0u);
 #pragma unroll 1
-    for (uint32_t row = 0; row < sq.count; ++row) {
+    for (uint32_t row = 0; row < d.seq_rows; ++row) {
         float q[R], k[R];
 #pragma unroll
         for (uint32_t i = 0; i < R; i += 8u) {
@@ -354,7 +347,7 @@ __global__ __launch_bounds__(256) void recurrent_kernel(DeltaArgs p) {
         }
         const uint2 vb = vn;
         const float av = f16_to_f32((uint16_t)an) + bias, bv = f16_to_f32((uint16_t)bn);
-        if (row + 1u < sq.count) fetch(row + 1u);
+        if (row + 1u < d.seq_rows) fetch(row + 1u);
         // sums over the key elements: |q|^2, |k|^2, q . k, S^T k, S^T q
         float sum[11];
 #pragma unroll
@@ -394,7 +387,7 @@ __global__ __launch_bounds__(256) void recurrent_kernel(DeltaArgs p) {
             uint2 h = make_uint2((uint32_t)f32_to_f16(o[0]) | (uint32_t)f32_to_f16(o[1]) << 16,
                                  (uint32_t)f32_to_f16(o[2]) | (uint32_t)f32_to_f16(o[3]) << 16);
             if (bad) h = make_uint2(kDeltaNan2, kDeltaNan2);
-            *reinterpret_cast<uint2*>(p.out + (uint64_t)(sq.first + row) * p.out_stride + vc) = h;
+            *reinterpret_cast<uint2*>(p.out + (uint64_t)(first + row) * p.out_stride + vc) = h;
         }
         if (d.kept > 1u) store(scalar_load(d.out_slots + s * d.kept + row));
     }
@@ -456,8 +449,6 @@ tsg_status delta_args(const tsg_delta* delta, const tsg_delta_states* states,
     return TSG_OK;
 }
 
-}  // namespace
-
 tsg_status launch_recurrent(const tsg_delta* delta, const DeltaArgs& a, tsg_stream stream) {
     const uint64_t waves =
         (uint64_t)a.seqs.num_seqs * a.value_heads * ((a.value_dim + 31u) / 32u);
@@ -473,6 +464,7 @@ tsg_status launch_recurrent(const tsg_delta* delta, const DeltaArgs& a, tsg_stre
     return check_launch("delta_recurrent");
 }
 
+}  // namespace
 }  // namespace tsg
 
 using namespace tsg;

@@ -55,21 +55,26 @@ __device__ __forceinline__ bool starts_wrong(const DeltaSeqs& d) {
     return __ballot(wrong) != 0;
 }
 
-struct DeltaSeq {
+struct DeltaSlot {
+    uint32_t in;  // to read; 0 where it is past the pool
+    bool fresh;   // no state before
+    bool bad;     // past the pool
+};
+__device__ __forceinline__ DeltaSlot delta_slot(const DeltaSeqs& d, uint32_t s) {
+    const uint32_t in = scalar_load(d.in_slots + s);
+    const bool fresh = in == TSG_NO_SLOT, inside = in < d.num_slots;
+    return DeltaSlot{inside ? in : 0u, fresh, !fresh && !inside};
+}
+struct DeltaSeq : DeltaSlot {
     uint32_t first, count;  // its rows
-    uint32_t in;            // slot to read; 0 where it is past the pool
-    bool fresh;             // no state before
-    bool bad;               // that slot is past the pool
 };
 // Sequence s, where no row start is wrong.
 __device__ __forceinline__ DeltaSeq delta_seq(const DeltaSeqs& d, uint32_t s) {
-    DeltaSeq r;
-    r.first = d.row_starts ? scalar_load(d.row_starts + s) : s * d.seq_rows;
-    r.count = d.row_starts ? scalar_load(d.row_starts + s + 1u) - r.first : d.seq_rows;
-    const uint32_t in = scalar_load(d.in_slots + s);
-    r.fresh = in == TSG_NO_SLOT;
-    r.bad = !r.fresh && in >= d.num_slots;
-    r.in = in < d.num_slots ? in : 0u;
+    DeltaSeq r{delta_slot(d, s), s * d.seq_rows, d.seq_rows};
+    if (d.row_starts) {
+        r.first = scalar_load(d.row_starts + s);
+        r.count = scalar_load(d.row_starts + s + 1u) - r.first;
+    }
     return r;
 }
 
@@ -146,9 +151,7 @@ __device__ __forceinline__ DeltaTile delta_tile(const DeltaSeqs& d, uint32_t id)
     return r;
 }
 
-// delta.hip
 constexpr uint32_t kDeltaNan2 = 0x7E007E00u;  // two fp16 NaN
-tsg_status launch_recurrent(const tsg_delta* delta, const DeltaArgs& a, tsg_stream stream);
 // delta_prefill.hip
 tsg_status prepare_delta(const tsg_delta* delta);  // once a plan, its device current
 uint64_t delta_scratch_bytes(const tsg_delta* delta, uint32_t rows, uint32_t num_seqs);
