@@ -81,19 +81,37 @@ __device__ __forceinline__ DeltaSeq delta_seq(const DeltaSeqs& d, uint32_t s) {
 // Whether an out slot of sequence s is past the pool, or another sequence's in or
 // out slot: the order of their reads and writes would be chance. Every kernel of
 // a call comes to the same answer, and writes none of the sequence's states then.
+// Every wave reads all sequences' slots, once, several loads in flight: quadratic in the
+// sequences, and less than the states' way through memory up to some thousand of them (512
+// sequences that keep 8 states of 4 heads of 64 x 64: 70 us; a pass over them for each state 176.
+// 4096 that keep one 154 for 383).
+template <uint32_t KEPT>
 __device__ __forceinline__ bool out_slots_clash(const DeltaSeqs& d, uint32_t s) {
-    const uint32_t lane = threadIdx.x & 63u, outs = d.num_seqs * d.kept;
-    bool clash = false;
-    for (uint32_t i = 0; i < d.kept; ++i) {
-        const uint32_t own = scalar_load(d.out_slots + s * d.kept + i);
-        if (own == TSG_NO_SLOT) continue;
-        clash = clash || own >= d.num_slots;
-        for (uint32_t t = lane; t < d.num_seqs; t += 64u)
-            clash = clash || (t != s && d.in_slots[t] == own);
-        for (uint32_t t = lane; t < outs; t += 64u)
-            clash = clash || (t - s * d.kept >= d.kept && d.out_slots[t] == own);
+    const uint32_t lane = threadIdx.x & 63u, outs = d.num_seqs * d.kept, first = s * d.kept;
+    uint32_t own[KEPT];
+    uint32_t any = 0, clash = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < KEPT; ++i) {
+        own[i] = i < d.kept ? scalar_load(d.out_slots + first + i) : TSG_NO_SLOT;
+        any |= own[i] != TSG_NO_SLOT;
+        clash |= (own[i] != TSG_NO_SLOT) & (own[i] >= d.num_slots);
     }
+    if (!any) return false;
+    const auto mine = [&](uint32_t slot) {
+        uint32_t hit = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < KEPT; ++i) hit |= slot == own[i];
+        return hit & (slot != TSG_NO_SLOT);
+    };
+#pragma unroll 4
+    for (uint32_t t = lane; t < d.num_seqs; t += 64u) clash |= (t != s) & mine(d.in_slots[t]);
+#pragma unroll 4
+    for (uint32_t t = lane; t < outs; t += 64u)
+        clash |= (t - first >= d.kept) & mine(d.out_slots[t]);
     return __ballot(clash) != 0;
+}
+__device__ __forceinline__ bool out_slots_clash(const DeltaSeqs& d, uint32_t s) {
+    return d.kept == 1u ? out_slots_clash<1u>(d, s) : out_slots_clash<kMaxDeltaKept>(d, s);
 }
 
 // The rows in tiles of R: sequence s's begin at id starts[s] / R + s (a sequence

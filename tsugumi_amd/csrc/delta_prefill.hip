@@ -486,7 +486,7 @@ __global__ __launch_bounds__(kScanThreads, (DKP <= 128u ? 4 : 2)) void scan_kern
     if (starts_wrong(d.seqs)) return;  // reported, and the rows made NaN, by the first kernel
     if (d.seqs.row_starts && d.seqs.num_seqs <= 64u) s = longest_first(d.seqs, s);
     const DeltaSeq sq = delta_seq(d.seqs, s);
-    const bool bad = out_slots_clash(d.seqs, s) || sq.bad;
+    const bool bad = out_slots_clash<1u>(d.seqs, s) || sq.bad;
     const uint32_t col4 = head * d.value_dim + c0 + 4u * (lane & 3u);
     if (bad) {
         if (at == 0u && kh == 0u && threadIdx.x == 0u) report(d.seqs.error, kErrDeltaSlot);
