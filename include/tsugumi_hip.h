@@ -943,14 +943,22 @@ tsg_status tsg_delta_conv(tsg_delta* delta, tsg_stream stream, const tsg_delta_s
 /* The rule for 1...8 rows of every sequence (a decoded token, a speculative
  * block); TSG_ERR_DECLINED for more; row_starts must be NULL. a_log, dt_bias
  * [value_heads] fp32. out [rows, value_heads * value_dim] fp16 shares no element
- * with the rows. q, k, v, out rows on 16 bytes. All in fp32. */
+ * with the rows. q, k, v, out rows on 16 bytes. Products, sums and states in fp32,
+ * outputs rounded once; states up to 1e30 (their products with rows are fp32 sums). */
 tsg_status tsg_delta_decode(tsg_delta* delta, tsg_stream stream, const tsg_delta_states* states,
                             const tsg_delta_batch* batch, const tsg_delta_rows* rows,
                             const float* a_log, const float* dt_bias, uint16_t* out,
                             uint32_t out_stride);
-/* The same for any number of rows of each sequence, ragged or uniform (kept is
- * 1). scratch: tsg_delta_prefill_scratch_bytes of device memory on 256 bytes,
- * for this call alone until it has run. */
+/* The rule for any number of rows of each sequence, ragged or uniform (kept is 1), 64
+ * rows at a time on fp16 matrix instructions. Operands other than q and k are split
+ * into two halves of fp16: 22 bits of each, or 2^-49 of a bound on its column, where
+ * decode has fp32's 24 bits. The bound is sqrt(key_dim) times the largest of the column
+ * of the state that the 64 rows begin with, and 65 times their largest value: with
+ * states and values up to 65,504 2^-49 of it is under fp16's least step. Sums and
+ * states in fp32, outputs rounded once.
+ * scratch: tsg_delta_prefill_scratch_bytes of device memory on 256 bytes, for this
+ * call alone until it has run: for every 64 rows, and once more a sequence, 25.25 KiB
+ * a value head and 24, 48 or 96 KiB a key head (key_dim up to 64, 128, 256). */
 size_t tsg_delta_prefill_scratch_bytes(const tsg_delta* delta, uint32_t rows, uint32_t num_seqs);
 tsg_status tsg_delta_prefill(tsg_delta* delta, tsg_stream stream, const tsg_delta_states* states,
                              const tsg_delta_batch* batch, const tsg_delta_rows* rows,

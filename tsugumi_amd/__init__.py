@@ -1255,7 +1255,8 @@ class GatedDelta:
         return DeltaBatch(self, in_slots, out_slots, rows, row_starts)
 
     def scratch_bytes(self, rows: int, num_seqs: int) -> int:
-        """Bytes of device memory that encode_prefill needs for such a call."""
+        """Bytes of device memory that encode_prefill needs for such a call: with 32 value and 16
+        key heads of 128 25 KB a row, and 1.6 MB a sequence."""
         _words(rows=rows, num_seqs=num_seqs)
         return int(self.lib.tsg_delta_prefill_scratch_bytes(self.handle, rows, num_seqs))
 

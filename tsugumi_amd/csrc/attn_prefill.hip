@@ -20,7 +20,8 @@
 //
 // The keys that a group of decoded sequences shares are taken the same way, the group's rows in
 // tiles of 128 (SHARED); the decode kernel joins these sums with each row's own keys'. 64
-// sequences of 8 key heads of 128 behind 16,000 keys: 44 us, and 24 the decode kernel's.
+// sequences of 32 query and 8 key heads of 128 behind 16,000 keys, with 11 to 501 of their own: 36
+// us, and 24 the decode kernel's.
 #include "attn_internal.hpp"
 
 namespace tsg {
@@ -824,8 +825,9 @@ tsg_status launch_prefixes(const tsg_attn* attn, const AttnArgs& a, PrefixArgs* 
     TSG_REQUIRE(rows * a.kv_heads <= kMaxPrefixRows, TSG_ERR_DECLINED,
                 "too many rows and query heads for the plan's scratch: tsg_attn_decode");
     // One workgroup a CU, of at least four key tiles: with two, the partial sums' way through
-    // memory costs what the shorter runs gain (64 sequences behind 16,000 tokens 57 us with one
-    // and with two, 32 sequences 50 and 62, 8 30 and 33; 8 groups of 8 behind 4000 49 and 47).
+    // memory costs what the shorter runs gain (both launches, 250 keys a sequence of its own
+    // behind 16,000: 64 sequences 58 us with one and with two, with heads of 256 72 and 86, 32
+    // sequences 54 and 64, 8 32 and 35; 8 groups of 8 behind 4096, 200 of their own, 49 and 48).
     // How many tiles there are, the device sees: a group that shares has two sequences at least,
     // and may end inside a tile.
     const uint64_t most = rows / kRows + std::min(x->num_groups, a.num_seqs / 2u);

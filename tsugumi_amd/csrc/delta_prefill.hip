@@ -117,9 +117,10 @@ __device__ __forceinline__ double wave_scan(double x) {
 }
 
 // A workgroup takes a chunk of a value head; those of one key head, which read the same rows,
-// come one after another on one XCD. Bound by the chain of its steps, with four workgroups a
-// CU (a key head's value heads in one workgroup, the rows' products once: 220 registers, 130 us
-// for 91 over 8192 rows and two value heads).
+// come one after another on one XCD. 8192 rows x 32 heads of 128 x 128: 85 us. Bound by the chain
+// of its steps, with four workgroups a CU: the vector units are busy 45 % of the time, LDS 19, the
+// matrix units 8 (a key head's value heads in one workgroup, the rows' products once: 220
+// registers, 130 us for what then took 91).
 template <uint32_t DKP>
 __global__ __launch_bounds__(256, 4) void prepare_kernel(ChunkArgs p) {
     constexpr uint32_t KS = DKP + 8u;  // halves of a key row in LDS
@@ -427,15 +428,19 @@ __global__ __launch_bounds__(256, 4) void prepare_kernel(ChunkArgs p) {
 // to 3) or of Q with the state; the first four go on to U, the others to the outputs. What
 // one wave's products need of the others' goes through LDS as operands of the matrix unit,
 // three exchanges a chunk: S, then R = beta (V - e^G K^ S), then U. Operands of the next
-// chunk are loaded as soon as this one's are used. Bound by the chain of a chunk's steps,
-// which leave the units mostly idle: 1.6 us each with one workgroup a CU (8192 rows x 32 heads
-// of 128 x 128: 202 us; four waves that do both, 260). 32 columns a workgroup halve the loads,
-// but one workgroup fits a CU then (11207 rows of 7 prompts: 292 us for 268).
+// chunk are loaded as soon as this one's are used. 8192 rows x 32 heads of 128 x 128: 214 us, 1.7
+// a chunk with one workgroup a CU; 7 prompts of 11207 rows 271, 1.5 with two. Bound by the
+// operands' way from L2, 84 KB a chunk and workgroup, 12 and 14 TB/s in these two: the
+// outputs' weights in two halves, 7 % more of them, took 8 % more time, where the chains of
+// products and the place of the outputs' step changed nothing. Vector units are busy 40 and 51 % of
+// the time, LDS 30 and 36 (conflicts 7 and 8), matrix units 13 and 16. When a chunk took 75 KB:
+// four waves for both roles 260 us for 202; 32 columns a workgroup, which halve the loads, but
+// of which one fits a CU, 292 for 268 (the prompts).
 
 constexpr uint32_t kScanThreads = 512;
 
 // The sequence of the n-th most rows, of up to 64: the longest chains are begun first (7
-// prompts of 201 to 3001 rows 251 us, in order 262).
+// prompts of 201 to 3001 rows 251 us, in order 262, at 75 KB of operands a chunk).
 __device__ __forceinline__ uint32_t longest_first(const DeltaSeqs& d, uint32_t n) {
     const uint32_t lane = threadIdx.x & 63u;
     const bool live = lane < d.num_seqs;
